@@ -478,6 +478,92 @@ int st_hip_merge_heads_f32_dev(size_t batch, size_t seq, size_t heads, size_t he
                                const float *contexts_in, float *out_f32, uint16_t *out_bf16,
                                void *stream);
 
+/* ---- decoding from a paged 8-bit cache ------------------------------------------------------------ */
+/* What a decoder needs to answer token by token: rotary positions, a cache of keys and values, its bookkeeping, and attention over it.
+ * No reference counterpart.  Device pointers, asynchronous on `stream`; nothing is read back, so that a step can be captured
+ * and replayed while lengths change.
+ *
+ * A batch is ragged: request r owns rows row_offsets[r] .. row_offsets[r+1]-1 of the step's matrices (row_offsets has requests+1
+ * entries, ascending from 0), holds lengths[r] tokens and finds token t in page page_table[r*table_width + t/page_size], at place
+ * t % page_size.  A step may be given more rows than the requests bring, as one captured for replay has to be: the slots of those
+ * behind are -1, which appending skips, and the attention does not touch their results.
+ *
+ * The cache's memory is the caller's: e4m3 values, and for every page and head one f32 scale for its keys and one for its values
+ * (value = code * scale).  Scales are powers of two, so that scaling never rounds: an e4m3 value keeps its four significant bits
+ * whatever the scale.  Values lie transposed, so that both products of the attention read whole 16-byte runs of what they sum over. */
+typedef struct {
+    size_t pages;     /* 1 or more */
+    size_t page_size; /* tokens: 16, 32, 64, 128 or 256 */
+    size_t kv_heads;
+    size_t head_dim;  /* 64, 128 or 256 */
+    uint8_t *k;       /* (pages, kv_heads, page_size, head_dim), 16-byte aligned, as is v */
+    uint8_t *v;       /* (pages, kv_heads, head_dim, page_size) */
+    float *k_scales;  /* (pages, kv_heads) */
+    float *v_scales;  /* (pages, kv_heads) */
+} st_hip_kv_cache;
+
+/* Page tables, slots and positions of a step, from what each request has in the cache (cached[r]) and brings (fresh[r] rows; 0 for one
+ * that waits).  Pages that the new tokens need are dealt in request order from free_pages, beginning at *taken_before (NULL: 0), and
+ * written into page_table, whose other entries stay as they are.  Written besides: row_offsets[requests+1]; lengths[r] =
+ * cached[r]+fresh[r]; for each of `rows` rows its position within its request and its slot, page*page_size + place, both -1 behind the
+ * last request's; and
+ * counts[3] = {pages taken from free_pages in all (the next step's *taken_before), rows used, requests refused}.
+ * A request is refused, alone, if a count of it is negative, its tokens pass table_width pages, its rows end behind `rows`, or it needs
+ * pages where the pages that it and those before it need (but for requests of the first two kinds) are more than are left: it takes
+ * none, lengths[r] is 0, and its rows' positions and slots are -1.  A slot is -1 too where its page's number is negative or the slot
+ * beyond int32.  Rows of a request with a negative fresh[r] are none; row_offsets never passes `rows`.
+ * What is written must not overlap what is read: cached may not be lengths, taken_before not counts. */
+int st_hip_page_tables_dev(size_t requests, size_t page_size, const int32_t *cached, const int32_t *fresh, size_t free_count,
+                           const int32_t *free_pages, const int32_t *taken_before, size_t table_width, int32_t *page_table,
+                           size_t rows, int32_t *row_offsets, int32_t *lengths, int32_t *positions, int32_t *slots, int32_t *counts,
+                           void *stream);
+
+/* Rotary positions.  The leading rotary_dim values of every head turn in pairs, (2i, 2i+1) if `interleaved`, else (i, i+rotary_dim/2):
+ * (a, b) -> magnitude * (a*cos - b*sin, a*sin + b*cos) of the angle position * w(i), with w(i) = base^(-2i/rotary_dim) / factor.
+ * original_length > 0 scales by parts instead, for contexts longer than a model was trained on: pairs that turn high_turns times or
+ * more within original_length positions keep base^(-2i/rotary_dim), those below low_turns times are divided by factor, and between the
+ * two the share that is kept rises evenly with the turns. */
+typedef struct {
+    size_t rotary_dim;  /* even, at most head_dim */
+    int interleaved;
+    float base;         /* 1 or more; usually 10000 and above */
+    float factor;       /* above 0; 1 for none */
+    float original_length, low_turns, high_turns; /* low_turns < high_turns; unused if original_length is 0 */
+    float magnitude;    /* 1 for a rotation */
+} st_hip_rotary;
+/* `heads` neighbouring heads of every row (row strides ld_in and ld_out in values), turned by the row's position, or by row % sequence
+ * if positions is NULL; what does not turn is copied.  `transposed` != 0 turns back: the gradient of the call without it.  Angles are
+ * reduced in 64 bits, so that far positions cost no accuracy; the products are f32, rounded once.  out may be in, with the same
+ * stride, or columns of the same rows that the input's do not meet; other overlaps are refused.  head_dim up to 1024. */
+int st_hip_rotary_f32_dev(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary *rotary, int transposed,
+                          const int32_t *positions, const float *in, size_t ld_in, float *out, size_t ld_out, void *stream);
+int st_hip_rotary_bf16_dev(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary *rotary, int transposed,
+                           const int32_t *positions, const uint16_t *in, size_t ld_in, uint16_t *out, size_t ld_out, void *stream);
+
+/* New keys and values into the cache: row i of k and v (kv_heads*head_dim values each, row stride ld) goes to slot slots[i]; slots
+ * outside the cache, -1 among them, are skipped.  The rows of a page stand together, as st_hip_page_tables_dev gives them, in any order;
+ * of rows for one slot the last counts.  Slots of one page that come apart, with another page's or a skipped row between them, race:
+ * the page's values are then unspecified (nothing else is touched).
+ * A page whose place 0 is among them begins anew.  Its scales become the smallest powers of two, at least 2^-118, with which the new
+ * rows' largest finite values are at most 448; those of other pages grow to that where it is larger, and what the page held is then
+ * rounded to the new scale (exact but for values below 2^-6 of the new scale).  Codes are rounded to nearest, ties to even; NaN and
+ * infinities become NaN. */
+int st_hip_kv_cache_append_f32_dev(const st_hip_kv_cache *cache, size_t rows, const int32_t *slots, const float *k, const float *v,
+                                   size_t ld, void *stream);
+int st_hip_kv_cache_append_bf16_dev(const st_hip_kv_cache *cache, size_t rows, const int32_t *slots, const uint16_t *k,
+                                    const uint16_t *v, size_t ld, void *stream);
+
+/* Attention of `rows` rows of bf16 queries (heads*head_dim values each, row stride ld_q) over the cache: out = softmax(scale * q.k) v,
+ * rounded to bf16.  heads is a multiple of kv_heads, and head h reads keys of head h / (heads/kv_heads).  `causal` != 0: a request's rows
+ * are its last tokens, the last row sees all lengths[r] keys and each one before it one key less; 0: every row sees all of them (an
+ * encoder's states).  Rows that see no key are 0.  A length counts as at most table_width pages; tokens of pages outside the cache
+ * are left out.  The products take bf16 and accumulate in f32, the softmax is f32; its weights enter the second product as bf16.
+ * q 16-byte and out 8-byte aligned, ld_q a multiple of 8 and ld_out of 4, otherwise ST_HIP_ERR_UNSUPPORTED.  Long contexts of few rows
+ * are cut over workgroups, whose parts go through the stream's scratch memory. */
+int st_hip_attention_kv_cache_bf16_dev(const st_hip_kv_cache *cache, size_t requests, size_t rows, size_t heads, float scale, int causal,
+                                       const int32_t *row_offsets, const int32_t *lengths, const int32_t *page_table,
+                                       size_t table_width, const uint16_t *q, size_t ld_q, uint16_t *out, size_t ld_out, void *stream);
+
 /* ---- measurement aid ---------------------------------------------------------------------------- */
 /* A loop of nothing but bf16 matrix instructions (v_mfma_f32_32x32x16_bf16) on register operands: `workgroups` × 4
  * wavefronts each issue 32·iterations of them (2·32·32·16 flop each) on fragments read once from `operands` (device,

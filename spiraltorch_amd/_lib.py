@@ -76,6 +76,16 @@ class DecoderConfig(ctypes.Structure):
     ]
 
 
+class KvCacheStruct(ctypes.Structure):
+    _fields_ = [(name, c_size_t) for name in ("pages", "page_size", "kv_heads", "head_dim")] + \
+        [(name, c_void_p) for name in ("k", "v", "k_scales", "v_scales")]
+
+
+class RotaryStruct(ctypes.Structure):
+    _fields_ = [("rotary_dim", c_size_t), ("interleaved", c_int)] + \
+        [(name, c_float) for name in ("base", "factor", "original_length", "low_turns", "high_turns", "magnitude")]
+
+
 # name -> (restype, argtypes); this table is also what the symbol-export test walks.
 SIGNATURES = {
     "st_hip_init": (c_int, []),
@@ -180,6 +190,16 @@ SIGNATURES = {
                                            c_void_p, c_void_p]),
     "st_hip_merge_heads_f32_dev": (c_int, [c_size_t, c_size_t, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p,
                                            c_void_p]),
+    "st_hip_page_tables_dev": (c_int, [c_size_t, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p,
+                                       c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "st_hip_rotary_f32_dev": (c_int, [c_size_t] * 4 + [POINTER(RotaryStruct), c_int, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t,
+                                                       c_void_p]),
+    "st_hip_rotary_bf16_dev": (c_int, [c_size_t] * 4 + [POINTER(RotaryStruct), c_int, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t,
+                                                        c_void_p]),
+    "st_hip_kv_cache_append_f32_dev": (c_int, [POINTER(KvCacheStruct), c_size_t, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "st_hip_kv_cache_append_bf16_dev": (c_int, [POINTER(KvCacheStruct), c_size_t, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "st_hip_attention_kv_cache_bf16_dev": (c_int, [POINTER(KvCacheStruct), c_size_t, c_size_t, c_size_t, c_float, c_int, c_void_p, c_void_p,
+                                                   c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
     "st_hip_decoder_weight_count": (c_size_t, [POINTER(DecoderConfig)]),
     "st_hip_decoder_create": (c_int, [POINTER(DecoderConfig), c_void_p, c_size_t, POINTER(c_void_p)]),
     "st_hip_decoder_forward_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),

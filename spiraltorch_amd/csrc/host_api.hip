@@ -301,6 +301,87 @@ int launch_status(hipError_t rc, const char *ctx)
     return ST_HIP_OK;
 }
 
+bool valid_page_size(size_t tokens) { return tokens >= 16 && tokens <= 256 && (tokens & (tokens - 1)) == 0; }
+
+// int32 values in device memory that a call reads or writes.
+struct Extent {
+    const int32_t *at;
+    size_t count;
+    bool meets(const Extent &other) const
+    {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(other.at);
+        return count && other.count && a < b + other.count * sizeof(int32_t) && b < a + count * sizeof(int32_t);
+    }
+};
+
+// Whether rows of `width` values, `ld_a` and `ld_b` apart, share memory: columns of one matrix that do not meet share none.
+bool overlaps_except_columns(const void *a, size_t ld_a, const void *b, size_t ld_b, size_t rows, size_t width, size_t size)
+{
+    const uintptr_t at_a = reinterpret_cast<uintptr_t>(a), at_b = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t end_a = at_a + ((rows - 1) * ld_a + width) * size, end_b = at_b + ((rows - 1) * ld_b + width) * size;
+    if (at_a >= end_b || at_b >= end_a) return false;
+    if (ld_a != ld_b) return true;
+    const uintptr_t apart = (at_a < at_b ? at_b - at_a : at_a - at_b) % (ld_a * size);
+    return apart < width * size || apart > (ld_a - width) * size;
+}
+
+int check_rotary(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary *r, const int32_t *positions, const void *in,
+                 size_t ld_in, const void *out, size_t ld_out, size_t size, bool *work)
+{
+    if (!r) return fail(ST_HIP_ERR_INVALID, "rotary configuration is null");
+    if (r->rotary_dim % 2 != 0 || r->rotary_dim > head_dim)
+        return fail(ST_HIP_ERR_INVALID, "rotary_dim %zu is odd or above head_dim %zu", r->rotary_dim, head_dim);
+    if (!(r->base >= 1.0f) || !std::isfinite(r->base) || !(r->factor > 0.0f) || !std::isfinite(r->factor) || !std::isfinite(r->magnitude))
+        return fail(ST_HIP_ERR_INVALID, "rotary base, factor and magnitude must be finite, the base at least 1 and the factor positive");
+    if (!(r->original_length >= 0.0f) || !std::isfinite(r->original_length) ||
+        (r->original_length > 0.0f && !(std::isfinite(r->low_turns) && std::isfinite(r->high_turns) && r->low_turns < r->high_turns)))
+        return fail(ST_HIP_ERR_INVALID, "rotary scaling by parts needs low_turns < high_turns and a finite original_length");
+    size_t width = 0, values = 0;
+    if (!checked_mul(heads, head_dim, &width) || !checked_mul(rows, width, &values)) return fail(ST_HIP_ERR_INVALID, "rotary dimensions overflow");
+    if (head_dim > 1024) return fail(ST_HIP_ERR_UNSUPPORTED, "rotary head_dim %zu is above 1024", head_dim);
+    if (rows > kMaxDim || width > kMaxDim || ld_in > kMaxDim || ld_out > kMaxDim || sequence > kMaxDim)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "rotary dimension exceeds i32");
+    if (values == 0) return ST_HIP_OK;
+    if (!in || !out) return fail(ST_HIP_ERR_INVALID, "rotary received a null pointer");
+    if (!positions && sequence == 0) return fail(ST_HIP_ERR_INVALID, "rotary needs positions or a sequence length");
+    if (ld_in < width || ld_out < width)
+        return fail(ST_HIP_ERR_INVALID, "rotary row stride %zu/%zu is smaller than heads*head_dim=%zu", ld_in, ld_out, width);
+    if (!(in == out && ld_in == ld_out) && overlaps_except_columns(in, ld_in, out, ld_out, rows, width, size))
+        return fail(ST_HIP_ERR_INVALID, "rotary output overlaps its input");
+    *work = true;
+    return ST_HIP_OK;
+}
+
+int check_kv_cache(const st_hip_kv_cache *c)
+{
+    if (!c) return fail(ST_HIP_ERR_INVALID, "kv cache is null");
+    if (!valid_page_size(c->page_size)) return fail(ST_HIP_ERR_UNSUPPORTED, "a page holds 16, 32, 64, 128 or 256 tokens, not %zu", c->page_size);
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache head_dim must be 64, 128 or 256, not %zu", c->head_dim);
+    if (c->pages == 0 || c->kv_heads == 0) return fail(ST_HIP_ERR_INVALID, "kv cache dimensions must be positive");
+    if (c->pages > kMaxDim || c->kv_heads > kMaxDim) return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache dimension exceeds i32");
+    size_t blocks = 0, bytes = 0;
+    if (!checked_mul(c->pages, c->kv_heads, &blocks) || !checked_mul(blocks, c->page_size * c->head_dim, &bytes))
+        return fail(ST_HIP_ERR_INVALID, "kv cache dimensions overflow");
+    if (!c->k || !c->v || !c->k_scales || !c->v_scales) return fail(ST_HIP_ERR_INVALID, "kv cache holds a null pointer");
+    if (reinterpret_cast<uintptr_t>(c->k) % 16 != 0 || reinterpret_cast<uintptr_t>(c->v) % 16 != 0)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache values must be 16-byte aligned");
+    return ST_HIP_OK;
+}
+
+int check_append(const st_hip_kv_cache *c, size_t rows, const int32_t *slots, const void *k, const void *v, size_t ld, size_t size)
+{
+    ST_HIP_CHECK(check_kv_cache(c));
+    const size_t width = c->kv_heads * c->head_dim;  // (below the cache's bytes)
+    size_t values = 0;
+    if (!checked_mul(rows, ld, &values) || values > static_cast<size_t>(-1) / size) return fail(ST_HIP_ERR_INVALID, "kv cache append dimensions overflow");
+    if (rows > kMaxDim - 256 || ld > kMaxDim || c->kv_heads > 65535) return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache append dimension exceeds the kernel's");
+    if (rows == 0) return ST_HIP_OK;
+    if (!slots || !k || !v) return fail(ST_HIP_ERR_INVALID, "kv cache append received a null pointer");
+    if (ld < width) return fail(ST_HIP_ERR_INVALID, "kv cache append row stride %zu is smaller than kv_heads*head_dim=%zu", ld, width);
+    return ST_HIP_OK;
+}
+
 // First non-finite value of a host slice, reported like TensorError::NonFiniteValue
 // (crates/st-tensor/src/pure.rs:5521-5533).
 int validate_finite_slice(const char *label, const float *values, size_t len)
@@ -1188,6 +1269,103 @@ int st_hip_attention_bf16_dev(size_t batch, size_t heads, size_t sequence, size_
                     head_dim);
     return launch_status(launch_attention_bf16(batch, heads, sequence, head_dim, scale, causal != 0, q, k, v, ld_in, out,
                                                ld_out, as_stream(stream)),
+                         "attention launch");
+}
+
+int st_hip_page_tables_dev(size_t requests, size_t page_size, const int32_t *cached, const int32_t *fresh, size_t free_count,
+                           const int32_t *free_pages, const int32_t *taken_before, size_t table_width, int32_t *page_table,
+                           size_t rows, int32_t *row_offsets, int32_t *lengths, int32_t *positions, int32_t *slots, int32_t *counts,
+                           void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    if (!valid_page_size(page_size)) return fail(ST_HIP_ERR_UNSUPPORTED, "a page holds 16, 32, 64, 128 or 256 tokens, not %zu", page_size);
+    size_t entries = 0;
+    if (!checked_mul(requests, table_width, &entries) || entries > static_cast<size_t>(-1) / 8)
+        return fail(ST_HIP_ERR_INVALID, "page table dimensions overflow");
+    if (requests >= kMaxDim || table_width >= kMaxDim || rows >= kMaxDim || free_count >= kMaxDim)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "page table dimension exceeds i32");
+    if (!row_offsets || !counts || (requests && (!cached || !fresh || !lengths)) || (entries && !page_table) || (rows && (!positions || !slots)) ||
+        (free_count && !free_pages))
+        return fail(ST_HIP_ERR_INVALID, "page tables received a null pointer");
+    const Extent read[] = {{cached, requests}, {fresh, requests}, {free_pages, free_count}, {taken_before, taken_before ? 1u : 0u}};
+    const Extent written[] = {{page_table, entries}, {row_offsets, requests + 1}, {lengths, requests}, {positions, rows}, {slots, rows}, {counts, 3}};
+    for (const Extent &w : written) {
+        for (const Extent &r : read)
+            if (w.meets(r)) return fail(ST_HIP_ERR_INVALID, "page tables: what is written overlaps what is read");
+        for (const Extent &other : written)
+            if (&other != &w && w.meets(other)) return fail(ST_HIP_ERR_INVALID, "page tables: results overlap");
+    }
+    return launch_status(launch_page_tables(requests, page_size, cached, fresh, free_count, free_pages, taken_before, table_width, page_table, rows,
+                                            row_offsets, lengths, positions, slots, counts, as_stream(stream)),
+                         "page tables launch");
+}
+
+int st_hip_rotary_f32_dev(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary *rotary, int transposed,
+                          const int32_t *positions, const float *in, size_t ld_in, float *out, size_t ld_out, void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    bool work = false;
+    ST_HIP_CHECK(check_rotary(rows, sequence, heads, head_dim, rotary, positions, in, ld_in, out, ld_out, sizeof(float), &work));
+    if (!work) return ST_HIP_OK;
+    return launch_status(launch_rotary_f32(rows, sequence, heads, head_dim, *rotary, transposed != 0, positions, in, ld_in, out, ld_out, as_stream(stream)),
+                         "rotary launch");
+}
+
+int st_hip_rotary_bf16_dev(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary *rotary, int transposed,
+                           const int32_t *positions, const uint16_t *in, size_t ld_in, uint16_t *out, size_t ld_out, void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    bool work = false;
+    ST_HIP_CHECK(check_rotary(rows, sequence, heads, head_dim, rotary, positions, in, ld_in, out, ld_out, sizeof(uint16_t), &work));
+    if (!work) return ST_HIP_OK;
+    return launch_status(launch_rotary_bf16(rows, sequence, heads, head_dim, *rotary, transposed != 0, positions, in, ld_in, out, ld_out, as_stream(stream)),
+                         "rotary launch");
+}
+
+int st_hip_kv_cache_append_f32_dev(const st_hip_kv_cache *cache, size_t rows, const int32_t *slots, const float *k, const float *v,
+                                   size_t ld, void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    ST_HIP_CHECK(check_append(cache, rows, slots, k, v, ld, sizeof(float)));
+    if (rows == 0) return ST_HIP_OK;
+    return launch_status(launch_kv_cache_append_f32(*cache, rows, slots, k, v, ld, as_stream(stream)), "kv cache append launch");
+}
+
+int st_hip_kv_cache_append_bf16_dev(const st_hip_kv_cache *cache, size_t rows, const int32_t *slots, const uint16_t *k,
+                                    const uint16_t *v, size_t ld, void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    ST_HIP_CHECK(check_append(cache, rows, slots, k, v, ld, sizeof(uint16_t)));
+    if (rows == 0) return ST_HIP_OK;
+    return launch_status(launch_kv_cache_append_bf16(*cache, rows, slots, k, v, ld, as_stream(stream)), "kv cache append launch");
+}
+
+int st_hip_attention_kv_cache_bf16_dev(const st_hip_kv_cache *cache, size_t requests, size_t rows, size_t heads, float scale, int causal,
+                                       const int32_t *row_offsets, const int32_t *lengths, const int32_t *page_table,
+                                       size_t table_width, const uint16_t *q, size_t ld_q, uint16_t *out, size_t ld_out, void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    ST_HIP_CHECK(check_kv_cache(cache));
+    if (heads == 0 || heads % cache->kv_heads != 0)
+        return fail(ST_HIP_ERR_INVALID, "attention heads %zu are not a multiple of the cache's %zu", heads, cache->kv_heads);
+    if (!std::isfinite(scale))
+        return fail(ST_HIP_ERR_NONFINITE, "non-finite value encountered in scaled_dot_attention_scale: %g", static_cast<double>(scale));
+    size_t width = 0, columns = 0, items = 0, entries = 0;
+    if (!checked_mul(heads, cache->head_dim, &width) || !checked_mul(rows, heads, &columns) || !checked_mul(requests, cache->kv_heads, &items) ||
+        !checked_mul(requests, table_width, &entries) || entries > static_cast<size_t>(-1) / 8)
+        return fail(ST_HIP_ERR_INVALID, "attention dimensions overflow");
+    if (width > kMaxDim || columns > kMaxDim || items > kMaxDim / 2 || requests >= kMaxDim || table_width > kMaxDim || ld_q > kMaxDim || ld_out > kMaxDim)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "attention dimension exceeds i32");
+    if (requests == 0 || rows == 0) return ST_HIP_OK;
+    if (!row_offsets || !lengths || (entries && !page_table) || !q || !out) return fail(ST_HIP_ERR_INVALID, "attention received a null pointer");
+    if (ld_q < width || ld_out < width)
+        return fail(ST_HIP_ERR_INVALID, "attention row stride %zu/%zu is smaller than heads*head_dim=%zu", ld_q, ld_out, width);
+    if (ld_q % 8 != 0 || ld_out % 4 != 0 || reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 8 != 0)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "attention over the cache needs ld_q %% 8 == 0, ld_out %% 4 == 0 and aligned buffers");
+    if (overlaps_except_columns(q, ld_q, out, ld_out, rows, width, sizeof(uint16_t)))
+        return fail(ST_HIP_ERR_INVALID, "attention output overlaps its queries");
+    return launch_status(launch_attention_kv_cache_bf16(*cache, requests, rows, heads, scale, causal != 0, row_offsets, lengths, page_table, table_width,
+                                                        q, ld_q, out, ld_out, as_stream(stream)),
                          "attention launch");
 }
 

@@ -200,6 +200,22 @@ hipError_t launch_attention_bf16(size_t batch, size_t heads, size_t sequence, si
                                  bool causal, const uint16_t *q, const uint16_t *k, const uint16_t *v,
                                  size_t ld_in, uint16_t *out, size_t ld_out, hipStream_t stream);
 
+// Decoding from a paged 8-bit cache (see st_hip.h).  Uses the stream's scratch memory where long contexts are cut over workgroups.
+hipError_t launch_attention_kv_cache_bf16(const st_hip_kv_cache &cache, size_t requests, size_t rows, size_t heads, float scale, bool causal,
+                                          const int32_t *row_offsets, const int32_t *lengths, const int32_t *page_table, size_t table_width,
+                                          const uint16_t *q, size_t ld_q, uint16_t *out, size_t ld_out, hipStream_t stream);
+hipError_t launch_page_tables(size_t requests, size_t page_size, const int32_t *cached, const int32_t *fresh, size_t free_count,
+                              const int32_t *free_pages, const int32_t *taken_before, size_t table_width, int32_t *page_table, size_t rows,
+                              int32_t *row_offsets, int32_t *lengths, int32_t *positions, int32_t *slots, int32_t *counts, hipStream_t stream);
+hipError_t launch_kv_cache_append_f32(const st_hip_kv_cache &cache, size_t rows, const int32_t *slots, const float *k, const float *v,
+                                      size_t ld, hipStream_t stream);
+hipError_t launch_kv_cache_append_bf16(const st_hip_kv_cache &cache, size_t rows, const int32_t *slots, const uint16_t *k, const uint16_t *v,
+                                       size_t ld, hipStream_t stream);
+hipError_t launch_rotary_f32(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary &rotary, bool transposed,
+                             const int32_t *positions, const float *in, size_t ld_in, float *out, size_t ld_out, hipStream_t stream);
+hipError_t launch_rotary_bf16(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary &rotary, bool transposed,
+                              const int32_t *positions, const uint16_t *in, size_t ld_in, uint16_t *out, size_t ld_out, hipStream_t stream);
+
 hipError_t launch_layer_norm_f32(size_t rows, size_t cols, const float *x, const float *residual,
                                  const float *gamma, const float *beta, float epsilon, float *out_f32,
                                  uint16_t *out_bf16, hipStream_t stream);

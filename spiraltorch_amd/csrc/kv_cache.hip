@@ -1,0 +1,350 @@
+// The paged 8-bit cache: page tables and slot maps of a step's ragged batch, and new keys and values into their pages.
+#include <algorithm>
+
+#include "device_math.h"
+#include "kernels.h"
+
+namespace sthip {
+
+namespace {
+
+// ---- page tables ----------------------------------------------------------------------------------------------------------------
+// Row r of the batch begins at the sum of fresh[] before it, and its new pages at the sum of the pages before it: two prefix sums over
+// the requests, and then a division for every row.  Both sums are taken with an addition that stops at 2^31 - 1 (still associative), so
+// that no counts can wrap, and rows and free_count are below that: a sum that stopped is never within them.
+constexpr unsigned kTablesStop = 0x7fffffffu;
+__device__ __forceinline__ unsigned stopping_add(unsigned a, unsigned b) { return min(a + b, kTablesStop); }
+
+struct TablesArgs {
+    const int *cached, *fresh, *free_pages, *taken_before;
+    int *page_table, *row_offsets, *lengths, *positions, *slots, *counts;
+    int requests, page_shift, free_count, rows;
+    long long table_width;
+};
+
+constexpr int kTablesThreads = 1024;
+constexpr int kTablesRequests = 256;  // whose own entries a workgroup writes
+constexpr int kTablesRows = 1024;     // of the batch, a workgroup
+
+// Every workgroup takes the sums over all requests up to its own (a few thousand at the most in earnest: each 1024 of them are one
+// load and one scan), which saves a second launch; then each row of its own finds its request in LDS.
+__global__ __launch_bounds__(kTablesThreads) void page_tables_kernel(TablesArgs p)
+{
+    __shared__ unsigned wave_rows[16], wave_pages[16];
+    __shared__ unsigned row_ends[kTablesThreads], page_starts[kTablesThreads];
+    __shared__ int had_pages[kTablesThreads], positions_at[kTablesThreads];  // (of the first row; -1 in had_pages: refused)
+    __shared__ int taken, refused;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int own_first = blockIdx.x * kTablesRequests, own_end = min(p.requests, own_first + kTablesRequests);
+    const unsigned row_first = static_cast<unsigned>(blockIdx.x) * kTablesRows;
+    const unsigned row_last = min(static_cast<unsigned>(p.rows), row_first + kTablesRows);
+    const int before = p.taken_before ? max(0, *p.taken_before) : 0;
+    const unsigned left = static_cast<unsigned>(max(0, p.free_count - before));
+    if (tid == 0) taken = refused = 0;
+    if (blockIdx.x == 0 && tid == 0) p.row_offsets[0] = 0;
+    unsigned rows_before = 0, pages_before = 0;
+    for (int first = 0; first < p.requests; first += kTablesThreads) {
+        // Workgroup 0 counts all of them; the others stop behind their own.
+        if (blockIdx.x != 0 && first >= own_end && rows_before >= row_last) break;
+        const int r = first + tid;
+        const bool is = r < p.requests;
+        const int cached = is ? p.cached[r] : 0, fresh = is ? p.fresh[r] : 0;
+        const long long after = static_cast<long long>(cached) + fresh;
+        const long long page_mask = (1ll << p.page_shift) - 1;
+        const long long had = (cached + page_mask) >> p.page_shift, used = (after + page_mask) >> p.page_shift;
+        const bool possible = cached >= 0 && fresh >= 0 && used <= p.table_width && after <= 0x7fffffff;
+        const unsigned my_rows = fresh > 0 ? fresh : 0, need = possible ? static_cast<unsigned>(used - had) : 0;
+        unsigned rows_to = my_rows, pages_to = need;
+#pragma unroll
+        for (int step = 1; step < 64; step <<= 1) {
+            const unsigned a = __shfl_up(rows_to, step), b = __shfl_up(pages_to, step);
+            if (lane >= step) {
+                rows_to = stopping_add(rows_to, a);
+                pages_to = stopping_add(pages_to, b);
+            }
+        }
+        if (lane == 63) {
+            wave_rows[wave] = rows_to;
+            wave_pages[wave] = pages_to;
+        }
+        __syncthreads();
+        unsigned chunk_rows = 0, chunk_pages = 0, rows_in = rows_before, pages_in = pages_before;
+#pragma unroll
+        for (int w = 0; w < kTablesThreads / 64; ++w) {
+            if (w == wave) {
+                rows_in = stopping_add(rows_in, chunk_rows);
+                pages_in = stopping_add(pages_in, chunk_pages);
+            }
+            chunk_rows = stopping_add(chunk_rows, wave_rows[w]);
+            chunk_pages = stopping_add(chunk_pages, wave_pages[w]);
+        }
+        rows_to = stopping_add(rows_to, rows_in);
+        pages_to = stopping_add(pages_to, pages_in);
+        const bool served = possible && rows_to <= static_cast<unsigned>(p.rows) && (need == 0 || pages_to <= left);
+        row_ends[tid] = rows_to;
+        page_starts[tid] = served ? pages_to - need : 0;
+        had_pages[tid] = served ? static_cast<int>(had) : -1;
+        positions_at[tid] = cached;
+        if (is && r >= own_first && r < own_end) {
+            p.lengths[r] = served ? static_cast<int>(after) : 0;
+            p.row_offsets[r + 1] = static_cast<int>(min(rows_to, static_cast<unsigned>(p.rows)));
+        }
+        if (blockIdx.x == 0) {
+            if (served && need) atomicMax(&taken, static_cast<int>(pages_to));  // those served are dealt in order
+            const unsigned long long no = __ballot(is && !served);
+            if (lane == 0 && no) atomicAdd(&refused, __popcll(no));
+        }
+        __syncthreads();
+        // The rows of these requests that are this workgroup's.
+        const unsigned ends = stopping_add(rows_before, chunk_rows);
+        for (unsigned row = max(row_first, rows_before) + tid; row < min(row_last, ends); row += kTablesThreads) {
+            int low = 0, high = kTablesThreads - 1;  // the first whose rows end behind this one
+            while (low < high) {
+                const int middle = (low + high) >> 1;
+                if (row_ends[middle] > row) high = middle;
+                else low = middle + 1;
+            }
+            const unsigned starts = low ? row_ends[low - 1] : rows_before;
+            int position = -1, slot = -1;
+            if (had_pages[low] >= 0) {
+                position = positions_at[low] + static_cast<int>(row - starts);
+                const int column = position >> p.page_shift, place = position & static_cast<int>(page_mask);
+                int *const entry = p.page_table + (first + low) * p.table_width + column;
+                int page;
+                if (column >= had_pages[low]) {
+                    page = p.free_pages[static_cast<long long>(before) + page_starts[low] + (column - had_pages[low])];
+                    if (place == 0) *entry = page;  // the first row of a new page stands at its place 0
+                } else {
+                    page = *entry;
+                }
+                const long long wide = (static_cast<long long>(page) << p.page_shift) + place;
+                if (page >= 0 && wide <= 0x7fffffff) slot = static_cast<int>(wide);
+            }
+            p.positions[row] = position;
+            p.slots[row] = slot;
+        }
+        rows_before = ends;
+        pages_before = stopping_add(pages_before, chunk_pages);
+        __syncthreads();
+    }
+    // (All requests have been looked at, or this workgroup's rows are all taken.)
+    for (unsigned row = max(row_first, rows_before) + tid; row < row_last; row += kTablesThreads) p.positions[row] = p.slots[row] = -1;
+    if (blockIdx.x == 0) {
+        __syncthreads();  // (no requests: the first barrier behind `taken` and `refused`)
+        if (tid == 0) {
+            p.counts[0] = before + taken;
+            p.counts[1] = static_cast<int>(min(rows_before, static_cast<unsigned>(p.rows)));
+            p.counts[2] = refused;
+        }
+    }
+}
+
+// ---- new keys and values --------------------------------------------------------------------------------------------------------
+// The smallest power of two s >= 2^-118 with largest <= 448 s: 448 is 1.75 * 2^8, so that the exponent follows from the value's own
+// and from whether its significand is above 1.75.
+__device__ __forceinline__ float needed_scale(float largest)
+{
+    const unsigned bits = __float_as_uint(largest);
+    const int exponent = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return __uint_as_float(static_cast<unsigned>(max(exponent, -118) + 127) << 23);
+}
+
+// What e4m3 cannot hold (infinities, NaN; nothing else is above 448 after scaling) becomes NaN.
+__device__ __forceinline__ float e4m3_or_nan(float x) { return fabsf(x) <= 448.0f ? x : NAN; }
+__device__ __forceinline__ unsigned e4m3_pair(float a, float b, unsigned old, std::bool_constant<false>)
+{
+    return __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_or_nan(a), e4m3_or_nan(b), old, false);
+}
+__device__ __forceinline__ unsigned e4m3_pair(float a, float b, unsigned old, std::bool_constant<true>)
+{
+    return __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_or_nan(a), e4m3_or_nan(b), old, true);
+}
+__device__ __forceinline__ unsigned e4m3_four(float a, float b, float c, float d)
+{
+    return e4m3_pair(c, d, e4m3_pair(a, b, 0, std::false_type{}), std::true_type{});
+}
+__device__ __forceinline__ unsigned rescaled_four(unsigned codes, float ratio)
+{
+    const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
+    return e4m3_four(low[0] * ratio, low[1] * ratio, high[0] * ratio, high[1] * ratio);
+}
+
+struct AppendArgs {
+    const void *k, *v;
+    const int *slots;
+    uint8_t *cache_k, *cache_v;
+    float *k_scales, *v_scales;
+    long long ld;
+    int rows, pages, page_shift, kv_heads, rows_per_block;
+};
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendMostPage = 256;  // tokens of the largest page
+
+// A workgroup takes the pages that begin (in the order of the rows) within its rows, for one head and for keys or values.  It first
+// notes for every place of the page the last row that is for it; everything behind that goes by place, so that no two threads
+// write the same.  VECTOR: rows of four values on 16-byte (f32) or 8-byte (bf16) boundaries.
+template <typename T, int HD, bool VECTOR>
+__global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
+{
+    constexpr int QUADS = HD / 4;                      // of a row
+    constexpr int PLACES = kAppendThreads / QUADS > 0 ? kAppendThreads / QUADS : 1;  // rows at a time
+    static_assert(QUADS <= kAppendThreads && kAppendThreads % QUADS == 0, "whole rows");
+    __shared__ int owners[kAppendMostPage];
+    __shared__ float wave_largest[kAppendThreads / 64];
+    __shared__ int run_end;
+    const int tid = threadIdx.x, page_size = 1 << p.page_shift;
+    const int head = blockIdx.y;
+    const bool keys = blockIdx.z == 0;
+    const T *const source = static_cast<const T *>(keys ? p.k : p.v) + static_cast<size_t>(head) * HD;
+    const int block_first = blockIdx.x * p.rows_per_block, block_end = min(p.rows, block_first + p.rows_per_block);
+
+    auto page_of = [&](int row) {  // -1: skipped
+        const int slot = p.slots[row];
+        const int page = slot < 0 ? -1 : slot >> p.page_shift;
+        return page < p.pages ? page : -1;
+    };
+    auto quad = [&](int row, int d) -> float4 {
+        const T *const at = source + static_cast<size_t>(row) * p.ld + d;
+        if constexpr (sizeof(T) == 4) {
+            if constexpr (VECTOR) return *reinterpret_cast<const float4 *>(at);
+            else return float4{at[0], at[1], at[2], at[3]};
+        } else {
+            unsigned low, high;
+            if constexpr (VECTOR) {
+                const uint2 both = *reinterpret_cast<const uint2 *>(at);
+                low = both.x;
+                high = both.y;
+            } else {
+                low = at[0] | static_cast<unsigned>(at[1]) << 16;
+                high = at[2] | static_cast<unsigned>(at[3]) << 16;
+            }
+            return float4{__uint_as_float(low << 16), __uint_as_float(low & 0xffff0000u), __uint_as_float(high << 16),
+                          __uint_as_float(high & 0xffff0000u)};
+        }
+    };
+
+    for (int first = block_first; first < block_end; ++first) {
+        const int page = page_of(first);
+        if (page < 0 || (first > 0 && page_of(first - 1) == page)) continue;  // (the same for the whole workgroup)
+        for (int place = tid; place < page_size; place += kAppendThreads) owners[place] = -1;
+        if (tid == 0) run_end = p.rows;
+        __syncthreads();
+        for (int at = first;; at += kAppendThreads) {
+            const int row = at + tid;
+            const bool mine = row < p.rows && page_of(row) == page;
+            if (!mine && row < p.rows) atomicMin(&run_end, row);
+            __syncthreads();
+            if (mine && row < run_end) atomicMax(&owners[p.slots[row] & (page_size - 1)], row);
+            if (run_end < at + kAppendThreads || at + kAppendThreads >= p.rows) break;
+        }
+        __syncthreads();
+
+        float largest = 0.0f;
+        const int quad_at = tid % QUADS * 4;
+        for (int place = tid / QUADS; place < page_size; place += PLACES) {
+            const int row = owners[place];
+            if (row < 0) continue;
+            const float4 x = quad(row, quad_at);
+            for (const float value : {x.x, x.y, x.z, x.w}) {
+                const float size = fabsf(value);
+                if (size < INFINITY) largest = fmaxf(largest, size);
+            }
+        }
+#pragma unroll
+        for (int step = 32; step > 0; step >>= 1) largest = fmaxf(largest, __shfl_xor(largest, step));
+        if ((tid & 63) == 0) wave_largest[tid >> 6] = largest;
+        __syncthreads();
+        for (int w = 0; w < kAppendThreads / 64; ++w) largest = fmaxf(largest, wave_largest[w]);
+
+        const size_t block = static_cast<size_t>(page) * p.kv_heads + head;
+        float *const scale_at = (keys ? p.k_scales : p.v_scales) + block;
+        const bool begun = owners[0] >= 0;
+        const float before = begun ? 0.0f : *scale_at;
+        const float scale = fmaxf(before, needed_scale(largest));
+        const bool grown = !begun && scale > before;
+        const float inverse = 1.0f / scale, ratio = before * inverse;
+        uint8_t *const codes = (keys ? p.cache_k : p.cache_v) + (block << p.page_shift) * HD;
+        if (keys) {
+            for (int place = tid / QUADS; place < page_size; place += PLACES) {
+                const int row = owners[place];
+                unsigned *const to = reinterpret_cast<unsigned *>(codes + place * HD + quad_at);
+                if (row >= 0) {
+                    const float4 x = quad(row, quad_at);
+                    *to = e4m3_four(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse);
+                } else if (grown) {
+                    *to = rescaled_four(*to, ratio);
+                }
+            }
+        } else {
+            for (int place = tid / QUADS; place < page_size; place += PLACES) {
+                const int row = owners[place];
+                uint8_t *const to = codes + (static_cast<size_t>(quad_at) << p.page_shift) + place;
+                unsigned four;
+                if (row >= 0) {
+                    const float4 x = quad(row, quad_at);
+                    four = e4m3_four(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse);
+                } else if (grown) {
+                    four = 0;
+                    for (int i = 0; i < 4; ++i) four |= static_cast<unsigned>(to[i << p.page_shift]) << 8 * i;
+                    four = rescaled_four(four, ratio);
+                } else {
+                    continue;
+                }
+                for (int i = 0; i < 4; ++i) to[i << p.page_shift] = static_cast<uint8_t>(four >> 8 * i);
+            }
+        }
+        __syncthreads();  // everyone has read the scale, and the next page takes `owners`
+        if (tid == 0) *scale_at = scale;
+    }
+}
+
+template <typename T, int HD>
+hipError_t launch_append(const st_hip_kv_cache &cache, size_t rows, const int32_t *slots, const T *k, const T *v, size_t ld, hipStream_t stream)
+{
+    AppendArgs args{k, v, slots, cache.k, cache.v, cache.k_scales, cache.v_scales, static_cast<long long>(ld), static_cast<int>(rows),
+                    static_cast<int>(cache.pages), __builtin_ctzll(cache.page_size), static_cast<int>(cache.kv_heads), 1};
+    const size_t units = rows * cache.kv_heads * 2;
+    args.rows_per_block = units <= 4096 ? 1 : 16;
+    const dim3 grid(static_cast<unsigned>((rows + args.rows_per_block - 1) / args.rows_per_block), static_cast<unsigned>(cache.kv_heads), 2);
+    constexpr size_t vector = 4 * sizeof(T);
+    const bool aligned = ld % 4 == 0 && reinterpret_cast<uintptr_t>(k) % vector == 0 && reinterpret_cast<uintptr_t>(v) % vector == 0;
+    if (aligned) kv_append_kernel<T, HD, true><<<grid, kAppendThreads, 0, stream>>>(args);
+    else kv_append_kernel<T, HD, false><<<grid, kAppendThreads, 0, stream>>>(args);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_append_any(const st_hip_kv_cache &cache, size_t rows, const int32_t *slots, const T *k, const T *v, size_t ld, hipStream_t stream)
+{
+    if (cache.head_dim == 64) return launch_append<T, 64>(cache, rows, slots, k, v, ld, stream);
+    if (cache.head_dim == 128) return launch_append<T, 128>(cache, rows, slots, k, v, ld, stream);
+    return launch_append<T, 256>(cache, rows, slots, k, v, ld, stream);
+}
+
+}  // namespace
+
+hipError_t launch_page_tables(size_t requests, size_t page_size, const int32_t *cached, const int32_t *fresh, size_t free_count,
+                              const int32_t *free_pages, const int32_t *taken_before, size_t table_width, int32_t *page_table, size_t rows,
+                              int32_t *row_offsets, int32_t *lengths, int32_t *positions, int32_t *slots, int32_t *counts, hipStream_t stream)
+{
+    const TablesArgs args{cached, fresh, free_pages, taken_before, page_table, row_offsets, lengths, positions, slots, counts,
+                          static_cast<int>(requests), __builtin_ctzll(page_size), static_cast<int>(free_count), static_cast<int>(rows),
+                          static_cast<long long>(table_width)};
+    const size_t by_requests = (requests + kTablesRequests - 1) / kTablesRequests, by_rows = (rows + kTablesRows - 1) / kTablesRows;
+    const size_t blocks = std::max<size_t>(1, std::max(by_requests, by_rows));
+    page_tables_kernel<<<static_cast<unsigned>(blocks), kTablesThreads, 0, stream>>>(args);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_cache_append_f32(const st_hip_kv_cache &cache, size_t rows, const int32_t *slots, const float *k, const float *v, size_t ld, hipStream_t stream)
+{
+    return launch_append_any(cache, rows, slots, k, v, ld, stream);
+}
+
+hipError_t launch_kv_cache_append_bf16(const st_hip_kv_cache &cache, size_t rows, const int32_t *slots, const uint16_t *k, const uint16_t *v, size_t ld, hipStream_t stream)
+{
+    return launch_append_any(cache, rows, slots, k, v, ld, stream);
+}
+
+}  // namespace sthip

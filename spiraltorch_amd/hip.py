@@ -434,6 +434,11 @@ def _dev(buf):
     return buf.ptr if isinstance(buf, DeviceBuffer) else buf
 
 
+def _address(buf):
+    ptr = _dev(buf)
+    return ptr.value if isinstance(ptr, ctypes.c_void_p) else ptr
+
+
 def release_scratch(stream=None) -> None:
     """Waits for the stream (None: the default stream) and frees the scratch buffers the library keeps for it."""
     _check(_lib.load().st_hip_release_scratch(_stream_ptr(stream)))
@@ -569,6 +574,74 @@ def attention_bf16_dev(batch, heads, sequence, head_dim, scale, causal, q, k, v,
     DeviceBuffers or raw device addresses (DeviceBuffer.at) of bf16 bit patterns."""
     _check(_lib.load().st_hip_attention_bf16_dev(batch, heads, sequence, head_dim, scale, int(bool(causal)), _dev(q),
                                                  _dev(k), _dev(v), ld_in, _dev(out), ld_out, _stream_ptr(stream)))
+
+
+class KvCache:
+    """A paged cache of e4m3 keys and values with a power-of-two scale for each page and head (st_hip_kv_cache of include/st_hip.h).
+
+    Without memory given, it owns its own: k (pages, kv_heads, page_size, head_dim) and v (pages, kv_heads, head_dim, page_size) bytes,
+    and k_scales, v_scales (pages, kv_heads) f32.  Pages need no clearing: one begins with the token at its place 0."""
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, k=None, v=None, k_scales=None, v_scales=None):
+        if min(pages, page_size, kv_heads, head_dim) <= 0:
+            raise ValueError("kv cache dimensions must be positive")
+        blocks = pages * kv_heads
+        self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
+        values = blocks * page_size * head_dim
+        self.k, self.v = (DeviceBuffer(values) if buf is None else buf for buf in (k, v))
+        self.k_scales, self.v_scales = (DeviceBuffer(blocks * 4) if buf is None else buf for buf in (k_scales, v_scales))
+        self._struct = _lib.KvCacheStruct(pages, page_size, kv_heads, head_dim, *(_address(buf) for buf in (self.k, self.v, self.k_scales,
+                                                                                                              self.v_scales)))
+        self._ref = ctypes.byref(self._struct)
+
+
+class Rotary:
+    """How rotary positions turn a head (st_hip_rotary of include/st_hip.h): its leading rotary_dim values in pairs, neighbours if
+    `interleaved`, by position * base^(-2i/rotary_dim) / factor; with original_length, scaled by parts between low_turns and high_turns."""
+
+    def __init__(self, rotary_dim: int, base: float = 10000.0, interleaved: bool = False, factor: float = 1.0, original_length: float = 0.0,
+                 low_turns: float = 1.0, high_turns: float = 4.0, magnitude: float = 1.0):
+        self._struct = _lib.RotaryStruct(rotary_dim, int(bool(interleaved)), base, factor, original_length, low_turns, high_turns, magnitude)
+        self._ref = ctypes.byref(self._struct)
+
+
+def page_tables_dev(requests, page_size, cached, fresh, free_count, free_pages, taken_before, table_width, page_table, rows, row_offsets,
+                    lengths, positions, slots, counts, stream=None) -> None:
+    """Page tables, row offsets, lengths, positions and slots of a step from what each request has in the cache and brings (int32
+    device buffers; see st_hip_page_tables_dev)."""
+    _check(_lib.load().st_hip_page_tables_dev(requests, page_size, _dev(cached), _dev(fresh), free_count, _dev(free_pages), _dev(taken_before),
+                                              table_width, _dev(page_table), rows, _dev(row_offsets), _dev(lengths), _dev(positions),
+                                              _dev(slots), _dev(counts), _stream_ptr(stream)))
+
+
+def rotary_f32_dev(rows, heads, head_dim, rotary: Rotary, positions, src, ld_in, dst, ld_out, transposed=False, sequence=0, stream=None) -> None:
+    """Rotary positions on neighbouring heads of rows; positions None: row % sequence.  `transposed`: the gradient."""
+    _check(_lib.load().st_hip_rotary_f32_dev(rows, sequence, heads, head_dim, rotary._ref, int(bool(transposed)), _dev(positions), _dev(src),
+                                             ld_in, _dev(dst), ld_out, _stream_ptr(stream)))
+
+
+def rotary_bf16_dev(rows, heads, head_dim, rotary: Rotary, positions, src, ld_in, dst, ld_out, transposed=False, sequence=0, stream=None) -> None:
+    """rotary_f32_dev on bf16 bit patterns."""
+    _check(_lib.load().st_hip_rotary_bf16_dev(rows, sequence, heads, head_dim, rotary._ref, int(bool(transposed)), _dev(positions), _dev(src),
+                                              ld_in, _dev(dst), ld_out, _stream_ptr(stream)))
+
+
+def kv_cache_append_f32_dev(cache: KvCache, rows, slots, k, v, ld, stream=None) -> None:
+    """Rows of keys and values (kv_heads*head_dim values, ld apart) into the cache's slots; negative slots are skipped."""
+    _check(_lib.load().st_hip_kv_cache_append_f32_dev(cache._ref, rows, _dev(slots), _dev(k), _dev(v), ld, _stream_ptr(stream)))
+
+
+def kv_cache_append_bf16_dev(cache: KvCache, rows, slots, k, v, ld, stream=None) -> None:
+    """kv_cache_append_f32_dev on bf16 bit patterns."""
+    _check(_lib.load().st_hip_kv_cache_append_bf16_dev(cache._ref, rows, _dev(slots), _dev(k), _dev(v), ld, _stream_ptr(stream)))
+
+
+def attention_kv_cache_bf16_dev(cache: KvCache, requests, rows, heads, scale, causal, row_offsets, lengths, page_table, table_width, q, ld_q,
+                                out, ld_out, stream=None) -> None:
+    """Attention of a ragged batch's bf16 query rows over the cache (see st_hip_attention_kv_cache_bf16_dev)."""
+    _check(_lib.load().st_hip_attention_kv_cache_bf16_dev(cache._ref, requests, rows, heads, scale, int(bool(causal)), _dev(row_offsets),
+                                                          _dev(lengths), _dev(page_table), table_width, _dev(q), ld_q, _dev(out), ld_out,
+                                                          _stream_ptr(stream)))
 
 
 def probe_mfma_bf16_dev(workgroups, iterations, operands, sink, stream=None) -> None:

@@ -14,11 +14,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(HERE, "..", "..", "include", "st_hip.h")
 TARGET = os.path.join(HERE, "st-backend-hip", "src", "ffi.rs")
 
-SCALARS = {"size_t": "usize", "int": "c_int", "float": "f32", "uint64_t": "u64", "uint16_t": "u16", "char": "c_char",
+SCALARS = {"size_t": "usize", "int": "c_int", "float": "f32", "uint64_t": "u64", "uint16_t": "u16", "int32_t": "i32", "uint8_t": "u8", "char": "c_char",
            "void": "c_void", "st_hip_device_props": "StHipDeviceProps", "st_hip_probe_result": "StHipProbeResult",
            "st_hip_decoder_config": "StHipDecoderConfig", "st_hip_attention_plan": "StHipAttentionPlan",
            "st_hip_gemm_tile_plan": "StHipGemmTilePlan", "st_hip_gemm_split_plan": "StHipGemmSplitPlan",
-           "st_hip_conv2d_split_plan": "StHipConv2dSplitPlan", "st_hip_conv2d_bf16_plan": "StHipConv2dBf16Plan"}
+           "st_hip_conv2d_split_plan": "StHipConv2dSplitPlan", "st_hip_conv2d_bf16_plan": "StHipConv2dBf16Plan",
+           "st_hip_kv_cache": "StHipKvCache", "st_hip_rotary": "StHipRotary"}
 RUST_KEYWORDS = {"in": "input", "type": "kind", "ref": "reference"}
 
 STRUCTS = '''/// `st_hip_device_props`.
@@ -136,6 +137,34 @@ pub struct StHipConv2dBf16Plan {
     pub items: u64,
     pub out_of_range: u64,
     pub duplicates: u64,
+}
+
+/// `st_hip_kv_cache`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct StHipKvCache {
+    pub pages: usize,
+    pub page_size: usize,
+    pub kv_heads: usize,
+    pub head_dim: usize,
+    pub k: *mut u8,
+    pub v: *mut u8,
+    pub k_scales: *mut f32,
+    pub v_scales: *mut f32,
+}
+
+/// `st_hip_rotary`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, PartialEq)]
+pub struct StHipRotary {
+    pub rotary_dim: usize,
+    pub interleaved: c_int,
+    pub base: f32,
+    pub factor: f32,
+    pub original_length: f32,
+    pub low_turns: f32,
+    pub high_turns: f32,
+    pub magnitude: f32,
 }
 '''
 

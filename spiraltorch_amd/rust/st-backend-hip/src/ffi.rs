@@ -122,6 +122,34 @@ pub struct StHipConv2dBf16Plan {
     pub duplicates: u64,
 }
 
+/// `st_hip_kv_cache`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct StHipKvCache {
+    pub pages: usize,
+    pub page_size: usize,
+    pub kv_heads: usize,
+    pub head_dim: usize,
+    pub k: *mut u8,
+    pub v: *mut u8,
+    pub k_scales: *mut f32,
+    pub v_scales: *mut f32,
+}
+
+/// `st_hip_rotary`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, PartialEq)]
+pub struct StHipRotary {
+    pub rotary_dim: usize,
+    pub interleaved: c_int,
+    pub base: f32,
+    pub factor: f32,
+    pub original_length: f32,
+    pub low_turns: f32,
+    pub high_turns: f32,
+    pub magnitude: f32,
+}
+
 #[link(name = "sthip")]
 extern "C" {
     pub fn st_hip_init() -> c_int;
@@ -200,6 +228,12 @@ extern "C" {
     pub fn st_hip_f32_to_bf16_dev(count: usize, input: *const f32, out: *mut u16, stream: *mut c_void) -> c_int;
     pub fn st_hip_split_heads_f32_dev(batch: usize, seq: usize, heads: usize, head_dim: usize, qkv: *const f32, q: *mut f32, k: *mut f32, v: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_merge_heads_f32_dev(batch: usize, seq: usize, heads: usize, head_dim: usize, contexts_in: *const f32, out_f32: *mut f32, out_bf16: *mut u16, stream: *mut c_void) -> c_int;
+    pub fn st_hip_page_tables_dev(requests: usize, page_size: usize, cached: *const i32, fresh: *const i32, free_count: usize, free_pages: *const i32, taken_before: *const i32, table_width: usize, page_table: *mut i32, rows: usize, row_offsets: *mut i32, lengths: *mut i32, positions: *mut i32, slots: *mut i32, counts: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn st_hip_rotary_f32_dev(rows: usize, sequence: usize, heads: usize, head_dim: usize, rotary: *const StHipRotary, transposed: c_int, positions: *const i32, input: *const f32, ld_in: usize, out: *mut f32, ld_out: usize, stream: *mut c_void) -> c_int;
+    pub fn st_hip_rotary_bf16_dev(rows: usize, sequence: usize, heads: usize, head_dim: usize, rotary: *const StHipRotary, transposed: c_int, positions: *const i32, input: *const u16, ld_in: usize, out: *mut u16, ld_out: usize, stream: *mut c_void) -> c_int;
+    pub fn st_hip_kv_cache_append_f32_dev(cache: *const StHipKvCache, rows: usize, slots: *const i32, k: *const f32, v: *const f32, ld: usize, stream: *mut c_void) -> c_int;
+    pub fn st_hip_kv_cache_append_bf16_dev(cache: *const StHipKvCache, rows: usize, slots: *const i32, k: *const u16, v: *const u16, ld: usize, stream: *mut c_void) -> c_int;
+    pub fn st_hip_attention_kv_cache_bf16_dev(cache: *const StHipKvCache, requests: usize, rows: usize, heads: usize, scale: f32, causal: c_int, row_offsets: *const i32, lengths: *const i32, page_table: *const i32, table_width: usize, q: *const u16, ld_q: usize, out: *mut u16, ld_out: usize, stream: *mut c_void) -> c_int;
     pub fn st_hip_probe_mfma_bf16_dev(workgroups: usize, iterations: usize, operands: *const u16, sink: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_probe_mfma_f32_dev(workgroups: usize, iterations: usize, operands: *const f32, sink: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_probe_stream_lds_dev(workgroups: usize, iterations: usize, region: *const c_void, region_bytes: usize, stream: *mut c_void) -> c_int;
