@@ -259,7 +259,10 @@ hipError_t device_malloc(void **out, size_t bytes);
 hipError_t stream_workspace(hipStream_t stream, size_t bytes, void **out);
 // A second buffer of the same kind (slot 1) for re-laid copies of a call's operands, which must stay where they are
 // while the kernels that read them take scratch from slot 0.
-hipError_t stream_workspace_slot(hipStream_t stream, int slot, size_t bytes, void **out);
+// `fresh` (if given) is set where the memory is not what the last call was handed.
+hipError_t stream_workspace_slot(hipStream_t stream, int slot, size_t bytes, void **out, bool *fresh = nullptr);
+// A third one, of 32-bit counters that are 0 when it is first handed out, and which every launch leaves 0.
+hipError_t stream_counters(hipStream_t stream, size_t count, unsigned **out);
 // Whether a launcher failed only because scratch memory could not grow (out of memory, or an allocation refused during capture):
 // nothing has been launched then, and a route that needs no scratch may still run.
 inline bool scratch_unavailable(hipError_t rc) { return rc == hipErrorOutOfMemory || rc == hipErrorStreamCaptureUnsupported; }

@@ -462,8 +462,9 @@ WorkspaceEntry *find_entry(hipStream_t stream, std::thread::id owner, int slot)
 
 hipError_t stream_workspace(hipStream_t stream, size_t bytes, void **out) { return stream_workspace_slot(stream, 0, bytes, out); }
 
-hipError_t stream_workspace_slot(hipStream_t stream, int slot, size_t bytes, void **out)
+hipError_t stream_workspace_slot(hipStream_t stream, int slot, size_t bytes, void **out, bool *fresh)
 {
+    if (fresh) *fresh = false;
     const std::thread::id me = std::this_thread::get_id();
     const size_t wanted = bytes ? bytes : 256;
     const bool capturing = being_captured(stream);
@@ -506,8 +507,8 @@ hipError_t stream_workspace_slot(hipStream_t stream, int slot, size_t bytes, voi
             return rc;
         }
     }
-    void *fresh = nullptr;
-    const hipError_t rc = scratch_malloc(&fresh, wanted, capturing);
+    void *memory = nullptr;
+    const hipError_t rc = scratch_malloc(&memory, wanted, capturing);
     std::lock_guard<std::mutex> lock(workspace_mutex());
     WorkspaceEntry *e = find_entry(stream, me, slot);
     if (rc != hipSuccess) {
@@ -515,15 +516,49 @@ hipError_t stream_workspace_slot(hipStream_t stream, int slot, size_t bytes, voi
         return rc;
     }
     if (e) {
-        e->ptr = fresh;
+        e->ptr = memory;
         e->capacity = wanted;
         e->growing = false;
         e->captured = capturing;
     } else {
-        workspace_entries().push_back(WorkspaceEntry{stream, me, fresh, wanted, slot, false, capturing});
+        workspace_entries().push_back(WorkspaceEntry{stream, me, memory, wanted, slot, false, capturing});
     }
-    *out = fresh;
+    *out = memory;
+    if (fresh) *fresh = true;
     return hipSuccess;
+}
+
+// New counters are cleared on a stream of their own and waited for: a launch that is being recorded must find them cleared when it is
+// replayed, and so must one that runs on the stream before that.
+hipError_t stream_counters(hipStream_t stream, size_t count, unsigned **out)
+{
+    constexpr int kSlot = 2;
+    constexpr size_t kLeast = 16u << 10;
+    const size_t bytes = std::max(kLeast, count * sizeof(unsigned));
+    void *memory = nullptr;
+    bool fresh = false;
+    hipError_t rc = stream_workspace_slot(stream, kSlot, bytes, &memory, &fresh);
+    if (rc != hipSuccess) return rc;
+    *out = static_cast<unsigned *>(memory);
+    if (!fresh) return hipSuccess;
+    const bool capturing = being_captured(stream);
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    if (capturing) rc = hipThreadExchangeStreamCaptureMode(&mode);
+    hipStream_t own = nullptr;
+    if (rc == hipSuccess) {
+        rc = hipStreamCreate(&own);
+        if (rc == hipSuccess) {
+            rc = hipMemsetAsync(memory, 0, bytes, own);
+            if (rc == hipSuccess) rc = hipStreamSynchronize(own);
+            (void)hipStreamDestroy(own);
+        }
+        if (capturing) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    }
+    if (rc == hipSuccess) return hipSuccess;
+    (void)hipGetLastError();
+    std::lock_guard<std::mutex> lock(workspace_mutex());
+    if (WorkspaceEntry *e = find_entry(stream, std::this_thread::get_id(), kSlot)) e->capacity = 0;  // not cleared: the next call replaces it
+    return hipErrorOutOfMemory;
 }
 
 // Called after the stream has been drained (before it is destroyed, or by st_hip_release_scratch).

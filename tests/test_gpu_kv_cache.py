@@ -203,13 +203,13 @@ def test_values_that_are_not_numbers(hip, kind):
 
 def check_attention(hip, rng, page, kv_heads, dim, group, lengths, fresh, causal, scale=None, behind=3, pages=None, width=None, edit=None,
                     stale=0x7f, extra=0, q_size=1.5, what=""):
-    """A ragged batch over a cache whose places behind the lengths, and unused pages, hold NaN (`stale`)."""
+    """A ragged batch over a cache whose places behind the lengths, and unused pages and their scales, hold NaN (`stale`)."""
     requests, heads = len(lengths), kv_heads * group
     used = [-(-max(0, n) // page) for n in lengths]
     width = max(used + [1]) if width is None else width
     pages = sum(used) + 2 if pages is None else pages
     store = Pages(hip, rng, pages, page, kv_heads, dim)
-    order, at = rng.permutation(pages), 0
+    order, at = np.append(1 + rng.permutation(pages - 1), 0), 0  # (page 0 stays unused: reads of pages that are none may go there)
     table = np.full((requests, width), SENTINEL)
     held = np.zeros((pages, page), bool)
     for r, n in enumerate(used):
@@ -219,6 +219,7 @@ def check_attention(hip, rng, page, kv_heads, dim, group, lengths, fresh, causal
         at += n
     if stale is not None:
         store.k[~held.any(1)], store.v[~held.any(1)] = stale, stale
+        store.k_scales[~held.any(1)] = store.v_scales[~held.any(1)] = np.nan
         store.k.transpose(0, 2, 1, 3)[~held], store.v.transpose(0, 3, 1, 2)[~held] = stale, stale
     offsets = np.concatenate([[0], np.cumsum(fresh)])
     rows = int(offsets[-1]) + behind

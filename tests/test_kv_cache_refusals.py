@@ -117,15 +117,14 @@ def test_attention(stub):
 
 
 def test_attention_goes_on_without_room_for_parts(stub):
-    """Long contexts of few rows are cut over workgroups and put together by a second launch; without scratch memory for the parts, one
-    launch does it all."""
+    """Long contexts of few rows are cut over workgroups; without scratch memory for the parts, one takes a context as it is."""
     out = run(stub, """
 for fail in (1, 0):
     no_memory.value, before = fail, launches.value
     hip.attention_kv_cache_bf16_dev(cache(pages=4000), 1, 1, 4, 0.1, True, M, 2 * M, 3 * M, 2000, 4 * M, 256, 5 * M, 256)
-    print(launches.value - before)
+    print(launches.value - before, grid.value)
 """)
-    assert out[0] == "1" and out[1] == "2"
+    assert out[:2] == ["1", "2"] and out[2] == "1" and int(out[3]) > 2
 
 
 def test_null_structures():
