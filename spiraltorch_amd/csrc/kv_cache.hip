@@ -175,127 +175,192 @@ struct AppendArgs {
     uint8_t *cache_k, *cache_v;
     float *k_scales, *v_scales;
     long long ld;
-    int rows, pages, page_shift, kv_heads, rows_per_block;
+    int rows, pages, page_shift, kv_heads;
+    unsigned sharers;
 };
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendMostPage = 256;  // tokens of the largest page
+constexpr int kAppendMostRows = 64;   // that a workgroup looks at for the beginnings of pages
 
-// A workgroup takes the pages that begin (in the order of the rows) within its rows, for one head and for keys or values.  It first
-// notes for every place of the page the last row that is for it; everything behind that goes by place, so that no two threads
-// write the same.  VECTOR: rows of four values on 16-byte (f32) or 8-byte (bf16) boundaries.
-template <typename T, int HD, bool VECTOR>
-__global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
+// Eight neighbouring values of a row, as they are.
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+struct Eight {
+    u32x4 raw[sizeof(T) / 2];
+    __device__ __forceinline__ float at(int i) const
+    {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(raw[i >> 2][i & 3]);
+        else return __uint_as_float(i & 1 ? raw[0][i >> 1] & 0xffff0000u : raw[0][i >> 1] << 16);
+    }
+};
+template <bool VECTOR, typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T *at)
 {
-    constexpr int QUADS = HD / 4;                      // of a row
-    constexpr int PLACES = kAppendThreads / QUADS > 0 ? kAppendThreads / QUADS : 1;  // rows at a time
-    static_assert(QUADS <= kAppendThreads && kAppendThreads % QUADS == 0, "whole rows");
+    Eight<T> x;
+    if constexpr (VECTOR) {
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(T) / 2; ++i) x.raw[i] = reinterpret_cast<const u32x4 *>(at)[i];
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.raw[i >> 2][i & 3] = __float_as_uint(at[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.raw[0][i] = at[2 * i] | static_cast<unsigned>(at[2 * i + 1]) << 16;
+    }
+    return x;
+}
+
+// A workgroup takes pages that begin (in the order of the rows) within its 64 rows, for one head: its lower half the keys, its upper half
+// the values.  Where every row begins a page, as in a decode step, several workgroups share the rows' pages.  For every place of a
+// page the last row that is for it is noted first; everything behind that goes by place, so that no two threads write the same.
+// A thread has eight values of four neighbouring places (of places a quarter of the page apart, for keys), so that both layouts are
+// read and written in runs: keys 8 bytes of a place at a time, 128 a row of lanes; values, which lie transposed, 4 bytes of a value at a
+// time, 64 in a page of 64.  Blocks of up to 8192 values (a page of 64 places and heads of 128 values) stay in registers between the
+// maximum and the rounding, larger ones are read again.  VECTOR: rows on 16-byte boundaries.
+template <typename T, int HD, bool VECTOR>
+__global__ __launch_bounds__(2 * kAppendThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 6 : 4))) void kv_append_kernel(AppendArgs p)
+{
+    constexpr int RUNS = HD / 8;  // of eight values
+    constexpr int WAVES = kAppendThreads / 64;
     __shared__ int owners[kAppendMostPage];
-    __shared__ float wave_largest[kAppendThreads / 64];
+    __shared__ float wave_largest[2 * WAVES];
+    __shared__ unsigned long long changes[WAVES], beginnings;
     __shared__ int run_end;
-    const int tid = threadIdx.x, page_size = 1 << p.page_shift;
-    const int head = blockIdx.y;
-    const bool keys = blockIdx.z == 0;
+    const int tid = threadIdx.x & (kAppendThreads - 1), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int page_size = 1 << p.page_shift, quarter = page_size >> 2;
+    const bool keys = __builtin_amdgcn_readfirstlane(threadIdx.x) < kAppendThreads;
+    const unsigned head = blockIdx.x % p.kv_heads, of_head = blockIdx.x / p.kv_heads;
+    const unsigned sharer = of_head & (p.sharers - 1);
+    const int block_first = static_cast<int>(of_head / p.sharers) * kAppendMostRows;
     const T *const source = static_cast<const T *>(keys ? p.k : p.v) + static_cast<size_t>(head) * HD;
-    const int block_first = blockIdx.x * p.rows_per_block, block_end = min(p.rows, block_first + p.rows_per_block);
 
     auto page_of = [&](int row) {  // -1: skipped
         const int slot = p.slots[row];
         const int page = slot < 0 ? -1 : slot >> p.page_shift;
         return page < p.pages ? page : -1;
     };
-    auto quad = [&](int row, int d) -> float4 {
-        const T *const at = source + static_cast<size_t>(row) * p.ld + d;
-        if constexpr (sizeof(T) == 4) {
-            if constexpr (VECTOR) return *reinterpret_cast<const float4 *>(at);
-            else return float4{at[0], at[1], at[2], at[3]};
-        } else {
-            unsigned low, high;
-            if constexpr (VECTOR) {
-                const uint2 both = *reinterpret_cast<const uint2 *>(at);
-                low = both.x;
-                high = both.y;
-            } else {
-                low = at[0] | static_cast<unsigned>(at[1]) << 16;
-                high = at[2] | static_cast<unsigned>(at[3]) << 16;
-            }
-            return float4{__uint_as_float(low << 16), __uint_as_float(low & 0xffff0000u), __uint_as_float(high << 16),
-                          __uint_as_float(high & 0xffff0000u)};
-        }
-    };
-
-    for (int first = block_first; first < block_end; ++first) {
+    // The 256 rows from the block's first on, one a thread; where the page is another one than the row's before.
+    const int own_row = block_first + tid;
+    const int own_page = own_row < p.rows ? page_of(own_row) : -2, own_place = own_row < p.rows ? p.slots[own_row] & (page_size - 1) : 0;
+    const bool change = own_row == 0 || (own_row <= p.rows ? page_of(own_row - 1) : -2) != own_page;
+    const unsigned long long changed = __ballot(change), begun_here = __ballot(change && own_page >= 0);
+    if (lane == 0 && keys) {
+        changes[wave] = changed;
+        if (wave == 0) beginnings = begun_here;
+    }
+    __syncthreads();
+    // Of the pages that begin here, this workgroup's: every sharers-th (a power of two).
+    const unsigned long long all_begun = beginnings;
+    const unsigned rank = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(all_begun >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(all_begun), 0));
+    for (unsigned long long pending = __ballot((all_begun >> lane & 1) != 0 && (rank & (p.sharers - 1)) == sharer); pending != 0; pending &= pending - 1) {
+        const int which = __builtin_ctzll(pending), first = block_first + which;
         const int page = page_of(first);
-        if (page < 0 || (first > 0 && page_of(first - 1) == page)) continue;  // (the same for the whole workgroup)
-        for (int place = tid; place < page_size; place += kAppendThreads) owners[place] = -1;
-        if (tid == 0) run_end = p.rows;
+        int end = kAppendThreads;  // of the page's rows, among the 256
+        for (int w = WAVES - 1; w >= 0; --w) {
+            const unsigned long long later = w == 0 ? changes[0] & (~1ull << which) : changes[w];
+            if (later != 0) end = 64 * w + __builtin_ctzll(later);
+        }
+        const size_t block = static_cast<size_t>(page) * p.kv_heads + head;
+        float *const scale_at = (keys ? p.k_scales : p.v_scales) + block;
+        const float held = *scale_at;
+        for (int place = threadIdx.x; place < page_size; place += 2 * kAppendThreads) owners[place] = -1;
+        if (threadIdx.x == 0) run_end = p.rows;
         __syncthreads();
-        for (int at = first;; at += kAppendThreads) {
-            const int row = at + tid;
-            const bool mine = row < p.rows && page_of(row) == page;
-            if (!mine && row < p.rows) atomicMin(&run_end, row);
-            __syncthreads();
-            if (mine && row < run_end) atomicMax(&owners[p.slots[row] & (page_size - 1)], row);
-            if (run_end < at + kAppendThreads || at + kAppendThreads >= p.rows) break;
+        if (keys && tid >= which && tid < end) atomicMax(&owners[own_place], own_row);
+        if (end == kAppendThreads) {  // repeated rows alone make a page's so many
+            for (int at = block_first + kAppendThreads; at < p.rows; at += kAppendThreads) {
+                const int row = at + tid;
+                const bool mine = row < p.rows && page_of(row) == page;
+                if (!mine && row < p.rows) atomicMin(&run_end, row);
+                __syncthreads();
+                if (mine && row < run_end) atomicMax(&owners[p.slots[row] & (page_size - 1)], row);
+                if (run_end < at + kAppendThreads) break;
+            }
         }
         __syncthreads();
 
+        const int items = quarter * RUNS;
+        // Item i: its four places, and its eight values.
+        auto item_run = [&](int i) { return keys ? i % RUNS : i / quarter; };
+        auto item_place = [&](int i, int j) { return keys ? i / RUNS + j * quarter : i % quarter * 4 + j; };
+        Eight<T> x[4];
+        int rows[4];
+        auto load = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                rows[j] = owners[item_place(i, j)];
+                if (rows[j] >= 0) x[j] = load_eight<VECTOR>(source + static_cast<size_t>(rows[j]) * p.ld + item_run(i) * 8);
+            }
+        };
         float largest = 0.0f;
-        const int quad_at = tid % QUADS * 4;
-        for (int place = tid / QUADS; place < page_size; place += PLACES) {
-            const int row = owners[place];
-            if (row < 0) continue;
-            const float4 x = quad(row, quad_at);
-            for (const float value : {x.x, x.y, x.z, x.w}) {
-                const float size = fabsf(value);
-                if (size < INFINITY) largest = fmaxf(largest, size);
+        for (int i = tid; i < items; i += kAppendThreads) {
+            load(i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (rows[j] < 0) continue;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float size = fabsf(x[j].at(e));
+                    largest = fmaxf(largest, size < INFINITY ? size : 0.0f);
+                }
             }
         }
 #pragma unroll
         for (int step = 32; step > 0; step >>= 1) largest = fmaxf(largest, __shfl_xor(largest, step));
-        if ((tid & 63) == 0) wave_largest[tid >> 6] = largest;
+        if (lane == 0) wave_largest[wave] = largest;
         __syncthreads();
-        for (int w = 0; w < kAppendThreads / 64; ++w) largest = fmaxf(largest, wave_largest[w]);
+        for (int w = 0; w < WAVES; ++w) largest = fmaxf(largest, wave_largest[(keys ? 0 : WAVES) + w]);
 
-        const size_t block = static_cast<size_t>(page) * p.kv_heads + head;
-        float *const scale_at = (keys ? p.k_scales : p.v_scales) + block;
         const bool begun = owners[0] >= 0;
-        const float before = begun ? 0.0f : *scale_at;
+        const float before = begun ? 0.0f : held;
         const float scale = fmaxf(before, needed_scale(largest));
         const bool grown = !begun && scale > before;
         const float inverse = 1.0f / scale, ratio = before * inverse;
         uint8_t *const codes = (keys ? p.cache_k : p.cache_v) + (block << p.page_shift) * HD;
-        if (keys) {
-            for (int place = tid / QUADS; place < page_size; place += PLACES) {
-                const int row = owners[place];
-                unsigned *const to = reinterpret_cast<unsigned *>(codes + place * HD + quad_at);
-                if (row >= 0) {
-                    const float4 x = quad(row, quad_at);
-                    *to = e4m3_four(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse);
-                } else if (grown) {
-                    *to = rescaled_four(*to, ratio);
+        for (int i = tid; i < items; i += kAppendThreads) {
+            if (items > kAppendThreads) load(i);
+            const int d = item_run(i) * 8;
+            auto four = [&](int j, int h) {  // codes 4h .. 4h+3 of place j
+                return e4m3_four(x[j].at(4 * h) * inverse, x[j].at(4 * h + 1) * inverse, x[j].at(4 * h + 2) * inverse, x[j].at(4 * h + 3) * inverse);
+            };
+            if (keys) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint2 *const to = reinterpret_cast<uint2 *>(codes + item_place(i, j) * HD + d);
+                    if (rows[j] >= 0) {
+                        *to = uint2{four(j, 0), four(j, 1)};
+                    } else if (grown) {
+                        const uint2 old = *to;
+                        *to = uint2{rescaled_four(old.x, ratio), rescaled_four(old.y, ratio)};
+                    }
                 }
+                continue;
             }
-        } else {
-            for (int place = tid / QUADS; place < page_size; place += PLACES) {
-                const int row = owners[place];
-                uint8_t *const to = codes + (static_cast<size_t>(quad_at) << p.page_shift) + place;
-                unsigned four;
-                if (row >= 0) {
-                    const float4 x = quad(row, quad_at);
-                    four = e4m3_four(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse);
-                } else if (grown) {
-                    four = 0;
-                    for (int i = 0; i < 4; ++i) four |= static_cast<unsigned>(to[i << p.page_shift]) << 8 * i;
-                    four = rescaled_four(four, ratio);
-                } else {
-                    continue;
+            const bool any = (rows[0] & rows[1] & rows[2] & rows[3]) >= 0, all = (rows[0] | rows[1] | rows[2] | rows[3]) >= 0;
+            if (!any && !grown) continue;
+            const unsigned mine = (rows[0] < 0 ? 0 : 0xffu) | (rows[1] < 0 ? 0 : 0xff00u) | (rows[2] < 0 ? 0 : 0xff0000u) | (rows[3] < 0 ? 0 : 0xff000000u);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                unsigned codes_of[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) codes_of[j] = rows[j] >= 0 ? four(j, h) : 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    unsigned *const to = reinterpret_cast<unsigned *>(codes + (static_cast<size_t>(d + 4 * h + e) << p.page_shift) + item_place(i, 0));
+                    // Byte e of the four places' words.
+                    const unsigned pick = 0x0c0c0400u + 0x0101u * e;
+                    unsigned word = __builtin_amdgcn_perm(codes_of[1], codes_of[0], pick) | __builtin_amdgcn_perm(codes_of[3], codes_of[2], pick) << 16;
+                    if (!all) {
+                        const unsigned old = *to;
+                        word = (word & mine) | ((grown ? rescaled_four(old, ratio) : old) & ~mine);
+                    }
+                    *to = word;
                 }
-                for (int i = 0; i < 4; ++i) to[i << p.page_shift] = static_cast<uint8_t>(four >> 8 * i);
             }
         }
         __syncthreads();  // everyone has read the scale, and the next page takes `owners`
-        if (tid == 0) *scale_at = scale;
+        if (tid == 0) *scale_at = scale;  // (the first thread of either half)
     }
 }
 
@@ -304,13 +369,16 @@ hipError_t launch_append(const st_hip_kv_cache &cache, size_t rows, const int32_
 {
     AppendArgs args{k, v, slots, cache.k, cache.v, cache.k_scales, cache.v_scales, static_cast<long long>(ld), static_cast<int>(rows),
                     static_cast<int>(cache.pages), __builtin_ctzll(cache.page_size), static_cast<int>(cache.kv_heads), 1};
-    const size_t units = rows * cache.kv_heads * 2;
-    args.rows_per_block = units <= 4096 ? 1 : 16;
-    const dim3 grid(static_cast<unsigned>((rows + args.rows_per_block - 1) / args.rows_per_block), static_cast<unsigned>(cache.kv_heads), 2);
-    constexpr size_t vector = 4 * sizeof(T);
-    const bool aligned = ld % 4 == 0 && reinterpret_cast<uintptr_t>(k) % vector == 0 && reinterpret_cast<uintptr_t>(v) % vector == 0;
-    if (aligned) kv_append_kernel<T, HD, true><<<grid, kAppendThreads, 0, stream>>>(args);
-    else kv_append_kernel<T, HD, false><<<grid, kAppendThreads, 0, stream>>>(args);
+    const size_t blocks = (rows + kAppendMostRows - 1) / kAppendMostRows * cache.kv_heads;
+    // Up to 1024 workgroups, which the chip holds at about once, share the rows' pages (us for 77 single rows of 5 heads at 256, 512, 1024 and
+    // 2048: 14.9, 8.8, 6.4, 6.4; for 8192 rows of 16 prompts, whose 64 rows begin a page or two: 22.5, 22.5, 22.5, 25.6).
+    args.sharers = 1;
+    while (args.sharers < kAppendMostRows && args.sharers < rows && blocks * args.sharers * 2 <= 1024) args.sharers *= 2;
+    const size_t grid = blocks * args.sharers;
+    if (grid > 0x7fffffffu) return hipErrorInvalidValue;
+    const bool aligned = ld * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
+    if (aligned) kv_append_kernel<T, HD, true><<<static_cast<unsigned>(grid), 2 * kAppendThreads, 0, stream>>>(args);
+    else kv_append_kernel<T, HD, false><<<static_cast<unsigned>(grid), 2 * kAppendThreads, 0, stream>>>(args);
     return hipGetLastError();
 }
 

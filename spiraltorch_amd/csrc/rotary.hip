@@ -14,10 +14,10 @@ struct RotaryArgs {
     void *out;
     const int *positions;
     long long ld_in, ld_out;
-    int rows, sequence, heads, head_dim, half, rows_per_block, heads_per_block;  // half: pairs of a head
+    int rows, sequence, heads, head_dim, half, rows_per_block, heads_per_block, head_blocks;  // half: pairs of a head
     bool interleaved, transposed, copies;                                        // copies: what does not turn has to be copied
     double log2_base_step;  // turns of pair i in a position, before scaling: 2^(-i * step) / 2 pi
-    double factor, original_length, low_turns, high_turns;
+    double by_factor, original_length, low_turns, by_turns;  // 1 / factor, 1 / (high - low)
     float magnitude;
 };
 
@@ -28,9 +28,9 @@ constexpr int kRotaryThreads = 256;
 __device__ __forceinline__ double turns_per_position(const RotaryArgs &p, int pair)
 {
     const double plain = exp2(-pair * p.log2_base_step) * 0.15915494309189535;  // 1 / 2 pi
-    if (p.original_length <= 0.0) return plain / p.factor;
-    const double kept = fmin(fmax((p.original_length * plain - p.low_turns) / (p.high_turns - p.low_turns), 0.0), 1.0);
-    return plain * (kept + (1.0 - kept) / p.factor);
+    if (p.original_length <= 0.0) return plain * p.by_factor;
+    const double kept = fmin(fmax((p.original_length * plain - p.low_turns) * p.by_turns, 0.0), 1.0);
+    return plain * (kept + (1.0 - kept) * p.by_factor);
 }
 
 // cos and sin of so many turns, times the magnitude: the nearest quarter of a turn is taken off in 64 bits, and the rest is an eighth
@@ -53,19 +53,25 @@ __device__ __forceinline__ float load_one(const uint16_t *at) { return __uint_as
 __device__ __forceinline__ void store_one(float *at, float x) { *at = x; }
 __device__ __forceinline__ void store_one(uint16_t *at, float x) { *at = f32_to_bf16_rne(x); }
 
+// cos and sin of the block's rows and all pairs, into LDS: (rows, pairs).
+__device__ __forceinline__ void fill_table(const RotaryArgs &p, int row_first, int block_rows, float2 *table)
+{
+    for (int i = threadIdx.x; i < block_rows * p.half; i += kRotaryThreads) {
+        const int row = row_first + i / p.half;
+        const int position = p.positions ? p.positions[row] : row % p.sequence;
+        table[i] = turned(position * turns_per_position(p, i % p.half), p.magnitude, p.transposed);
+    }
+}
+
 // One pair a thread, of any stride and alignment.
 template <typename T>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_pairs_kernel(RotaryArgs p)
 {
-    extern __shared__ __attribute__((aligned(16))) float2 rotary_lds[];  // (rows, pairs)
+    extern __shared__ __attribute__((aligned(16))) float2 rotary_lds[];
     const int tid = threadIdx.x, half = p.half;
-    const int row_first = blockIdx.x * p.rows_per_block, block_rows = min(p.rows - row_first, p.rows_per_block);
-    const int head_first = blockIdx.y * p.heads_per_block, block_heads = min(p.heads - head_first, p.heads_per_block);
-    for (int i = tid; i < block_rows * half; i += kRotaryThreads) {
-        const int row = row_first + i / half;
-        const int position = p.positions ? p.positions[row] : row % p.sequence;
-        rotary_lds[i] = turned(position * turns_per_position(p, i % half), p.magnitude, p.transposed);
-    }
+    const int row_first = blockIdx.x / p.head_blocks * p.rows_per_block, block_rows = min(p.rows - row_first, p.rows_per_block);
+    const int head_first = blockIdx.x % p.head_blocks * p.heads_per_block, block_heads = min(p.heads - head_first, p.heads_per_block);
+    fill_table(p, row_first, block_rows, rotary_lds);
     __syncthreads();
     const int rest = p.copies ? p.head_dim - 2 * half : 0, units = half + rest;
     const long long total = static_cast<long long>(block_rows) * block_heads * units;
@@ -87,6 +93,107 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_pairs_kernel(RotaryArgs
     }
 }
 
+// Sixteen bytes of values.
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+constexpr int kRunValues = 16 / sizeof(T);
+template <typename T>
+__device__ __forceinline__ float run_at(const u32x4 &run, int i)
+{
+    if constexpr (sizeof(T) == 4) return __uint_as_float(run[i]);
+    else return __uint_as_float(i & 1 ? run[i >> 1] & 0xffff0000u : run[i >> 1] << 16);
+}
+template <typename T>
+__device__ __forceinline__ u32x4 run_of(const float (&values)[kRunValues<T>])
+{
+    u32x4 run;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) run[i] = __float_as_uint(values[i]);
+        else run[i] = pack_bf16x2_rne(values[2 * i], values[2 * i + 1]);
+    }
+    return run;
+}
+
+// The same 32 bytes at a time, as many pairs as 16 bytes hold values: two runs half a rotary_dim apart, or beside each other.  A thread
+// has BATCH of them at once, and loads the first ones before the angles are worked out.
+template <typename T, bool INTERLEAVED, int BATCH>
+__global__ __launch_bounds__(kRotaryThreads) void rotary_runs_kernel(RotaryArgs p)
+{
+    constexpr int COUNT = kRunValues<T>;
+    extern __shared__ __attribute__((aligned(16))) float2 rotary_lds[];
+    const int tid = threadIdx.x, half = p.half;
+    const int row_first = blockIdx.x / p.head_blocks * p.rows_per_block, block_rows = min(p.rows - row_first, p.rows_per_block);
+    const int head_first = blockIdx.x % p.head_blocks * p.heads_per_block, block_heads = min(p.heads - head_first, p.heads_per_block);
+    const int turning = half / COUNT, units = turning + (p.copies ? (p.head_dim - 2 * half) / COUNT : 0);
+    const int total = block_rows * block_heads * units;  // (a block's share is small)
+    const int second = INTERLEAVED ? COUNT : half;
+    u32x4 x[BATCH][2];
+    struct Place {
+        int unit, row;
+        long long head, at;  // offsets within a row, and of the first run within the head
+    };
+    auto place_of = [&](int i) {
+        Place w;
+        const int of = i / units;
+        w.unit = i - of * units;
+        w.row = of / block_heads;
+        w.head = static_cast<long long>(head_first + of - w.row * block_heads) * p.head_dim;
+        w.at = w.unit >= turning ? half + w.unit * COUNT : INTERLEAVED ? 2 * w.unit * COUNT : w.unit * COUNT;
+        return w;
+    };
+    auto load = [&](int first) {
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const int i = first + b * kRotaryThreads;
+            if (i < total) {
+                const Place w = place_of(i);
+                const T *const in = static_cast<const T *>(p.in) + (row_first + w.row) * p.ld_in + w.head + w.at;
+                x[b][0] = *reinterpret_cast<const u32x4 *>(in);
+                if (w.unit < turning) x[b][1] = *reinterpret_cast<const u32x4 *>(in + second);
+            }
+        }
+    };
+    load(tid);
+    fill_table(p, row_first, block_rows, rotary_lds);
+    __syncthreads();
+    for (int first = tid; first < total; first += BATCH * kRotaryThreads) {
+        if (first != tid) load(first);
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const int i = first + b * kRotaryThreads;
+            if (i < total) {
+                const Place w = place_of(i);
+                T *const out = static_cast<T *>(p.out) + (row_first + w.row) * p.ld_out + w.head + w.at;
+                u32x4 low = x[b][0];
+                if (w.unit < turning) {
+                    const float2 *const by = rotary_lds + w.row * half + w.unit * COUNT;
+                    float values[2][COUNT];  // in the order in which the runs hold them
+#pragma unroll
+                    for (int e = 0; e < COUNT; ++e) {
+                        const float2 cs = by[e];
+                        const int ra = INTERLEAVED ? 2 * e / COUNT : 0, ia = INTERLEAVED ? 2 * e % COUNT : e;
+                        const int rb = INTERLEAVED ? ra : 1, ib = INTERLEAVED ? ia + 1 : e;
+                        const float a = run_at<T>(x[b][ra], ia), c = run_at<T>(x[b][rb], ib);
+                        values[ra][ia] = a * cs.x - c * cs.y;
+                        values[rb][ib] = a * cs.y + c * cs.x;
+                    }
+                    low = run_of<T>(values[0]);
+                    *reinterpret_cast<u32x4 *>(out + second) = run_of<T>(values[1]);
+                }
+                *reinterpret_cast<u32x4 *>(out) = low;
+            }
+        }
+    }
+}
+
+template <typename T, int BATCH>
+void launch_runs(dim3 grid, size_t table, const RotaryArgs &args, hipStream_t stream)
+{
+    if (args.interleaved) rotary_runs_kernel<T, true, BATCH><<<grid, kRotaryThreads, table, stream>>>(args);
+    else rotary_runs_kernel<T, false, BATCH><<<grid, kRotaryThreads, table, stream>>>(args);
+}
+
 template <typename T>
 hipError_t launch_rotary(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary &r, bool transposed,
                          const int32_t *positions, const T *in, size_t ld_in, T *out, size_t ld_out, hipStream_t stream)
@@ -106,16 +213,29 @@ hipError_t launch_rotary(size_t rows, size_t sequence, size_t heads, size_t head
     args.transposed = transposed;
     args.copies = in != out;
     args.log2_base_step = std::log2(static_cast<double>(r.base)) / (r.rotary_dim ? args.half : 1);
-    args.factor = r.factor;
+    args.by_factor = 1.0 / r.factor;
     args.original_length = r.original_length;
     args.low_turns = r.low_turns;
-    args.high_turns = r.high_turns;
+    args.by_turns = 1.0 / (static_cast<double>(r.high_turns) - r.low_turns);
     args.magnitude = r.magnitude;
-    args.rows_per_block = 4;
-    args.heads_per_block = static_cast<int>(std::min<size_t>(heads, 16));
-    const size_t by_rows = (rows + args.rows_per_block - 1) / args.rows_per_block, by_heads = (heads + args.heads_per_block - 1) / args.heads_per_block;
-    const dim3 grid(static_cast<unsigned>(by_rows), static_cast<unsigned>(by_heads));
-    rotary_pairs_kernel<T><<<grid, kRotaryThreads, static_cast<size_t>(args.rows_per_block) * args.half * sizeof(float2), stream>>>(args);
+    // Runs of 16 bytes wherever every one of them begins on their boundary.
+    constexpr size_t COUNT = kRunValues<T>;
+    const bool runs = args.half % COUNT == 0 && head_dim % COUNT == 0 && ld_in % COUNT == 0 && ld_out % COUNT == 0 &&
+                      reinterpret_cast<uintptr_t>(in) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    const size_t turning = runs ? args.half / COUNT : args.half, copied = args.copies ? (head_dim - r.rotary_dim) / (runs ? COUNT : 1) : 0;
+    const size_t units = std::max<size_t>(1, turning + copied);  // of a head
+    // A block of 256 threads takes as many whole rows as give each thread a batch, or a part of a row's heads.
+    const size_t batch = runs && rows * heads * units >= size_t(1) << 19 ? 4 : 1, wanted = batch * kRotaryThreads;
+    args.heads_per_block = static_cast<int>(std::max<size_t>(1, std::min(heads, wanted / units)));
+    args.head_blocks = static_cast<int>((heads + args.heads_per_block - 1) / args.heads_per_block);
+    args.rows_per_block = static_cast<int>(std::max<size_t>(1, std::min({rows, wanted / (units * args.heads_per_block), size_t(2048) / std::max(1, args.half)})));
+    const size_t blocks = (rows + args.rows_per_block - 1) / args.rows_per_block * args.head_blocks;
+    if (blocks > 0x7fffffffu) return hipErrorInvalidValue;
+    const size_t table = static_cast<size_t>(args.rows_per_block) * args.half * sizeof(float2);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (!runs) rotary_pairs_kernel<T><<<grid, kRotaryThreads, table, stream>>>(args);
+    else if (batch == 4) launch_runs<T, 4>(grid, table, args, stream);
+    else launch_runs<T, 1>(grid, table, args, stream);
     return hipGetLastError();
 }
 
