@@ -23,6 +23,9 @@ namespace {
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
+// s_waitcnt vmcnt(n) alone.
+#define KV_WAIT_LOADS(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | (7 << 4) | (15 << 8) | ((((n) >> 4) & 3) << 14))
+
 struct KvAttentionArgs {
     const uint8_t *k, *v;
     const float *k_scales, *v_scales;
@@ -49,12 +52,13 @@ constexpr int kKvLeastShare = 4;  // tiles that a workgroup takes at the least: 
 __device__ __forceinline__ int clamped(int x, int low, int high) { return min(max(x, low), high); }
 
 struct KvRequest {
-    int first_row, rows, length;
+    int first_row, rows, length, id;
 };
 
 __device__ __forceinline__ KvRequest load_request(const KvAttentionArgs &p, int r)
 {
     KvRequest q;
+    q.id = r;
     q.first_row = clamped(p.row_offsets[r], 0, p.rows);
     q.rows = max(0, clamped(p.row_offsets[r + 1], 0, p.rows) - q.first_row);
     q.length = static_cast<int>(min(static_cast<long long>(max(0, p.lengths[r])), p.table_width << p.page_shift));
@@ -96,7 +100,6 @@ __device__ __forceinline__ unsigned wave_scan(unsigned v)
 // request where there are no more than 64.
 struct KvFound {
     KvRequest of;
-    int request;
     unsigned offset;  // of the item within its request's
     unsigned before;  // sum of `other` over the requests before it
 };
@@ -133,11 +136,11 @@ __device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvR
         low += which * step;
         left = min(step, left - which * step);
         if (step > 1) continue;
-        found->request = low;
         found->offset = item - items_before;
         found->of.first_row = __builtin_amdgcn_readlane(q.first_row, which);
         found->of.rows = __builtin_amdgcn_readlane(q.rows, which);
         found->of.length = __builtin_amdgcn_readlane(q.length, which);
+        found->of.id = __builtin_amdgcn_readlane(q.id, which);
         return true;
     }
 }
@@ -146,9 +149,25 @@ __device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvR
 __device__ __forceinline__ KvRequest own_request(const KvAttentionArgs &p)
 {
     const int lane = threadIdx.x & 63;
-    KvRequest q{0, 0, 0};
+    KvRequest q{0, 0, 0, 0};
     if (p.requests <= 64 && lane < p.requests) q = load_request(p, lane);
     return q;
+}
+
+// The same in the order of their lengths, so that the longest work begins first.
+__device__ __forceinline__ KvRequest longest_first(const KvAttentionArgs &p, const KvRequest &own)
+{
+    const int lane = threadIdx.x & 63;
+    int rank = lane;
+    if (p.requests <= 64 && lane < p.requests) {
+        rank = 0;
+        for (int i = 0; i < p.requests; ++i) {
+            const int other = __builtin_amdgcn_readlane(own.length, i);
+            rank += other > own.length || (other == own.length && i < lane);
+        }
+    }
+    auto moved = [&](int x) { return __builtin_amdgcn_ds_permute(4 * rank, x); };
+    return KvRequest{moved(own.first_row), moved(own.rows), moved(own.length), moved(own.id)};
 }
 
 // The 64-key tiles that a workgroup takes of a context at the most: all the tiles that there are, over `target` workgroups.  Contexts of
@@ -182,6 +201,20 @@ __device__ __forceinline__ bf16x8 widened(unsigned low, unsigned high, float sca
 // 1 in the bytes of `codes` that hold NaN, else 0.
 __device__ __forceinline__ unsigned nan_bytes(unsigned codes) { return (((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; }
 
+// NaN becomes 0; not 0 where there was one.
+__device__ __forceinline__ unsigned drop_nan(u32x4 &codes)
+{
+    asm volatile("");  // (a branch where this is called in one)
+    unsigned any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned is = nan_bytes(codes[i]);
+        any |= is;
+        codes[i] &= ~((is << 8) - is);
+    }
+    return any;
+}
+
 __device__ __forceinline__ float across_groups_max(float v)  // over the four lane groups, same column
 {
     const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -199,7 +232,8 @@ __device__ __forceinline__ float across_groups_sum(float v)
 template <int HD, int NC>
 struct KvColumnsState {
     f32x4 out[NC][HD / 16];
-    float run_max[NC], run_sum[NC];  // in log2, of scaled scores; this lane's share of the sum
+    f32x4 sum[NC];      // of the weights, as they go into `out`: a product with ones, four times the same
+    float run_max[NC];  // in log2, of scaled scores
     int limit[NC];                   // keys that the column sees
     int keys, fewest;                // the most and the fewest that any of them does
 };
@@ -212,7 +246,7 @@ __device__ __forceinline__ void begin_columns(const KvAttentionArgs &p, const Kv
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         s.run_max[c] = -INFINITY;
-        s.run_sum[c] = 0.0f;
+        s.sum[c] = f32x4{0.f, 0.f, 0.f, 0.f};
         s.limit[c] = sees(min(columns - 1, first + 16 * c + n));
 #pragma unroll
         for (int t = 0; t < HD / 16; ++t) s.out[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -221,9 +255,133 @@ __device__ __forceinline__ void begin_columns(const KvAttentionArgs &p, const Kv
     s.keys = sees(min(columns, first + 16 * NC) - 1);
 }
 
+// Q^T of a wavefront's columns: value 64j + 16g + 8h + (0..7) of the column, for step (j, h) of the first product; keys are loaded alike.  A
+// negative scale goes into its signs, so that the largest score is that of the largest product.
+template <int HD, int NC>
+__device__ __forceinline__ void load_queries(const KvAttentionArgs &p, const KvRequest &of, int kv_head, int first, bf16x8 (&query)[NC][HD / 32])
+{
+    const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, columns = of.rows * p.group;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int column = min(columns - 1, first + 16 * c + n);
+        const uint16_t *const q = p.q + (static_cast<size_t>(of.first_row) + column / p.group) * p.ld_q +
+                                  static_cast<size_t>(kv_head * p.group + column % p.group) * HD;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+            u32x4 raw = *reinterpret_cast<const u32x4 *>(q + 64 * (j / 2) + 16 * g + 8 * (j % 2));
+            if (p.negative) raw ^= 0x80008000u;
+            query[c][j] = __builtin_bit_cast(bf16x8, raw);
+        }
+    }
+}
+
+// -infinity for the scores of keys that a column does not see; `fits`: whether this lane's 16 keys are on a page of the cache.
+template <int HD, int NC>
+__device__ __forceinline__ void hide_unseen(const KvColumnsState<HD, NC> &s, unsigned key0, bool fits, f32x4 (&scores)[NC][4])
+{
+    asm volatile("");  // (a branch, not selects in every tile)
+    const int group = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int seen = fits ? s.limit[c] - static_cast<int>(key0) - 16 * group : 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (i >= seen) scores[c][i >> 2][i & 3] = -INFINITY;
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (comparisons one by one take no scalar registers)
+        }
+    }
+}
+
+// A tile's scores (products of queries and keys; -infinity where a column does not see the key) to the weights of its values, and the
+// columns' maxima, sums and outputs with them.
+template <int HD, int NC>
+__device__ __forceinline__ void weigh(const KvAttentionArgs &p, f32x4 (&scores)[NC][4], KvColumnsState<HD, NC> &s, bf16x8 (&weights)[NC][2])
+{
+    float most[NC];
+    bool grows = false;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        most[c] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            most[c] = fmaxf(fmaxf(most[c], scores[c][i][0]), scores[c][i][1]);
+            most[c] = fmaxf(fmaxf(most[c], scores[c][i][2]), scores[c][i][3]);
+        }
+        most[c] = across_groups_max(most[c]) * p.scale_log2;
+        grows |= most[c] > s.run_max[c] + 8.0f;
+    }
+    // The maximum may lag behind by a factor of 2^8: weights are that much larger then, and nothing has to be scaled for most tiles.
+    if (__any(grows)) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const float up = fmaxf(s.run_max[c], most[c]), shrink = up == s.run_max[c] ? 1.0f : __builtin_amdgcn_exp2f(s.run_max[c] - up);
+            s.run_max[c] = up;
+            s.sum[c] *= shrink;
+#pragma unroll
+            for (int t = 0; t < HD / 16; ++t) s.out[c][t] *= shrink;
+        }
+    }
+    // Weights are summed as they are rounded for the second product: what their rounding adds to it, it adds to the sum as well.
+    const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const float base = s.run_max[c] == -INFINITY ? 0.0f : s.run_max[c];  // (a column that has seen nothing: its weights are 2^-inf)
+        u32x4 packed[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(scores[c][i][e], p.scale_log2, -base));
+            packed[i >> 1][2 * (i & 1)] = pack_bf16x2_rne(w[0], w[1]);
+            packed[i >> 1][2 * (i & 1) + 1] = pack_bf16x2_rne(w[2], w[3]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            weights[c][h] = __builtin_bit_cast(bf16x8, packed[h]);
+            s.sum[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), weights[c][h], s.sum[c], 0, 0, 0);
+        }
+    }
+}
+
+// Values that a column does not see may be anything, above all those behind the last key or on a page outside the cache, and 0 * NaN is not
+// 0.  In a tile that not every column sees whole, NaN among the values goes into the product as 0, and this makes up for it, in tiles
+// `tile`, tile + step, ... below `end`: every sum that met one is NaN.  The same product, of 1 where a value is NaN and 1 where it is seen, says
+// which.
+template <int HD, int NC>
+__device__ __forceinline__ void mark_nan(const KvAttentionArgs &p, const KvRequest &of, int kv_head, unsigned tile, unsigned end, unsigned step, KvColumnsState<HD, NC> &s)
+{
+    const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, page_mask = (1 << p.page_shift) - 1;
+    for (; tile < end; tile += step) {
+        const unsigned key = tile * kKvTile + 16 * g;
+        int page = key < static_cast<unsigned>(of.length) ? p.page_table[of.id * p.table_width + (key >> p.page_shift)] : -1;
+        const bool fits = page >= 0 && page < p.pages;
+        if (!fits) page = 0;
+        const uint8_t *const v = p.v + (((static_cast<size_t>(page) * p.kv_heads + kv_head) * HD + n) << p.page_shift) + (key & page_mask);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int seen = fits ? s.limit[c] - static_cast<int>(key) : 0;
+            u32x4 sees[2];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sees[i >> 2][i & 3] = (2 * i < seen ? 0x3f80u : 0u) | (2 * i + 1 < seen ? 0x3f800000u : 0u);
+#pragma unroll
+            for (int t = 0; t < HD / 16; ++t) {
+                u32x4 is = *reinterpret_cast<const u32x4 *>(v + (static_cast<size_t>(16 * t) << p.page_shift));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) is[i] = nan_bytes(is[i]) * 0x38u;  // 1.0
+                f32x4 met = {0.f, 0.f, 0.f, 0.f};
+                met = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(is[0], is[1], 1.0f), __builtin_bit_cast(bf16x8, sees[0]), met, 0, 0, 0);
+                met = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(is[2], is[3], 1.0f), __builtin_bit_cast(bf16x8, sees[1]), met, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (met[i] > 0.0f) s.out[c][t][i] = NAN;
+            }
+        }
+    }
+}
+
 // Tiles `tile`, tile + step, ... below `end` of the request's keys for a wavefront's columns.
 template <int HD, int NC>
-__device__ __forceinline__ void attend(const KvAttentionArgs &p, const KvRequest &of, int request, int kv_head, int first, unsigned tile_first,
+__device__ __forceinline__ void attend(const KvAttentionArgs &p, const KvRequest &of, int kv_head, int first, unsigned tile_first,
                                        unsigned end, unsigned step, KvColumnsState<HD, NC> &s)
 {
     constexpr int KL = HD / 64;  // 16-byte loads of a key's row, per lane
@@ -231,23 +389,10 @@ __device__ __forceinline__ void attend(const KvAttentionArgs &p, const KvRequest
     if (tile_first >= end) return;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, columns = of.rows * p.group;
 
-    // Q^T: value 64j + 16g + 8h + (0..7) of the column, for step (j, h) of the first product; keys are loaded alike.  A negative scale
-    // goes into its signs, so that the largest score is that of the largest product.
     bf16x8 query[NC][2 * KL];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int column = min(columns - 1, first + 16 * c + n);
-        const uint16_t *const q = p.q + (static_cast<size_t>(of.first_row) + column / p.group) * p.ld_q +
-                                  static_cast<size_t>(kv_head * p.group + column % p.group) * HD;
-#pragma unroll
-        for (int j = 0; j < 2 * KL; ++j) {
-            u32x4 raw = *reinterpret_cast<const u32x4 *>(q + 64 * (j / 2) + 16 * g + 8 * (j % 2));
-            if (p.negative) raw ^= 0x80008000u;
-            query[c][j] = __builtin_bit_cast(bf16x8, raw);
-        }
-    }
+    load_queries<HD, NC>(p, of, kv_head, first, query);
 
-    const int *const table = p.page_table + request * p.table_width;
+    const int *const table = p.page_table + of.id * p.table_width;
     const int page_mask = (1 << p.page_shift) - 1;
     // The pages of the 16 keys that this lane loads (a row of the first product: group n/4), and of those whose scores it holds.
     const int key_group = 16 * (n >> 2), value_group = 16 * g;
@@ -302,60 +447,11 @@ __device__ __forceinline__ void attend(const KvAttentionArgs &p, const KvRequest
         __builtin_amdgcn_sched_barrier(0);  // (what is widened too early takes registers)
         if (more) load_keys(next, key_page);
 
-        int seen[NC];  // of this lane's 16 keys
-#pragma unroll
-        for (int c = 0; c < NC; ++c) seen[c] = value_fits ? s.limit[c] - static_cast<int>(key0) - value_group : 0;
-        if (!whole) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (i >= seen[c]) scores[c][i >> 2][i & 3] = -INFINITY;
-        }
-        float most[NC];
-        bool grows = false;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            most[c] = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) most[c] = fmaxf(most[c], fmaxf(fmaxf(scores[c][i][0], scores[c][i][1]), fmaxf(scores[c][i][2], scores[c][i][3])));
-            most[c] = across_groups_max(most[c]) * p.scale_log2;
-            grows |= most[c] > s.run_max[c] + 8.0f;
-        }
-        // The maximum may lag behind by a factor of 2^8: weights are that much larger then, and nothing has to be scaled for most tiles.
-        if (__any(grows)) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const float up = fmaxf(s.run_max[c], most[c]), shrink = up == s.run_max[c] ? 1.0f : __builtin_amdgcn_exp2f(s.run_max[c] - up);
-                s.run_max[c] = up;
-                s.run_sum[c] *= shrink;
-#pragma unroll
-                for (int t = 0; t < VT; ++t) s.out[c][t] *= shrink;
-            }
-        }
+        if (!whole) hide_unseen<HD, NC>(s, key0, value_fits, scores);
         bf16x8 weights[NC][2];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const float base = s.run_max[c] == -INFINITY ? 0.0f : s.run_max[c];  // (a column that has seen nothing: its weights are 2^-inf)
-            u32x4 packed[2];
-            float sums[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(scores[c][i][e], p.scale_log2, -base));
-                sums[i] = (w[0] + w[1]) + (w[2] + w[3]);
-                packed[i >> 1][2 * (i & 1)] = pack_bf16x2_rne(w[0], w[1]);
-                packed[i >> 1][2 * (i & 1) + 1] = pack_bf16x2_rne(w[2], w[3]);
-            }
-            s.run_sum[c] += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-            weights[c][0] = __builtin_bit_cast(bf16x8, packed[0]);
-            weights[c][1] = __builtin_bit_cast(bf16x8, packed[1]);
-        }
+        weigh<HD, NC>(p, scores, s, weights);
         if (!whole) {
-            // Values that a column does not see may be anything, above all those behind the last key or on a page outside the cache, and
-            // 0 * NaN is not 0: NaN goes in as 0, and where it is seen is looked for below.
-            unsigned is = 0;
+            unsigned is = 0;  // (see mark_nan)
 #pragma unroll
             for (int t = 0; t < VT; ++t)
 #pragma unroll
@@ -383,34 +479,7 @@ __device__ __forceinline__ void attend(const KvAttentionArgs &p, const KvRequest
             value_page = page_at(next + step * kKvTile + value_group);
         }
     }
-
-    // From the first tile on where NaN was left out: every sum that met one is one.  The same product, of 1 where a value is NaN and 1
-    // where it is seen, says which.
-    for (tile = masked_first; tile < end; tile += step) {
-        const unsigned key0 = tile * kKvTile;
-        const int page = page_at(key0 + value_group);
-        const uint8_t *const v = values_at(key0, page);
-        value_fits = fits(page);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int seen = value_fits ? s.limit[c] - static_cast<int>(key0) - value_group : 0;
-            u32x4 sees[2];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sees[i >> 2][i & 3] = (2 * i < seen ? 0x3f80u : 0u) | (2 * i + 1 < seen ? 0x3f800000u : 0u);
-#pragma unroll
-            for (int t = 0; t < VT; ++t) {
-                u32x4 is = *reinterpret_cast<const u32x4 *>(v + (static_cast<size_t>(16 * t) << p.page_shift));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) is[i] = nan_bytes(is[i]) * 0x38u;  // 1.0
-                f32x4 met = {0.f, 0.f, 0.f, 0.f};
-                met = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(is[0], is[1], 1.0f), __builtin_bit_cast(bf16x8, sees[0]), met, 0, 0, 0);
-                met = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(is[2], is[3], 1.0f), __builtin_bit_cast(bf16x8, sees[1]), met, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (met[i] > 0.0f) s.out[c][t][i] = NAN;
-            }
-        }
-    }
+    mark_nan<HD, NC>(p, of, kv_head, masked_first, end, step, s);
 }
 
 __device__ __forceinline__ uint16_t *out_at(const KvAttentionArgs &p, const KvRequest &of, int kv_head, int column, int head_dim)
@@ -439,15 +508,17 @@ __device__ __forceinline__ float2 load_shared(const float *at)
 // A sum of 0 is a column without keys.  (Scores of NaN make it NaN.)
 __device__ __forceinline__ float inverse_of(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
 
+template <int HD>
+constexpr int kKvFewFloats = 4 * kKvColumns * (HD + 4);
+
 // Few columns: a workgroup takes sixteen of them and a share of their keys, which its four wavefronts deal out among themselves.  Where
 // a context is cut over workgroups, the last of them to finish puts their parts together, in the parts' order: the result does not
 // depend on who that was.
 template <int HD>
-__device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned unit)
+__device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned unit, float *lds_out)
 {
     constexpr int VT = HD / 16;
     constexpr int OS = HD + 4;  // row stride of the wavefronts' sums in LDS
-    __shared__ __attribute__((aligned(16))) float lds_out[4 * kKvColumns * OS];
     __shared__ float lds_max[4][kKvColumns], lds_sum[4][kKvColumns];
     __shared__ bool is_last;
 
@@ -467,13 +538,12 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
     KvColumnsState<HD, 1> s;
     begin_columns<HD, 1>(p, at.of, first, s);
     const unsigned tiles = key_tiles(s.keys), tile_first = part * own_share, tile_end = min(tiles, tile_first + min(own_share, 0x40000000u));
-    attend<HD, 1>(p, at.of, at.request, kv_head, first, tile_first + wave, tile_end, 4, s);
+    attend<HD, 1>(p, at.of, kv_head, first, tile_first + wave, tile_end, 4, s);
 
     // The four wavefronts' sums, each on its own maximum, put together.
-    const float wave_sum_of = across_groups_sum(s.run_sum[0]);
     if (g == 0) {
         lds_max[wave][n] = s.run_max[0];
-        lds_sum[wave][n] = wave_sum_of;
+        lds_sum[wave][n] = s.sum[0][0];
     }
 #pragma unroll
     for (int t = 0; t < VT; ++t) *reinterpret_cast<f32x4 *>(&lds_out[(wave * kKvColumns + n) * OS + 16 * t + 4 * g]) = s.out[0][t];
@@ -517,7 +587,7 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
 
     auto place = [&](unsigned of_part, int c) { return (static_cast<size_t>(unit) + (static_cast<size_t>(of_part) - part) * p.kv_heads) * kKvColumns + c; };
     float *const factors = lds_out;  // (parts, 16)
-    static_assert(kKvMostParts * kKvColumns + 256 * 4 <= 4 * kKvColumns * (64 + 4), "factors and the threads' sums");
+    static_assert(kKvMostParts * kKvColumns + 256 * 4 <= kKvFewFloats<64>, "factors and the threads' sums");
     constexpr int MINE = kKvMostParts / 16;
     const int slice = tid >> 4;
     float2 held[MINE];
@@ -571,41 +641,208 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
     }
 }
 
-// Many columns: each wavefront has 16 NC of its own, and all keys that they see.
-template <int HD, int NC>
-__device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned tile)
+// Many columns: each wavefront has 16 NC of its own, and the workgroup brings the keys and values that all of them read through LDS, as the
+// cache holds them, in a ring of stages that is filled two tiles ahead by loads that write LDS themselves: the wavefronts' registers
+// hold columns, and a tile is read from memory once for four of them.  A stage holds 64 keys' rows and the values' HD rows of 64
+// bytes; their 16-byte pieces are stored at places that keep the sixteen rows that a fragment reads on banks of their own.
+typedef __attribute__((address_space(3))) void *kv_lds_ptr;
+typedef __attribute__((address_space(1))) const void *kv_global_ptr;
+typedef __attribute__((address_space(4))) int kv_constant_int;
+typedef __attribute__((address_space(4))) float kv_constant_float;
+// One for each 16 keys of a tile.
+template <typename T>
+struct Four {
+    T a, b, c, d;
+};
+// (Values, not places: a choice among places would put them into memory.)
+template <typename T>
+__device__ __forceinline__ T pick(T a, T b, T c, T d, int group)
 {
-    constexpr int WIDTH = 4 * 16 * NC;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const T low = group & 1 ? b : a, high = group & 1 ? d : c;
+    return group & 2 ? high : low;
+}
+template <typename T>
+__device__ __forceinline__ T pick(const Four<T> of, int group) { return pick(of.a, of.b, of.c, of.d, group); }
+constexpr int kKvStages = 3;
+template <int HD>
+constexpr int kKvStageBytes = 2 * kKvTile * HD + 4 * 256;
+
+// Which piece of a key's row stands at a place is the exclusive or of the place and this: by the bits in which the sixteen rows of a
+// fragment differ (0 and 1, 4 and 5) beyond those that choose among the rows in the 256 bytes of all banks.
+template <int HD>
+__device__ __forceinline__ int key_swizzle(int row)
+{
+    if constexpr (HD == 64) return row >> 4 & 3;
+    else if constexpr (HD == 128) return (row >> 1 & 1) | (row >> 4 & 3) << 1;
+    else return (row & 3) | (row >> 4 & 3) << 2;
+}
+
+#ifndef PF
+#define PF 2
+#endif
+template <int HD, int NC>
+__device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned item, unsigned char *lds)
+{
+    constexpr int WIDTH = 4 * 16 * NC, VT = HD / 16, KL = HD / 64, LOADS = kKvTile * HD / 4096;  // of 16 bytes, a thread, for keys and for values
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int kv_head = tile % p.kv_heads;
+    const int kv_head = item % p.kv_heads;
     KvFound at;
-    auto tiles = [&](const KvRequest &q) {
+    auto tiles_of = [&](const KvRequest &q) {
         const int columns = q.rows * p.group;
         return columns > p.few ? (static_cast<unsigned>(columns) + WIDTH - 1) / WIDTH : 0;
     };
-    if (!find_request(p, own_request(p), tile / p.kv_heads, p.wide / p.kv_heads, tiles, [](const KvRequest &) { return 0u; }, &at)) return;
+    if (!find_request(p, longest_first(p, own_request(p)), item / p.kv_heads, p.wide / p.kv_heads, tiles_of, [](const KvRequest &) { return 0u; }, &at)) return;
+    const KvRequest of = at.of;
     // (the last columns see the most keys: they come first)
-    const int columns = at.of.rows * p.group, first = static_cast<int>(tiles(at.of) - 1 - at.offset) * WIDTH + wave * 16 * NC;
-    if (first >= columns) return;
+    const int columns = of.rows * p.group, block_first = static_cast<int>(tiles_of(of) - 1 - at.offset) * WIDTH, first = block_first + wave * 16 * NC;
     KvColumnsState<HD, NC> s;
-    begin_columns<HD, NC>(p, at.of, first, s);
-    attend<HD, NC>(p, at.of, at.request, kv_head, first, 0, key_tiles(s.keys), 1, s);
+    begin_columns<HD, NC>(p, of, first, s);
+    const int last_column = min(columns, block_first + WIDTH) - 1;
+    const unsigned end = key_tiles(p.causal ? max(0, of.length - of.rows + last_column / p.group + 1) : of.length);
+    const unsigned own_end = first < columns ? key_tiles(s.keys) : 0;  // (behind the last column a wavefront helps with the loads)
+    bf16x8 query[NC][2 * KL];
+    load_queries<HD, NC>(p, of, kv_head, first, query);
+
+    // What a tile's four groups of keys are on, the same for all threads: read by the scalar unit, whose loads the counting of vector loads
+    // below does not meet.
+    struct Pages {
+        Four<int> block;  // page * kv_heads + head, of page 0 for none
+        int fits;         // bit i: there is one
+    };
+    const kv_constant_int *const table = (const kv_constant_int *)(p.page_table + of.id * p.table_width);
+    const int page_mask = (1 << p.page_shift) - 1;
+    auto look_up = [&](unsigned tile) {
+        Pages pages;
+        pages.fits = 0;
+        auto one = [&](int i) {
+            const unsigned key = tile * kKvTile + 16 * i, there = min(key, static_cast<unsigned>(of.length - 1));
+            const int page = table[there >> p.page_shift];
+            const bool fits = key == there && page >= 0 && page < p.pages;
+            pages.fits |= fits << i;
+            return (fits ? page : 0) * p.kv_heads + kv_head;
+        };
+        pages.block = Four<int>{one(0), one(1), one(2), one(3)};
+        return pages;
+    };
+    // Where a thread's pieces stand: 16-byte loads of keys begin at a place of the wavefront's 16-key group, those of values at one of the
+    // thread's own group, but for pages that hold whole tiles at one of all threads' page.
+    unsigned key_offset[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int place = i * 256 + tid, row = place / (HD / 16);
+        key_offset[i] = (row & 15) * HD + (place % (HD / 16) ^ key_swizzle<HD>(row)) * 16;
+    }
+    const int load_group = (lane & 3) ^ (lane >> 4);
+    const unsigned value_offset = (static_cast<unsigned>(tid >> 2) << p.page_shift) + (p.page_shift >= 6 ? 16 * load_group : 0);
+    const float *const scales = lane & 4 ? p.v_scales : p.k_scales;
+    auto request = [&](unsigned tile, unsigned char *stage_at, const Pages &pages) {
+        const unsigned key0 = tile * kKvTile;
+        unsigned char *const to = stage_at + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const unsigned group = (i * 256u + wave * 64u) / HD;  // (a wavefront's rows are of one)
+            const uint8_t *const from = p.k + ((static_cast<size_t>(static_cast<unsigned>(pick(pages.block, group))) << p.page_shift) + ((key0 + 16 * group) & page_mask)) * HD;
+            __builtin_amdgcn_global_load_lds((kv_global_ptr)(from + key_offset[i]), (kv_lds_ptr)(to + i * 4096), 16, 0, 0);
+        }
+        const uint8_t *values;
+        if (p.page_shift >= 6) values = p.v + ((static_cast<size_t>(static_cast<unsigned>(pages.block.a)) * HD) << p.page_shift) + (key0 & page_mask);
+        else values = p.v + ((static_cast<size_t>(static_cast<unsigned>(pick(pages.block, load_group))) * HD) << p.page_shift) + ((key0 + 16 * load_group) & page_mask);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            __builtin_amdgcn_global_load_lds((kv_global_ptr)(values + (static_cast<size_t>(i * 64) << p.page_shift) + value_offset), (kv_lds_ptr)(to + kKvTile * HD + i * 4096), 16, 0, 0);
+        // (each wavefront its own: the keys' four scales, then the values', again and again)
+        __builtin_amdgcn_global_load_lds((kv_global_ptr)(scales + static_cast<unsigned>(pick(pages.block, lane))), (kv_lds_ptr)(stage_at + 2 * kKvTile * HD + wave * 256), 4, 0, 0);
+    };
+    const int key_at = ((n >> 2) * 16 + (n & 3)) * HD, key_turn = key_swizzle<HD>((n >> 2) * 16 + (n & 3));
+    const int value_at = kKvTile * HD + n * 64 + ((g ^ (n >> 2)) * 16), scale_at = 2 * kKvTile * HD + wave * 256;
+    unsigned nan_first = own_end;  // see mark_nan
+    // One tile from its stage, while the tile two behind it comes into another.  (That the two do not meet has to be said, or every read of
+    // the one waits for all of the other.)
+    auto take_tile = [&](const unsigned char *__restrict held, unsigned char *__restrict coming, unsigned tile, const Pages &pages, const Pages &after) __attribute__((always_inline)) {
+        if (tile + 2 < end) request(tile + 2, coming, after);
+        if (tile >= own_end) return;
+        const unsigned key0 = tile * kKvTile;
+        const float scale_of_keys = *reinterpret_cast<const float *>(held + scale_at + 4 * (n >> 2));
+        const float held_scale = *reinterpret_cast<const float *>(held + scale_at + 16 + 4 * g);
+        const float scale_of_values = pages.fits >> g & 1 ? held_scale : 1.0f;
+        // Pieces are read PF ahead of their use.
+        f32x4 scores[NC][4];
+        auto key_piece = [&](int i) { return *reinterpret_cast<const u32x4 *>(held + key_at + 4 * (i / KL) * HD + ((4 * (i % KL) + g) ^ key_turn) * 16); };
+        auto value_piece = [&](int t) { return *reinterpret_cast<const u32x4 *>(held + value_at + t * 1024); };
+        u32x4 ahead[PF];
+#pragma unroll
+        for (int i = 0; i < PF; ++i) ahead[i] = key_piece(i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) scores[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KL; ++j) {
+                const int at = i * KL + j;
+                const u32x4 codes = ahead[at % PF];
+                if (at + PF < 4 * KL) ahead[at % PF] = key_piece(at + PF);
+                else ahead[at % PF] = value_piece(at + PF - 4 * KL);
+                const bf16x8 low = widened(codes[0], codes[1], scale_of_keys), high = widened(codes[2], codes[3], scale_of_keys);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) scores[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(low, query[c][2 * j], scores[c][i], 0, 0, 0);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) scores[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(high, query[c][2 * j + 1], scores[c][i], 0, 0, 0);
+            }
+        }
+        const bool whole = pages.fits == 15 && key0 + kKvTile <= static_cast<unsigned>(s.fewest);
+        if (!whole) hide_unseen<HD, NC>(s, key0, pages.fits >> g & 1, scores);
+        bf16x8 weights[NC][2];
+        weigh<HD, NC>(p, scores, s, weights);
+        unsigned nan = 0;
+#pragma unroll
+        for (int t = 0; t < VT; ++t) {
+            u32x4 codes = ahead[t % PF];
+            if (t + PF < VT) ahead[t % PF] = value_piece(t + PF);
+            if (!whole) nan |= drop_nan(codes);
+            const bf16x8 low = widened(codes[0], codes[1], scale_of_values), high = widened(codes[2], codes[3], scale_of_values);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(low, weights[c][0], s.out[c][t], 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(high, weights[c][1], s.out[c][t], 0, 0, 0);
+        }
+        if (__any(nan != 0)) nan_first = min(nan_first, tile);
+    };
+    if (end != 0) {
+        Pages pages = look_up(0), next = look_up(1), after = look_up(2);
+        unsigned char *now = lds, *soon = lds + kKvStageBytes<HD>, *then = lds + 2 * kKvStageBytes<HD>;
+        request(0, now, pages);
+        if (end > 1) request(1, soon, next);
+        for (unsigned tile = 0; tile < end; ++tile) {
+            // This tile has landed in every wavefront's share of it, and everyone is done with the one before, whose stage is next.
+            if (tile + 1 < end) KV_WAIT_LOADS(2 * LOADS + 1);
+            else KV_WAIT_LOADS(0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            take_tile(now, then, tile, pages, after);
+            pages = next, next = after, after = look_up(tile + 3);
+            unsigned char *const done = now;
+            now = soon, soon = then, then = done;
+        }
+    }
+    mark_nan<HD, NC>(p, of, kv_head, nan_first, own_end, 1, s);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int column = first + 16 * c + n;
-        const float inverse = inverse_of(across_groups_sum(s.run_sum[c]));
+        const float inverse = inverse_of(s.sum[c][0]);
         if (column >= columns) continue;
-        uint16_t *const out = out_at(p, at.of, kv_head, column, HD) + 4 * g;
+        uint16_t *const out = out_at(p, of, kv_head, column, HD) + 4 * g;
 #pragma unroll
-        for (int t = 0; t < HD / 16; ++t) *reinterpret_cast<u32x2 *>(out + 16 * t) = rounded_four(s.out[c][t], inverse);
+        for (int t = 0; t < VT; ++t) *reinterpret_cast<u32x2 *>(out + 16 * t) = rounded_four(s.out[c][t], inverse);
     }
 }
 
 template <int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : HD == 128 ? 3 : 2))) void kv_attention_few_kernel(KvAttentionArgs p)
 {
-    few_columns<HD>(p, blockIdx.x);
+    __shared__ __attribute__((aligned(16))) float lds[kKvFewFloats<HD>];
+    few_columns<HD>(p, blockIdx.x, lds);
 }
 
 // Batches that may hold requests of either kind.
@@ -614,8 +851,10 @@ constexpr int kKvWideTiles = HD == 64 ? 4 : 2;
 template <int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void kv_attention_mixed_kernel(KvAttentionArgs p)
 {
-    if (blockIdx.x < p.wide) many_columns<HD, kKvWideTiles<HD>>(p, blockIdx.x);
-    else few_columns<HD>(p, blockIdx.x - p.wide);
+    constexpr size_t few = kKvFewFloats<HD> * sizeof(float), wide = kKvStages * kKvStageBytes<HD>;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[few > wide ? few : wide];
+    if (blockIdx.x < p.wide) many_columns<HD, kKvWideTiles<HD>>(p, blockIdx.x, lds);
+    else few_columns<HD>(p, blockIdx.x - p.wide, reinterpret_cast<float *>(lds));
 }
 
 // Requests of more columns go to wide tiles: keys and values are widened once for four or two times as many columns there, but a
