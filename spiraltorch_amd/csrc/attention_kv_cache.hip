@@ -33,12 +33,15 @@ struct KvAttentionArgs {
     const uint16_t *q;
     uint16_t *out;
     float *parts;       // where keys are cut over workgroups: for each of `units` of them 16 columns of head_dim sums, and then 16 maxima and sums
-    unsigned *arrived;  // and for every tile of columns how many of its workgroups are done: 0 before a launch and after it
+    float *wide_parts;  // the same for wide tiles
+    unsigned *arrived;  // and for every tile of columns, `items` narrow ones and the wide ones, how many of its workgroups are done: 0 before a
+                        // launch and after it
     long long ld_q, ld_out, table_width;
     int requests, rows, heads, kv_heads, group, pages, page_shift;
     int few;         // requests of so many columns or fewer go to the kernel whose wavefronts share them, others to the one of wide tiles
     unsigned units;  // workgroups of the former
     unsigned wide;   // and of the latter
+    unsigned items;  // the most that there can be of (narrow tile of columns, key head) pairs
     float heads_by_target;
     float scale_log2;  // |scale| * log2(e), not quite 0
     bool causal, negative;
@@ -46,7 +49,7 @@ struct KvAttentionArgs {
 
 constexpr int kKvTile = 64;     // keys
 constexpr int kKvColumns = 16;  // (token, head) pairs of a tile
-constexpr int kKvMostParts = 128;
+constexpr int kKvMostParts = 128, kKvMostWideParts = 16;
 constexpr int kKvLeastShare = 4;  // tiles that a workgroup takes at the least: one for each of its wavefronts
 
 __device__ __forceinline__ int clamped(int x, int low, int high) { return min(max(x, low), high); }
@@ -71,28 +74,39 @@ __device__ __forceinline__ unsigned few_tiles(const KvAttentionArgs &p, const Kv
     const int columns = q.rows * p.group;
     return columns <= p.few ? (static_cast<unsigned>(columns) + kKvColumns - 1) / kKvColumns : 0;
 }
-// A context in parts of `share` tiles, or more where they would be too many to put together.
-__device__ __forceinline__ unsigned share_of(const KvRequest &q, unsigned share) { return max(share, (key_tiles(q.length) + kKvMostParts - 1) / kKvMostParts); }
-__device__ __forceinline__ unsigned parts_of(const KvRequest &q, unsigned share)
+// A context in parts of `share` tiles, or more where they would be too many to put together; whole, if it is not much longer, or short and
+// not longer than two: putting parts together takes 3 us, and its last part would leave a workgroup with little to do.  (16 contexts of 300 to
+// 1000 keys with 64 columns each took 26 us when cut at every share, and 19 so; 12 heads' 16 contexts of 1500 keys, 24 tiles at a share
+// of 12, 14.4 and 12.0; decoding 64 contexts of up to 8192 41.2 and 40.2, and 43.5 with contexts of up to two shares whole.)
+__device__ __forceinline__ unsigned share_of(const KvRequest &q, unsigned share, unsigned most = kKvMostParts)
 {
-    const unsigned mine = share_of(q, share);
+    const unsigned tiles = key_tiles(q.length), mine = max(share, ((tiles + most - 1) / most + 3u) & ~3u);
+    return tiles <= max(mine + mine / 2, min(2 * mine, 24u)) ? max(tiles, 1u) : mine;
+}
+__device__ __forceinline__ unsigned parts_of(const KvRequest &q, unsigned share, unsigned most = kKvMostParts)
+{
+    const unsigned mine = share_of(q, share, most);
     return max(1u, (key_tiles(q.length) + mine - 1) / mine);
 }
 
-// Sum over the lanes up to and with this one.
-__device__ __forceinline__ unsigned wave_scan(unsigned v)
+// `of(x, y)` over the lanes up to and with this one, where of(x, 0) is x.
+template <class Of>
+__device__ __forceinline__ unsigned wave_scan(unsigned v, Of &&of)
 {
     auto shifted = [](unsigned x, auto control, auto rows) {
         return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(control)::value, decltype(rows)::value, 0xf, false));
     };
     using All = std::integral_constant<int, 0xf>;
-    v += shifted(v, std::integral_constant<int, 0x111>{}, All{});  // within rows of sixteen: from 1, 2, 4 and 8 lanes before
-    v += shifted(v, std::integral_constant<int, 0x112>{}, All{});
-    v += shifted(v, std::integral_constant<int, 0x114>{}, All{});
-    v += shifted(v, std::integral_constant<int, 0x118>{}, All{});
-    v += shifted(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // the last of a row to the next one, in rows 1 and 3
-    v += shifted(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // lane 31 to rows 2 and 3
-    return v;
+    v = of(v, shifted(v, std::integral_constant<int, 0x111>{}, All{}));  // within rows of sixteen: from 1, 2, 4 and 8 lanes before
+    v = of(v, shifted(v, std::integral_constant<int, 0x112>{}, All{}));
+    v = of(v, shifted(v, std::integral_constant<int, 0x114>{}, All{}));
+    v = of(v, shifted(v, std::integral_constant<int, 0x118>{}, All{}));
+    v = of(v, shifted(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}));  // the last of a row to the next one, in rows 1 and 3
+    return of(v, shifted(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}));  // lane 31 to rows 2 and 3
+}
+__device__ __forceinline__ unsigned wave_scan(unsigned v)
+{
+    return wave_scan(v, [](unsigned x, unsigned y) { return x + y; });
 }
 
 // Work is numbered by prefix sums over the requests, which every wavefront takes for itself: `count(request)` items each, and the
@@ -154,37 +168,62 @@ __device__ __forceinline__ KvRequest own_request(const KvAttentionArgs &p)
     return q;
 }
 
-// The same in the order of their lengths, so that the longest work begins first.
+// What one wavefront found for all of a workgroup's.
+__device__ __forceinline__ KvFound uniform(const KvFound &f)
+{
+    auto one = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    return KvFound{{one(f.of.first_row), one(f.of.rows), one(f.of.length), one(f.of.id)}, static_cast<unsigned>(one(f.offset)), static_cast<unsigned>(one(f.before))};
+}
+
+// The same with the longest first, so that the longest work begins first: sorted, or by eight classes half an octave wide and the rest.
+// (Sorting took 2.8 us for 64 requests, for 16 it takes 0.6 us.  What is done in a few microseconds goes without, and work that takes
+// long has requests in the order of their lengths.)
+template <bool SORT>
 __device__ __forceinline__ KvRequest longest_first(const KvAttentionArgs &p, const KvRequest &own)
 {
+    if (p.requests > 64) return own;
     const int lane = threadIdx.x & 63;
-    int rank = lane;
-    if (p.requests <= 64 && lane < p.requests) {
-        rank = 0;
+    int rank = 0;
+    if (SORT && p.requests <= 16) {
         for (int i = 0; i < p.requests; ++i) {
             const int other = __builtin_amdgcn_readlane(own.length, i);
             rank += other > own.length || (other == own.length && i < lane);
+        }
+        if (lane >= p.requests) rank = lane;
+    } else {
+        const unsigned width = own.rows == 0 ? 0 : __float_as_uint(static_cast<float>(own.length)) >> 22;  // exponent and a bit more
+        const unsigned widest = __builtin_amdgcn_readlane(wave_scan(width, [](unsigned x, unsigned y) { return max(x, y); }), 63);
+        const int of_class = static_cast<int>(min(widest - width, 8u));
+        if (__all(of_class == 0 || own.rows == 0)) return own;
+        int before = 0;
+#pragma unroll
+        for (int i = 0; i <= 8; ++i) {
+            const unsigned long long in = __ballot(of_class == i);
+            const int among = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(in >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(in), 0));
+            if (of_class == i) rank = before + among;
+            before += __popcll(in);
         }
     }
     auto moved = [&](int x) { return __builtin_amdgcn_ds_permute(4 * rank, x); };
     return KvRequest{moved(own.first_row), moved(own.rows), moved(own.length), moved(own.id)};
 }
 
-// The 64-key tiles that a workgroup takes of a context at the most: all the tiles that there are, over `target` workgroups.  Contexts of
-// very different lengths fill the chip evenly so, whatever the host knows of them (it knows the table's width alone).
-__device__ __forceinline__ unsigned find_share(const KvAttentionArgs &p, const KvRequest &own)
+// The 64-key tiles that a workgroup takes of a context at the most: all the tiles that there are, `count(request)` for one, over the
+// workgroups that there should be.  Contexts of very different lengths fill the chip evenly so, whatever the host knows of them (it
+// knows the table's width alone).
+template <class Count>
+__device__ __forceinline__ unsigned find_share(const KvAttentionArgs &p, const KvRequest &own, Count &&count)
 {
-    if (p.parts == nullptr) return 0x7fffffffu;
     float tiles = 0.0f;  // (rounded, but alike in every workgroup, and what it may fall short of the sum by is added below)
-    auto add = [&](const KvRequest &q) { tiles += static_cast<float>(few_tiles(p, q)) * static_cast<float>(key_tiles(q.length)); };
     if (p.requests <= 64) {
-        add(own);
+        tiles = count(own);
     } else {
         const int step = (p.requests + 63) / 64, first = (threadIdx.x & 63) * step, end = min(p.requests, first + step);
-        for (int r = first; r < end; ++r) add(load_request(p, r));
+        for (int r = first; r < end; ++r) tiles += count(load_request(p, r));
     }
     const float share = wave_sum(tiles) * p.heads_by_target * 1.001f + 1.0f;
-    return __builtin_amdgcn_readfirstlane(max(static_cast<unsigned>(kKvLeastShare), static_cast<unsigned>(fminf(share, 1073741824.0f))));
+    const unsigned whole = (static_cast<unsigned>(fminf(share, 1073741824.0f)) + 3u) & ~3u;  // (the same for each of four wavefronts)
+    return __builtin_amdgcn_readfirstlane(max(static_cast<unsigned>(kKvLeastShare), whole));
 }
 
 // Eight e4m3 values times a power of two, as bf16: both are exact.
@@ -521,16 +560,28 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
     constexpr int OS = HD + 4;  // row stride of the wavefronts' sums in LDS
     __shared__ float lds_max[4][kKvColumns], lds_sum[4][kKvColumns];
     __shared__ bool is_last;
+    __shared__ KvFound found;
+    __shared__ unsigned found_share;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int kv_head = unit % p.kv_heads;  // neighbouring workgroups, on different XCDs, share nothing
-    const KvRequest own = own_request(p);
-    const unsigned share = find_share(p, own);
-    KvFound at;
-    if (!find_request(p, own, unit / p.kv_heads, p.units / p.kv_heads, [&](const KvRequest &q) { return few_tiles(p, q) * parts_of(q, share); },
-                      [&](const KvRequest &q) { return few_tiles(p, q); }, &at))
-        return;
+    if (wave == 0) {
+        const KvRequest own = longest_first<false>(p, own_request(p));
+        unsigned share = 0x7fffffffu;
+        if (p.parts) share = find_share(p, own, [&](const KvRequest &q) { return static_cast<float>(few_tiles(p, q)) * static_cast<float>(key_tiles(q.length)); });
+        KvFound at;
+        const bool is = find_request(p, own, unit / p.kv_heads, p.units / p.kv_heads, [&](const KvRequest &q) { return few_tiles(p, q) * parts_of(q, share); },
+                                     [&](const KvRequest &q) { return few_tiles(p, q); }, &at);
+        if (lane == 0) {
+            found = at;
+            found_share = is ? share : 0;
+        }
+    }
+    __syncthreads();
+    const unsigned share = __builtin_amdgcn_readfirstlane(found_share);
+    if (share == 0) return;
+    const KvFound at = uniform(found);
     const unsigned parts = parts_of(at.of, share), part = at.offset % parts, own_share = share_of(at.of, share);
     const unsigned column_tile = at.offset / parts;
     const int first = static_cast<int>(column_tile) * kKvColumns, columns = min(kKvColumns, at.of.rows * p.group - first);
@@ -586,6 +637,26 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
     if (!is_last) return;
 
     auto place = [&](unsigned of_part, int c) { return (static_cast<size_t>(unit) + (static_cast<size_t>(of_part) - part) * p.kv_heads) * kKvColumns + c; };
+    // Sixteen bytes a thread; where there are fewer columns than rows of threads, several rows share a column's parts.  A thread asks for its
+    // first parts before their factors are known: what this takes is one memory latency after the other.
+    constexpr int LANES = HD / 4, ROWS = 256 / LANES, AHEAD = 16;
+    const int across = min(ROWS, columns > 8 ? 16 : columns > 4 ? 8 : columns > 2 ? 4 : columns);
+    const int d = tid % LANES * 4, thread_row = tid / LANES, slices = ROWS / across, mine = thread_row / across;
+    float2 low[AHEAD], high[AHEAD];
+    auto ask = [&](int c, unsigned from) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const unsigned of_part = from + i * slices;
+            low[i] = high[i] = float2{0.0f, 0.0f};
+            if (c < columns && of_part < parts) {
+                const float *const at_part = p.parts + place(of_part, c) * HD + d;
+                low[i] = load_shared(at_part);
+                high[i] = load_shared(at_part + 2);
+            }
+        }
+    };
+    ask(thread_row % across, mine);
+
     float *const factors = lds_out;  // (parts, 16)
     static_assert(kKvMostParts * kKvColumns + 256 * 4 <= kKvFewFloats<64>, "factors and the threads' sums");
     constexpr int MINE = kKvMostParts / 16;
@@ -597,8 +668,9 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
         const unsigned of_part = slice + 16 * i;
         held[i] = float2{-INFINITY, 0.0f};
         if (of_part < parts && n < columns) held[i] = load_shared(statistics + 2 * place(of_part, n));
-        most = fmaxf(most, held[i].x);
     }
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) most = fmaxf(most, held[i].x);
     most = across_groups_max(most);
     if (g == 0) lds_max[wave][n] = most;
     __syncthreads();
@@ -614,20 +686,16 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
     sum = across_groups_sum(sum);
     if (g == 0) lds_sum[wave][n] = sum;
     __syncthreads();
-    // Sixteen bytes a thread; where there are fewer columns than rows of threads, several rows share a column's parts.
-    constexpr int LANES = HD / 4, ROWS = 256 / LANES;
-    const int across = min(ROWS, columns > 8 ? 16 : columns > 4 ? 8 : columns > 2 ? 4 : columns);
-    const int d = tid % LANES * 4, thread_row = tid / LANES, slices = ROWS / across, mine = thread_row / across;
     f32x4 *const sums = reinterpret_cast<f32x4 *>(lds_out + kKvMostParts * kKvColumns);
     for (int c0 = 0; c0 < columns; c0 += across) {
         const int c = c0 + thread_row % across;
         f32x4 total = {0.f, 0.f, 0.f, 0.f};
-        if (c < columns) {
-#pragma unroll 4
-            for (unsigned of_part = mine; of_part < parts; of_part += slices) {
-                const float *const from = p.parts + place(of_part, c) * HD + d;
-                const float2 low = load_shared(from), high = load_shared(from + 2);
-                total += f32x4{low.x, low.y, high.x, high.y} * factors[of_part * kKvColumns + c];
+        for (unsigned from = mine; from < parts; from += AHEAD * slices) {
+            if (c0 != 0 || from != mine) ask(c, from);
+            if (c < columns) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i)
+                    if (from + i * slices < parts) total += f32x4{low[i].x, low[i].y, high[i].x, high[i].y} * factors[(from + i * slices) * kKvColumns + c];
             }
         }
         sums[tid] = total;
@@ -677,30 +745,57 @@ __device__ __forceinline__ int key_swizzle(int row)
     else return (row & 3) | (row >> 4 & 3) << 2;
 }
 
-#ifndef PF
-#define PF 2
-#endif
-template <int HD, int NC>
+template <int HD, int NC, bool CUT>
 __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned item, unsigned char *lds)
 {
     constexpr int WIDTH = 4 * 16 * NC, VT = HD / 16, KL = HD / 64, LOADS = kKvTile * HD / 4096;  // of 16 bytes, a thread, for keys and for values
+    constexpr int AHEAD = 2;  // pieces that are read before their use
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int kv_head = item % p.kv_heads;
-    KvFound at;
+    __shared__ KvFound found;
+    __shared__ unsigned found_share;
+    __shared__ bool is_last;
     auto tiles_of = [&](const KvRequest &q) {
         const int columns = q.rows * p.group;
         return columns > p.few ? (static_cast<unsigned>(columns) + WIDTH - 1) / WIDTH : 0;
     };
-    if (!find_request(p, longest_first(p, own_request(p)), item / p.kv_heads, p.wide / p.kv_heads, tiles_of, [](const KvRequest &) { return 0u; }, &at)) return;
+    if (wave == 0) {
+        const KvRequest own = longest_first<true>(p, own_request(p));
+        unsigned share = 0x7fffffffu;
+        if (CUT)  // (of the rows that see their own keys one by one, each sees half of them on average)
+            share = find_share(p, own, [&](const KvRequest &q) {
+                return static_cast<float>(tiles_of(q)) * (static_cast<float>(key_tiles(q.length)) - (p.causal ? 0.5f / kKvTile * min(q.rows, q.length) : 0.0f));
+            });
+        KvFound at;
+        const bool is = find_request(p, own, item / p.kv_heads, p.wide / p.kv_heads, [&](const KvRequest &q) { return tiles_of(q) * (CUT ? parts_of(q, share, kKvMostWideParts) : 1); },
+                                     tiles_of, &at);
+        if (lane == 0) {
+            found = at;
+            found_share = is ? share : 0;
+        }
+    }
+    __syncthreads();
+    const unsigned share = __builtin_amdgcn_readfirstlane(found_share);
+    if (share == 0) return;
+    const KvFound at = uniform(found);
     const KvRequest of = at.of;
     // (the last columns see the most keys: they come first)
-    const int columns = of.rows * p.group, block_first = static_cast<int>(tiles_of(of) - 1 - at.offset) * WIDTH, first = block_first + wave * 16 * NC;
+    const unsigned most_parts = CUT ? parts_of(of, share, kKvMostWideParts) : 1;
+    const unsigned part = at.offset % most_parts, column_tile = tiles_of(of) - 1 - at.offset / most_parts;
+    const int columns = of.rows * p.group, block_first = static_cast<int>(column_tile) * WIDTH, first = block_first + wave * 16 * NC;
+    const int last_column = min(columns, block_first + WIDTH) - 1;
+    unsigned tile_first = 0, end = key_tiles(p.causal ? max(0, of.length - of.rows + last_column / p.group + 1) : of.length), parts = 1;
+    if constexpr (CUT) {
+        const unsigned own_share = share_of(of, share, kKvMostWideParts);
+        parts = max(1u, (end + own_share - 1) / own_share);
+        if (part >= parts) return;  // (these columns see fewer keys than others of the request)
+        tile_first = part * own_share;
+        end = min(end, tile_first + own_share);
+    }
     KvColumnsState<HD, NC> s;
     begin_columns<HD, NC>(p, of, first, s);
-    const int last_column = min(columns, block_first + WIDTH) - 1;
-    const unsigned end = key_tiles(p.causal ? max(0, of.length - of.rows + last_column / p.group + 1) : of.length);
-    const unsigned own_end = first < columns ? key_tiles(s.keys) : 0;  // (behind the last column a wavefront helps with the loads)
+    const unsigned own_end = first < columns ? min(end, key_tiles(s.keys)) : 0;  // (behind the last column a wavefront helps with the loads)
     bf16x8 query[NC][2 * KL];
     load_queries<HD, NC>(p, of, kv_head, first, query);
 
@@ -766,13 +861,12 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
         const float scale_of_keys = *reinterpret_cast<const float *>(held + scale_at + 4 * (n >> 2));
         const float held_scale = *reinterpret_cast<const float *>(held + scale_at + 16 + 4 * g);
         const float scale_of_values = pages.fits >> g & 1 ? held_scale : 1.0f;
-        // Pieces are read PF ahead of their use.
         f32x4 scores[NC][4];
         auto key_piece = [&](int i) { return *reinterpret_cast<const u32x4 *>(held + key_at + 4 * (i / KL) * HD + ((4 * (i % KL) + g) ^ key_turn) * 16); };
         auto value_piece = [&](int t) { return *reinterpret_cast<const u32x4 *>(held + value_at + t * 1024); };
-        u32x4 ahead[PF];
+        u32x4 ahead[AHEAD];
 #pragma unroll
-        for (int i = 0; i < PF; ++i) ahead[i] = key_piece(i);
+        for (int i = 0; i < AHEAD; ++i) ahead[i] = key_piece(i);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -780,9 +874,9 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
 #pragma unroll
             for (int j = 0; j < KL; ++j) {
                 const int at = i * KL + j;
-                const u32x4 codes = ahead[at % PF];
-                if (at + PF < 4 * KL) ahead[at % PF] = key_piece(at + PF);
-                else ahead[at % PF] = value_piece(at + PF - 4 * KL);
+                const u32x4 codes = ahead[at % AHEAD];
+                if (at + AHEAD < 4 * KL) ahead[at % AHEAD] = key_piece(at + AHEAD);
+                else ahead[at % AHEAD] = value_piece(at + AHEAD - 4 * KL);
                 const bf16x8 low = widened(codes[0], codes[1], scale_of_keys), high = widened(codes[2], codes[3], scale_of_keys);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) scores[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(low, query[c][2 * j], scores[c][i], 0, 0, 0);
@@ -797,8 +891,8 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
         unsigned nan = 0;
 #pragma unroll
         for (int t = 0; t < VT; ++t) {
-            u32x4 codes = ahead[t % PF];
-            if (t + PF < VT) ahead[t % PF] = value_piece(t + PF);
+            u32x4 codes = ahead[t % AHEAD];
+            if (t + AHEAD < VT) ahead[t % AHEAD] = value_piece(t + AHEAD);
             if (!whole) nan |= drop_nan(codes);
             const bf16x8 low = widened(codes[0], codes[1], scale_of_values), high = widened(codes[2], codes[3], scale_of_values);
 #pragma unroll
@@ -808,12 +902,12 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
         }
         if (__any(nan != 0)) nan_first = min(nan_first, tile);
     };
-    if (end != 0) {
-        Pages pages = look_up(0), next = look_up(1), after = look_up(2);
+    if (tile_first < end) {
+        Pages pages = look_up(tile_first), next = look_up(tile_first + 1), after = look_up(tile_first + 2);
         unsigned char *now = lds, *soon = lds + kKvStageBytes<HD>, *then = lds + 2 * kKvStageBytes<HD>;
-        request(0, now, pages);
-        if (end > 1) request(1, soon, next);
-        for (unsigned tile = 0; tile < end; ++tile) {
+        request(tile_first, now, pages);
+        if (tile_first + 1 < end) request(tile_first + 1, soon, next);
+        for (unsigned tile = tile_first; tile < end; ++tile) {
             // This tile has landed in every wavefront's share of it, and everyone is done with the one before, whose stage is next.
             if (tile + 1 < end) KV_WAIT_LOADS(2 * LOADS + 1);
             else KV_WAIT_LOADS(0);
@@ -827,6 +921,54 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
         }
     }
     mark_nan<HD, NC>(p, of, kv_head, nan_first, own_end, 1, s);
+
+    // Parts lie as the lanes hold them, 8 bytes of each beside the next one's, and are put together by the last workgroup likewise.
+    if (CUT && parts > 1) {
+        const size_t all = static_cast<size_t>(p.wide) * WIDTH;
+        auto sums_at = [&](size_t unit, int c, int t, int half) {
+            return p.wide_parts + ((((unit * 4 + wave) * NC + c) * VT + t) * 2 + half) * 128 + 2 * lane;
+        };
+        auto statistics_at = [&](size_t unit, int c) { return p.wide_parts + all * HD + 2 * (unit * WIDTH + wave * 16 * NC + 16 * c + n); };
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int t = 0; t < VT; ++t) {
+                store_shared(sums_at(item, c, t, 0), float2{s.out[c][t][0], s.out[c][t][1]});
+                store_shared(sums_at(item, c, t, 1), float2{s.out[c][t][2], s.out[c][t][3]});
+            }
+            if (g == 0) store_shared(statistics_at(item, c), float2{s.run_max[c], s.sum[c][0]});
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) {
+            unsigned *const arrived = p.arrived + p.items + (static_cast<size_t>(at.before) + column_tile) * p.kv_heads + kv_head;
+            is_last = atomicAdd(arrived, 1u) == parts - 1;
+            if (is_last) atomicExch(arrived, 0u);
+        }
+        __syncthreads();
+        if (!is_last) return;
+        auto unit_of = [&](unsigned of_part) { return static_cast<size_t>(item) + (static_cast<size_t>(of_part) - part) * p.kv_heads; };
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float most = -INFINITY;
+            for (unsigned of_part = 0; of_part < parts; ++of_part) most = fmaxf(most, load_shared(statistics_at(unit_of(of_part), c)).x);
+            const float base = most == -INFINITY ? 0.0f : most;
+            s.sum[c][0] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < VT; ++t) s.out[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (unsigned of_part = 0; of_part < parts; ++of_part) {
+                const size_t unit = unit_of(of_part);
+                const float2 own = load_shared(statistics_at(unit, c));
+                const float factor = __builtin_amdgcn_exp2f(own.x - base);
+                s.sum[c][0] += own.y * factor;
+#pragma unroll
+                for (int t = 0; t < VT; ++t) {
+                    const float2 low = load_shared(sums_at(unit, c, t, 0)), high = load_shared(sums_at(unit, c, t, 1));
+                    s.out[c][t] += f32x4{low.x, low.y, high.x, high.y} * factor;
+                }
+            }
+        }
+    }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int column = first + 16 * c + n;
@@ -839,7 +981,7 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
 }
 
 template <int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : HD == 128 ? 3 : 2))) void kv_attention_few_kernel(KvAttentionArgs p)
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : HD == 128 ? 2 : 1, HD == 64 ? 4 : HD == 128 ? 2 : 1))) void kv_attention_few_kernel(KvAttentionArgs p)
 {
     __shared__ __attribute__((aligned(16))) float lds[kKvFewFloats<HD>];
     few_columns<HD>(p, blockIdx.x, lds);
@@ -848,52 +990,65 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 
 // Batches that may hold requests of either kind.
 template <int HD>
 constexpr int kKvWideTiles = HD == 64 ? 4 : 2;
-template <int HD>
+template <int HD, bool CUT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void kv_attention_mixed_kernel(KvAttentionArgs p)
 {
     constexpr size_t few = kKvFewFloats<HD> * sizeof(float), wide = kKvStages * kKvStageBytes<HD>;
     __shared__ __attribute__((aligned(16))) unsigned char lds[few > wide ? few : wide];
-    if (blockIdx.x < p.wide) many_columns<HD, kKvWideTiles<HD>>(p, blockIdx.x, lds);
+    if (blockIdx.x < p.wide) many_columns<HD, kKvWideTiles<HD>, CUT>(p, blockIdx.x, lds);
     else few_columns<HD>(p, blockIdx.x - p.wide, reinterpret_cast<float *>(lds));
 }
 
-// Requests of more columns go to wide tiles: keys and values are widened once for four or two times as many columns there, but a
-// context cannot be shared by several workgroups.
-constexpr int kKvFew = 32;
-// Workgroups that all contexts are cut over, beside one for each tile of columns.
-constexpr int kKvTarget = 512;
+// Requests of more columns than half a wide tile go to wide tiles: keys and values are widened once for four or two times as many columns
+// there.  Below that the wide tile's other wavefronts would have nothing to do.  (At 128 columns of head dimension 64, 4 contexts of 5000
+// keys: 60 us in wide tiles, 25 without.  At 64 columns, 16 contexts of 2000: 39 and 33 of dimension 128, 95 and 73 of 256.)
+template <int HD>
+constexpr int kKvFew = kKvWideTiles<HD> * 32;
+// Workgroups that all contexts are cut over, beside one for each tile of columns: as many as the chip holds at once of the kernel's registers
+// for 128 and 256 values.  (64 contexts of 16 to 8192 keys and eight heads took 45, 41, 41 and 46 us with 256, 384, 512 and 768 of them at
+// dimension 128, 24, 22 and 22 with 256, 512 and 1024 at 64; at 256, two heads, 30, 34 and 43.)
+template <int HD>
+constexpr int kKvTarget = HD == 256 ? 256 : 512;
 
 template <int HD>
 hipError_t launch_kv_attention(KvAttentionArgs args, hipStream_t stream)
 {
-    constexpr int WIDTH = 4 * 16 * kKvWideTiles<HD>;
+    constexpr long long WIDTH = 4 * 16 * kKvWideTiles<HD>;
     const long long columns = static_cast<long long>(args.rows) * args.group;
-    long long tiles = columns / kKvColumns + args.requests;  // of sixteen columns: each request has one that is not full
+    long long tiles = columns / kKvColumns + args.requests, wide_tiles = 0;  // of sixteen columns: each request has one that is not full
     args.few = 0x7fffffff;
-    if (static_cast<long long>(args.rows - args.requests) * args.group > kKvFew) {
-        args.few = kKvFew;
+    if (static_cast<long long>(args.rows - args.requests) * args.group > kKvFew<HD>) {
+        args.few = kKvFew<HD>;
         // Requests that are wide have more than `few` columns: so many at the most.
-        args.wide = static_cast<unsigned>((columns / WIDTH + std::min<long long>(args.requests, columns / (args.few + 1))) * args.kv_heads);
+        wide_tiles = columns / WIDTH + std::min<long long>(args.requests, columns / (args.few + 1));
         tiles = std::min<long long>(tiles, static_cast<long long>(args.requests) * ((args.few + kKvColumns - 1) / kKvColumns));
     }
-    const long long items = tiles * args.kv_heads;
-    args.heads_by_target = static_cast<float>(args.kv_heads) / kKvTarget;
-    long long units = items;
-    if (items <= 4096 && (args.table_width << args.page_shift) > kKvLeastShare * kKvTile) {
-        units = items + kKvTarget;
+    const long long items = tiles * args.kv_heads, wide_items = wide_tiles * args.kv_heads;
+    args.items = static_cast<unsigned>(items);
+    args.heads_by_target = static_cast<float>(args.kv_heads) / kKvTarget<HD>;
+    // Contexts are cut where there may be too few tiles of columns for the chip.
+    const bool cuts = (args.table_width << args.page_shift) > kKvLeastShare * kKvTile;
+    const bool cut = cuts && items <= 4096, wide_cut = cuts && wide_items != 0 && wide_items <= kKvTarget<HD>;
+    long long units = items + (cut ? kKvTarget<HD> : 0), wide_units = wide_items + (wide_cut ? 2 * kKvTarget<HD> : 0);
+    if (cut || wide_cut) {
+        const size_t floats = cut ? static_cast<size_t>(units) * kKvColumns * (HD + 2) : 0;
         void *scratch = nullptr;
-        hipError_t rc = stream_workspace(stream, static_cast<size_t>(units) * kKvColumns * (HD + 2) * sizeof(float), &scratch);
-        if (rc == hipSuccess) rc = stream_counters(stream, static_cast<size_t>(items), &args.arrived);
+        hipError_t rc = stream_workspace(stream, (floats + (wide_cut ? static_cast<size_t>(wide_units) * WIDTH * (HD + 2) : 0)) * sizeof(float), &scratch);
+        if (rc == hipSuccess) rc = stream_counters(stream, static_cast<size_t>(items + wide_items), &args.arrived);
         if (rc == hipSuccess) {
-            args.parts = static_cast<float *>(scratch);
+            if (cut) args.parts = static_cast<float *>(scratch);
+            if (wide_cut) args.wide_parts = static_cast<float *>(scratch) + floats;
         } else if (scratch_unavailable(rc)) {
             units = items;
+            wide_units = wide_items;
         } else {
             return rc;
         }
     }
     args.units = static_cast<unsigned>(units);
-    if (args.wide) kv_attention_mixed_kernel<HD><<<args.wide + args.units, 256, 0, stream>>>(args);
+    args.wide = static_cast<unsigned>(wide_units);
+    if (args.wide_parts) kv_attention_mixed_kernel<HD, true><<<args.wide + args.units, 256, 0, stream>>>(args);
+    else if (args.wide) kv_attention_mixed_kernel<HD, false><<<args.wide + args.units, 256, 0, stream>>>(args);
     else kv_attention_few_kernel<HD><<<args.units, 256, 0, stream>>>(args);
     return hipGetLastError();
 }

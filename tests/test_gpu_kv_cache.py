@@ -284,6 +284,16 @@ def test_long_contexts(hip, page, dim, kv_heads, group, length, fresh):
     check_attention(hip, rng, page, kv_heads, dim, group, [length // 3, 70], [fresh, 1], False, width=20000 // page)
 
 
+@pytest.mark.parametrize("page,dim,kv_heads,group,lengths,fresh", [(64, 128, 1, 4, [2000, 130, 900, 0], [100, 70, 1, 40]), (16, 64, 2, 3, [1500, 64], [333, 50]),
+                                                                   (128, 256, 1, 2, [1111, 2100], [200, 80]), (32, 128, 2, 1, [700, 1900], [700, 150]),
+                                                                   (64, 64, 8, 1, [4096], [4096])])
+def test_long_prompts(hip, page, dim, kv_heads, group, lengths, fresh):
+    """Many rows of few requests, whose contexts are shared by several workgroups though rows have tiles of their own."""
+    rng = np.random.default_rng(sum(lengths))
+    for causal in (True, False) if max(fresh) < 1000 else (True,):
+        check_attention(hip, rng, page, kv_heads, dim, group, lengths, fresh, causal)
+
+
 def test_rows_without_keys(hip):
     """More rows than tokens: the first see none, and are 0; requests of no length, of a negative one."""
     rng = np.random.default_rng(1)
@@ -503,5 +513,58 @@ def test_serving_from_a_graph(hip):
             other.check(f"eager {i}")
     finally:
         del graph
+        hip.release_scratch(stream.cuda_stream)
+        hip.release_scratch(None)
+
+
+@pytest.mark.parametrize("rows", [1, 90])
+def test_contexts_of_a_graph(hip, rows):
+    """Two recorded calls of one stream, of different sizes, replayed in turn over contexts that one workgroup takes and that several share,
+    with eager calls between."""
+    import torch
+    rng = np.random.default_rng(rows)
+    dim, kv_heads, group, page = 64, 2, 2, 64
+    heads, width = kv_heads * group, 40
+    store = Pages(hip, rng, 100, page, kv_heads, dim)
+    requests = [3, 2]
+    tables = [rng.permutation(100)[:r * width].reshape(r, width) for r in (2, 2)]
+    tables = [np.concatenate([tables[0], tables[0][:1]]), tables[1]]
+    offsets = [np.arange(r + 1) * rows for r in requests]
+    q_bits = [inputs.to_bf16(rng.normal(size=(r * rows, heads * dim)).astype(np.float32)) for r in requests]
+    d_offsets, d_tables, d_q = ([dev(hip, a) for a in offsets], [dev(hip, a) for a in tables], [hip.DeviceBuffer.from_array(a) for a in q_bits])
+    d_lengths = [dev(hip, np.zeros(r)) for r in requests]
+    outs = [hip.DeviceBuffer(r * rows * heads * dim * 2) for r in requests]
+
+    def call(i, stream=None):
+        hip.attention_kv_cache_bf16_dev(store.cache, requests[i], requests[i] * rows, heads, 0.125, True, d_offsets[i], d_lengths[i], d_tables[i], width,
+                                        d_q[i], heads * dim, outs[i], heads * dim, stream=stream)
+
+    def check(i, lengths, what):
+        want, mine, bound = plain.attention(store.k, store.v, store.k_scales, store.v_scales, offsets[i], lengths, tables[i],
+                                            inputs.from_bf16(q_bits[i].ravel()).astype(np.float64).reshape(-1, heads, dim), 0.125, True)
+        got = inputs.from_bf16(outs[i].to_array(np.uint16, requests[i] * rows * heads * dim)).reshape(-1, heads, dim)
+        assert mine.all() and (np.abs(got - want) <= bound).all(), what
+
+    graphs, stream = [torch.cuda.CUDAGraph() for _ in requests], torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph, stream=stream):
+            call(i, torch.cuda.current_stream().cuda_stream)
+    try:
+        for lengths in ([2560, 700, 3], [1, 0, 2], [64, 2560, 2500], [2000, 2000, 2000]):
+            for i, r in enumerate(requests):
+                d_lengths[i].upload(np.array(lengths[:r], np.int32))
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                for graph in graphs * 2:
+                    graph.replay()
+            torch.cuda.synchronize()
+            for i, r in enumerate(requests):
+                check(i, lengths[:r], f"replay of {i}, {lengths}")
+                call(i)
+                hip.device_synchronize()
+                check(i, lengths[:r], f"eager {i}, {lengths}")
+    finally:
+        del graphs, graph
         hip.release_scratch(stream.cuda_stream)
         hip.release_scratch(None)
