@@ -89,22 +89,8 @@ __device__ __forceinline__ unsigned parts_of(const KvRequest &q, unsigned share,
     return max(1u, (key_tiles(q.length) + mine - 1) / mine);
 }
 
-// `of(x, y)` over the lanes up to and with this one, where of(x, 0) is x.
-template <class Of>
-__device__ __forceinline__ unsigned wave_scan(unsigned v, Of &&of)
-{
-    auto shifted = [](unsigned x, auto control, auto rows) {
-        return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(control)::value, decltype(rows)::value, 0xf, false));
-    };
-    using All = std::integral_constant<int, 0xf>;
-    v = of(v, shifted(v, std::integral_constant<int, 0x111>{}, All{}));  // within rows of sixteen: from 1, 2, 4 and 8 lanes before
-    v = of(v, shifted(v, std::integral_constant<int, 0x112>{}, All{}));
-    v = of(v, shifted(v, std::integral_constant<int, 0x114>{}, All{}));
-    v = of(v, shifted(v, std::integral_constant<int, 0x118>{}, All{}));
-    v = of(v, shifted(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}));  // the last of a row to the next one, in rows 1 and 3
-    return of(v, shifted(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}));  // lane 31 to rows 2 and 3
-}
-__device__ __forceinline__ unsigned wave_scan(unsigned v)
+// Sum over the lanes up to and with this one.
+__device__ __forceinline__ unsigned wave_scan_sum(unsigned v)
 {
     return wave_scan(v, [](unsigned x, unsigned y) { return x + y; });
 }
@@ -141,7 +127,7 @@ __device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvR
                 others += other(q);
             }
         }
-        const unsigned to = wave_scan(items), to_other = wave_scan(others);
+        const unsigned to = wave_scan_sum(items), to_other = wave_scan_sum(others);
         const unsigned long long behind = __ballot(items_before + to > item);
         if (behind == 0 || (left == p.requests && __builtin_amdgcn_readlane(to, 63) > most)) return false;
         const int which = __builtin_ctzll(behind);

@@ -97,6 +97,22 @@ __device__ __forceinline__ float wave_sum(float v)
     return v;
 }
 
+// `of(x, y)` over the lanes up to and with this one, where of(x, 0) is x.
+template <class Of>
+__device__ __forceinline__ unsigned wave_scan(unsigned v, Of &&of)
+{
+    auto shifted = [](unsigned x, auto control, auto rows) {
+        return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(control)::value, decltype(rows)::value, 0xf, false));
+    };
+    using All = std::integral_constant<int, 0xf>;
+    v = of(v, shifted(v, std::integral_constant<int, 0x111>{}, All{}));  // within rows of sixteen: from 1, 2, 4 and 8 lanes before
+    v = of(v, shifted(v, std::integral_constant<int, 0x112>{}, All{}));
+    v = of(v, shifted(v, std::integral_constant<int, 0x114>{}, All{}));
+    v = of(v, shifted(v, std::integral_constant<int, 0x118>{}, All{}));
+    v = of(v, shifted(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}));  // the last of a row to the next one, in rows 1 and 3
+    return of(v, shifted(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}));  // lane 31 to rows 2 and 3
+}
+
 // The normalisation of a row whose sum and sum of squares are known.
 struct LayerNormRow {
     float mean, denom, inv;

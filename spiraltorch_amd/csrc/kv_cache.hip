@@ -149,24 +149,26 @@ __device__ __forceinline__ float needed_scale(float largest)
     return __uint_as_float(static_cast<unsigned>(max(exponent, -118) + 127) << 23);
 }
 
-// What e4m3 cannot hold (infinities, NaN; nothing else is above 448 after scaling) becomes NaN.
-__device__ __forceinline__ float e4m3_or_nan(float x) { return fabsf(x) <= 448.0f ? x : NAN; }
-__device__ __forceinline__ unsigned e4m3_pair(float a, float b, unsigned old, std::bool_constant<false>)
+// Codes of four values over a power of two, none of them above 448 times it; infinities go in as NaN.
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned e4m3_four(float a, float b, float c, float d, float scale)
 {
-    return __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_or_nan(a), e4m3_or_nan(b), old, false);
+    s16x2 codes = {0, 0};
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(codes, a, b, scale, false);
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(codes, c, d, scale, true));
 }
-__device__ __forceinline__ unsigned e4m3_pair(float a, float b, unsigned old, std::bool_constant<true>)
+__device__ __forceinline__ unsigned e4m3_four(unsigned low, unsigned high, float scale)  // of bf16 pairs
 {
-    return __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_or_nan(a), e4m3_or_nan(b), old, true);
-}
-__device__ __forceinline__ unsigned e4m3_four(float a, float b, float c, float d)
-{
-    return e4m3_pair(c, d, e4m3_pair(a, b, 0, std::false_type{}), std::true_type{});
+    s16x2 codes = {0, 0};
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(codes, __builtin_bit_cast(bf16x2, low), scale, false);
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(codes, __builtin_bit_cast(bf16x2, high), scale, true));
 }
 __device__ __forceinline__ unsigned rescaled_four(unsigned codes, float ratio)
 {
     const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
-    return e4m3_four(low[0] * ratio, low[1] * ratio, high[0] * ratio, high[1] * ratio);
+    return e4m3_four(low[0] * ratio, low[1] * ratio, high[0] * ratio, high[1] * ratio, 1.0f);
 }
 
 struct AppendArgs {
@@ -181,17 +183,51 @@ struct AppendArgs {
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendMostPage = 256;  // tokens of the largest page
+static_assert(kAppendMostPage <= kAppendThreads, "a place for each thread");
 constexpr int kAppendMostRows = 64;   // that a workgroup looks at for the beginnings of pages
 
 // Eight neighbouring values of a row, as they are.
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
 struct Eight {
     u32x4 raw[sizeof(T) / 2];
-    __device__ __forceinline__ float at(int i) const
+    // The sizes' bits, as an unsigned number as large as they are; of bf16 two at a time.
+    __device__ __forceinline__ void widen(unsigned &largest) const
     {
-        if constexpr (sizeof(T) == 4) return __uint_as_float(raw[i >> 2][i & 3]);
-        else return __uint_as_float(i & 1 ? raw[0][i >> 1] & 0xffff0000u : raw[0][i >> 1] << 16);
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(T) * 2; ++i) {
+            const unsigned bits = raw[i >> 2][i & 3];
+            if constexpr (sizeof(T) == 4) {
+                largest = max(largest, bits & 0x7fffffffu);
+            } else {
+                typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+                largest = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, largest), __builtin_bit_cast(u16x2, bits & 0x7fff7fffu)));
+            }
+        }
+    }
+    // What e4m3 cannot hold, infinities and NaN, as another value (its bits).
+    __device__ __forceinline__ void replace(unsigned with)
+    {
+        constexpr unsigned all = sizeof(T) == 4 ? 0x7f800000u : 0x7f80u;
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(T) * 2; ++i) {
+            unsigned bits = raw[i >> 2][i & 3];
+            if constexpr (sizeof(T) == 4) {
+                if ((bits & all) == all) bits = with;
+            } else {
+                if ((bits & all) == all) bits = (bits & 0xffff0000u) | with;
+                if ((bits >> 16 & all) == all) bits = (bits & 0xffffu) | with << 16;
+            }
+            raw[i >> 2][i & 3] = bits;
+        }
+    }
+    __device__ __forceinline__ unsigned codes(int half, float scale) const
+    {
+        if constexpr (sizeof(T) == 4) {
+            const u32x4 x = raw[half];
+            return e4m3_four(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3]), scale);
+        } else {
+            return e4m3_four(raw[0][2 * half], raw[0][2 * half + 1], scale);
+        }
     }
 };
 template <bool VECTOR, typename T>
@@ -211,26 +247,29 @@ __device__ __forceinline__ Eight<T> load_eight(const T *at)
     return x;
 }
 
-// A workgroup takes pages that begin (in the order of the rows) within its 64 rows, for one head: its lower half the keys, its upper half
-// the values.  Where every row begins a page, as in a decode step, several workgroups share the rows' pages.  For every place of a
+// A workgroup takes pages that begin (in the order of the rows) within its 64 rows, for one head, and their keys or their values.  Where
+// every row begins a page, as in a decode step, several workgroups share the rows' pages.  For every place of a
 // page the last row that is for it is noted first; everything behind that goes by place, so that no two threads write the same.
 // A thread has eight values of four neighbouring places (of places a quarter of the page apart, for keys), so that both layouts are
 // read and written in runs: keys 8 bytes of a place at a time, 128 a row of lanes; values, which lie transposed, 4 bytes of a value at a
 // time, 64 in a page of 64.  Blocks of up to 8192 values (a page of 64 places and heads of 128 values) stay in registers between the
 // maximum and the rounding, larger ones are read again.  VECTOR: rows on 16-byte boundaries.
+// What bounds it is instructions and their latencies as much as memory: sizes are compared as integers, two of bf16 at a time, and values are
+// scaled and rounded by the instruction that makes two codes of them.  (8192 rows of bf16, 8 heads of 128 values, in pages of 64: 17.1 us,
+// 2.9 TB/s; 22.4 when each value was widened, compared and scaled by itself, 18.2 when a workgroup had both keys and values.)
 template <typename T, int HD, bool VECTOR>
-__global__ __launch_bounds__(2 * kAppendThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 6 : 4))) void kv_append_kernel(AppendArgs p)
+__global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
 {
     constexpr int RUNS = HD / 8;  // of eight values
     constexpr int WAVES = kAppendThreads / 64;
     __shared__ int owners[kAppendMostPage];
-    __shared__ float wave_largest[2 * WAVES];
+    __shared__ unsigned wave_largest[WAVES];
     __shared__ unsigned long long changes[WAVES], beginnings;
-    __shared__ int run_end;
-    const int tid = threadIdx.x & (kAppendThreads - 1), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ int run_end, pages[kAppendMostRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int page_size = 1 << p.page_shift, quarter = page_size >> 2;
-    const bool keys = __builtin_amdgcn_readfirstlane(threadIdx.x) < kAppendThreads;
-    const unsigned head = blockIdx.x % p.kv_heads, of_head = blockIdx.x / p.kv_heads;
+    const bool keys = (blockIdx.x & 1) == 0;
+    const unsigned head = blockIdx.x / 2 % p.kv_heads, of_head = blockIdx.x / 2 / p.kv_heads;
     const unsigned sharer = of_head & (p.sharers - 1);
     const int block_first = static_cast<int>(of_head / p.sharers) * kAppendMostRows;
     const T *const source = static_cast<const T *>(keys ? p.k : p.v) + static_cast<size_t>(head) * HD;
@@ -245,17 +284,17 @@ __global__ __launch_bounds__(2 * kAppendThreads) __attribute__((amdgpu_waves_per
     const int own_page = own_row < p.rows ? page_of(own_row) : -2, own_place = own_row < p.rows ? p.slots[own_row] & (page_size - 1) : 0;
     const bool change = own_row == 0 || (own_row <= p.rows ? page_of(own_row - 1) : -2) != own_page;
     const unsigned long long changed = __ballot(change), begun_here = __ballot(change && own_page >= 0);
-    if (lane == 0 && keys) {
+    if (lane == 0) {
         changes[wave] = changed;
         if (wave == 0) beginnings = begun_here;
     }
+    if (tid < kAppendMostRows) pages[tid] = own_page;
     __syncthreads();
     // Of the pages that begin here, this workgroup's: every sharers-th (a power of two).
     const unsigned long long all_begun = beginnings;
     const unsigned rank = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(all_begun >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(all_begun), 0));
     for (unsigned long long pending = __ballot((all_begun >> lane & 1) != 0 && (rank & (p.sharers - 1)) == sharer); pending != 0; pending &= pending - 1) {
-        const int which = __builtin_ctzll(pending), first = block_first + which;
-        const int page = page_of(first);
+        const int which = __builtin_ctzll(pending), page = __builtin_amdgcn_readfirstlane(pages[which]);
         int end = kAppendThreads;  // of the page's rows, among the 256
         for (int w = WAVES - 1; w >= 0; --w) {
             const unsigned long long later = w == 0 ? changes[0] & (~1ull << which) : changes[w];
@@ -264,10 +303,10 @@ __global__ __launch_bounds__(2 * kAppendThreads) __attribute__((amdgpu_waves_per
         const size_t block = static_cast<size_t>(page) * p.kv_heads + head;
         float *const scale_at = (keys ? p.k_scales : p.v_scales) + block;
         const float held = *scale_at;
-        for (int place = threadIdx.x; place < page_size; place += 2 * kAppendThreads) owners[place] = -1;
-        if (threadIdx.x == 0) run_end = p.rows;
+        if (tid < page_size) owners[tid] = -1;
+        if (tid == 0) run_end = p.rows;
         __syncthreads();
-        if (keys && tid >= which && tid < end) atomicMax(&owners[own_place], own_row);
+        if (tid >= which && tid < end) atomicMax(&owners[own_place], own_row);
         if (end == kAppendThreads) {  // repeated rows alone make a page's so many
             for (int at = block_first + kAppendThreads; at < p.rows; at += kAppendThreads) {
                 const int row = at + tid;
@@ -293,43 +332,51 @@ __global__ __launch_bounds__(2 * kAppendThreads) __attribute__((amdgpu_waves_per
                 if (rows[j] >= 0) x[j] = load_eight<VECTOR>(source + static_cast<size_t>(rows[j]) * p.ld + item_run(i) * 8);
             }
         };
-        float largest = 0.0f;
-        for (int i = tid; i < items; i += kAppendThreads) {
-            load(i);
+        // The largest size, by its bits; where a value is none, which its bits show, once more without those.
+        auto measure = [&](bool finite) {
+            unsigned sizes = 0;
+            for (int i = tid; i < items; i += kAppendThreads) {
+                load(i);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (rows[j] < 0) continue;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float size = fabsf(x[j].at(e));
-                    largest = fmaxf(largest, size < INFINITY ? size : 0.0f);
+                for (int j = 0; j < 4; ++j) {
+                    if (finite) x[j].replace(0);
+                    if (rows[j] >= 0) x[j].widen(sizes);
                 }
             }
+            if constexpr (sizeof(T) == 2) sizes = max(sizes << 16, sizes & 0xffff0000u);
+            sizes = wave_scan(sizes, [](unsigned a, unsigned b) { return max(a, b); });
+            if (lane == 63) wave_largest[wave] = sizes;
+            __syncthreads();
+        };
+        measure(false);
+        auto largest_of_all = [&] { return __builtin_amdgcn_readfirstlane(max(max(wave_largest[0], wave_largest[1]), max(wave_largest[2], wave_largest[3]))); };
+        unsigned largest = largest_of_all();
+        const bool special = largest >= 0x7f800000u;
+        if (special) {
+            __syncthreads();
+            measure(true);
+            largest = largest_of_all();
         }
-#pragma unroll
-        for (int step = 32; step > 0; step >>= 1) largest = fmaxf(largest, __shfl_xor(largest, step));
-        if (lane == 0) wave_largest[wave] = largest;
-        __syncthreads();
-        for (int w = 0; w < WAVES; ++w) largest = fmaxf(largest, wave_largest[(keys ? 0 : WAVES) + w]);
 
         const bool begun = owners[0] >= 0;
         const float before = begun ? 0.0f : held;
-        const float scale = fmaxf(before, needed_scale(largest));
+        const float scale = fmaxf(before, needed_scale(__uint_as_float(largest)));
         const bool grown = !begun && scale > before;
-        const float inverse = 1.0f / scale, ratio = before * inverse;
+        const float ratio = before / scale;
         uint8_t *const codes = (keys ? p.cache_k : p.cache_v) + (block << p.page_shift) * HD;
         for (int i = tid; i < items; i += kAppendThreads) {
-            if (items > kAppendThreads) load(i);
+            if (items > kAppendThreads || special) load(i);
+            if (special) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j].replace(sizeof(T) == 4 ? 0x7fc00000u : 0x7fc0u);
+            }
             const int d = item_run(i) * 8;
-            auto four = [&](int j, int h) {  // codes 4h .. 4h+3 of place j
-                return e4m3_four(x[j].at(4 * h) * inverse, x[j].at(4 * h + 1) * inverse, x[j].at(4 * h + 2) * inverse, x[j].at(4 * h + 3) * inverse);
-            };
             if (keys) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     uint2 *const to = reinterpret_cast<uint2 *>(codes + item_place(i, j) * HD + d);
                     if (rows[j] >= 0) {
-                        *to = uint2{four(j, 0), four(j, 1)};
+                        *to = uint2{x[j].codes(0, scale), x[j].codes(1, scale)};
                     } else if (grown) {
                         const uint2 old = *to;
                         *to = uint2{rescaled_four(old.x, ratio), rescaled_four(old.y, ratio)};
@@ -344,13 +391,16 @@ __global__ __launch_bounds__(2 * kAppendThreads) __attribute__((amdgpu_waves_per
             for (int h = 0; h < 2; ++h) {
                 unsigned codes_of[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) codes_of[j] = rows[j] >= 0 ? four(j, h) : 0;
+                for (int j = 0; j < 4; ++j) codes_of[j] = rows[j] >= 0 ? x[j].codes(h, scale) : 0;
+                // Bytes e of the four places: a word of value 4h + e.
+                const unsigned low_ab = __builtin_amdgcn_perm(codes_of[1], codes_of[0], 0x05010400u), high_ab = __builtin_amdgcn_perm(codes_of[1], codes_of[0], 0x07030602u);
+                const unsigned low_cd = __builtin_amdgcn_perm(codes_of[3], codes_of[2], 0x05010400u), high_cd = __builtin_amdgcn_perm(codes_of[3], codes_of[2], 0x07030602u);
+                const unsigned words[4] = {__builtin_amdgcn_perm(low_cd, low_ab, 0x05040100u), __builtin_amdgcn_perm(low_cd, low_ab, 0x07060302u),
+                                           __builtin_amdgcn_perm(high_cd, high_ab, 0x05040100u), __builtin_amdgcn_perm(high_cd, high_ab, 0x07060302u)};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     unsigned *const to = reinterpret_cast<unsigned *>(codes + (static_cast<size_t>(d + 4 * h + e) << p.page_shift) + item_place(i, 0));
-                    // Byte e of the four places' words.
-                    const unsigned pick = 0x0c0c0400u + 0x0101u * e;
-                    unsigned word = __builtin_amdgcn_perm(codes_of[1], codes_of[0], pick) | __builtin_amdgcn_perm(codes_of[3], codes_of[2], pick) << 16;
+                    unsigned word = words[e];
                     if (!all) {
                         const unsigned old = *to;
                         word = (word & mine) | ((grown ? rescaled_four(old, ratio) : old) & ~mine);
@@ -360,7 +410,7 @@ __global__ __launch_bounds__(2 * kAppendThreads) __attribute__((amdgpu_waves_per
             }
         }
         __syncthreads();  // everyone has read the scale, and the next page takes `owners`
-        if (tid == 0) *scale_at = scale;  // (the first thread of either half)
+        if (tid == 0) *scale_at = scale;
     }
 }
 
@@ -369,16 +419,16 @@ hipError_t launch_append(const st_hip_kv_cache &cache, size_t rows, const int32_
 {
     AppendArgs args{k, v, slots, cache.k, cache.v, cache.k_scales, cache.v_scales, static_cast<long long>(ld), static_cast<int>(rows),
                     static_cast<int>(cache.pages), __builtin_ctzll(cache.page_size), static_cast<int>(cache.kv_heads), 1};
-    const size_t blocks = (rows + kAppendMostRows - 1) / kAppendMostRows * cache.kv_heads;
-    // Up to 1024 workgroups, which the chip holds at about once, share the rows' pages (us for 77 single rows of 5 heads at 256, 512, 1024 and
-    // 2048: 14.9, 8.8, 6.4, 6.4; for 8192 rows of 16 prompts, whose 64 rows begin a page or two: 22.5, 22.5, 22.5, 25.6).
+    const size_t blocks = (rows + kAppendMostRows - 1) / kAppendMostRows * cache.kv_heads * 2;
+    // Up to 2048 workgroups, which the chip holds at once, share the rows' pages (us for 77 single rows of 5 heads at 1024, 2048 and
+    // 4096: 7.7, 5.6, 5.6; for 8192 rows of 16 prompts, whose 64 rows begin a page or two: 17.1, 17.1, 19.5).
     args.sharers = 1;
-    while (args.sharers < kAppendMostRows && args.sharers < rows && blocks * args.sharers * 2 <= 1024) args.sharers *= 2;
+    while (args.sharers < kAppendMostRows && args.sharers < rows && blocks * args.sharers * 2 <= 2048) args.sharers *= 2;
     const size_t grid = blocks * args.sharers;
     if (grid > 0x7fffffffu) return hipErrorInvalidValue;
     const bool aligned = ld * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
-    if (aligned) kv_append_kernel<T, HD, true><<<static_cast<unsigned>(grid), 2 * kAppendThreads, 0, stream>>>(args);
-    else kv_append_kernel<T, HD, false><<<static_cast<unsigned>(grid), 2 * kAppendThreads, 0, stream>>>(args);
+    if (aligned) kv_append_kernel<T, HD, true><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(args);
+    else kv_append_kernel<T, HD, false><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(args);
     return hipGetLastError();
 }
 
