@@ -803,7 +803,13 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
             pages.fits |= fits << i;
             return (fits ? page : 0) * p.kv_heads + kv_head;
         };
-        pages.block = Four<int>{one(0), one(1), one(2), one(3)};
+        if (p.page_shift >= 6) {
+            const int block = one(0);
+            pages.fits *= 15;
+            pages.block = Four<int>{block, block, block, block};
+        } else {
+            pages.block = Four<int>{one(0), one(1), one(2), one(3)};
+        }
         return pages;
     };
     // Where a thread's pieces stand: 16-byte loads of keys begin at a place of the wavefront's 16-key group, those of values at one of the
