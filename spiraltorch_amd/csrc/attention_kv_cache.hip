@@ -717,7 +717,7 @@ __device__ __forceinline__ T pick(T a, T b, T c, T d, int group)
 }
 template <typename T>
 __device__ __forceinline__ T pick(const Four<T> of, int group) { return pick(of.a, of.b, of.c, of.d, group); }
-constexpr int kKvStages = 3;
+constexpr int kKvStages = 4;
 template <int HD>
 constexpr int kKvStageBytes = 2 * kKvTile * HD + 4 * 256;
 
@@ -846,13 +846,13 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
     unsigned nan_first = own_end;  // see mark_nan
     // One tile from its stage, while the tile two behind it comes into another.  (That the two do not meet has to be said, or every read of
     // the one waits for all of the other.)
-    auto take_tile = [&](const unsigned char *__restrict held, unsigned char *__restrict coming, unsigned tile, const Pages &pages, const Pages &after) __attribute__((always_inline)) {
+    auto take_tile = [&](const unsigned char *__restrict held, unsigned char *__restrict coming, unsigned tile, int fits, const Pages &after) __attribute__((always_inline)) {
         if (tile + 2 < end) request(tile + 2, coming, after);
         if (tile >= own_end) return;
         const unsigned key0 = tile * kKvTile;
         const float scale_of_keys = *reinterpret_cast<const float *>(held + scale_at + 4 * (n >> 2));
         const float held_scale = *reinterpret_cast<const float *>(held + scale_at + 16 + 4 * g);
-        const float scale_of_values = pages.fits >> g & 1 ? held_scale : 1.0f;
+        const float scale_of_values = fits >> g & 1 ? held_scale : 1.0f;
         f32x4 scores[NC][4];
         auto key_piece = [&](int i) { return *reinterpret_cast<const u32x4 *>(held + key_at + 4 * (i / KL) * HD + ((4 * (i % KL) + g) ^ key_turn) * 16); };
         auto value_piece = [&](int t) { return *reinterpret_cast<const u32x4 *>(held + value_at + t * 1024); };
@@ -876,8 +876,8 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
                 for (int c = 0; c < NC; ++c) scores[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(high, query[c][2 * j + 1], scores[c][i], 0, 0, 0);
             }
         }
-        const bool whole = pages.fits == 15 && key0 + kKvTile <= static_cast<unsigned>(s.fewest);
-        if (!whole) hide_unseen<HD, NC>(s, key0, pages.fits >> g & 1, scores);
+        const bool whole = fits == 15 && key0 + kKvTile <= static_cast<unsigned>(s.fewest);
+        if (!whole) hide_unseen<HD, NC>(s, key0, fits >> g & 1, scores);
         bf16x8 weights[NC][2];
         weigh<HD, NC>(p, scores, s, weights);
         unsigned nan = 0;
@@ -895,21 +895,29 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
         if (__any(nan != 0)) nan_first = min(nan_first, tile);
     };
     if (tile_first < end) {
-        Pages pages = look_up(tile_first), next = look_up(tile_first + 1), after = look_up(tile_first + 2);
-        unsigned char *now = lds, *soon = lds + kKvStageBytes<HD>, *then = lds + 2 * kKvStageBytes<HD>;
-        request(tile_first, now, pages);
-        if (tile_first + 1 < end) request(tile_first + 1, soon, next);
-        for (unsigned tile = tile_first; tile < end; ++tile) {
-            // This tile has landed in every wavefront's share of it, and everyone is done with the one before, whose stage is next.
-            if (tile + 1 < end) KV_WAIT_LOADS(2 * LOADS + 1);
-            else KV_WAIT_LOADS(0);
+        // Two tiles at a time: the pair has landed in every wavefront's share of it, and everyone is done with the pair before, whose stages
+        // the next one's loads take.
+        int fits = 0, other_fits = 0;
+        auto begin = [&](unsigned tile, unsigned char *stage_at) {
+            const Pages pages = look_up(tile);
+            if (tile < end) request(tile, stage_at, pages);
+            return pages.fits;
+        };
+        unsigned char *now = lds, *then = lds + 2 * kKvStageBytes<HD>;
+        fits = begin(tile_first, now);
+        other_fits = begin(tile_first + 1, now + kKvStageBytes<HD>);
+        Pages next = look_up(tile_first + 2), after = look_up(tile_first + 3);
+        for (unsigned tile = tile_first; tile < end; tile += 2) {
+            KV_WAIT_LOADS(0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            take_tile(now, then, tile, pages, after);
-            pages = next, next = after, after = look_up(tile + 3);
+            take_tile(now, then, tile, fits, next);
+            take_tile(now + kKvStageBytes<HD>, then + kKvStageBytes<HD>, tile + 1, other_fits, after);
+            fits = next.fits, other_fits = after.fits;
+            next = look_up(tile + 4), after = look_up(tile + 5);
             unsigned char *const done = now;
-            now = soon, soon = then, then = done;
+            now = then, then = done;
         }
     }
     mark_nan<HD, NC>(p, of, kv_head, nan_first, own_end, 1, s);
