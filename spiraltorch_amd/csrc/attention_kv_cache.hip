@@ -336,7 +336,7 @@ __device__ __forceinline__ void weigh(const KvAttentionArgs &p, f32x4 (&scores)[
         grows |= most[c] > s.run_max[c] + 8.0f;
     }
     // The maximum may lag behind by a factor of 2^8: weights are that much larger then, and nothing has to be scaled for most tiles.
-    if (__any(grows)) {
+    if (__builtin_expect(__any(grows), 0)) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const float up = fmaxf(s.run_max[c], most[c]), shrink = up == s.run_max[c] ? 1.0f : __builtin_amdgcn_exp2f(s.run_max[c] - up);
@@ -877,7 +877,7 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
             }
         }
         const bool whole = fits == 15 && key0 + kKvTile <= static_cast<unsigned>(s.fewest);
-        if (!whole) hide_unseen<HD, NC>(s, key0, fits >> g & 1, scores);
+        if (__builtin_expect(!whole, 0)) hide_unseen<HD, NC>(s, key0, fits >> g & 1, scores);
         bf16x8 weights[NC][2];
         weigh<HD, NC>(p, scores, s, weights);
         unsigned nan = 0;
@@ -885,7 +885,7 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
         for (int t = 0; t < VT; ++t) {
             u32x4 codes = ahead[t % AHEAD];
             if (t + AHEAD < VT) ahead[t % AHEAD] = value_piece(t + AHEAD);
-            if (!whole) nan |= drop_nan(codes);
+            if (__builtin_expect(!whole, 0)) nan |= drop_nan(codes);
             const bf16x8 low = widened(codes[0], codes[1], scale_of_values), high = widened(codes[2], codes[3], scale_of_values);
 #pragma unroll
             for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(low, weights[c][0], s.out[c][t], 0, 0, 0);
