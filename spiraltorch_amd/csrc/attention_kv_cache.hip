@@ -23,9 +23,6 @@ namespace {
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
-// s_waitcnt vmcnt(n) alone.
-#define KV_WAIT_LOADS(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | (7 << 4) | (15 << 8) | ((((n) >> 4) & 3) << 14))
-
 struct KvAttentionArgs {
     const uint8_t *k, *v;
     const float *k_scales, *v_scales;
@@ -696,9 +693,15 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
 }
 
 // Many columns: each wavefront has 16 NC of its own, and the workgroup brings the keys and values that all of them read through LDS, as the
-// cache holds them, in a ring of stages that is filled two tiles ahead by loads that write LDS themselves: the wavefronts' registers
-// hold columns, and a tile is read from memory once for four of them.  A stage holds 64 keys' rows and the values' HD rows of 64
-// bytes; their 16-byte pieces are stored at places that keep the sixteen rows that a fragment reads on banks of their own.
+// cache holds them, in a ring of four stages: two tiles are worked on between barriers while loads that write LDS themselves fill the other
+// two stages.  The wavefronts' registers hold columns, and a tile is read from memory once for four of them.  A stage holds 64 keys' rows and
+// the values' HD rows of 64 bytes; their 16-byte pieces are stored at places that keep the sixteen rows that a fragment reads on banks of
+// their own.
+// What bounds this is the issue of vector instructions.  A tile of 64 keys and 32 columns of 128 values has 68 products, which take 8 cycles of it
+// each, and 343 others, 128 of them conversions of codes, at 5 cycles (exponentials 8.5): 2340 cycles, and the matrix cores' own 1088 hide among
+// them.  8 prompts of 500 rows over 1000 to 4000 keys, 32 heads on 8 of 128 values: 145 us, 0.86 PFLOP/s.  (Ways there: 158 us when each 16
+// keys' page was looked up for itself, 149 with a barrier for each tile.  Three wavefronts a SIMD: 180, for spilled registers; 48 columns a
+// wavefront: 143 to 157; priority to wavefronts within products: 143 to 147.)
 typedef __attribute__((address_space(3))) void *kv_lds_ptr;
 typedef __attribute__((address_space(1))) const void *kv_global_ptr;
 typedef __attribute__((address_space(4))) int kv_constant_int;
@@ -908,8 +911,7 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
         other_fits = begin(tile_first + 1, now + kKvStageBytes<HD>);
         Pages next = look_up(tile_first + 2), after = look_up(tile_first + 3);
         for (unsigned tile = tile_first; tile < end; tile += 2) {
-            KV_WAIT_LOADS(0);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             take_tile(now, then, tile, fits, next);
