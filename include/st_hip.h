@@ -547,7 +547,7 @@ int st_hip_rotary_bf16_dev(size_t rows, size_t sequence, size_t heads, size_t he
  * A page whose place 0 is among them begins anew.  Its scales become the smallest powers of two, at least 2^-118, with which the new
  * rows' largest finite values are at most 448; those of other pages grow to that where it is larger, and what the page held is then
  * rounded to the new scale (exact but for values below 2^-6 of the new scale).  Codes are rounded to nearest, ties to even; NaN and
- * infinities become NaN. */
+ * infinities become NaN.  The rows must not overlap the cache. */
 int st_hip_kv_cache_append_f32_dev(const st_hip_kv_cache *cache, size_t rows, const int32_t *slots, const float *k, const float *v,
                                    size_t ld, void *stream);
 int st_hip_kv_cache_append_bf16_dev(const st_hip_kv_cache *cache, size_t rows, const int32_t *slots, const uint16_t *k,

@@ -1036,7 +1036,7 @@ hipError_t launch_kv_attention(KvAttentionArgs args, hipStream_t stream)
         const size_t floats = cut ? static_cast<size_t>(units) * kKvColumns * (HD + 2) : 0;
         void *scratch = nullptr;
         hipError_t rc = stream_workspace(stream, (floats + (wide_cut ? static_cast<size_t>(wide_units) * WIDTH * (HD + 2) : 0)) * sizeof(float), &scratch);
-        if (rc == hipSuccess) rc = stream_counters(stream, static_cast<size_t>(items + wide_items), &args.arrived);
+        if (rc == hipSuccess) rc = stream_counters(stream, static_cast<size_t>(items + (wide_cut ? wide_items : 0)), &args.arrived);
         if (rc == hipSuccess) {
             if (cut) args.parts = static_cast<float *>(scratch);
             if (wide_cut) args.wide_parts = static_cast<float *>(scratch) + floats;

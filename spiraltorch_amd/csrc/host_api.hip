@@ -314,6 +314,13 @@ struct Extent {
     }
 };
 
+// Whether `rows` rows, `ld` values of `size` bytes apart, can be in memory at all.
+bool addressable(size_t rows, size_t ld, size_t size)
+{
+    size_t values = 0;
+    return checked_mul(rows, ld, &values) && values <= static_cast<size_t>(-1) / 2 / size;
+}
+
 // Whether rows of `width` values, `ld_a` and `ld_b` apart, share memory: columns of one matrix that do not meet share none.
 bool overlaps_except_columns(const void *a, size_t ld_a, const void *b, size_t ld_b, size_t rows, size_t width, size_t size)
 {
@@ -337,7 +344,8 @@ int check_rotary(size_t rows, size_t sequence, size_t heads, size_t head_dim, co
         (r->original_length > 0.0f && !(std::isfinite(r->low_turns) && std::isfinite(r->high_turns) && r->low_turns < r->high_turns)))
         return fail(ST_HIP_ERR_INVALID, "rotary scaling by parts needs low_turns < high_turns and a finite original_length");
     size_t width = 0, values = 0;
-    if (!checked_mul(heads, head_dim, &width) || !checked_mul(rows, width, &values)) return fail(ST_HIP_ERR_INVALID, "rotary dimensions overflow");
+    if (!checked_mul(heads, head_dim, &width) || !checked_mul(rows, width, &values) || !addressable(rows, ld_in, size) || !addressable(rows, ld_out, size))
+        return fail(ST_HIP_ERR_INVALID, "rotary dimensions overflow");
     if (head_dim > 1024) return fail(ST_HIP_ERR_UNSUPPORTED, "rotary head_dim %zu is above 1024", head_dim);
     if (rows > kMaxDim || width > kMaxDim || ld_in > kMaxDim || ld_out > kMaxDim || sequence > kMaxDim)
         return fail(ST_HIP_ERR_UNSUPPORTED, "rotary dimension exceeds i32");
@@ -363,22 +371,36 @@ int check_kv_cache(const st_hip_kv_cache *c)
     size_t blocks = 0, bytes = 0;
     if (!checked_mul(c->pages, c->kv_heads, &blocks) || !checked_mul(blocks, c->page_size * c->head_dim, &bytes))
         return fail(ST_HIP_ERR_INVALID, "kv cache dimensions overflow");
+    if (blocks > kMaxDim) return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache pages*kv_heads exceeds i32");
     if (!c->k || !c->v || !c->k_scales || !c->v_scales) return fail(ST_HIP_ERR_INVALID, "kv cache holds a null pointer");
     if (reinterpret_cast<uintptr_t>(c->k) % 16 != 0 || reinterpret_cast<uintptr_t>(c->v) % 16 != 0)
         return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache values must be 16-byte aligned");
     return ST_HIP_OK;
 }
 
+// Whether rows of `width` values, `ld` apart, share memory with the cache.
+bool meets_cache(const st_hip_kv_cache &c, const void *rows_at, size_t rows, size_t ld, size_t width, size_t size)
+{
+    const uintptr_t first = reinterpret_cast<uintptr_t>(rows_at), end = first + ((rows - 1) * ld + width) * size;
+    const size_t blocks = c.pages * c.kv_heads, bytes = blocks * c.page_size * c.head_dim;
+    auto meets = [&](const void *at, size_t held) {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(at);
+        return first < from + held && from < end;
+    };
+    return meets(c.k, bytes) || meets(c.v, bytes) || meets(c.k_scales, blocks * sizeof(float)) || meets(c.v_scales, blocks * sizeof(float));
+}
+
 int check_append(const st_hip_kv_cache *c, size_t rows, const int32_t *slots, const void *k, const void *v, size_t ld, size_t size)
 {
     ST_HIP_CHECK(check_kv_cache(c));
     const size_t width = c->kv_heads * c->head_dim;  // (below the cache's bytes)
-    size_t values = 0;
-    if (!checked_mul(rows, ld, &values) || values > static_cast<size_t>(-1) / size) return fail(ST_HIP_ERR_INVALID, "kv cache append dimensions overflow");
+    if (!addressable(rows, ld, size)) return fail(ST_HIP_ERR_INVALID, "kv cache append dimensions overflow");
     if (rows > kMaxDim - 256 || ld > kMaxDim || c->kv_heads > 65535) return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache append dimension exceeds the kernel's");
     if (rows == 0) return ST_HIP_OK;
     if (!slots || !k || !v) return fail(ST_HIP_ERR_INVALID, "kv cache append received a null pointer");
     if (ld < width) return fail(ST_HIP_ERR_INVALID, "kv cache append row stride %zu is smaller than kv_heads*head_dim=%zu", ld, width);
+    if (meets_cache(*c, k, rows, ld, width, size) || meets_cache(*c, v, rows, ld, width, size))
+        return fail(ST_HIP_ERR_INVALID, "kv cache append: the new rows overlap the cache");
     return ST_HIP_OK;
 }
 
@@ -1352,7 +1374,8 @@ int st_hip_attention_kv_cache_bf16_dev(const st_hip_kv_cache *cache, size_t requ
         return fail(ST_HIP_ERR_NONFINITE, "non-finite value encountered in scaled_dot_attention_scale: %g", static_cast<double>(scale));
     size_t width = 0, columns = 0, items = 0, entries = 0;
     if (!checked_mul(heads, cache->head_dim, &width) || !checked_mul(rows, heads, &columns) || !checked_mul(requests, cache->kv_heads, &items) ||
-        !checked_mul(requests, table_width, &entries) || entries > static_cast<size_t>(-1) / 8)
+        !checked_mul(requests, table_width, &entries) || entries > static_cast<size_t>(-1) / 8 || !addressable(rows, ld_q, sizeof(uint16_t)) ||
+        !addressable(rows, ld_out, sizeof(uint16_t)))
         return fail(ST_HIP_ERR_INVALID, "attention dimensions overflow");
     if (width > kMaxDim || columns > kMaxDim || items > kMaxDim / 2 || requests >= kMaxDim || table_width > kMaxDim || ld_q > kMaxDim || ld_out > kMaxDim)
         return fail(ST_HIP_ERR_UNSUPPORTED, "attention dimension exceeds i32");
@@ -1364,6 +1387,7 @@ int st_hip_attention_kv_cache_bf16_dev(const st_hip_kv_cache *cache, size_t requ
         return fail(ST_HIP_ERR_UNSUPPORTED, "attention over the cache needs ld_q %% 8 == 0, ld_out %% 4 == 0 and aligned buffers");
     if (overlaps_except_columns(q, ld_q, out, ld_out, rows, width, sizeof(uint16_t)))
         return fail(ST_HIP_ERR_INVALID, "attention output overlaps its queries");
+    if (meets_cache(*cache, out, rows, ld_out, width, sizeof(uint16_t))) return fail(ST_HIP_ERR_INVALID, "attention output overlaps the cache");
     return launch_status(launch_attention_kv_cache_bf16(*cache, requests, rows, heads, scale, causal != 0, row_offsets, lengths, page_table, table_width,
                                                         q, ld_q, out, ld_out, as_stream(stream)),
                          "attention launch");

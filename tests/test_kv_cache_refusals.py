@@ -81,6 +81,7 @@ def test_rotary(stub):
                     "rotary=hip.Rotary(64, original_length=0.0, low_turns=4.0, high_turns=4.0)": "taken",
                     "src=None": "invalid", "dst=None": "invalid", "ld_in=127": "invalid", "ld_out=127": "invalid",
                     "head_dim=1026, ld_in=4096, ld_out=4096": "unsupported", "rows=2**40": "unsupported", "rows=2**62": "invalid",
+                    "rows=2**31 - 1, ld_in=2**31 - 1": "invalid", "rows=2**31 - 1, ld_out=2**31 - 1": "invalid",
                     # overlaps: other strides, shifted, columns that meet and that do not
                     "dst=2*M, ld_out=256": "invalid", f"dst=2*M + {size}": "invalid",
                     f"ld_in=256, ld_out=256, dst=2*M + {128 * size}": "taken", f"ld_in=256, ld_out=256, dst=2*M + {127 * size}": "invalid",
@@ -91,14 +92,18 @@ def test_rotary(stub):
 
 CACHES = {"cache=cache(page=8)": "unsupported", "cache=cache(page=96)": "unsupported", "cache=cache(dim=32)": "unsupported", "cache=cache(dim=96)": "unsupported",
           "cache=cache(k=8 + M)": "unsupported", "cache=cache(v=4 + M)": "unsupported", "cache=cache(k=0)": "invalid", "cache=cache(vs=0)": "invalid",
-          "cache=cache(pages=2**31)": "unsupported", "cache=cache(heads=2**32)": "unsupported"}
+          "cache=cache(pages=2**31)": "unsupported", "cache=cache(heads=2**32)": "unsupported",
+          "cache=cache(pages=2**20, heads=2**12)": "unsupported"}
 
 
 def test_append(stub):
     for call in ("hip.kv_cache_append_f32_dev", "hip.kv_cache_append_bf16_dev"):
         base = "cache=cache(), rows=5, slots=1*M, k=2*M, v=3*M, ld=128"
         expected = {"": "taken", "ld=131, k=2*M + 2": "taken", "rows=0, slots=None, k=None, v=None": "taken", "slots=None": "invalid", "k=None": "invalid",
-                    "v=None": "invalid", "ld=127": "invalid", "rows=2**31": "unsupported", "ld=2**40": "unsupported", "rows=2**40, ld=2**40": "invalid", **CACHES}
+                    "v=None": "invalid", "ld=127": "invalid", "rows=2**31": "unsupported", "ld=2**40": "unsupported", "rows=2**40, ld=2**40": "invalid", "rows=2**31 - 300, ld=2**31 - 1": "invalid",
+                    # rows within the cache's 65536 bytes of keys or values, or its 64 of scales
+                    "k=16*M + 65532": "invalid", "k=16*M + 65536": "taken", "v=32*M": "invalid", "k=48*M - 8": "invalid", "v=64*M + 60": "invalid",
+                    "v=64*M + 64": "taken", **CACHES}
         assert answers(stub, call, base, expected) == list(expected.values())
 
 
@@ -112,7 +117,9 @@ def test_attention(stub):
                 "ld_q=255": "invalid", "ld_q=248": "invalid", "ld_out=252": "invalid", "ld_q=257": "unsupported", "ld_out=258": "unsupported",
                 "q=4*M + 8": "unsupported", "out=5*M + 4": "unsupported", "out=5*M + 8": "taken",
                 "rows=2**30": "unsupported", "rows=2**63": "invalid", "requests=2**31": "unsupported", "requests=2**62": "invalid",
-                "out=4*M": "invalid", "out=4*M + 512": "invalid", "ld_q=512, ld_out=512, out=4*M + 512": "taken", **CACHES}
+                "out=4*M": "invalid", "out=4*M + 512": "invalid", "ld_q=512, ld_out=512, out=4*M + 512": "taken",
+                "rows=2**29 - 1, heads=4, ld_q=2**31 - 8, ld_out=2**31 - 4": "invalid", "out=16*M + 65528": "invalid", "out=16*M + 65536": "taken",
+                "out=32*M - 8": "invalid", "out=64*M": "invalid", **CACHES}
     assert answers(stub, "hip.attention_kv_cache_bf16_dev", base, expected) == list(expected.values())
 
 
@@ -125,6 +132,13 @@ for fail in (1, 0):
     print(launches.value - before, grid.value)
 """)
     assert out[:2] == ["1", "2"] and out[2] == "1" and int(out[3]) > 2
+    out = run(stub, """
+for fail in (1, 0):
+    no_memory.value = fail
+    hip.attention_kv_cache_bf16_dev(cache(pages=4000), 1, 300, 4, 0.1, True, M, 2 * M, 3 * M, 2000, 4 * M, 256, 5 * M, 256)
+    print(grid.value)
+""")
+    assert out[0] == "22" and int(out[1]) > 22  # eight narrow tiles of columns and three wide ones, of two heads
 
 
 def test_null_structures():
