@@ -396,15 +396,16 @@ def test_a_page_beyond_32_bits(hip):
     hip.kv_cache_append_bf16_dev(store, 100, dev(hip, slots), d_k, d_v, heads * dim)
     plain.append(host_k, scales[0], np.arange(100), values[0], False)
     plain.append(host_v, scales[1], np.arange(100), values[1], True)
-    q_bits = inputs.to_bf16(rng.normal(size=(2, heads * dim)).astype(np.float32))
-    out = hip.DeviceBuffer(2 * heads * dim * 2)
-    hip.attention_kv_cache_bf16_dev(store, 1, 2, heads, 1 / 16, True, dev(hip, [0, 2]), dev(hip, [100]), dev(hip, [[last]]), 1,
-                                    hip.DeviceBuffer.from_array(q_bits), heads * dim, out, heads * dim)
-    hip.device_synchronize()
-    q = inputs.from_bf16(q_bits.ravel()).astype(np.float64).reshape(2, heads, dim)
-    want, _, bound = plain.attention(host_k, host_v, *scales, [0, 2], [100], np.array([[0]]), q, 1 / 16, True)
-    got = inputs.from_bf16(out.to_array(np.uint16, 2 * heads * dim)).reshape(2, heads, dim)
-    assert (np.abs(got - want) <= bound).all()
+    for n in (2, 100):  # a narrow tile of columns, and a wide one
+        q_bits = inputs.to_bf16(rng.normal(size=(n, heads * dim)).astype(np.float32))
+        out = hip.DeviceBuffer(n * heads * dim * 2)
+        hip.attention_kv_cache_bf16_dev(store, 1, n, heads, 1 / 16, True, dev(hip, [0, n]), dev(hip, [100]), dev(hip, [[last]]), 1,
+                                        hip.DeviceBuffer.from_array(q_bits), heads * dim, out, heads * dim)
+        hip.device_synchronize()
+        q = inputs.from_bf16(q_bits.ravel()).astype(np.float64).reshape(n, heads, dim)
+        want, _, bound = plain.attention(host_k, host_v, *scales, [0, n], [100], np.array([[0]]), q, 1 / 16, True)
+        got = inputs.from_bf16(out.to_array(np.uint16, n * heads * dim)).reshape(n, heads, dim)
+        assert (np.abs(got - want) <= bound).all(), n
 
 
 # ---- a run of them together -------------------------------------------------------------------------------------------------------
@@ -568,3 +569,51 @@ def test_contexts_of_a_graph(hip, rows):
         del graphs, graph
         hip.release_scratch(stream.cuda_stream)
         hip.release_scratch(None)
+
+
+def test_two_streams_from_two_threads(hip):
+    """Steps on two streams at once, each from a thread of its own, with contexts that several workgroups share: nothing of theirs meets."""
+    import threading
+    rng = np.random.default_rng(21)
+    dim, kv_heads, group, page, width = 128, 2, 4, 64, 60
+    heads = kv_heads * group
+    store = Pages(hip, rng, 150, page, kv_heads, dim)
+    works, errors = [], []
+    for rows, lengths in ((1, [3800, 100, 2000]), (40, [3000, 2500])):
+        n = len(lengths)
+        table = rng.integers(0, 150, (n, width))
+        q_bits = inputs.to_bf16(rng.normal(size=(n * rows, heads * dim)).astype(np.float32))
+        q = inputs.from_bf16(q_bits.ravel()).astype(np.float64).reshape(-1, heads, dim)
+        offsets = np.arange(n + 1) * rows
+        want = plain.attention(store.k, store.v, store.k_scales, store.v_scales, offsets, lengths, table, q, 0.09, True)
+        works.append((n, rows, hip.Stream(), [dev(hip, a) for a in (offsets, lengths, table)], hip.DeviceBuffer.from_array(q_bits),
+                      hip.DeviceBuffer(q_bits.nbytes), want))
+
+    def serve(n, rows, stream, d, d_q, out, want):
+        try:
+            for i in range(30):
+                hip.attention_kv_cache_bf16_dev(store.cache, n, n * rows, heads, 0.09, True, *d, width, d_q, heads * dim, out, heads * dim, stream=stream)
+                if i % 10 == 9:
+                    stream.synchronize()
+                    got = inputs.from_bf16(out.to_array(np.uint16, n * rows * heads * dim)).reshape(-1, heads, dim)
+                    assert (np.abs(got - want[0]) <= want[2]).all(), (rows, i)
+            hip.release_scratch(stream)
+        except BaseException as e:
+            errors.append(e)
+
+    hip.device_synchronize()
+    threads = [threading.Thread(target=serve, args=w) for w in works]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def test_the_same_twice(hip):
+    """Whichever workgroup puts a context's parts together, the bits are the same."""
+    rng = np.random.default_rng(22)
+    for rows, dim, page in ((1, 128, 64), (3, 256, 16), (80, 64, 32)):
+        lengths = [int(n) for n in rng.integers(600, 4000, 3)]
+        seeds = [check_attention(hip, np.random.default_rng(5), page, 2, dim, 2, lengths, [rows] * 3, True) for _ in range(4)]
+        assert all((s == seeds[0]).all() for s in seeds)
