@@ -181,9 +181,7 @@ struct AppendArgs {
     unsigned sharers;
 };
 
-constexpr int kAppendThreads = 256;
 constexpr int kAppendMostPage = 256;  // tokens of the largest page
-static_assert(kAppendMostPage <= kAppendThreads, "a place for each thread");
 constexpr int kAppendMostRows = 64;   // that a workgroup looks at for the beginnings of pages
 
 // Eight neighbouring values of a row, as they are.
@@ -253,15 +251,16 @@ __device__ __forceinline__ Eight<T> load_eight(const T *at)
 // A thread has eight values of four neighbouring places (of places a quarter of the page apart, for keys), so that both layouts are
 // read and written in runs: keys 8 bytes of a place at a time, 128 a row of lanes; values, which lie transposed, 4 bytes of a value at a
 // time, 64 in a page of 64.  Blocks of up to 8192 values (a page of 64 places and heads of 128 values) stay in registers between the
-// maximum and the rounding, larger ones are read again.  VECTOR: rows on 16-byte boundaries.
+// maximum and the rounding, larger ones are read again where threads have more than one such share.  VECTOR: rows on 16-byte boundaries.
 // What bounds it is instructions and their latencies as much as memory: sizes are compared as integers, two of bf16 at a time, and values are
 // scaled and rounded by the instruction that makes two codes of them.  (8192 rows of bf16, 8 heads of 128 values, in pages of 64: 17.1 us,
 // 2.9 TB/s; 22.4 when each value was widened, compared and scaled by itself, 18.2 when a workgroup had both keys and values.)
-template <typename T, int HD, bool VECTOR>
-__global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
+template <typename T, int HD, bool VECTOR, int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs p)
 {
     constexpr int RUNS = HD / 8;  // of eight values
-    constexpr int WAVES = kAppendThreads / 64;
+    constexpr int WAVES = THREADS / 64;
+    static_assert(kAppendMostPage <= THREADS, "a place for each thread");
     __shared__ int owners[kAppendMostPage];
     __shared__ unsigned wave_largest[WAVES];
     __shared__ unsigned long long changes[WAVES], beginnings;
@@ -279,7 +278,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
         const int page = slot < 0 ? -1 : slot >> p.page_shift;
         return page < p.pages ? page : -1;
     };
-    // The 256 rows from the block's first on, one a thread; where the page is another one than the row's before.
+    // The THREADS rows from the block's first on, one a thread; where the page is another one than the row's before.
     const int own_row = block_first + tid;
     const int own_page = own_row < p.rows ? page_of(own_row) : -2, own_place = own_row < p.rows ? p.slots[own_row] & (page_size - 1) : 0;
     const bool change = own_row == 0 || (own_row <= p.rows ? page_of(own_row - 1) : -2) != own_page;
@@ -295,7 +294,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
     const unsigned rank = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(all_begun >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(all_begun), 0));
     for (unsigned long long pending = __ballot((all_begun >> lane & 1) != 0 && (rank & (p.sharers - 1)) == sharer); pending != 0; pending &= pending - 1) {
         const int which = __builtin_ctzll(pending), page = __builtin_amdgcn_readfirstlane(pages[which]);
-        int end = kAppendThreads;  // of the page's rows, among the 256
+        int end = THREADS;  // of the page's rows, among those
         for (int w = WAVES - 1; w >= 0; --w) {
             const unsigned long long later = w == 0 ? changes[0] & (~1ull << which) : changes[w];
             if (later != 0) end = 64 * w + __builtin_ctzll(later);
@@ -307,14 +306,14 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
         if (tid == 0) run_end = p.rows;
         __syncthreads();
         if (tid >= which && tid < end) atomicMax(&owners[own_place], own_row);
-        if (end == kAppendThreads) {  // repeated rows alone make a page's so many
-            for (int at = block_first + kAppendThreads; at < p.rows; at += kAppendThreads) {
+        if (end == THREADS) {  // repeated rows alone make a page's so many
+            for (int at = block_first + THREADS; at < p.rows; at += THREADS) {
                 const int row = at + tid;
                 const bool mine = row < p.rows && page_of(row) == page;
                 if (!mine && row < p.rows) atomicMin(&run_end, row);
                 __syncthreads();
                 if (mine && row < run_end) atomicMax(&owners[p.slots[row] & (page_size - 1)], row);
-                if (run_end < at + kAppendThreads) break;
+                if (run_end < at + THREADS) break;
             }
         }
         __syncthreads();
@@ -335,7 +334,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
         // The largest size, by its bits; where a value is none, which its bits show, once more without those.
         auto measure = [&](bool finite) {
             unsigned sizes = 0;
-            for (int i = tid; i < items; i += kAppendThreads) {
+            for (int i = tid; i < items; i += THREADS) {
                 load(i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -349,7 +348,12 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
             __syncthreads();
         };
         measure(false);
-        auto largest_of_all = [&] { return __builtin_amdgcn_readfirstlane(max(max(wave_largest[0], wave_largest[1]), max(wave_largest[2], wave_largest[3]))); };
+        auto largest_of_all = [&] {
+            unsigned most = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) most = max(most, wave_largest[w]);
+            return __builtin_amdgcn_readfirstlane(most);
+        };
         unsigned largest = largest_of_all();
         const bool special = largest >= 0x7f800000u;
         if (special) {
@@ -364,8 +368,8 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs p)
         const bool grown = !begun && scale > before;
         const float ratio = before / scale;
         uint8_t *const codes = (keys ? p.cache_k : p.cache_v) + (block << p.page_shift) * HD;
-        for (int i = tid; i < items; i += kAppendThreads) {
-            if (items > kAppendThreads || special) load(i);
+        for (int i = tid; i < items; i += THREADS) {
+            if (items > THREADS || special) load(i);
             if (special) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j].replace(sizeof(T) == 4 ? 0x7fc00000u : 0x7fc0u);
@@ -419,16 +423,22 @@ hipError_t launch_append(const st_hip_kv_cache &cache, size_t rows, const int32_
 {
     AppendArgs args{k, v, slots, cache.k, cache.v, cache.k_scales, cache.v_scales, static_cast<long long>(ld), static_cast<int>(rows),
                     static_cast<int>(cache.pages), __builtin_ctzll(cache.page_size), static_cast<int>(cache.kv_heads), 1};
+    // A thread has 32 values at once; where a page has more than 256 threads do, it takes 512.  (us for 49 times 8 rows in pages of 256, 4 heads of
+    // 128 values: 28.4, 15.8 with 512 and 13.7 with 1024; 88 times 3 rows, 10 heads of 64 values: 25.0, 21.3 and 64.)
+    const bool large = cache.page_size * HD > 256 * 32;
     const size_t blocks = (rows + kAppendMostRows - 1) / kAppendMostRows * cache.kv_heads * 2;
-    // Up to 2048 workgroups, which the chip holds at once, share the rows' pages (us for 77 single rows of 5 heads at 1024, 2048 and
+    // Up to 2048 workgroups of four wavefronts, which the chip holds at once, share the rows' pages (us for 77 single rows of 5 heads at 1024, 2048 and
     // 4096: 7.7, 5.6, 5.6; for 8192 rows of 16 prompts, whose 64 rows begin a page or two: 17.1, 17.1, 19.5).
     args.sharers = 1;
-    while (args.sharers < kAppendMostRows && args.sharers < rows && blocks * args.sharers * 2 <= 2048) args.sharers *= 2;
+    while (args.sharers < kAppendMostRows && args.sharers < rows && blocks * args.sharers * 2 <= (large ? 1024u : 2048u)) args.sharers *= 2;
     const size_t grid = blocks * args.sharers;
     if (grid > 0x7fffffffu) return hipErrorInvalidValue;
     const bool aligned = ld * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0;
-    if (aligned) kv_append_kernel<T, HD, true><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(args);
-    else kv_append_kernel<T, HD, false><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(args);
+    const dim3 blocks_of(static_cast<unsigned>(grid));
+    if (large && aligned) kv_append_kernel<T, HD, true, 512><<<blocks_of, 512, 0, stream>>>(args);
+    else if (large) kv_append_kernel<T, HD, false, 512><<<blocks_of, 512, 0, stream>>>(args);
+    else if (aligned) kv_append_kernel<T, HD, true, 256><<<blocks_of, 256, 0, stream>>>(args);
+    else kv_append_kernel<T, HD, false, 256><<<blocks_of, 256, 0, stream>>>(args);
     return hipGetLastError();
 }
 

@@ -1,6 +1,7 @@
 // Rotary positions: the leading values of every head turn in pairs by an angle that grows with the row's position.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "device_math.h"
 #include "kernels.h"
@@ -48,10 +49,6 @@ __device__ __forceinline__ float2 turned(double turns, float magnitude, bool bac
     return float2{cosine * magnitude, (back ? -sine : sine) * magnitude};
 }
 
-__device__ __forceinline__ float load_one(const float *at) { return *at; }
-__device__ __forceinline__ float load_one(const uint16_t *at) { return __uint_as_float(static_cast<unsigned>(*at) << 16); }
-__device__ __forceinline__ void store_one(float *at, float x) { *at = x; }
-__device__ __forceinline__ void store_one(uint16_t *at, float x) { *at = f32_to_bf16_rne(x); }
 
 // cos and sin of the block's rows and all pairs, into LDS: (rows, pairs).
 __device__ __forceinline__ void fill_table(const RotaryArgs &p, int row_first, int block_rows, float2 *table)
@@ -63,64 +60,38 @@ __device__ __forceinline__ void fill_table(const RotaryArgs &p, int row_first, i
     }
 }
 
-// One pair a thread, of any stride and alignment.
-template <typename T>
-__global__ __launch_bounds__(kRotaryThreads) void rotary_pairs_kernel(RotaryArgs p)
-{
-    extern __shared__ __attribute__((aligned(16))) float2 rotary_lds[];
-    const int tid = threadIdx.x, half = p.half;
-    const int row_first = blockIdx.x / p.head_blocks * p.rows_per_block, block_rows = min(p.rows - row_first, p.rows_per_block);
-    const int head_first = blockIdx.x % p.head_blocks * p.heads_per_block, block_heads = min(p.heads - head_first, p.heads_per_block);
-    fill_table(p, row_first, block_rows, rotary_lds);
-    __syncthreads();
-    const int rest = p.copies ? p.head_dim - 2 * half : 0, units = half + rest;
-    const long long total = static_cast<long long>(block_rows) * block_heads * units;
-    for (long long i = tid; i < total; i += kRotaryThreads) {
-        const int unit = static_cast<int>(i % units);
-        const long long of = i / units;
-        const int head = head_first + static_cast<int>(of % block_heads), row = static_cast<int>(of / block_heads);
-        const T *const in = static_cast<const T *>(p.in) + (row_first + row) * p.ld_in + static_cast<long long>(head) * p.head_dim;
-        T *const out = static_cast<T *>(p.out) + (row_first + row) * p.ld_out + static_cast<long long>(head) * p.head_dim;
-        if (unit >= half) {
-            out[half + unit] = in[half + unit];
-            continue;
-        }
-        const int first = p.interleaved ? 2 * unit : unit, second = p.interleaved ? first + 1 : unit + half;
-        const float2 by = rotary_lds[row * half + unit];
-        const float a = load_one(in + first), b = load_one(in + second);
-        store_one(out + first, a * by.x - b * by.y);
-        store_one(out + second, a * by.y + b * by.x);
+// COUNT neighbouring values, up to 16 bytes, loaded and stored at once: words of two bf16 or one f32, or a single bf16.
+template <typename T, int COUNT>
+struct alignas(COUNT * sizeof(T)) Run {
+    static constexpr int WORDS = COUNT * sizeof(T) / 4;
+    std::conditional_t<WORDS == 0, uint16_t, uint32_t> word[WORDS == 0 ? 1 : WORDS];
+    __device__ __forceinline__ float at(int i) const
+    {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(word[i]);
+        else if constexpr (WORDS == 0) return __uint_as_float(static_cast<uint32_t>(word[0]) << 16);
+        else return __uint_as_float(i & 1 ? word[i >> 1] & 0xffff0000u : word[i >> 1] << 16);
     }
-}
-
-// Sixteen bytes of values.
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-template <typename T>
-constexpr int kRunValues = 16 / sizeof(T);
-template <typename T>
-__device__ __forceinline__ float run_at(const u32x4 &run, int i)
-{
-    if constexpr (sizeof(T) == 4) return __uint_as_float(run[i]);
-    else return __uint_as_float(i & 1 ? run[i >> 1] & 0xffff0000u : run[i >> 1] << 16);
-}
-template <typename T>
-__device__ __forceinline__ u32x4 run_of(const float (&values)[kRunValues<T>])
-{
-    u32x4 run;
+    static __device__ __forceinline__ Run of(const float (&values)[COUNT])
+    {
+        Run run;
+        if constexpr (WORDS == 0) {
+            run.word[0] = f32_to_bf16_rne(values[0]);
+        } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) run[i] = __float_as_uint(values[i]);
-        else run[i] = pack_bf16x2_rne(values[2 * i], values[2 * i + 1]);
+            for (int i = 0; i < WORDS; ++i) {
+                if constexpr (sizeof(T) == 4) run.word[i] = __float_as_uint(values[i]);
+                else run.word[i] = pack_bf16x2_rne(values[2 * i], values[2 * i + 1]);
+            }
+        }
+        return run;
     }
-    return run;
-}
+};
 
-// The same 32 bytes at a time, as many pairs as 16 bytes hold values: two runs half a rotary_dim apart, or beside each other.  A thread
-// has BATCH of them at once, and loads the first ones before the angles are worked out.
-template <typename T, bool INTERLEAVED, int BATCH>
+// COUNT pairs at a time: two runs half a rotary_dim apart, or beside each other.  A thread has BATCH of them at once, and loads the first
+// ones before the angles are worked out.
+template <typename T, int COUNT, bool INTERLEAVED, int BATCH>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_runs_kernel(RotaryArgs p)
 {
-    constexpr int COUNT = kRunValues<T>;
     extern __shared__ __attribute__((aligned(16))) float2 rotary_lds[];
     const int tid = threadIdx.x, half = p.half;
     const int row_first = blockIdx.x / p.head_blocks * p.rows_per_block, block_rows = min(p.rows - row_first, p.rows_per_block);
@@ -128,7 +99,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_runs_kernel(RotaryArgs 
     const int turning = half / COUNT, units = turning + (p.copies ? (p.head_dim - 2 * half) / COUNT : 0);
     const int total = block_rows * block_heads * units;  // (a block's share is small)
     const int second = INTERLEAVED ? COUNT : half;
-    u32x4 x[BATCH][2];
+    using Values = Run<T, COUNT>;
+    Values x[BATCH][2];
     struct Place {
         int unit, row;
         long long head, at;  // offsets within a row, and of the first run within the head
@@ -149,8 +121,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_runs_kernel(RotaryArgs 
             if (i < total) {
                 const Place w = place_of(i);
                 const T *const in = static_cast<const T *>(p.in) + (row_first + w.row) * p.ld_in + w.head + w.at;
-                x[b][0] = *reinterpret_cast<const u32x4 *>(in);
-                if (w.unit < turning) x[b][1] = *reinterpret_cast<const u32x4 *>(in + second);
+                x[b][0] = *reinterpret_cast<const Values *>(in);
+                if (w.unit < turning) x[b][1] = *reinterpret_cast<const Values *>(in + second);
             }
         }
     };
@@ -165,7 +137,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_runs_kernel(RotaryArgs 
             if (i < total) {
                 const Place w = place_of(i);
                 T *const out = static_cast<T *>(p.out) + (row_first + w.row) * p.ld_out + w.head + w.at;
-                u32x4 low = x[b][0];
+                Values low = x[b][0];
                 if (w.unit < turning) {
                     const float2 *const by = rotary_lds + w.row * half + w.unit * COUNT;
                     float values[2][COUNT];  // in the order in which the runs hold them
@@ -173,25 +145,27 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_runs_kernel(RotaryArgs 
                     for (int e = 0; e < COUNT; ++e) {
                         const float2 cs = by[e];
                         const int ra = INTERLEAVED ? 2 * e / COUNT : 0, ia = INTERLEAVED ? 2 * e % COUNT : e;
-                        const int rb = INTERLEAVED ? ra : 1, ib = INTERLEAVED ? ia + 1 : e;
-                        const float a = run_at<T>(x[b][ra], ia), c = run_at<T>(x[b][rb], ib);
+                        const int rb = INTERLEAVED ? (2 * e + 1) / COUNT : 1, ib = INTERLEAVED ? (2 * e + 1) % COUNT : e;
+                        const float a = x[b][ra].at(ia), c = x[b][rb].at(ib);
                         values[ra][ia] = a * cs.x - c * cs.y;
                         values[rb][ib] = a * cs.y + c * cs.x;
                     }
-                    low = run_of<T>(values[0]);
-                    *reinterpret_cast<u32x4 *>(out + second) = run_of<T>(values[1]);
+                    low = Values::of(values[0]);
+                    *reinterpret_cast<Values *>(out + second) = Values::of(values[1]);
                 }
-                *reinterpret_cast<u32x4 *>(out) = low;
+                *reinterpret_cast<Values *>(out) = low;
             }
         }
     }
 }
 
-template <typename T, int BATCH>
-void launch_runs(dim3 grid, size_t table, const RotaryArgs &args, hipStream_t stream)
+template <typename T, int COUNT>
+void launch_runs(dim3 grid, size_t table, size_t batch, const RotaryArgs &args, hipStream_t stream)
 {
-    if (args.interleaved) rotary_runs_kernel<T, true, BATCH><<<grid, kRotaryThreads, table, stream>>>(args);
-    else rotary_runs_kernel<T, false, BATCH><<<grid, kRotaryThreads, table, stream>>>(args);
+    if (batch == 4 && args.interleaved) rotary_runs_kernel<T, COUNT, true, 4><<<grid, kRotaryThreads, table, stream>>>(args);
+    else if (batch == 4) rotary_runs_kernel<T, COUNT, false, 4><<<grid, kRotaryThreads, table, stream>>>(args);
+    else if (args.interleaved) rotary_runs_kernel<T, COUNT, true, 1><<<grid, kRotaryThreads, table, stream>>>(args);
+    else rotary_runs_kernel<T, COUNT, false, 1><<<grid, kRotaryThreads, table, stream>>>(args);
 }
 
 template <typename T>
@@ -218,14 +192,14 @@ hipError_t launch_rotary(size_t rows, size_t sequence, size_t heads, size_t head
     args.low_turns = r.low_turns;
     args.by_turns = 1.0 / (static_cast<double>(r.high_turns) - r.low_turns);
     args.magnitude = r.magnitude;
-    // Runs of 16 bytes wherever every one of them begins on their boundary.
-    constexpr size_t COUNT = kRunValues<T>;
-    const bool runs = args.half % COUNT == 0 && head_dim % COUNT == 0 && ld_in % COUNT == 0 && ld_out % COUNT == 0 &&
-                      reinterpret_cast<uintptr_t>(in) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-    const size_t turning = runs ? args.half / COUNT : args.half, copied = args.copies ? (head_dim - r.rotary_dim) / (runs ? COUNT : 1) : 0;
+    // Runs as long as every one of them begins on a boundary of its length, up to 16 bytes.  (6815 rows of 33 bf16 heads of 80 values, 40 of
+    // which turn, 8 bytes at a time: 20 us, 70 by single values.)
+    const size_t together = args.half | head_dim | ld_in | ld_out | reinterpret_cast<uintptr_t>(in) / sizeof(T) | reinterpret_cast<uintptr_t>(out) / sizeof(T) | 16 / sizeof(T);
+    const size_t count = together & -together;
+    const size_t turning = args.half / count, copied = args.copies ? (head_dim - r.rotary_dim) / count : 0;
     const size_t units = std::max<size_t>(1, turning + copied);  // of a head
     // A block of 256 threads takes as many whole rows as give each thread a batch, or a part of a row's heads.
-    const size_t batch = runs && rows * heads * units >= size_t(1) << 19 ? 4 : 1, wanted = batch * kRotaryThreads;
+    const size_t batch = rows * heads * units >= size_t(1) << 19 ? 4 : 1, wanted = batch * kRotaryThreads;
     args.heads_per_block = static_cast<int>(std::max<size_t>(1, std::min(heads, wanted / units)));
     args.head_blocks = static_cast<int>((heads + args.heads_per_block - 1) / args.heads_per_block);
     args.rows_per_block = static_cast<int>(std::max<size_t>(1, std::min({rows, wanted / (units * args.heads_per_block), size_t(2048) / std::max(1, args.half)})));
@@ -233,9 +207,12 @@ hipError_t launch_rotary(size_t rows, size_t sequence, size_t heads, size_t head
     if (blocks > 0x7fffffffu) return hipErrorInvalidValue;
     const size_t table = static_cast<size_t>(args.rows_per_block) * args.half * sizeof(float2);
     const dim3 grid(static_cast<unsigned>(blocks));
-    if (!runs) rotary_pairs_kernel<T><<<grid, kRotaryThreads, table, stream>>>(args);
-    else if (batch == 4) launch_runs<T, 4>(grid, table, args, stream);
-    else launch_runs<T, 1>(grid, table, args, stream);
+    if constexpr (sizeof(T) == 2) {
+        if (count == 8) launch_runs<T, 8>(grid, table, batch, args, stream);
+    }
+    if (count == 4) launch_runs<T, 4>(grid, table, batch, args, stream);
+    if (count == 2) launch_runs<T, 2>(grid, table, batch, args, stream);
+    if (count == 1) launch_runs<T, 1>(grid, table, batch, args, stream);
     return hipGetLastError();
 }
 

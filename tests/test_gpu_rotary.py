@@ -123,6 +123,19 @@ def test_in_place_and_between_columns_of_one_matrix(hip, kind, interleaved, dim,
     check(got[:, width:], x[:, :width], heads, dim, config, positions, False, kind, "into other columns")
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,heads,dim,turned", [(3000, 14, 96, 36), (2500, 9, 65, 22), (5000, 12, 80, 40)])
+def test_many_rows_of_short_runs(hip, kind, rows, heads, dim, turned):
+    """Runs of two values, one and four, where a thread has several at once."""
+    rng = np.random.default_rng(rows)
+    x = make(rng, (rows, heads * dim), kind)
+    positions = rng.integers(0, 3000, rows)
+    for interleaved in (False, True):
+        config = {"rotary_dim": turned, "interleaved": interleaved}
+        got, _ = run(hip, x, heads * dim, heads, dim, config, positions, heads * dim)
+        check(got, x, heads, dim, config, positions, False, kind, f"interleaved {interleaved}")
+
+
 def test_positions_from_the_row(hip):
     x = make(np.random.default_rng(4), (3 * 37, 64), "f32")
     config = {"rotary_dim": 64, "interleaved": True}
