@@ -949,25 +949,49 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
         }
         __syncthreads();
         if (!is_last) return;
+        // Lane group g asks for the statistics of parts g, g + 4, ...; what each part counts for goes to all four through LDS, each
+        // wavefront's to a place of its own.  A part's sums are asked for all at once: this takes one memory latency after the other.
         auto unit_of = [&](unsigned of_part) { return static_cast<size_t>(item) + (static_cast<size_t>(of_part) - part) * p.kv_heads; };
+        static_assert(kKvMostWideParts == 16 && 4 * NC * 16 * kKvMostWideParts * sizeof(float) <= kKvStages * kKvStageBytes<HD>, "factors");
+        float *const factors = reinterpret_cast<float *>(lds) + wave * NC * 16 * kKvMostWideParts;  // (NC, parts, 16 columns)
+        float2 held[NC][4];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                held[c][i] = float2{-INFINITY, 0.0f};
+                if (g + 4 * i < parts) held[c][i] = load_shared(statistics_at(unit_of(g + 4 * i), c));
+            }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            float most = -INFINITY;
-            for (unsigned of_part = 0; of_part < parts; ++of_part) most = fmaxf(most, load_shared(statistics_at(unit_of(of_part), c)).x);
+            const float most = across_groups_max(fmaxf(fmaxf(held[c][0].x, held[c][1].x), fmaxf(held[c][2].x, held[c][3].x)));
             const float base = most == -INFINITY ? 0.0f : most;
-            s.sum[c][0] = 0.0f;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float factor = __builtin_amdgcn_exp2f(held[c][i].x - base);
+                sum += held[c][i].y * factor;
+                factors[(c * kKvMostWideParts + g + 4 * i) * 16 + n] = factor;
+            }
+            s.sum[c][0] = across_groups_sum(sum);
 #pragma unroll
             for (int t = 0; t < VT; ++t) s.out[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            for (unsigned of_part = 0; of_part < parts; ++of_part) {
-                const size_t unit = unit_of(of_part);
-                const float2 own = load_shared(statistics_at(unit, c));
-                const float factor = __builtin_amdgcn_exp2f(own.x - base);
-                s.sum[c][0] += own.y * factor;
+        }
+#pragma unroll 1
+        for (unsigned of_part = 0; of_part < parts; ++of_part) {
+            float2 low[NC][VT], high[NC][VT];
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int t = 0; t < VT; ++t) {
-                    const float2 low = load_shared(sums_at(unit, c, t, 0)), high = load_shared(sums_at(unit, c, t, 1));
-                    s.out[c][t] += f32x4{low.x, low.y, high.x, high.y} * factor;
+                    low[c][t] = load_shared(sums_at(unit_of(of_part), c, t, 0));
+                    high[c][t] = load_shared(sums_at(unit_of(of_part), c, t, 1));
                 }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float factor = factors[(c * kKvMostWideParts + of_part) * 16 + n];
+#pragma unroll
+                for (int t = 0; t < VT; ++t) s.out[c][t] += f32x4{low[c][t].x, low[c][t].y, high[c][t].x, high[c][t].y} * factor;
             }
         }
     }
