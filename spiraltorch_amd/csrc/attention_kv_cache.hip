@@ -40,6 +40,7 @@ struct KvAttentionArgs {
     unsigned wide;   // and of the latter
     unsigned items;  // the most that there can be of (narrow tile of columns, key head) pairs
     float heads_by_target;
+    bool halves_own;  // whether a share of wide tiles counts half of a request's own rows
     float scale_log2;  // |scale| * log2(e), not quite 0
     bool causal, negative;
 };
@@ -734,54 +735,22 @@ __device__ __forceinline__ int key_swizzle(int row)
     else return (row & 3) | (row >> 4 & 3) << 2;
 }
 
-template <int HD, int NC, bool CUT>
-__device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned item, unsigned char *lds)
+// A tile of columns and the tiles of keys tile_first .. end-1 of their context: all of it, or part `part` of `parts`.
+struct KvWideWork {
+    KvRequest of;
+    unsigned column_tile, tile_first, end, part, parts, arrived;
+};
+
+template <int HD, int NC, bool JOINS>
+__device__ __forceinline__ void attend_wide(const KvAttentionArgs &p, const KvWideWork &work, int kv_head, unsigned item, unsigned char *lds)
 {
     constexpr int WIDTH = 4 * 16 * NC, VT = HD / 16, KL = HD / 64, LOADS = kKvTile * HD / 4096;  // of 16 bytes, a thread, for keys and for values
     constexpr int AHEAD = 2;  // pieces that are read before their use
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int kv_head = item % p.kv_heads;
-    __shared__ KvFound found;
-    __shared__ unsigned found_share;
-    __shared__ bool is_last;
-    auto tiles_of = [&](const KvRequest &q) {
-        const int columns = q.rows * p.group;
-        return columns > p.few ? (static_cast<unsigned>(columns) + WIDTH - 1) / WIDTH : 0;
-    };
-    if (wave == 0) {
-        const KvRequest own = longest_first<true>(p, own_request(p));
-        unsigned share = 0x7fffffffu;
-        if (CUT)  // (of the rows that see their own keys one by one, each sees half of them on average)
-            share = find_share(p, own, [&](const KvRequest &q) {
-                return static_cast<float>(tiles_of(q)) * (static_cast<float>(key_tiles(q.length)) - (p.causal ? 0.5f / kKvTile * min(q.rows, q.length) : 0.0f));
-            });
-        KvFound at;
-        const bool is = find_request(p, own, item / p.kv_heads, p.wide / p.kv_heads, [&](const KvRequest &q) { return tiles_of(q) * (CUT ? parts_of(q, share, kKvMostWideParts) : 1); },
-                                     tiles_of, &at);
-        if (lane == 0) {
-            found = at;
-            found_share = is ? share : 0;
-        }
-    }
-    __syncthreads();
-    const unsigned share = __builtin_amdgcn_readfirstlane(found_share);
-    if (share == 0) return;
-    const KvFound at = uniform(found);
-    const KvRequest of = at.of;
-    // (the last columns see the most keys: they come first)
-    const unsigned most_parts = CUT ? parts_of(of, share, kKvMostWideParts) : 1;
-    const unsigned part = at.offset % most_parts, column_tile = tiles_of(of) - 1 - at.offset / most_parts;
-    const int columns = of.rows * p.group, block_first = static_cast<int>(column_tile) * WIDTH, first = block_first + wave * 16 * NC;
-    const int last_column = min(columns, block_first + WIDTH) - 1;
-    unsigned tile_first = 0, end = key_tiles(p.causal ? max(0, of.length - of.rows + last_column / p.group + 1) : of.length), parts = 1;
-    if constexpr (CUT) {
-        const unsigned own_share = share_of(of, share, kKvMostWideParts);
-        parts = max(1u, (end + own_share - 1) / own_share);
-        if (part >= parts) return;  // (these columns see fewer keys than others of the request)
-        tile_first = part * own_share;
-        end = min(end, tile_first + own_share);
-    }
+    const KvRequest &of = work.of;
+    const unsigned tile_first = JOINS ? work.tile_first : 0, end = work.end;
+    const int columns = of.rows * p.group, first = static_cast<int>(work.column_tile) * WIDTH + wave * 16 * NC;
     KvColumnsState<HD, NC> s;
     begin_columns<HD, NC>(p, of, first, s);
     const unsigned own_end = first < columns ? min(end, key_tiles(s.keys)) : 0;  // (behind the last column a wavefront helps with the loads)
@@ -925,7 +894,9 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
     mark_nan<HD, NC>(p, of, kv_head, nan_first, own_end, 1, s);
 
     // Parts lie as the lanes hold them, 8 bytes of each beside the next one's, and are put together by the last workgroup likewise.
-    if (CUT && parts > 1) {
+    if constexpr (JOINS) {
+        const unsigned part = work.part, parts = work.parts;
+        __shared__ bool is_last;
         const size_t all = static_cast<size_t>(p.wide) * WIDTH;
         auto sums_at = [&](size_t unit, int c, int t, int half) {
             return p.wide_parts + ((((unit * 4 + wave) * NC + c) * VT + t) * 2 + half) * 128 + 2 * lane;
@@ -943,7 +914,7 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (tid == 0) {
-            unsigned *const arrived = p.arrived + p.items + (static_cast<size_t>(at.before) + column_tile) * p.kv_heads + kv_head;
+            unsigned *const arrived = p.arrived + p.items + static_cast<size_t>(work.arrived) * p.kv_heads + kv_head;
             is_last = atomicAdd(arrived, 1u) == parts - 1;
             if (is_last) atomicExch(arrived, 0u);
         }
@@ -1006,6 +977,56 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
     }
 }
 
+template <int HD, int NC, bool CUT>
+__device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned item, unsigned char *lds)
+{
+    constexpr int WIDTH = 4 * 16 * NC;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kv_head = item % p.kv_heads;
+    __shared__ KvFound found;
+    __shared__ unsigned found_share;
+    auto tiles_of = [&](const KvRequest &q) {
+        const int columns = q.rows * p.group;
+        return columns > p.few ? (static_cast<unsigned>(columns) + WIDTH - 1) / WIDTH : 0;
+    };
+    if (wave == 0) {
+        const KvRequest own = longest_first<true>(p, own_request(p));
+        unsigned share = 0x7fffffffu;
+        if (CUT)  // (of the rows that see their own keys one by one, each sees half of them on average)
+            share = find_share(p, own, [&](const KvRequest &q) {
+                return static_cast<float>(tiles_of(q)) * (static_cast<float>(key_tiles(q.length)) - (p.halves_own ? 0.5f / kKvTile * min(q.rows, q.length) : 0.0f));
+            });
+        KvFound at;
+        const bool is = find_request(p, own, item / p.kv_heads, p.wide / p.kv_heads, [&](const KvRequest &q) { return tiles_of(q) * (CUT ? parts_of(q, share, kKvMostWideParts) : 1); },
+                                     tiles_of, &at);
+        if (lane == 0) {
+            found = at;
+            found_share = is ? share : 0;
+        }
+    }
+    __syncthreads();
+    const unsigned share = __builtin_amdgcn_readfirstlane(found_share);
+    if (share == 0) return;
+    const KvFound at = uniform(found);
+    const KvRequest of = at.of;
+    // (the last columns see the most keys: they come first)
+    const unsigned most_parts = CUT ? parts_of(of, share, kKvMostWideParts) : 1;
+    KvWideWork work{of, tiles_of(of) - 1 - at.offset / most_parts, 0, 0, at.offset % most_parts, 1, 0};
+    const int last_column = min(of.rows * p.group, static_cast<int>(work.column_tile + 1) * WIDTH) - 1;
+    work.end = key_tiles(p.causal ? max(0, of.length - of.rows + last_column / p.group + 1) : of.length);
+    work.arrived = at.before + work.column_tile;
+    if constexpr (CUT) {
+        const unsigned own_share = share_of(of, share, kKvMostWideParts);
+        work.parts = max(1u, (work.end + own_share - 1) / own_share);
+        if (work.part >= work.parts) return;  // (these columns see fewer keys than others of the request)
+        work.tile_first = work.part * own_share;
+        work.end = min(work.end, work.tile_first + own_share);
+        // (A loop of its own for whole contexts: 145 us instead of 150 for 8 prompts none of which is cut.)
+        if (work.parts > 1) return attend_wide<HD, NC, true>(p, work, kv_head, item, lds);
+    }
+    attend_wide<HD, NC, false>(p, work, kv_head, item, lds);
+}
+
 template <int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : HD == 128 ? 2 : 1, HD == 64 ? 4 : HD == 128 ? 2 : 1))) void kv_attention_few_kernel(KvAttentionArgs p)
 {
@@ -1052,10 +1073,15 @@ hipError_t launch_kv_attention(KvAttentionArgs args, hipStream_t stream)
     const long long items = tiles * args.kv_heads, wide_items = wide_tiles * args.kv_heads;
     args.items = static_cast<unsigned>(items);
     args.heads_by_target = static_cast<float>(args.kv_heads) / kKvTarget<HD>;
-    // Contexts are cut where there may be too few tiles of columns for the chip.
+    const bool fills = wide_items > kKvTarget<HD>;
+    args.halves_own = args.causal && !fills;
+    // Contexts are cut where there may be too few tiles of columns for the chip, or few enough that a context much longer than the others is
+    // what is waited for.  (47 prompts of 24 rows over 16 to 6834 keys, 80 heads on 5: 166 us uncut, 105; 55 of 108 rows over up to 3537,
+    // 16 on 1: 82 and 55.  Even batches pay for it: 8 of 500 rows 147 and 148 at dimension 128, 106 and 117 at 64.)
+    // Cuts add at most a target of workgroups, and another where half of a prompt's own keys were left out of the sum that they share.
     const bool cuts = (args.table_width << args.page_shift) > kKvLeastShare * kKvTile;
-    const bool cut = cuts && items <= 4096, wide_cut = cuts && wide_items != 0 && wide_items <= kKvTarget<HD>;
-    long long units = items + (cut ? kKvTarget<HD> : 0), wide_units = wide_items + (wide_cut ? 2 * kKvTarget<HD> : 0);
+    const bool cut = cuts && items <= 4096, wide_cut = cuts && wide_items != 0 && wide_items <= 4 * kKvTarget<HD>;
+    long long units = items + (cut ? kKvTarget<HD> : 0), wide_units = wide_items + (wide_cut ? fills ? kKvTarget<HD> : 2 * kKvTarget<HD> : 0);
     if (cut || wide_cut) {
         const size_t floats = cut ? static_cast<size_t>(units) * kKvColumns * (HD + 2) : 0;
         void *scratch = nullptr;

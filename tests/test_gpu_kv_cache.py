@@ -294,6 +294,16 @@ def test_long_prompts(hip, page, dim, kv_heads, group, lengths, fresh):
         check_attention(hip, rng, page, kv_heads, dim, group, lengths, fresh, causal)
 
 
+@pytest.mark.parametrize("dim,kv_heads,group,fresh", [(128, 8, 4, 20), (64, 8, 8, 20), (256, 7, 4, 18)])
+def test_many_prompts_of_uneven_lengths(hip, dim, kv_heads, group, fresh):
+    """More wide tiles than the chip holds at once, two contexts of which are long enough to be cut."""
+    rng = np.random.default_rng(dim)
+    lengths = [int(n) for n in rng.integers(0, 90, 64)]
+    lengths[7], lengths[40] = 3000, 2111
+    for causal in (True, False):
+        check_attention(hip, rng, 64, kv_heads, dim, group, lengths, [fresh] * 64, causal)
+
+
 def test_rows_without_keys(hip):
     """More rows than tokens: the first see none, and are 0; requests of no length, of a negative one."""
     rng = np.random.default_rng(1)
