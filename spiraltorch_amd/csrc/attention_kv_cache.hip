@@ -921,7 +921,8 @@ __device__ __forceinline__ void attend_wide(const KvAttentionArgs &p, const KvWi
         __syncthreads();
         if (!is_last) return;
         // Lane group g asks for the statistics of parts g, g + 4, ...; what each part counts for goes to all four through LDS, each
-        // wavefront's to a place of its own.  A part's sums are asked for all at once: this takes one memory latency after the other.
+        // wavefront's to a place of its own.  The sums of two parts are asked for at once (registers
+        // end there; one, for heads of 256): this takes one memory latency after the other.
         auto unit_of = [&](unsigned of_part) { return static_cast<size_t>(item) + (static_cast<size_t>(of_part) - part) * p.kv_heads; };
         static_assert(kKvMostWideParts == 16 && 4 * NC * 16 * kKvMostWideParts * sizeof(float) <= kKvStages * kKvStageBytes<HD>, "factors");
         float *const factors = reinterpret_cast<float *>(lds) + wave * NC * 16 * kKvMostWideParts;  // (NC, parts, 16 columns)
@@ -948,22 +949,35 @@ __device__ __forceinline__ void attend_wide(const KvAttentionArgs &p, const KvWi
 #pragma unroll
             for (int t = 0; t < VT; ++t) s.out[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-#pragma unroll 1
-        for (unsigned of_part = 0; of_part < parts; ++of_part) {
-            float2 low[NC][VT], high[NC][VT];
+        auto ask = [&](unsigned of_part, float2 (&sums)[NC][VT][2]) __attribute__((always_inline)) {
+            const float *const at = sums_at(unit_of(of_part), 0, 0, 0);
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int t = 0; t < VT; ++t) {
-                    low[c][t] = load_shared(sums_at(unit_of(of_part), c, t, 0));
-                    high[c][t] = load_shared(sums_at(unit_of(of_part), c, t, 1));
-                }
+            for (int i = 0; i < 2 * NC * VT; ++i) sums[i / (2 * VT)][i / 2 % VT][i % 2] = load_shared(at + i * 128);
+        };
+        auto add = [&](unsigned of_part, const float2 (&sums)[NC][VT][2]) __attribute__((always_inline)) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const float factor = factors[(c * kKvMostWideParts + of_part) * 16 + n];
 #pragma unroll
-                for (int t = 0; t < VT; ++t) s.out[c][t] += f32x4{low[c][t].x, low[c][t].y, high[c][t].x, high[c][t].y} * factor;
+                for (int t = 0; t < VT; ++t) s.out[c][t] += f32x4{sums[c][t][0].x, sums[c][t][0].y, sums[c][t][1].x, sums[c][t][1].y} * factor;
             }
+        };
+        float2 one[NC][VT][2];
+        unsigned of_part = 0;
+        if constexpr (HD < 256) {
+            float2 two[NC][VT][2];
+#pragma unroll 1
+            for (; of_part + 1 < parts; of_part += 2) {
+                ask(of_part, one);
+                ask(of_part + 1, two);
+                add(of_part, one);
+                add(of_part + 1, two);
+            }
+        }
+#pragma unroll 1
+        for (; of_part < parts; ++of_part) {
+            ask(of_part, one);
+            add(of_part, one);
         }
     }
 #pragma unroll
