@@ -701,7 +701,7 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
 // their own.
 // What bounds this is the issue of vector instructions.  A tile of 64 keys and 32 columns of 128 values has 68 products, which take 8 cycles of it
 // each, and 343 others, 128 of them conversions of codes, at 5 cycles (exponentials 8.5): 2340 cycles, and the matrix cores' own 1088 hide among
-// them.  8 prompts of 500 rows over 1000 to 4000 keys, 32 heads on 8 of 128 values: 145 us, 0.86 PFLOP/s.  (Ways there: 158 us when each 16
+// them.  8 prompts of 500 rows over 1000 to 4000 keys, 32 heads on 8 of 128 values: 148 us, 0.85 PFLOP/s.  (Ways there: 158 us when each 16
 // keys' page was looked up for itself, 149 with a barrier for each tile.  Three wavefronts a SIMD: 180, for spilled registers; 48 columns a
 // wavefront: 143 to 157; priority to wavefronts within products: 143 to 147.)
 typedef __attribute__((address_space(3))) void *kv_lds_ptr;
