@@ -93,7 +93,7 @@ __device__ __forceinline__ unsigned wave_scan_sum(unsigned v)
     return wave_scan(v, [](unsigned x, unsigned y) { return x + y; });
 }
 
-// Work is numbered by prefix sums over the requests, which every wavefront takes for itself: `count(request)` items each, and the
+// Work is numbered by prefix sums over the requests, which a wavefront of every workgroup takes: `count(request)` items each, and the
 // request of item number `item` is found by 64 sums at a time (one round of loads for up to 64 requests, two for 4096 ...).  `own`: this lane's
 // request where there are no more than 64.
 struct KvFound {
