@@ -252,11 +252,17 @@ __device__ __forceinline__ float across_groups_sum(float v)
 }
 
 // A wavefront's columns: NC tiles of sixteen, tile c at `first + 16c`, of the request's rows*group; behind the last one they repeat it.
+// Sums of weighted values are divided by the weights' only at the end, and weights may be 2^8 (see weigh): for 2^31 keys on pages of scale 2^70 or
+// less they stay below 2^31 * 2^8 * 448 * 2^70, 2^118.  From the first page above that on, weights are 2^-64 of what they were, so that the largest
+// values that there are, averaged over as many keys as there can be, keep as far from f32's border.
+constexpr float kKvLargeScale = 0x1p70f, kKvLowered = 64.0f;
+
 template <int HD, int NC>
 struct KvColumnsState {
     f32x4 out[NC][HD / 16];
     f32x4 sum[NC];      // of the weights, as they go into `out`: a product with ones, four times the same
-    float run_max[NC];  // in log2, of scaled scores
+    float run_max[NC];  // in log2, of scaled scores, and `lowered` more
+    float lowered;      // weights are smaller by that power of two: 0, or kKvLowered once values have been met that are as large as kKvLargeScale
     int limit[NC];                   // keys that the column sees
     int keys, fewest;                // the most and the fewest that any of them does
 };
@@ -269,6 +275,7 @@ __device__ __forceinline__ void begin_columns(const KvAttentionArgs &p, const Kv
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         s.run_max[c] = -INFINITY;
+        s.lowered = 0.0f;
         s.sum[c] = f32x4{0.f, 0.f, 0.f, 0.f};
         s.limit[c] = sees(min(columns - 1, first + 16 * c + n));
 #pragma unroll
@@ -315,6 +322,21 @@ __device__ __forceinline__ void hide_unseen(const KvColumnsState<HD, NC> &s, uns
     }
 }
 
+// Before a tile's values count, if one of them is on a page of a scale above kKvLargeScale.
+template <int HD, int NC>
+__device__ __forceinline__ void lower_for(float value_scale, KvColumnsState<HD, NC> &s)
+{
+    if (__builtin_expect(!__any(value_scale > kKvLargeScale), 1) || s.lowered != 0.0f) return;
+    s.lowered = kKvLowered;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        s.run_max[c] += kKvLowered;
+        s.sum[c] *= 0x1p-64f;
+#pragma unroll
+        for (int t = 0; t < HD / 16; ++t) s.out[c][t] *= 0x1p-64f;
+    }
+}
+
 // A tile's scores (products of queries and keys; -infinity where a column does not see the key) to the weights of its values, and the
 // columns' maxima, sums and outputs with them.
 template <int HD, int NC>
@@ -330,7 +352,7 @@ __device__ __forceinline__ void weigh(const KvAttentionArgs &p, f32x4 (&scores)[
             most[c] = fmaxf(fmaxf(most[c], scores[c][i][0]), scores[c][i][1]);
             most[c] = fmaxf(fmaxf(most[c], scores[c][i][2]), scores[c][i][3]);
         }
-        most[c] = across_groups_max(most[c]) * p.scale_log2;
+        most[c] = fmaf(across_groups_max(most[c]), p.scale_log2, s.lowered);
         grows |= most[c] > s.run_max[c] + 8.0f;
     }
     // The maximum may lag behind by a factor of 2^8: weights are that much larger then, and nothing has to be scaled for most tiles.
@@ -471,6 +493,7 @@ __device__ __forceinline__ void attend(const KvAttentionArgs &p, const KvRequest
         if (more) load_keys(next, key_page);
 
         if (!whole) hide_unseen<HD, NC>(s, key0, value_fits, scores);
+        lower_for<HD, NC>(value_scale, s);
         bf16x8 weights[NC][2];
         weigh<HD, NC>(p, scores, s, weights);
         if (!whole) {
@@ -852,6 +875,7 @@ __device__ __forceinline__ void attend_wide(const KvAttentionArgs &p, const KvWi
         }
         const bool whole = fits == 15 && key0 + kKvTile <= static_cast<unsigned>(s.fewest);
         if (__builtin_expect(!whole, 0)) hide_unseen<HD, NC>(s, key0, fits >> g & 1, scores);
+        lower_for<HD, NC>(scale_of_values, s);
         bf16x8 weights[NC][2];
         weigh<HD, NC>(p, scores, s, weights);
         unsigned nan = 0;

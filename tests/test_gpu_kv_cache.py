@@ -390,6 +390,24 @@ def test_pages_of_very_different_sizes(hip):
     check_attention(hip, rng, 16, 2, 64, 2, [100, 90], [3, 50], True, edit=edit)
 
 
+@pytest.mark.parametrize("dim,kv_heads,group,lengths,fresh", [(64, 2, 2, [300, 7], [1, 3]), (128, 1, 4, [5000, 900], [1, 2]), (256, 1, 2, [2500, 40], [2, 1]),
+                                                              (64, 1, 8, [400, 30], [60, 2]), (128, 2, 4, [2600, 500], [40, 33]), (256, 1, 4, [1500], [70])])
+def test_averages_of_values_near_the_largest(hip, dim, kv_heads, group, lengths, fresh):
+    """Their sum is beyond f32, their average is not: on all pages, on the later ones alone, and on every fourth beside pages of 2^-20."""
+    def edit(where):
+        def change(store, table, q):
+            store.v[...] &= 0x7f
+            for r, n in enumerate(lengths):
+                pages = table[r, :-(-n // 64)]
+                store.v_scales[pages] = 2.0**-20
+                store.v_scales[pages[where(len(pages))]] = 2.0**119
+        return change
+
+    for where in (lambda n: slice(None), lambda n: slice(n // 2, None), lambda n: slice(n % 4, None, 4)):
+        got = check_attention(hip, np.random.default_rng(23), 64, kv_heads, dim, group, lengths, fresh, True, edit=edit(where))
+        assert np.isfinite(got).all() and got.max() > 2.0**120
+
+
 def test_a_page_beyond_32_bits(hip):
     """Codes more than 2^32 bytes into the cache's memory, appended and read."""
     pages, page, heads, dim = 2200, 256, 32, 256  # 4.6 GB each of keys and values
