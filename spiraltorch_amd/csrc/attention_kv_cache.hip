@@ -11,6 +11,7 @@
 // Every 16-key group lies within a page whatever its size, so that a tile may span up to four pages.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "device_math.h"
@@ -1171,8 +1172,9 @@ hipError_t launch_attention_kv_cache_bf16(const st_hip_kv_cache &cache, size_t r
     args.group = static_cast<int>(heads / cache.kv_heads);
     args.pages = static_cast<int>(cache.pages);
     args.page_shift = __builtin_ctzll(cache.page_size);
-    // (Not quite 0, so that masked scores of -infinity keep their weight of 0 where the scale is.)
-    args.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
+    // (Not quite 0, so that masked scores of -infinity keep their weight of 0 where the scale is: so small that it makes nothing of any other.)
+    args.scale_log2 = std::fabs(scale) * 1.4426950408889634f;
+    if (!(args.scale_log2 > 0.0f)) args.scale_log2 = std::numeric_limits<float>::denorm_min();
     args.negative = scale < 0.0f;
     args.causal = causal;
     if (cache.head_dim == 64) return launch_kv_attention<64>(args, stream);

@@ -1372,6 +1372,7 @@ int st_hip_attention_kv_cache_bf16_dev(const st_hip_kv_cache *cache, size_t requ
         return fail(ST_HIP_ERR_INVALID, "attention heads %zu are not a multiple of the cache's %zu", heads, cache->kv_heads);
     if (!std::isfinite(scale))
         return fail(ST_HIP_ERR_NONFINITE, "non-finite value encountered in scaled_dot_attention_scale: %g", static_cast<double>(scale));
+    if (!std::isfinite(scale * 1.4426950408889634f)) return fail(ST_HIP_ERR_UNSUPPORTED, "attention scale %g times log2(e) exceeds f32", static_cast<double>(scale));
     size_t width = 0, columns = 0, items = 0, entries = 0;
     if (!checked_mul(heads, cache->head_dim, &width) || !checked_mul(rows, heads, &columns) || !checked_mul(requests, cache->kv_heads, &items) ||
         !checked_mul(requests, table_width, &entries) || entries > static_cast<size_t>(-1) / 8 || !addressable(rows, ld_q, sizeof(uint16_t)) ||

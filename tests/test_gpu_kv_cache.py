@@ -372,6 +372,18 @@ def test_scales_of_the_scores(hip, scale):
         check_attention(hip, rng, 64, 1, 128, 4, [200, 17], [5, 17], causal, scale=scale)
 
 
+@pytest.mark.parametrize("scale", [0.0, 1e-45, 1e-41, -1e-38, 1e-36])
+def test_small_scales_of_large_scores(hip, scale):
+    """Products of queries and keys of 10^36, on narrow tiles of columns and on wide ones, with masked keys beside them."""
+    def edit(store, table, q):
+        store.k_scales[table[table >= 0]] = 2.0**60
+
+    rng = np.random.default_rng(24)
+    for dim in (64, 128, 256):
+        for lengths, fresh in (([200, 17], [5, 17]), ([300], [150])):
+            check_attention(hip, rng, 64, 1, dim, 2, lengths, fresh, True, scale=scale, edit=edit, q_size=1e15)
+
+
 def test_strides(hip):
     rng = np.random.default_rng(8)
     for extra in (1, 3):

@@ -123,6 +123,14 @@ def test_attention(stub):
     assert answers(stub, "hip.attention_kv_cache_bf16_dev", base, expected) == list(expected.values())
 
 
+def test_attention_scales(stub):
+    """A scale that f32 holds, but not times log2(e)."""
+    base = ("cache=cache(), requests=3, rows=7, heads=4, scale=0.1, causal=True, row_offsets=1*M, lengths=2*M, page_table=3*M, table_width=4, "
+            "q=4*M, ld_q=256, out=5*M, ld_out=256")
+    expected = {"scale=2.3e38": "taken", "scale=-2.3e38": "taken", "scale=2.4e38": "unsupported", "scale=-3.4e38": "unsupported", "scale=1e-45": "taken"}
+    assert answers(stub, "hip.attention_kv_cache_bf16_dev", base, expected) == list(expected.values())
+
+
 def test_attention_goes_on_without_room_for_parts(stub):
     """Long contexts of few rows are cut over workgroups; without scratch memory for the parts, one takes a context as it is."""
     out = run(stub, """
