@@ -39,7 +39,7 @@ struct KvAttentionArgs {
     int few;         // requests of so many columns or fewer go to the kernel whose wavefronts share them, others to the one of wide tiles
     unsigned units;  // workgroups of the former
     unsigned wide;   // and of the latter
-    unsigned items;  // the most that there can be of (narrow tile of columns, key head) pairs
+    unsigned items, wide_items;  // the most that there can be of (tile of columns, key head) pairs, narrow and wide: a counter for each
     float heads_by_target;
     bool halves_own;  // whether a share of wide tiles counts half of a request's own rows
     float scale_log2;  // |scale| * log2(e), not quite 0
@@ -88,10 +88,12 @@ __device__ __forceinline__ unsigned parts_of(const KvRequest &q, unsigned share,
     return max(1u, (key_tiles(q.length) + mine - 1) / mine);
 }
 
+// Sums stop at 2^32 - 1 (and stay associative): those of any row offsets can be compared with what there is room for.
+__device__ __forceinline__ unsigned stopping_sum(unsigned x, unsigned y) { return __builtin_elementwise_add_sat(x, y); }
 // Sum over the lanes up to and with this one.
 __device__ __forceinline__ unsigned wave_scan_sum(unsigned v)
 {
-    return wave_scan(v, [](unsigned x, unsigned y) { return x + y; });
+    return wave_scan(v, stopping_sum);
 }
 
 // Work is numbered by prefix sums over the requests, which a wavefront of every workgroup takes: `count(request)` items each, and the
@@ -102,10 +104,10 @@ struct KvFound {
     unsigned offset;  // of the item within its request's
     unsigned before;  // sum of `other` over the requests before it
 };
-// False behind the last item; and for all items where they are more than `most`, which row offsets out of order can make them: a launch
-// does all of its work or none.
+// False behind the last item; and for all items where they, or `other`, are more than there is room for, which row offsets out of order can make
+// them: a launch does all the work of one kind or none of it, and its counters are within their buffer and 0 after it.
 template <class Count, class Other>
-__device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvRequest &own, unsigned item, unsigned most, Count &&count, Other &&other, KvFound *found)
+__device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvRequest &own, unsigned item, unsigned most, unsigned most_other, Count &&count, Other &&other, KvFound *found)
 {
     const int lane = threadIdx.x & 63;
     int low = 0, left = p.requests;
@@ -122,13 +124,14 @@ __device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvR
             const int first = low + lane * step, end = min(low + left, first + step);
             for (int r = first; r < end; ++r) {
                 q = load_request(p, r);
-                items += count(q);
-                others += other(q);
+                items = stopping_sum(items, count(q));
+                others = stopping_sum(others, other(q));
             }
         }
         const unsigned to = wave_scan_sum(items), to_other = wave_scan_sum(others);
         const unsigned long long behind = __ballot(items_before + to > item);
-        if (behind == 0 || (left == p.requests && __builtin_amdgcn_readlane(to, 63) > most)) return false;
+        if (behind == 0) return false;
+        if (left == p.requests && (__builtin_amdgcn_readlane(to, 63) > most || __builtin_amdgcn_readlane(to_other, 63) > most_other)) return false;
         const int which = __builtin_ctzll(behind);
         items_before += __builtin_amdgcn_readlane(to - items, which);
         found->before += __builtin_amdgcn_readlane(to_other - others, which);
@@ -580,7 +583,7 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
         unsigned share = 0x7fffffffu;
         if (p.parts) share = find_share(p, own, [&](const KvRequest &q) { return static_cast<float>(few_tiles(p, q)) * static_cast<float>(key_tiles(q.length)); });
         KvFound at;
-        const bool is = find_request(p, own, unit / p.kv_heads, p.units / p.kv_heads, [&](const KvRequest &q) { return few_tiles(p, q) * parts_of(q, share); },
+        const bool is = find_request(p, own, unit / p.kv_heads, p.units / p.kv_heads, p.items / p.kv_heads, [&](const KvRequest &q) { return few_tiles(p, q) * parts_of(q, share); },
                                      [&](const KvRequest &q) { return few_tiles(p, q); }, &at);
         if (lane == 0) {
             found = at;
@@ -1038,7 +1041,7 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
                 return static_cast<float>(tiles_of(q)) * (static_cast<float>(key_tiles(q.length)) - (p.halves_own ? 0.5f / kKvTile * min(q.rows, q.length) : 0.0f));
             });
         KvFound at;
-        const bool is = find_request(p, own, item / p.kv_heads, p.wide / p.kv_heads, [&](const KvRequest &q) { return tiles_of(q) * (CUT ? parts_of(q, share, kKvMostWideParts) : 1); },
+        const bool is = find_request(p, own, item / p.kv_heads, p.wide / p.kv_heads, p.wide_items / p.kv_heads, [&](const KvRequest &q) { return tiles_of(q) * (CUT ? parts_of(q, share, kKvMostWideParts) : 1); },
                                      tiles_of, &at);
         if (lane == 0) {
             found = at;
@@ -1113,6 +1116,7 @@ hipError_t launch_kv_attention(KvAttentionArgs args, hipStream_t stream)
     }
     const long long items = tiles * args.kv_heads, wide_items = wide_tiles * args.kv_heads;
     args.items = static_cast<unsigned>(items);
+    args.wide_items = static_cast<unsigned>(wide_items);
     args.heads_by_target = static_cast<float>(args.kv_heads) / kKvTarget<HD>;
     const bool fills = wide_items > kKvTarget<HD>;
     args.halves_own = args.causal && !fills;

@@ -313,6 +313,26 @@ def test_rows_without_keys(hip):
         check_attention(hip, rng, 16, 2, dim, 3, [0, 0, -2**31], [3, 1, 1], False)
 
 
+@pytest.mark.parametrize("requests,rows,dim,group", [(8, 40, 64, 1), (130, 50, 64, 2), (6, 300, 64, 1), (200, 700, 128, 1), (7, 130, 256, 2)])
+def test_row_offsets_out_of_order(hip, requests, rows, dim, group):
+    """Offsets that rise and fall claim more tiles of columns than the rows have, by more than there are counters for but less than there are
+    workgroups: nothing is written, and the calls after it are right."""
+    rng = np.random.default_rng(rows)
+    store = Pages(hip, rng, 20, 64, 1, dim)
+    width = 40
+    d_q = hip.DeviceBuffer.from_array(inputs.to_bf16(rng.normal(size=(rows, group * dim)).astype(np.float32)))
+    out = hip.DeviceBuffer.from_array(np.full((rows, group * dim), 0x4321, np.uint16))
+    d_table, d_lengths = dev(hip, rng.integers(0, 20, (requests, width))), dev(hip, rng.integers(1000, 2500, requests))
+    offsets = np.where(np.arange(requests + 1) % 2 == 1, rows, 0)
+    for causal in (True, False):
+        hip.attention_kv_cache_bf16_dev(store.cache, requests, rows, group, 0.1, causal, dev(hip, offsets), d_lengths, d_table, width, d_q, group * dim,
+                                        out, group * dim)
+        hip.device_synchronize()
+        assert (out.to_array(np.uint16, (rows, group * dim)) == 0x4321).all()
+        check_attention(hip, rng, 64, 1, dim, group, [2100, 5, 1500], [1, 1, 2], causal)
+        check_attention(hip, rng, 64, 1, dim, group, [1500, 300], [rows // 2, 1], causal)
+
+
 def test_lengths_beyond_the_table(hip):
     rng = np.random.default_rng(2)
     for causal in (True, False):
