@@ -395,12 +395,14 @@ int check_append(const st_hip_kv_cache *c, size_t rows, const int32_t *slots, co
     ST_HIP_CHECK(check_kv_cache(c));
     const size_t width = c->kv_heads * c->head_dim;  // (below the cache's bytes)
     if (!addressable(rows, ld, size)) return fail(ST_HIP_ERR_INVALID, "kv cache append dimensions overflow");
-    if (rows > kMaxDim - 256 || ld > kMaxDim || c->kv_heads > 65535) return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache append dimension exceeds the kernel's");
+    if (rows > kMaxDim || ld > kMaxDim || c->kv_heads > 65535) return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache append dimension exceeds the kernel's");
     if (rows == 0) return ST_HIP_OK;
     if (!slots || !k || !v) return fail(ST_HIP_ERR_INVALID, "kv cache append received a null pointer");
     if (ld < width) return fail(ST_HIP_ERR_INVALID, "kv cache append row stride %zu is smaller than kv_heads*head_dim=%zu", ld, width);
     if (meets_cache(*c, k, rows, ld, width, size) || meets_cache(*c, v, rows, ld, width, size))
         return fail(ST_HIP_ERR_INVALID, "kv cache append: the new rows overlap the cache");
+    // (a workgroup looks up to 512 rows, its threads, beyond the last)
+    if (rows > kMaxDim - 512) return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache append rows %zu exceed the kernel's", rows);
     return ST_HIP_OK;
 }
 

@@ -107,6 +107,14 @@ def test_append(stub):
         assert answers(stub, call, base, expected) == list(expected.values())
 
 
+def test_append_of_the_most_rows(stub):
+    """The kernel's row numbers go up to 512 beyond the rows, within int32."""
+    for call in ("hip.kv_cache_append_f32_dev", "hip.kv_cache_append_bf16_dev"):
+        base = "cache=cache(page=256, dim=256), rows=5, slots=2**44, k=2**46, v=2**47, ld=512"
+        expected = {"rows=2**31 - 1 - 512": "taken", "rows=2**31 - 512": "unsupported", "rows=2**31 - 1 - 256": "unsupported"}
+        assert answers(stub, call, base, expected) == list(expected.values())
+
+
 def test_attention(stub):
     base = ("cache=cache(), requests=3, rows=7, heads=4, scale=0.1, causal=True, row_offsets=1*M, lengths=2*M, page_table=3*M, table_width=4, "
             "q=4*M, ld_q=256, out=5*M, ld_out=256")
