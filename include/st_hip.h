@@ -534,7 +534,7 @@ typedef struct {
 /* `heads` neighbouring heads of every row (row strides ld_in and ld_out in values), turned by the row's position, or by row % sequence
  * if positions is NULL; what does not turn is copied.  `transposed` != 0 turns back: the gradient of the call without it.  Angles are
  * reduced in 64 bits, so that far positions cost no accuracy; the products are f32, rounded once.  out may be in, with the same
- * stride, or columns of the same rows that the input's do not meet; other overlaps are refused.  head_dim up to 1024. */
+ * stride, or columns of the same rows that the input's do not meet; other overlaps are refused, those with positions among them.  head_dim up to 1024. */
 int st_hip_rotary_f32_dev(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary *rotary, int transposed,
                           const int32_t *positions, const float *in, size_t ld_in, float *out, size_t ld_out, void *stream);
 int st_hip_rotary_bf16_dev(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary *rotary, int transposed,
@@ -547,7 +547,7 @@ int st_hip_rotary_bf16_dev(size_t rows, size_t sequence, size_t heads, size_t he
  * A page whose place 0 is among them begins anew.  Its scales become the smallest powers of two, at least 2^-118, with which the new
  * rows' largest finite values are at most 448; those of other pages grow to that where it is larger, and what the page held is then
  * rounded to the new scale (exact but for values below 2^-6 of the new scale).  Codes are rounded to nearest, ties to even; NaN and
- * infinities become NaN.  The rows must not overlap the cache. */
+ * infinities become NaN.  Neither the rows nor slots may overlap the cache. */
 int st_hip_kv_cache_append_f32_dev(const st_hip_kv_cache *cache, size_t rows, const int32_t *slots, const float *k, const float *v,
                                    size_t ld, void *stream);
 int st_hip_kv_cache_append_bf16_dev(const st_hip_kv_cache *cache, size_t rows, const int32_t *slots, const uint16_t *k,
@@ -558,6 +558,7 @@ int st_hip_kv_cache_append_bf16_dev(const st_hip_kv_cache *cache, size_t rows, c
  * are its last tokens, the last row sees all lengths[r] keys and each one before it one key less; 0: every row sees all of them (an
  * encoder's states).  Rows that see no key are 0.  A length counts as at most table_width pages; tokens of pages outside the cache
  * are left out.  scale times log2(e) has to be within f32 (ST_HIP_ERR_UNSUPPORTED).  The products take bf16 and accumulate in f32, the softmax is f32; its weights enter the second product as bf16.
+ * out may be columns of q's rows that q does not meet, and overlaps nothing else that is read.
  * q 16-byte and out 8-byte aligned, ld_q a multiple of 8 and ld_out of 4, otherwise ST_HIP_ERR_UNSUPPORTED.  Long contexts of few rows
  * are cut over workgroups, whose parts go through the stream's scratch memory. */
 int st_hip_attention_kv_cache_bf16_dev(const st_hip_kv_cache *cache, size_t requests, size_t rows, size_t heads, float scale, int causal,

@@ -332,6 +332,17 @@ bool overlaps_except_columns(const void *a, size_t ld_a, const void *b, size_t l
     return apart < width * size || apart > (ld_a - width) * size;
 }
 
+// Whether rows of `width` values, `ld` apart, share memory with `held` (which may stand between them).
+bool meets_rows(const Extent &held, const void *rows_at, size_t rows, size_t ld, size_t width, size_t size)
+{
+    const uintptr_t first = reinterpret_cast<uintptr_t>(rows_at), end = first + ((rows - 1) * ld + width) * size;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(held.at), to = from + held.count * sizeof(int32_t);
+    if (held.count == 0 || from >= end || to <= first) return false;
+    if (from < first) return true;
+    const uintptr_t within = (from - first) % (ld * size);
+    return within < width * size || to - from > ld * size - within;
+}
+
 int check_rotary(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary *r, const int32_t *positions, const void *in,
                  size_t ld_in, const void *out, size_t ld_out, size_t size, bool *work)
 {
@@ -356,6 +367,8 @@ int check_rotary(size_t rows, size_t sequence, size_t heads, size_t head_dim, co
         return fail(ST_HIP_ERR_INVALID, "rotary row stride %zu/%zu is smaller than heads*head_dim=%zu", ld_in, ld_out, width);
     if (!(in == out && ld_in == ld_out) && overlaps_except_columns(in, ld_in, out, ld_out, rows, width, size))
         return fail(ST_HIP_ERR_INVALID, "rotary output overlaps its input");
+    if (positions && meets_rows({positions, rows}, out, rows, ld_out, width, size))
+        return fail(ST_HIP_ERR_INVALID, "rotary output overlaps the positions");
     *work = true;
     return ST_HIP_OK;
 }
@@ -401,6 +414,7 @@ int check_append(const st_hip_kv_cache *c, size_t rows, const int32_t *slots, co
     if (ld < width) return fail(ST_HIP_ERR_INVALID, "kv cache append row stride %zu is smaller than kv_heads*head_dim=%zu", ld, width);
     if (meets_cache(*c, k, rows, ld, width, size) || meets_cache(*c, v, rows, ld, width, size))
         return fail(ST_HIP_ERR_INVALID, "kv cache append: the new rows overlap the cache");
+    if (meets_cache(*c, slots, 1, rows, rows, sizeof(int32_t))) return fail(ST_HIP_ERR_INVALID, "kv cache append: the slots overlap the cache");
     // (a workgroup looks up to 512 rows, its threads, beyond the last)
     if (rows > kMaxDim - 512) return fail(ST_HIP_ERR_UNSUPPORTED, "kv cache append rows %zu exceed the kernel's", rows);
     return ST_HIP_OK;
@@ -1391,6 +1405,9 @@ int st_hip_attention_kv_cache_bf16_dev(const st_hip_kv_cache *cache, size_t requ
     if (overlaps_except_columns(q, ld_q, out, ld_out, rows, width, sizeof(uint16_t)))
         return fail(ST_HIP_ERR_INVALID, "attention output overlaps its queries");
     if (meets_cache(*cache, out, rows, ld_out, width, sizeof(uint16_t))) return fail(ST_HIP_ERR_INVALID, "attention output overlaps the cache");
+    for (const Extent &held : {Extent{row_offsets, requests + 1}, Extent{lengths, requests}, Extent{page_table, entries}})
+        if (meets_rows(held, out, rows, ld_out, width, sizeof(uint16_t)))
+            return fail(ST_HIP_ERR_INVALID, "attention output overlaps the row offsets, lengths or page table");
     return launch_status(launch_attention_kv_cache_bf16(*cache, requests, rows, heads, scale, causal != 0, row_offsets, lengths, page_table, table_width,
                                                         q, ld_q, out, ld_out, as_stream(stream)),
                          "attention launch");

@@ -139,6 +139,31 @@ def test_attention_scales(stub):
     assert answers(stub, "hip.attention_kv_cache_bf16_dev", base, expected) == list(expected.values())
 
 
+def test_results_over_what_is_read(stub):
+    """Positions, slots, offsets, lengths and page tables within what a call writes; beside it, and between its rows, they may be."""
+    for call, size in (("hip.rotary_f32_dev", 4), ("hip.rotary_bf16_dev", 2)):
+        base = "rows=3, heads=2, head_dim=64, rotary=hip.Rotary(64), positions=3*M, src=2*M, ld_in=128, dst=3*M, ld_out=128"
+        rows = 3 * 128 * size
+        expected = {"": "invalid", "positions=3*M - 8": "invalid", "positions=3*M - 12": "taken", f"positions=3*M + {rows - 4}": "invalid",
+                    f"positions=3*M + {rows}": "taken", f"ld_out=200, positions=3*M + {128 * size}": "taken",
+                    f"ld_out=200, positions=3*M + {200 * size - 12}": "taken", f"ld_out=200, positions=3*M + {200 * size - 8}": "invalid",
+                    f"ld_out=200, positions=3*M + {300 * size}": "invalid", f"ld_out=200, positions=3*M + {328 * size}": "taken",
+                    "positions=2*M": "taken", "src=3*M, positions=3*M + 4": "invalid", "positions=None, sequence=2": "taken"}
+        assert answers(stub, call, base, expected) == list(expected.values())
+    for call in ("hip.kv_cache_append_f32_dev", "hip.kv_cache_append_bf16_dev"):
+        base = "cache=cache(), rows=5, slots=1*M, k=2*M, v=3*M, ld=128"
+        expected = {"slots=16*M - 16": "invalid", "slots=16*M - 20": "taken", "slots=32*M + 65532": "invalid", "slots=32*M + 65536": "taken",
+                    "slots=48*M + 8": "invalid", "slots=64*M + 60": "invalid", "slots=2*M": "taken"}
+        assert answers(stub, call, base, expected) == list(expected.values())
+    base = ("cache=cache(), requests=3, rows=7, heads=4, scale=0.1, causal=True, row_offsets=1*M, lengths=2*M, page_table=3*M, table_width=4, "
+            "q=4*M, ld_q=256, out=5*M, ld_out=256")
+    expected = {"out=1*M": "invalid", "out=1*M + 8": "invalid", "out=1*M + 16": "taken", "out=2*M": "invalid", "out=2*M + 16": "taken", "out=3*M + 40": "invalid",
+                "out=3*M + 48": "taken", "row_offsets=5*M + 3580": "invalid", "row_offsets=5*M + 3584": "taken", "lengths=5*M - 12": "taken",
+                "page_table=5*M - 44": "invalid", "ld_out=512, page_table=5*M + 512": "taken", "ld_out=512, page_table=5*M + 1536": "taken",
+                "ld_out=512, page_table=5*M + 1000": "invalid", "table_width=0, page_table=5*M": "taken"}
+    assert answers(stub, "hip.attention_kv_cache_bf16_dev", base, expected) == list(expected.values())
+
+
 def test_attention_goes_on_without_room_for_parts(stub):
     """Long contexts of few rows are cut over workgroups; without scratch memory for the parts, one takes a context as it is."""
     out = run(stub, """
