@@ -30,16 +30,18 @@ struct KvAttentionArgs {
     const int *row_offsets, *lengths, *page_table;
     const uint16_t *q;
     uint16_t *out;
-    float *parts;       // where keys are cut over workgroups: for each of `units` of them 16 columns of head_dim sums, and then 16 maxima and sums
-    float *wide_parts;  // the same for wide tiles
-    unsigned *arrived;  // and for every tile of columns, `items` narrow ones and the wide ones, how many of its workgroups are done: 0 before a
-                        // launch and after it
+    float *parts;       // where keys are cut over workgroups: for each part, up to `room` for a key head, 16 columns of head_dim sums, and then 16
+                        // maxima and sums
+    float *wide_parts;  // the same for each workgroup of wide tiles
+    unsigned *arrived;  // and for every tile of columns, as many narrow ones as there is room for parts and the wide ones, how many of its workgroups
+                        // are done: 0 before a launch and after it
     long long ld_q, ld_out, table_width;
     int requests, rows, heads, kv_heads, group, pages, page_shift;
     int few;         // requests of so many columns or fewer go to the kernel whose wavefronts share them, others to the one of wide tiles
     unsigned units;  // workgroups of the former
     unsigned wide;   // and of the latter
-    unsigned items, wide_items;  // the most that there can be of (tile of columns, key head) pairs, narrow and wide: a counter for each
+    unsigned room;        // see kKvRoom
+    unsigned wide_items;  // the most that there can be of (wide tile of columns, key head) pairs: a counter for each
     float heads_by_target;
     bool halves_own;  // whether a share of wide tiles counts half of a request's own rows
     float scale_log2;  // |scale| * log2(e), not quite 0
@@ -88,6 +90,20 @@ __device__ __forceinline__ unsigned parts_of(const KvRequest &q, unsigned share,
     return max(1u, (key_tiles(q.length) + mine - 1) / mine);
 }
 
+// Calls `with` for requests first, first + stride, ... below end, whose loads are AHEAD at a time: a plan of many requests is a chain of them.
+template <int AHEAD, class With>
+__device__ __forceinline__ void for_requests(const KvAttentionArgs &p, int first, int end, int stride, With &&with)
+{
+    for (int r = first; r < end; r += AHEAD * stride) {
+        KvRequest q[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) q[i] = load_request(p, min(r + i * stride, end - 1));
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (r + i * stride < end) with(q[i]);
+    }
+}
+
 // Sums stop at 2^32 - 1 (and stay associative): those of any row offsets can be compared with what there is room for.
 __device__ __forceinline__ unsigned stopping_sum(unsigned x, unsigned y) { return __builtin_elementwise_add_sat(x, y); }
 // Sum over the lanes up to and with this one.
@@ -122,11 +138,13 @@ __device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvR
             others = other(q);
         } else {
             const int first = low + lane * step, end = min(low + left, first + step);
-            for (int r = first; r < end; ++r) {
-                q = load_request(p, r);
-                items = stopping_sum(items, count(q));
-                others = stopping_sum(others, other(q));
-            }
+            auto add = [&](const KvRequest &of) {
+                q = of;
+                items = stopping_sum(items, count(of));
+                others = stopping_sum(others, other(of));
+            };
+            if (step <= 2) for_requests<2>(p, first, end, 1, add);
+            else for_requests<8>(p, first, end, 1, add);
         }
         const unsigned to = wave_scan_sum(items), to_other = wave_scan_sum(others);
         const unsigned long long behind = __ballot(items_before + to > item);
@@ -206,8 +224,9 @@ __device__ __forceinline__ unsigned find_share(const KvAttentionArgs &p, const K
     if (p.requests <= 64) {
         tiles = count(own);
     } else {
-        const int step = (p.requests + 63) / 64, first = (threadIdx.x & 63) * step, end = min(p.requests, first + step);
-        for (int r = first; r < end; ++r) tiles += count(load_request(p, r));
+        auto add = [&](const KvRequest &q) { tiles += count(q); };
+        if (p.requests <= 128) for_requests<2>(p, threadIdx.x & 63, p.requests, 64, add);
+        else for_requests<8>(p, threadIdx.x & 63, p.requests, 64, add);
     }
     const float share = wave_sum(tiles) * p.heads_by_target * 1.001f + 1.0f;
     const unsigned whole = (static_cast<unsigned>(fminf(share, 1073741824.0f)) + 3u) & ~3u;  // (the same for each of four wavefronts)
@@ -583,8 +602,8 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
         unsigned share = 0x7fffffffu;
         if (p.parts) share = find_share(p, own, [&](const KvRequest &q) { return static_cast<float>(few_tiles(p, q)) * static_cast<float>(key_tiles(q.length)); });
         KvFound at;
-        const bool is = find_request(p, own, unit / p.kv_heads, p.units / p.kv_heads, p.items / p.kv_heads, [&](const KvRequest &q) { return few_tiles(p, q) * parts_of(q, share); },
-                                     [&](const KvRequest &q) { return few_tiles(p, q); }, &at);
+        const bool is = find_request(p, own, unit / p.kv_heads, p.units / p.kv_heads, p.room, [&](const KvRequest &q) { return few_tiles(p, q) * parts_of(q, share); },
+                                     [&](const KvRequest &q) { return parts_of(q, share) > 1 ? few_tiles(p, q) * parts_of(q, share) : 0; }, &at);
         if (lane == 0) {
             found = at;
             found_share = is ? share : 0;
@@ -611,7 +630,9 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
 #pragma unroll
     for (int t = 0; t < VT; ++t) *reinterpret_cast<f32x4 *>(&lds_out[(wave * kKvColumns + n) * OS + 16 * t + 4 * g]) = s.out[0][t];
     __syncthreads();
-    float *const statistics = p.parts + static_cast<size_t>(p.units) * kKvColumns * HD;
+    float *const statistics = p.parts + static_cast<size_t>(p.room) * p.kv_heads * kKvColumns * HD;
+    const size_t parts_before = at.before + static_cast<size_t>(column_tile) * parts;  // those of contexts that are cut
+    auto place = [&](unsigned of_part, int c) { return ((parts_before + of_part) * p.kv_heads + kv_head) * kKvColumns + c; };
     for (int i = tid; i < columns * (HD / 4); i += 256) {
         const int c = i / (HD / 4), d = i % (HD / 4) * 4;
         float most = -INFINITY;
@@ -627,10 +648,10 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
             total += *reinterpret_cast<const f32x4 *>(&lds_out[(w * kKvColumns + c) * OS + d]) * factor;
         }
         if (parts > 1) {
-            const size_t place = static_cast<size_t>(unit) * kKvColumns + c;
-            store_shared(p.parts + place * HD + d, float2{total[0], total[1]});
-            store_shared(p.parts + place * HD + d + 2, float2{total[2], total[3]});
-            if (d == 0) store_shared(statistics + 2 * place, float2{most, sum});
+            const size_t at_part = place(part, c);
+            store_shared(p.parts + at_part * HD + d, float2{total[0], total[1]});
+            store_shared(p.parts + at_part * HD + d + 2, float2{total[2], total[3]});
+            if (d == 0) store_shared(statistics + 2 * at_part, float2{most, sum});
         } else {
             *reinterpret_cast<u32x2 *>(out_at(p, at.of, kv_head, first + c, HD) + d) = rounded_four(total, inverse_of(sum));
         }
@@ -641,14 +662,13 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0) {
-        unsigned *const arrived = p.arrived + static_cast<size_t>(at.before + column_tile) * p.kv_heads + kv_head;
+        unsigned *const arrived = p.arrived + parts_before * p.kv_heads + kv_head;
         is_last = atomicAdd(arrived, 1u) == parts - 1;
         if (is_last) atomicExch(arrived, 0u);
     }
     __syncthreads();
     if (!is_last) return;
 
-    auto place = [&](unsigned of_part, int c) { return (static_cast<size_t>(unit) + (static_cast<size_t>(of_part) - part) * p.kv_heads) * kKvColumns + c; };
     // Sixteen bytes a thread; where there are fewer columns than rows of threads, several rows share a column's parts.  A thread asks for its
     // first parts before their factors are known: what this takes is one memory latency after the other, and what it asks for.  (One context of
     // 1000 keys and eight heads of 128 values: 8.8 us with 8 parts ahead, 9.5 with 16.)
@@ -944,7 +964,7 @@ __device__ __forceinline__ void attend_wide(const KvAttentionArgs &p, const KvWi
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (tid == 0) {
-            unsigned *const arrived = p.arrived + p.items + static_cast<size_t>(work.arrived) * p.kv_heads + kv_head;
+            unsigned *const arrived = p.arrived + (static_cast<size_t>(p.room) + work.arrived) * p.kv_heads + kv_head;
             is_last = atomicAdd(arrived, 1u) == parts - 1;
             if (is_last) atomicExch(arrived, 0u);
         }
@@ -1101,6 +1121,11 @@ constexpr int kKvFew = kKvWideTiles<HD> * 32;
 template <int HD>
 constexpr int kKvTarget = HD == 256 ? 256 : 512;
 
+// And the room for parts, for each key head: contexts that are cut are longer than one and a half shares, so that they are cut into fewer parts than 5/3
+// of their length in shares, and all contexts together are as many shares as there should be workgroups.
+template <int HD>
+constexpr int kKvRoom = kKvTarget<HD> * 5 / 3;
+
 template <int HD>
 hipError_t launch_kv_attention(KvAttentionArgs args, hipStream_t stream)
 {
@@ -1115,25 +1140,28 @@ hipError_t launch_kv_attention(KvAttentionArgs args, hipStream_t stream)
         tiles = std::min<long long>(tiles, static_cast<long long>(args.requests) * ((args.few + kKvColumns - 1) / kKvColumns));
     }
     const long long items = tiles * args.kv_heads, wide_items = wide_tiles * args.kv_heads;
-    args.items = static_cast<unsigned>(items);
+    args.room = static_cast<unsigned>(kKvRoom<HD> / args.kv_heads) + 1;
     args.wide_items = static_cast<unsigned>(wide_items);
     args.heads_by_target = static_cast<float>(args.kv_heads) / kKvTarget<HD>;
     const bool fills = wide_items > kKvTarget<HD>;
     args.halves_own = args.causal && !fills;
-    // Contexts are cut where there may be too few tiles of columns for the chip, or few enough that a context much longer than the others is
+    // Contexts of narrow tiles are cut wherever one may be longer than the least share, however many requests there are: a long one among many
+    // is what is waited for, and shares of a batch without such are longer than its contexts.  (420 and 1024 requests of 16 to 500 keys and one of 131072,
+    // a token each, 32 heads on 8 of 128 values: 1041 and 1106 us uncut, 115 and 261.  The plan reads all lengths once more for it: 1024 of 16
+    // to 2000 keys 299 uncut, 312.)
+    // Those of wide tiles are cut where there may be too few of these for the chip, or few enough that a context much longer than the others is
     // what is waited for.  (47 prompts of 24 rows over 16 to 6834 keys, 80 heads on 5: 166 us uncut, 105; 55 of 108 rows over up to 3537,
     // 16 on 1: 82 and 55.  Even batches pay for it: 8 of 500 rows 147 and 148 at dimension 128, 106 and 117 at 64.)
     // Cuts add at most a target of workgroups, and another where half of a prompt's own keys were left out of the sum that they share.
-    const bool cuts = (args.table_width << args.page_shift) > kKvLeastShare * kKvTile;
-    const bool cut = cuts && items <= 4096, wide_cut = cuts && wide_items != 0 && wide_items <= 4 * kKvTarget<HD>;
+    const bool cut = (args.table_width << args.page_shift) > kKvLeastShare * kKvTile, wide_cut = cut && wide_items != 0 && wide_items <= 4 * kKvTarget<HD>;
     long long units = items + (cut ? kKvTarget<HD> : 0), wide_units = wide_items + (wide_cut ? fills ? kKvTarget<HD> : 2 * kKvTarget<HD> : 0);
-    if (cut || wide_cut) {
-        const size_t floats = cut ? static_cast<size_t>(units) * kKvColumns * (HD + 2) : 0;
+    if (cut) {
+        const size_t room = static_cast<size_t>(args.room) * args.kv_heads, floats = room * kKvColumns * (HD + 2);
         void *scratch = nullptr;
         hipError_t rc = stream_workspace(stream, (floats + (wide_cut ? static_cast<size_t>(wide_units) * WIDTH * (HD + 2) : 0)) * sizeof(float), &scratch);
-        if (rc == hipSuccess) rc = stream_counters(stream, static_cast<size_t>(items + (wide_cut ? wide_items : 0)), &args.arrived);
+        if (rc == hipSuccess) rc = stream_counters(stream, room + (wide_cut ? static_cast<size_t>(wide_items) : 0), &args.arrived);
         if (rc == hipSuccess) {
-            if (cut) args.parts = static_cast<float *>(scratch);
+            args.parts = static_cast<float *>(scratch);
             if (wide_cut) args.wide_parts = static_cast<float *>(scratch) + floats;
         } else if (scratch_unavailable(rc)) {
             units = items;

@@ -304,6 +304,26 @@ def test_many_prompts_of_uneven_lengths(hip, dim, kv_heads, group, fresh):
         check_attention(hip, rng, 64, kv_heads, dim, group, lengths, [fresh] * 64, causal)
 
 
+@pytest.mark.parametrize("requests,dim,kv_heads,group", [(65, 64, 2, 1), (130, 128, 1, 4), (600, 64, 1, 2), (70, 256, 1, 2)])
+def test_many_requests_of_long_contexts(hip, requests, dim, kv_heads, group):
+    """More than 64 requests, with contexts long enough that some are cut; some bring no row, some several."""
+    rng = np.random.default_rng(requests + dim)
+    lengths, fresh = rng.integers(300, 1000, requests), rng.integers(0, 3, requests)
+    lengths[rng.permutation(requests)[:4]] = 5000, 4095, 3001, 4500
+    for causal in (True, False):
+        check_attention(hip, rng, 64, kv_heads, dim, group, lengths.tolist(), fresh.tolist(), causal)
+
+
+@pytest.mark.parametrize("requests,dim", [(1100, 64), (700, 128)])
+def test_a_long_context_among_very_many(hip, requests, dim):
+    """The one long context is first, last and between, and short ones are next to it."""
+    rng = np.random.default_rng(requests)
+    for at in (0, requests // 2 + 1, requests - 1):
+        lengths = rng.integers(0, 20, requests)
+        lengths[at] = 9000
+        check_attention(hip, rng, 16, 6, dim, 1, lengths.tolist(), [1] * requests, True)
+
+
 def test_rows_without_keys(hip):
     """More rows than tokens: the first see none, and are 0; requests of no length, of a negative one."""
     rng = np.random.default_rng(1)
@@ -315,20 +335,20 @@ def test_rows_without_keys(hip):
 
 @pytest.mark.parametrize("requests,rows,dim,group", [(8, 40, 64, 1), (130, 50, 64, 2), (6, 300, 64, 1), (200, 700, 128, 1), (7, 130, 256, 2)])
 def test_row_offsets_out_of_order(hip, requests, rows, dim, group):
-    """Offsets that rise and fall claim more tiles of columns than the rows have, by more than there are counters for but less than there are
-    workgroups: nothing is written, and the calls after it are right."""
+    """Offsets that rise and fall claim more tiles of columns than the rows have: nothing behind the rows is written, and the calls after it, which
+    count in the same places, are right."""
     rng = np.random.default_rng(rows)
     store = Pages(hip, rng, 20, 64, 1, dim)
     width = 40
     d_q = hip.DeviceBuffer.from_array(inputs.to_bf16(rng.normal(size=(rows, group * dim)).astype(np.float32)))
-    out = hip.DeviceBuffer.from_array(np.full((rows, group * dim), 0x4321, np.uint16))
+    out = hip.DeviceBuffer.from_array(np.full((rows + 9, group * dim), 0x4321, np.uint16))
     d_table, d_lengths = dev(hip, rng.integers(0, 20, (requests, width))), dev(hip, rng.integers(1000, 2500, requests))
     offsets = np.where(np.arange(requests + 1) % 2 == 1, rows, 0)
     for causal in (True, False):
         hip.attention_kv_cache_bf16_dev(store.cache, requests, rows, group, 0.1, causal, dev(hip, offsets), d_lengths, d_table, width, d_q, group * dim,
                                         out, group * dim)
         hip.device_synchronize()
-        assert (out.to_array(np.uint16, (rows, group * dim)) == 0x4321).all()
+        assert (out.to_array(np.uint16, (rows + 9, group * dim))[rows:] == 0x4321).all()
         check_attention(hip, rng, 64, 1, dim, group, [2100, 5, 1500], [1, 1, 2], causal)
         check_attention(hip, rng, 64, 1, dim, group, [1500, 300], [rows // 2, 1], causal)
 

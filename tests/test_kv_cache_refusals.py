@@ -182,6 +182,18 @@ for fail in (1, 0):
     assert out[0] == "22" and int(out[1]) > 22  # eight narrow tiles of columns and three wide ones, of two heads
 
 
+def test_contexts_are_cut_among_any_number_of_requests(stub):
+    """Two key heads, a narrow tile of columns for each request and one for each sixteen columns, and 512 workgroups more for parts; none more for
+    a table of no more keys than a workgroup takes."""
+    out = run(stub, """
+for requests in (60, 2040, 5000):
+    for width in (2000, 4):
+        hip.attention_kv_cache_bf16_dev(cache(pages=4000), requests, requests, 4, 0.1, True, M, 2 * M, 2**40, width, 2**41, 256, 2**42, 256)
+        print(grid.value - 2 * (requests + requests * 2 // 16))
+""")
+    assert out == ["512", "0"] * 3
+
+
 def test_null_structures():
     from spiraltorch_amd import hip
     with pytest.raises(ValueError):
