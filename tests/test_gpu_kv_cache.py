@@ -324,6 +324,23 @@ def test_a_long_context_among_very_many(hip, requests, dim):
         check_attention(hip, rng, 16, 6, dim, 1, lengths.tolist(), [1] * requests, True)
 
 
+@pytest.mark.parametrize("dim,group,length,fresh", [(64, 1, 32700, 1), (128, 1, 65530, 2), (256, 1, 32768, 1), (64, 16, 40000, 1), (128, 16, 32701, 1),
+                                                    (64, 4, 12200, 70), (128, 4, 12280, 70), (256, 4, 12200, 35), (128, 2, 20000, 40)])
+def test_as_many_parts_as_there_can_be(hip, dim, group, length, fresh):
+    """One context on one key head, cut into up to 128 parts of narrow tiles of columns or up to 16 of wide ones, whose shares then grow."""
+    check_attention(hip, np.random.default_rng(length), 256, 1, dim, group, [length], [fresh], True)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_long_prompts_among_many_requests(hip, dim):
+    """More than 64 requests, three of them with prompts that are cut, beside single tokens and requests that wait."""
+    rng = np.random.default_rng(dim)
+    lengths, fresh = rng.integers(1, 200, 90), rng.integers(0, 2, 90)
+    for r, n, rows in ((3, 2500, 75), (64, 1800, 80), (89, 3000, 70)):
+        lengths[r], fresh[r] = n, rows
+    check_attention(hip, rng, 64, 1, dim, 2, lengths.tolist(), fresh.tolist(), True)
+
+
 def test_rows_without_keys(hip):
     """More rows than tokens: the first see none, and are 0; requests of no length, of a negative one."""
     rng = np.random.default_rng(1)
