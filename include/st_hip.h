@@ -103,7 +103,9 @@ int st_hip_device_synchronize(void);
 /* Scratch memory (split-k partial sums, re-laid weights, padded operand copies) is kept per (stream, host thread) and
  * grows on demand; a buffer whose host thread has exited is re-used by the next thread that launches on that stream,
  * and st_hip_stream_destroy frees its stream's buffers.  A call recorded into a graph keeps the buffers it was handed, which
- * later calls on the stream and thread use as well: replay the graph on that stream, or ordered with its work.  A buffer
+ * later calls on the stream and thread use as well: replay the graph on that stream, or ordered with its work.  (Beside it, both read what the
+ * other wrote; and attention over a paged cache, which counts its parts there, may then be wrong in later calls too, until
+ * st_hip_release_scratch.)  A buffer
  * that a graph may hold is not freed when the stream's scratch grows past it, only with the stream or by
  * st_hip_release_scratch; the graph must not be replayed after that.  What is kept is what the largest call on a stream
  * needed, up to 2 GiB of re-laid operands for f32 products and convolutions beside the partial sums.  st_hip_release_scratch waits for `stream` (NULL = the default
