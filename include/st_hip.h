@@ -559,7 +559,8 @@ int st_hip_kv_cache_append_bf16_dev(const st_hip_kv_cache *cache, size_t rows, c
  * rounded to bf16.  heads is a multiple of kv_heads, and head h reads keys of head h / (heads/kv_heads).  `causal` != 0: a request's rows
  * are its last tokens, the last row sees all lengths[r] keys and each one before it one key less; 0: every row sees all of them (an
  * encoder's states).  Rows that see no key are 0.  A length counts as at most table_width pages; tokens of pages outside the cache
- * are left out.  scale times log2(e) has to be within f32 (ST_HIP_ERR_UNSUPPORTED).  The products take bf16 and accumulate in f32, the softmax is f32; its weights enter the second product as bf16.
+ * are left out.  scale times log2(e) has to be within f32 (ST_HIP_ERR_UNSUPPORTED).  The products take bf16 and accumulate in f32, the softmax
+ * is f32; its weights enter the second product as two pieces of bf16 for requests of few rows, as one (2^-8 of each weight) for others.
  * out may be columns of q's rows that q does not meet, and overlaps nothing else that is read.
  * q 16-byte and out 8-byte aligned, ld_q a multiple of 8 and ld_out of 4, otherwise ST_HIP_ERR_UNSUPPORTED.  Long contexts of few rows
  * are cut over workgroups, whose parts go through the stream's scratch memory. */

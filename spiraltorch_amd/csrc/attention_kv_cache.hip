@@ -362,8 +362,8 @@ __device__ __forceinline__ void lower_for(float value_scale, KvColumnsState<HD, 
 
 // A tile's scores (products of queries and keys; -infinity where a column does not see the key) to the weights of its values, and the
 // columns' maxima, sums and outputs with them.
-template <int HD, int NC>
-__device__ __forceinline__ void weigh(const KvAttentionArgs &p, f32x4 (&scores)[NC][4], KvColumnsState<HD, NC> &s, bf16x8 (&weights)[NC][2])
+template <int HD, int NC, int PIECES>
+__device__ __forceinline__ void weigh(const KvAttentionArgs &p, f32x4 (&scores)[NC][4], KvColumnsState<HD, NC> &s, bf16x8 (&weights)[PIECES][NC][2])
 {
     float most[NC];
     bool grows = false;
@@ -389,28 +389,38 @@ __device__ __forceinline__ void weigh(const KvAttentionArgs &p, f32x4 (&scores)[
             for (int t = 0; t < HD / 16; ++t) s.out[c][t] *= shrink;
         }
     }
-    // Weights are rounded to bf16 for the second product, which is that of bf16, and summed as they are rounded: what their rounding adds to it, it
-    // adds to the sum as well.  The result's error is 0.0017 to 0.0019 of its size (root mean square) so, and 0.00166, its own rounding to bf16,
-    // with what their rounding leaves as a second piece.  That piece costs half of a tile's products again and 40 other instructions: of narrow tiles, decode_64x8192 41.1 and 42.1 us, cross_16x1500 12.2 and 13.1, 16 contexts of 2000 keys with 16 rows of 64 values 20.9 and
-    // 22.7; wide ones are bound by the issue of just these.
+    // Weights go into the second product, which is that of bf16, as two pieces of it (the second is what the first's rounding leaves: 2^-16 of a
+    // weight is lost) or as one, and are summed as they go in: what their rounding adds to the values' sum, it adds to the weights' as well.  With
+    // two the result's error is that of its own rounding to bf16, 0.00166 of its size (root mean square), with one 0.0017 to 0.0019.  The second
+    // piece costs half of a tile's products again and 40 other instructions.  Narrow tiles wait for memory most of the time and have it
+    // (decode_64x8192 41.0 us with one piece and 42.0 with two, decode_1x4097 10.8 and 11.0, cross_16x1500 12.1 and 12.9, 16 contexts of 2000 keys
+    // with 16 rows of 64 values 21.2 and 23.2); wide ones are bound by the issue of just these (prefill_8x500 148 and 189, the same at 64 values 117
+    // and 166) and have one.
     const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const float base = s.run_max[c] == -INFINITY ? 0.0f : s.run_max[c];  // (a column that has seen nothing: its weights are 2^-inf)
-        u32x4 packed[2];
+        u32x4 packed[PIECES][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(scores[c][i][e], p.scale_log2, -base));
-            packed[i >> 1][2 * (i & 1)] = pack_bf16x2_rne(w[0], w[1]);
-            packed[i >> 1][2 * (i & 1) + 1] = pack_bf16x2_rne(w[2], w[3]);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const unsigned pair = pack_bf16x2_rne(w[2 * half], w[2 * half + 1]);
+                packed[0][i >> 1][2 * (i & 1) + half] = pair;
+                if constexpr (PIECES == 2)
+                    packed[1][i >> 1][2 * (i & 1) + half] = pack_bf16x2_rne(w[2 * half] - __uint_as_float(pair << 16), w[2 * half + 1] - __uint_as_float(pair & 0xffff0000u));
+            }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            weights[c][h] = __builtin_bit_cast(bf16x8, packed[h]);
-            s.sum[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), weights[c][h], s.sum[c], 0, 0, 0);
-        }
+        for (int piece = 0; piece < PIECES; ++piece)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                weights[piece][c][h] = __builtin_bit_cast(bf16x8, packed[piece][h]);
+                s.sum[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), weights[piece][c][h], s.sum[c], 0, 0, 0);
+            }
     }
 }
 
@@ -520,8 +530,8 @@ __device__ __forceinline__ void attend(const KvAttentionArgs &p, const KvRequest
 
         if (!whole) hide_unseen<HD, NC>(s, key0, value_fits, scores);
         lower_for<HD, NC>(value_scale, s);
-        bf16x8 weights[NC][2];
-        weigh<HD, NC>(p, scores, s, weights);
+        bf16x8 weights[2][NC][2];
+        weigh<HD, NC, 2>(p, scores, s, weights);
         if (!whole) {
             unsigned is = 0;  // (see mark_nan)
 #pragma unroll
@@ -541,9 +551,12 @@ __device__ __forceinline__ void attend(const KvAttentionArgs &p, const KvRequest
         for (int t = 0; t < VT; ++t) {
             const bf16x8 low = widened(value_codes[t][0], value_codes[t][1], value_scale), high = widened(value_codes[t][2], value_codes[t][3], value_scale);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(low, weights[c][0], s.out[c][t], 0, 0, 0);
+            for (int piece = 0; piece < 2; ++piece) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(high, weights[c][1], s.out[c][t], 0, 0, 0);
+                for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(low, weights[piece][c][0], s.out[c][t], 0, 0, 0);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(high, weights[piece][c][1], s.out[c][t], 0, 0, 0);
+            }
         }
         if (more) {
             load_values(next, value_page);
@@ -902,8 +915,8 @@ __device__ __forceinline__ void attend_wide(const KvAttentionArgs &p, const KvWi
         const bool whole = fits == 15 && key0 + kKvTile <= static_cast<unsigned>(s.fewest);
         if (__builtin_expect(!whole, 0)) hide_unseen<HD, NC>(s, key0, fits >> g & 1, scores);
         lower_for<HD, NC>(scale_of_values, s);
-        bf16x8 weights[NC][2];
-        weigh<HD, NC>(p, scores, s, weights);
+        bf16x8 weights[1][NC][2];
+        weigh<HD, NC, 1>(p, scores, s, weights);
         unsigned nan = 0;
 #pragma unroll
         for (int t = 0; t < VT; ++t) {
@@ -912,9 +925,9 @@ __device__ __forceinline__ void attend_wide(const KvAttentionArgs &p, const KvWi
             if (__builtin_expect(!whole, 0)) nan |= drop_nan(codes);
             const bf16x8 low = widened(codes[0], codes[1], scale_of_values), high = widened(codes[2], codes[3], scale_of_values);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(low, weights[c][0], s.out[c][t], 0, 0, 0);
+            for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(low, weights[0][c][0], s.out[c][t], 0, 0, 0);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(high, weights[c][1], s.out[c][t], 0, 0, 0);
+            for (int c = 0; c < NC; ++c) s.out[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(high, weights[0][c][1], s.out[c][t], 0, 0, 0);
         }
         if (__any(nan != 0)) nan_first = min(nan_first, tile);
     };

@@ -108,13 +108,13 @@ def append(codes, scales, slots, rows, transposed):
                 block[place] = narrow(np.where(np.abs(y) <= 448.0, y, np.nan))
 
 
-def attention(k, v, k_scales, v_scales, offsets, lengths, table, q, scale, causal):
+def attention(k, v, k_scales, v_scales, offsets, lengths, table, q, scale, causal, weight_step=2.0**-8):
     """k (pages, heads, page, dim), v (pages, heads, dim, page) codes; q (rows, heads, dim) float64.  The result, the rows that belong to
     a request, and how far a result may be off that is computed as the kernel does it:
 
       a score is a sum of head_dim products in f32 in any order, times two scales and log2(e): (head_dim + 4) half steps of the sum of
       the sizes, and one more for the difference to the maximum; a weight carries twice that, as the largest score shifts all of them;
-      its power of two a few steps; weights are rounded to bf16 (2^-8 of each), in the sum of the weights as in that of the values: a
+      its power of two a few steps; weights are rounded to bf16 (2^-8 of each, or weight_step where they are in pieces), in the sum of the weights as in that of the values: a
       result sum(w v) / sum(w) moves by sum(dw (v - result)) / sum(w); both are summed in f32 (a half step per key at the most), and
       the result is rounded to bf16."""
     rows, heads, dim = q.shape
@@ -144,6 +144,6 @@ def attention(k, v, k_scales, v_scales, offsets, lengths, table, q, scale, causa
                         out[i, head] = weights @ values[seen] / total
                         sizes = (weights @ np.abs(values[seen])) / total
                         off = (dim + 8) * 2.0**-24 * np.max(np.abs(keys[seen]) @ np.abs(x)) * abs(scale)
-                    weights_off = 2.0**-8 * 1.01 + 4 * off + (8 + seen.sum()) * 2.0**-24
+                    weights_off = weight_step * 1.01 + 4 * off + (8 + seen.sum()) * 2.0**-24
                     bound[i, head] = 2.0**-8 * np.abs(out[i, head]) + weights_off * (sizes + np.abs(out[i, head]))
     return out, mine, bound

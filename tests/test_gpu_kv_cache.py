@@ -202,7 +202,7 @@ def test_values_that_are_not_numbers(hip, kind):
 # ---- attention ------------------------------------------------------------------------------------------------------------------
 
 def check_attention(hip, rng, page, kv_heads, dim, group, lengths, fresh, causal, scale=None, behind=3, pages=None, width=None, edit=None,
-                    stale=0x7f, extra=0, q_size=1.5, what=""):
+                    stale=0x7f, extra=0, q_size=1.5, weight_step=2.0**-8, what=""):
     """A ragged batch over a cache whose places behind the lengths, and unused pages and their scales, hold NaN (`stale`)."""
     requests, heads = len(lengths), kv_heads * group
     used = [-(-max(0, n) // page) for n in lengths]
@@ -237,7 +237,8 @@ def check_attention(hip, rng, page, kv_heads, dim, group, lengths, fresh, causal
     hip.device_synchronize()
     bits = out.to_array(np.uint16, (rows, ld_out))
     q = inputs.from_bf16(q_bits[:, :heads * dim].ravel()).astype(np.float64).reshape(rows, heads, dim)
-    want, mine, bound = plain.attention(store.k, store.v, store.k_scales, store.v_scales, offsets, lengths, table, q, float(np.float32(scale)), causal)
+    want, mine, bound = plain.attention(store.k, store.v, store.k_scales, store.v_scales, offsets, lengths, table, q, float(np.float32(scale)), causal,
+                                        weight_step)
     assert (bits[~mine] == 0x4321).all() and (bits[:, heads * dim:] == 0x4321).all(), f"{what}: rows or columns behind the batch's"
     got = inputs.from_bf16(bits[:, :heads * dim].ravel()).astype(np.float64).reshape(rows, heads, dim)[mine]
     want, bound = want[mine], bound[mine]
@@ -420,6 +421,12 @@ def test_numbers_that_are_none(hip, dim):
     got = check_attention(hip, rng, 16, 2, dim, 2, [100, 90], [40, 40], True, edit=edit, stale=0x7f)
     assert np.isnan(got).any() and not np.isnan(got).all()
     check_attention(hip, rng, 16, 2, dim, 2, [100, 90], [40, 40], False, edit=edit, stale=0xff)
+
+
+@pytest.mark.parametrize("dim,group,lengths,fresh", [(64, 4, [700, 90], [1, 3]), (128, 4, [6000, 5], [1, 1]), (256, 2, [900, 2000], [2, 10]), (64, 16, [500], [8])])
+def test_weights_of_few_rows(hip, dim, group, lengths, fresh):
+    """Two pieces of bf16 hold a weight: the first is off by 2^-8 of it at the most, the second by 2^-8 of that."""
+    check_attention(hip, np.random.default_rng(dim), 64, 2, dim, group, lengths, fresh, True, weight_step=2.0**-16)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 3.0, 1e-30])
