@@ -79,29 +79,38 @@ __device__ __forceinline__ unsigned few_tiles(const KvAttentionArgs &p, const Kv
 // not longer than two: putting parts together takes 3 us, and its last part would leave a workgroup with little to do.  (16 contexts of 300 to
 // 1000 keys with 64 columns each took 26 us when cut at every share, and 19 so; 12 heads' 16 contexts of 1500 keys, 24 tiles at a share
 // of 12, 14.4 and 12.0; decoding 64 contexts of up to 8192 41.2 and 40.2, and 43.5 with contexts of up to two shares whole.)
-__device__ __forceinline__ unsigned share_of(const KvRequest &q, unsigned share, unsigned most = kKvMostParts)
+__device__ __forceinline__ unsigned share_of_tiles(unsigned tiles, unsigned share, unsigned most)
 {
-    const unsigned tiles = key_tiles(q.length), mine = max(share, ((tiles + most - 1) / most + 3u) & ~3u);
+    const unsigned mine = max(share, ((tiles + most - 1) / most + 3u) & ~3u);
     return tiles <= max(mine + mine / 2, min(2 * mine, 24u)) ? max(tiles, 1u) : mine;
 }
+__device__ __forceinline__ unsigned share_of(const KvRequest &q, unsigned share, unsigned most = kKvMostParts) { return share_of_tiles(key_tiles(q.length), share, most); }
 __device__ __forceinline__ unsigned parts_of(const KvRequest &q, unsigned share, unsigned most = kKvMostParts)
 {
     const unsigned mine = share_of(q, share, most);
     return max(1u, (key_tiles(q.length) + mine - 1) / mine);
 }
 
-// Calls `with` for requests first, first + stride, ... below end, whose loads are AHEAD at a time: a plan of many requests is a chain of them.
+// Calls `with` for this lane's requests, `step` of them from low + lane * step on and below end, whose loads are two or eight at a time: a plan
+// of many requests is a chain of them.
 template <int AHEAD, class With>
-__device__ __forceinline__ void for_requests(const KvAttentionArgs &p, int first, int end, int stride, With &&with)
+__device__ __forceinline__ void for_requests_by(const KvAttentionArgs &p, int first, int end, With &&with)
 {
-    for (int r = first; r < end; r += AHEAD * stride) {
+    for (int r = first; r < end; r += AHEAD) {
         KvRequest q[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) q[i] = load_request(p, min(r + i * stride, end - 1));
+        for (int i = 0; i < AHEAD; ++i) q[i] = load_request(p, min(r + i, end - 1));
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
-            if (r + i * stride < end) with(q[i]);
+            if (r + i < end) with(q[i]);
     }
+}
+template <class With>
+__device__ __forceinline__ void for_requests(const KvAttentionArgs &p, int low, int end, int step, With &&with)
+{
+    const int first = low + (threadIdx.x & 63) * step;
+    if (step <= 2) for_requests_by<2>(p, first, min(end, first + step), with);
+    else for_requests_by<8>(p, first, min(end, first + step), with);
 }
 
 // Sums stop at 2^32 - 1 (and stay associative): those of any row offsets can be compared with what there is room for.
@@ -115,17 +124,19 @@ __device__ __forceinline__ unsigned wave_scan_sum(unsigned v)
 // Work is numbered by prefix sums over the requests, which a wavefront of every workgroup takes: `count(request)` items each, and the
 // request of item number `item` is found by 64 sums at a time (one round of loads for up to 64 requests, two for 4096 ...).  `own`: this lane's
 // request where there are no more than 64.
+constexpr unsigned kKvWhole = 0x7fffffffu;  // as a share: no context is cut
 struct KvFound {
     KvRequest of;
     unsigned offset;  // of the item within its request's
     unsigned before;  // sum of `other` over the requests before it
 };
 // False behind the last item; and for all items where they, or `other`, are more than there is room for, which row offsets out of order can make
-// them: a launch does all the work of one kind or none of it, and its counters are within their buffer and 0 after it.
+// them: a launch does all the work of one kind or none of it, and its counters are within their buffer and 0 after it.  `known`, if it is: the sum
+// of `count` over this lane's requests of the first level, where `before` will not be looked at.
 template <class Count, class Other>
-__device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvRequest &own, unsigned item, unsigned most, unsigned most_other, Count &&count, Other &&other, KvFound *found)
+__device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvRequest &own, unsigned item, unsigned most, unsigned most_other, Count &&count, Other &&other, KvFound *found,
+                                             bool is_known, unsigned known)
 {
-    const int lane = threadIdx.x & 63;
     int low = 0, left = p.requests;
     unsigned items_before = 0;
     found->before = 0;
@@ -136,15 +147,14 @@ __device__ __forceinline__ bool find_request(const KvAttentionArgs &p, const KvR
         if (p.requests <= 64) {
             items = count(q);
             others = other(q);
+        } else if (is_known && left == p.requests) {
+            items = known;
         } else {
-            const int first = low + lane * step, end = min(low + left, first + step);
-            auto add = [&](const KvRequest &of) {
+            for_requests(p, low, low + left, step, [&](const KvRequest &of) {
                 q = of;
                 items = stopping_sum(items, count(of));
                 others = stopping_sum(others, other(of));
-            };
-            if (step <= 2) for_requests<2>(p, first, end, 1, add);
-            else for_requests<8>(p, first, end, 1, add);
+            });
         }
         const unsigned to = wave_scan_sum(items), to_other = wave_scan_sum(others);
         const unsigned long long behind = __ballot(items_before + to > item);
@@ -214,23 +224,42 @@ __device__ __forceinline__ KvRequest longest_first(const KvAttentionArgs &p, con
     return KvRequest{moved(own.first_row), moved(own.rows), moved(own.length), moved(own.id)};
 }
 
-// The 64-key tiles that a workgroup takes of a context at the most: all the tiles that there are, `count(request)` for one, over the
+// Workgroups that all contexts are cut over, beside one for each tile of columns: as many as the chip holds at once of the kernel's registers
+// for 128 and 256 values.  (64 contexts of 16 to 8192 keys and eight heads took 45, 41, 41 and 46 us with 256, 384, 512 and 768 of them at
+// dimension 128, 24, 22 and 22 with 256, 512 and 1024 at 64; at 256, two heads, 30, 34 and 43.)
+template <int HD>
+constexpr int kKvTarget = HD == 256 ? 256 : 512;
+
+// The 64-key tiles that a workgroup takes of a context at the most: all the tiles that there are, `work(request)` for one, over the
 // workgroups that there should be.  Contexts of very different lengths fill the chip evenly so, whatever the host knows of them (it
-// knows the table's width alone).
-template <class Count>
-__device__ __forceinline__ unsigned find_share(const KvAttentionArgs &p, const KvRequest &own, Count &&count)
+// knows the table's width alone).  `work` is 0 where `tiles(request)`, the tiles of columns, are.  The one look at more than 64 requests also says
+// whether even the longest is not cut (kKvWhole), and how many items there are at the most, where cuts add up to `more`: 1024 requests with a
+// token each, none cut, 267 us, 318 when all were counted once more; a prompt of 500 rows beside 511 that wait 80 and 92.
+struct KvShare {
+    unsigned share, tiles, most_items;  // tiles: this lane's, of columns
+};
+template <class Tiles, class Work>
+__device__ __forceinline__ KvShare find_share(const KvAttentionArgs &p, const KvRequest &own, unsigned most_parts, unsigned more, Tiles &&tiles, Work &&work)
 {
-    float tiles = 0.0f;  // (rounded, but alike in every workgroup, and what it may fall short of the sum by is added below)
+    float all = 0.0f;  // (rounded, but alike in every workgroup, and what it may fall short of the sum by is added below)
+    unsigned longest = 0, mine = 0;
     if (p.requests <= 64) {
-        tiles = count(own);
+        all = work(own);
     } else {
-        auto add = [&](const KvRequest &q) { tiles += count(q); };
-        if (p.requests <= 128) for_requests<2>(p, threadIdx.x & 63, p.requests, 64, add);
-        else for_requests<8>(p, threadIdx.x & 63, p.requests, 64, add);
+        for_requests(p, 0, p.requests, (p.requests + 63) / 64, [&](const KvRequest &q) {
+            const unsigned columns = tiles(q);
+            mine = stopping_sum(mine, columns);
+            all += work(q);
+            if (columns != 0) longest = max(longest, key_tiles(q.length));
+        });
     }
-    const float share = wave_sum(tiles) * p.heads_by_target * 1.001f + 1.0f;
-    const unsigned whole = (static_cast<unsigned>(fminf(share, 1073741824.0f)) + 3u) & ~3u;  // (the same for each of four wavefronts)
-    return __builtin_amdgcn_readfirstlane(max(static_cast<unsigned>(kKvLeastShare), whole));
+    const float even = wave_sum(all) * p.heads_by_target * 1.001f + 1.0f;
+    const unsigned whole = (static_cast<unsigned>(fminf(even, 1073741824.0f)) + 3u) & ~3u;  // (the same for each of four wavefronts)
+    const unsigned share = __builtin_amdgcn_readfirstlane(max(static_cast<unsigned>(kKvLeastShare), whole));
+    if (p.requests <= 64) return KvShare{share, 0, ~0u};
+    longest = __builtin_amdgcn_readlane(wave_scan(longest, [](unsigned x, unsigned y) { return max(x, y); }), 63);
+    const unsigned most_items = stopping_sum(__builtin_amdgcn_readlane(wave_scan_sum(mine), 63), more);
+    return KvShare{share_of_tiles(longest, share, most_parts) >= longest ? kKvWhole : share, mine, most_items};
 }
 
 // Eight e4m3 values times a power of two, as bf16: both are exact.
@@ -615,11 +644,15 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
     const int kv_head = unit % p.kv_heads;  // neighbouring workgroups, on different XCDs, share nothing
     if (wave == 0) {
         const KvRequest own = longest_first<false>(p, own_request(p));
-        unsigned share = 0x7fffffffu;
-        if (p.parts) share = find_share(p, own, [&](const KvRequest &q) { return static_cast<float>(few_tiles(p, q)) * static_cast<float>(key_tiles(q.length)); });
+        auto tiles = [&](const KvRequest &q) { return few_tiles(p, q); };
+        KvShare even{kKvWhole, 0, ~0u};
+        if (p.parts)
+            even = find_share(p, own, kKvMostParts, kKvTarget<HD>, tiles, [&](const KvRequest &q) { return static_cast<float>(tiles(q)) * static_cast<float>(key_tiles(q.length)); });
+        const unsigned share = even.share;
         KvFound at;
-        const bool is = find_request(p, own, unit / p.kv_heads, p.units / p.kv_heads, p.room, [&](const KvRequest &q) { return few_tiles(p, q) * parts_of(q, share); },
-                                     [&](const KvRequest &q) { return parts_of(q, share) > 1 ? few_tiles(p, q) * parts_of(q, share) : 0; }, &at);
+        const bool is = unit / p.kv_heads < even.most_items && find_request(p, own, unit / p.kv_heads, p.units / p.kv_heads, p.room, [&](const KvRequest &q) { return tiles(q) * parts_of(q, share); },
+                                     [&](const KvRequest &q) { return parts_of(q, share) > 1 ? tiles(q) * parts_of(q, share) : 0; }, &at,
+                                     p.parts && share == kKvWhole, even.tiles);
         if (lane == 0) {
             found = at;
             found_share = is ? share : 0;
@@ -1070,14 +1103,15 @@ __device__ __forceinline__ void many_columns(const KvAttentionArgs &p, unsigned 
     };
     if (wave == 0) {
         const KvRequest own = longest_first<true>(p, own_request(p));
-        unsigned share = 0x7fffffffu;
+        KvShare even{kKvWhole, 0, ~0u};
         if (CUT)  // (of the rows that see their own keys one by one, each sees half of them on average)
-            share = find_share(p, own, [&](const KvRequest &q) {
+            even = find_share(p, own, kKvMostWideParts, 2 * kKvTarget<HD>, tiles_of, [&](const KvRequest &q) {
                 return static_cast<float>(tiles_of(q)) * (static_cast<float>(key_tiles(q.length)) - (p.halves_own ? 0.5f / kKvTile * min(q.rows, q.length) : 0.0f));
             });
+        const unsigned share = even.share;
         KvFound at;
-        const bool is = find_request(p, own, item / p.kv_heads, p.wide / p.kv_heads, p.wide_items / p.kv_heads, [&](const KvRequest &q) { return tiles_of(q) * (CUT ? parts_of(q, share, kKvMostWideParts) : 1); },
-                                     tiles_of, &at);
+        const bool is = item / p.kv_heads < even.most_items && find_request(p, own, item / p.kv_heads, p.wide / p.kv_heads, p.wide_items / p.kv_heads, [&](const KvRequest &q) { return tiles_of(q) * (CUT ? parts_of(q, share, kKvMostWideParts) : 1); },
+                                     tiles_of, &at, CUT && share == kKvWhole, even.tiles);
         if (lane == 0) {
             found = at;
             found_share = is ? share : 0;
@@ -1130,12 +1164,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 ?
 // keys: 60 us in wide tiles, 25 without.  At 64 columns, 16 contexts of 2000: 39 and 33 of dimension 128, 95 and 73 of 256.)
 template <int HD>
 constexpr int kKvFew = kKvWideTiles<HD> * 32;
-// Workgroups that all contexts are cut over, beside one for each tile of columns: as many as the chip holds at once of the kernel's registers
-// for 128 and 256 values.  (64 contexts of 16 to 8192 keys and eight heads took 45, 41, 41 and 46 us with 256, 384, 512 and 768 of them at
-// dimension 128, 24, 22 and 22 with 256, 512 and 1024 at 64; at 256, two heads, 30, 34 and 43.)
-template <int HD>
-constexpr int kKvTarget = HD == 256 ? 256 : 512;
-
 // And the room for parts, for each key head: contexts that are cut are longer than one and a half shares, so that they are cut into fewer parts than 5/3
 // of their length in shares, and all contexts together are as many shares as there should be workgroups.
 template <int HD>
@@ -1149,9 +1177,9 @@ hipError_t launch_kv_attention(KvAttentionArgs args, hipStream_t stream)
     long long tiles = columns / kKvColumns + args.requests, wide_tiles = 0;  // of sixteen columns: each request has one that is not full
     args.few = 0x7fffffff;
     // Each request counts as one row, so that single tokens, however many requests they are of, have the kernel of narrow tiles alone (64 of up to
-    // 4096 keys 23.7 us there and 26.1 in the other, 256 of 64 values 61.5 and 84.9).  A prompt among as many that wait goes there as well: one of 300
-    // rows behind 2000 keys beside 511 that wait takes 57 us in either, one of 100 34 and 48, one of 500 85 and 76.  A caller to whom the latter matters
-    // leaves out who waits, or gives more rows.
+    // 4096 keys 24.4 us there and 27.4 in the other, 256 of 64 values 61.4 and 82.6).  A prompt among as many that wait goes there as well: one of 300
+    // rows behind 2000 keys beside 511 that wait takes 54 us there and 53 in wide tiles, one of 100 49 and 44, one of 500 80 and 70, at 64 values 38 and
+    // 49.  A caller to whom that matters leaves out who waits, or gives more rows.
     if (static_cast<long long>(args.rows - args.requests) * args.group > kKvFew<HD>) {
         args.few = kKvFew<HD>;
         // Requests that are wide have more than `few` columns: so many at the most.
@@ -1166,8 +1194,8 @@ hipError_t launch_kv_attention(KvAttentionArgs args, hipStream_t stream)
     args.halves_own = args.causal && !fills;
     // Contexts of narrow tiles are cut wherever one may be longer than the least share, however many requests there are: a long one among many
     // is what is waited for, and shares of a batch without such are longer than its contexts.  (420 and 1024 requests of 16 to 500 keys and one of 131072,
-    // a token each, 32 heads on 8 of 128 values: 1041 and 1106 us uncut, 115 and 261.  The plan reads all lengths once more for it: 1024 of 16
-    // to 2000 keys 299 uncut, 312.)
+    // a token each, 32 heads on 8 of 128 values: 1163 and 1223 us uncut, 121 and 276.  1024 of 16 to 2000 keys, none of which is cut: 279 and 267.  A
+    // prompt of 100 rows behind 2000 keys beside 511 requests that wait, cut into three: 33 and 49, of 500, not cut, 82 and 80.)
     // Those of wide tiles are cut where there may be too few of these for the chip, or few enough that a context much longer than the others is
     // what is waited for.  (47 prompts of 24 rows over 16 to 6834 keys, 80 heads on 5: 166 us uncut, 105; 55 of 108 rows over up to 3537,
     // 16 on 1: 82 and 55.  Even batches pay for it: 8 of 500 rows 147 and 148 at dimension 128, 106 and 117 at 64.)
