@@ -797,8 +797,8 @@ __device__ __forceinline__ void few_columns(const KvAttentionArgs &p, unsigned u
 // the values' HD rows of 64 bytes; their 16-byte pieces are stored at places that keep the sixteen rows that a fragment reads on banks of
 // their own.
 // What bounds this is the issue of vector instructions.  A tile of 64 keys and 32 columns of 128 values has 68 products, which take 8 cycles of it
-// each, and 343 others, 128 of them conversions of codes, at 5 cycles (exponentials 8.5): 2340 cycles, and the matrix cores' own 1088 hide among
-// them.  8 prompts of 500 rows over 1000 to 4000 keys, 32 heads on 8 of 128 values: 148 us, 0.85 PFLOP/s.  (Ways there: 158 us when each 16
+// each, and 338 others, 128 of them conversions of codes, at 5 cycles (exponentials 8.5): 2350 cycles, and the matrix cores' own 1088 hide among
+// them.  8 prompts of 500 rows over 1000 to 4000 keys, 32 heads on 8 of 128 values: 150 us, 0.83 PFLOP/s.  (Ways there: 158 us when each 16
 // keys' page was looked up for itself, 149 with a barrier for each tile.  Three wavefronts a SIMD: 180, for spilled registers; 48 columns a
 // wavefront: 143 to 157; priority to wavefronts within products: 143 to 147.)
 typedef __attribute__((address_space(3))) void *kv_lds_ptr;
