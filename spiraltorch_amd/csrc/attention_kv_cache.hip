@@ -1200,7 +1200,8 @@ hipError_t launch_kv_attention(KvAttentionArgs args, hipStream_t stream)
     // what is waited for.  (47 prompts of 24 rows over 16 to 6834 keys, 80 heads on 5: 166 us uncut, 105; 55 of 108 rows over up to 3537,
     // 16 on 1: 82 and 55.  Even batches pay for it: 8 of 500 rows 147 and 148 at dimension 128, 106 and 117 at 64.)
     // Cuts add at most a target of workgroups, and another where half of a prompt's own keys were left out of the sum that they share.
-    const bool cut = (args.table_width << args.page_shift) > kKvLeastShare * kKvTile, wide_cut = cut && wide_items != 0 && wide_items <= 4 * kKvTarget<HD>;
+    // (More key heads than that target are more shares than there should be workgroups: no context is as long as one.)
+    const bool cut = (args.table_width << args.page_shift) > kKvLeastShare * kKvTile && args.kv_heads <= kKvTarget<HD>, wide_cut = cut && wide_items != 0 && wide_items <= 4 * kKvTarget<HD>;
     long long units = items + (cut ? kKvTarget<HD> : 0), wide_units = wide_items + (wide_cut ? fills ? kKvTarget<HD> : 2 * kKvTarget<HD> : 0);
     if (cut) {
         const size_t room = static_cast<size_t>(args.room) * args.kv_heads, floats = room * kKvColumns * (HD + 2);

@@ -342,6 +342,12 @@ def test_long_prompts_among_many_requests(hip, dim):
     check_attention(hip, rng, 64, 1, dim, 2, lengths.tolist(), fresh.tolist(), True)
 
 
+@pytest.mark.parametrize("kv_heads,dim,length", [(520, 64, 700), (400, 64, 1500), (200, 128, 900), (260, 256, 400)])
+def test_many_key_heads(hip, kv_heads, dim, length):
+    """As many key heads as there should be workgroups, and more and fewer."""
+    check_attention(hip, np.random.default_rng(kv_heads), 64, kv_heads, dim, 1, [length, 20], [1, 2], True)
+
+
 def test_rows_without_keys(hip):
     """More rows than tokens: the first see none, and are 0; requests of no length, of a negative one."""
     rng = np.random.default_rng(1)

@@ -194,6 +194,20 @@ for requests in (60, 2040, 5000):
     assert out == ["512", "0"] * 3
 
 
+def test_no_parts_where_key_heads_fill_the_chip(stub):
+    """A share of as many workgroups as there should be is longer than any context then: nothing is cut, and no memory is kept for parts."""
+    out = run(stub, """
+memory = ctypes.c_ulonglong.in_dll(stub, "stub_memory_used")
+for heads in (512, 513, 5000):
+    hip.release_scratch()
+    before = memory.value
+    c = cache(pages=100, heads=heads, k=2**43, v=2**44, ks=2**45, vs=2**46)
+    hip.attention_kv_cache_bf16_dev(c, 1, 1, heads, 0.1, True, M, 2 * M, 2**40, 2000, 2**41, heads * 64, 2**42, heads * 64)
+    print(grid.value - heads, memory.value - before > 0)
+""")
+    assert out == ["512", "True", "0", "False", "0", "False"]
+
+
 def test_null_structures():
     from spiraltorch_amd import hip
     with pytest.raises(ValueError):
