@@ -568,6 +568,49 @@ int st_hip_attention_kv_cache_bf16_dev(const st_hip_kv_cache *cache, size_t requ
                                        const int32_t *row_offsets, const int32_t *lengths, const int32_t *page_table,
                                        size_t table_width, const uint16_t *q, size_t ld_q, uint16_t *out, size_t ld_out, void *stream);
 
+/* ---- training a decoder --------------------------------------------------------------------------- */
+/* A bias of the attention's scores that is learned by buckets of the distance n = key - query: table[bucket(n)*heads + h] for head h.
+ * If `bidirectional`, the lower half of the buckets is for keys up to the query and the upper half for keys behind it, by m = |n|; else
+ * all are for keys up to the query, m = max(-n, 0).  Of a side's buckets, half (rounded down: e of s) hold one distance each, m itself;
+ * m >= e is in bucket e + floor((s - e) * log(m/e) / log(max_distance/e)), or in the last one (floor of a number that is whole to within 1e-9
+ * takes it as whole). */
+#define ST_HIP_POSITION_BIAS_MOST_BUCKETS 256
+#define ST_HIP_POSITION_BIAS_MOST_DISTANCE 2048
+typedef struct {
+    size_t buckets;      /* a side has 2 or more; 256 in all at the most; even if bidirectional */
+    size_t max_distance; /* above e, 2048 at the most */
+    int bidirectional;
+    const float *table;  /* (buckets, heads) */
+} st_hip_position_bias;
+
+/* Attention that is trained: bf16, softmax(scale * q.k + bias) v, heads in the columns of row-major matrices as for
+ * st_hip_attention_bf16_dev, sequence b in rows b*sequence .. b*sequence + sequence-1. */
+typedef struct {
+    size_t batch, heads;
+    size_t kv_heads;  /* heads is a multiple of it: head h reads keys and values of head h / (heads/kv_heads) */
+    size_t sequence, head_dim; /* head_dim 64 or 128 */
+    float scale;
+    int causal;             /* a query sees keys up to its own place */
+    const int32_t *lengths; /* (batch), device: how much of each sequence there is (taken as 0..sequence); NULL: all of it */
+    const st_hip_position_bias *position_bias; /* host; NULL: none */
+} st_hip_attention_training;
+/* The forward pass, which keeps lse (batch, heads, sequence): the natural log of the sum of the row's exponentials, -infinity for a row that
+ * sees no key.  q, out: heads*head_dim columns; k, v: kv_heads*head_dim columns, row stride ld_kv.  Rows behind a sequence's length are
+ * not read, and their results are 0 (lse: -infinity), as are those of rows whose every key has a bias of -infinity.
+ * The products take bf16 and accumulate in f32, the softmax is f32; its weights are rounded to bf16 for the second product, and so is out.
+ * Row strides (values) multiples of 8, buffers 16-byte aligned, and a sequence of a head within 2 GiB of its first row, else
+ * ST_HIP_ERR_UNSUPPORTED.  What is written overlaps nothing else; columns of one matrix that do not meet may be given. */
+int st_hip_attention_training_bf16_dev(const st_hip_attention_training *shape, const uint16_t *q, size_t ld_q, const uint16_t *k,
+                                       const uint16_t *v, size_t ld_kv, uint16_t *out, size_t ld_out, float *lse, void *stream);
+/* The backward pass, from what the forward pass was given and gave, and out's gradient: grad_q, grad_k, grad_v (bf16; those of shared
+ * heads summed in f32, rows behind a length 0) and, if grad_table is not NULL, that of the position bias's table (f32, (buckets, heads)),
+ * all overwritten.  The probabilities are worked out again; results do not depend on the order in which workgroups run.  grad_out is read
+ * within the lengths only.  The rows' sums go through the stream's scratch memory. */
+int st_hip_attention_backward_bf16_dev(const st_hip_attention_training *shape, const uint16_t *q, size_t ld_q, const uint16_t *k,
+                                       const uint16_t *v, size_t ld_kv, const uint16_t *out, size_t ld_out, const float *lse,
+                                       const uint16_t *grad_out, size_t ld_grad_out, uint16_t *grad_q, size_t ld_grad_q, uint16_t *grad_k,
+                                       uint16_t *grad_v, size_t ld_grad_kv, float *grad_table, void *stream);
+
 /* ---- measurement aid ---------------------------------------------------------------------------- */
 /* A loop of nothing but bf16 matrix instructions (v_mfma_f32_32x32x16_bf16) on register operands: `workgroups` × 4
  * wavefronts each issue 32·iterations of them (2·32·32·16 flop each) on fragments read once from `operands` (device,

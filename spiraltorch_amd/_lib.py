@@ -86,6 +86,15 @@ class RotaryStruct(ctypes.Structure):
         [(name, c_float) for name in ("base", "factor", "original_length", "low_turns", "high_turns", "magnitude")]
 
 
+class PositionBiasStruct(ctypes.Structure):
+    _fields_ = [("buckets", c_size_t), ("max_distance", c_size_t), ("bidirectional", c_int), ("table", c_void_p)]
+
+
+class AttentionTrainingStruct(ctypes.Structure):
+    _fields_ = [(name, c_size_t) for name in ("batch", "heads", "kv_heads", "sequence", "head_dim")] + \
+        [("scale", c_float), ("causal", c_int), ("lengths", c_void_p), ("position_bias", POINTER(PositionBiasStruct))]
+
+
 # name -> (restype, argtypes); this table is also what the symbol-export test walks.
 SIGNATURES = {
     "st_hip_init": (c_int, []),
@@ -200,6 +209,11 @@ SIGNATURES = {
     "st_hip_kv_cache_append_bf16_dev": (c_int, [POINTER(KvCacheStruct), c_size_t, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "st_hip_attention_kv_cache_bf16_dev": (c_int, [POINTER(KvCacheStruct), c_size_t, c_size_t, c_size_t, c_float, c_int, c_void_p, c_void_p,
                                                    c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
+    "st_hip_attention_training_bf16_dev": (c_int, [POINTER(AttentionTrainingStruct), c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p,
+                                                   c_size_t, c_void_p, c_void_p]),
+    "st_hip_attention_backward_bf16_dev": (c_int, [POINTER(AttentionTrainingStruct), c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p,
+                                                   c_size_t, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p, c_size_t,
+                                                   c_void_p, c_void_p]),
     "st_hip_decoder_weight_count": (c_size_t, [POINTER(DecoderConfig)]),
     "st_hip_decoder_create": (c_int, [POINTER(DecoderConfig), c_void_p, c_size_t, POINTER(c_void_p)]),
     "st_hip_decoder_forward_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),

@@ -373,6 +373,82 @@ int check_rotary(size_t rows, size_t sequence, size_t heads, size_t head_dim, co
     return ST_HIP_OK;
 }
 
+// Rows of `width` bytes, `stride` apart, that a call reads or writes.
+struct Region {
+    const void *at;
+    size_t rows, stride, width;
+    // Whether two share memory: columns of one matrix that do not meet share none.
+    bool meets(const Region &other) const
+    {
+        if (!at || !other.at || rows == 0 || width == 0 || other.rows == 0 || other.width == 0) return false;
+        const uintptr_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(other.at);
+        if (a >= b + (other.rows - 1) * other.stride + other.width || b >= a + (rows - 1) * stride + width) return false;
+        if (stride != other.stride) return true;
+        const uintptr_t behind = a <= b ? (b - a) % stride : (stride - (a - b) % stride) % stride;  // where the other's rows begin in this one's
+        return behind < width || behind > stride - other.width;
+    }
+};
+Region flat(const void *at, size_t bytes) { return Region{at, 1, bytes, bytes}; }
+
+// Refuses results (none of them empty) that share memory with each other or with what is read.
+template <size_t READ, size_t WRITTEN>
+int check_regions(const char *what, const Region (&read)[READ], const Region (&written)[WRITTEN])
+{
+    for (size_t i = 0; i < WRITTEN; ++i) {
+        for (const Region &r : read)
+            if (written[i].meets(r)) return fail(ST_HIP_ERR_INVALID, "%s: what is written overlaps what is read", what);
+        for (size_t j = 0; j < i; ++j)
+            if (written[i].meets(written[j])) return fail(ST_HIP_ERR_INVALID, "%s: results overlap", what);
+    }
+    return ST_HIP_OK;
+}
+
+int check_attention_training(const st_hip_attention_training *a, bool *work)
+{
+    *work = false;
+    if (!a) return fail(ST_HIP_ERR_INVALID, "attention training shape is null");
+    if (a->kv_heads == 0 ? a->heads != 0 : a->heads % a->kv_heads != 0)
+        return fail(ST_HIP_ERR_INVALID, "attention heads %zu are not a multiple of kv_heads %zu", a->heads, a->kv_heads);
+    if (a->head_dim != 64 && a->head_dim != 128)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "attention training needs head_dim 64 or 128, not %zu", a->head_dim);
+    if (!std::isfinite(a->scale))
+        return fail(ST_HIP_ERR_NONFINITE, "non-finite value encountered in scaled_dot_attention_scale: %g", static_cast<double>(a->scale));
+    if (!std::isfinite(a->scale * 1.4426950408889634f))
+        return fail(ST_HIP_ERR_UNSUPPORTED, "attention scale %g times log2(e) exceeds f32", static_cast<double>(a->scale));
+    size_t contexts = 0, rows = 0, values = 0, width = 0;
+    if (!checked_mul(a->batch, a->heads, &contexts) || !checked_mul(contexts, a->sequence, &rows) || !checked_mul(rows, a->head_dim * 8, &values) ||
+        !checked_mul(a->heads, a->head_dim, &width))
+        return fail(ST_HIP_ERR_INVALID, "attention dimensions overflow");
+    // (the kernels look up to a tile of 128 rows behind the last)
+    if (a->batch > kMaxDim || width > kMaxDim || a->sequence > kMaxDim - 256 || rows > kMaxDim)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "attention dimension exceeds i32");
+    if (const st_hip_position_bias *b = a->position_bias) {
+        if (b->bidirectional && b->buckets % 2 != 0) return fail(ST_HIP_ERR_INVALID, "position bias buckets %zu are odd on two sides", b->buckets);
+        const size_t side = b->bidirectional ? b->buckets / 2 : b->buckets;
+        if (side < 2 || b->max_distance <= side / 2)
+            return fail(ST_HIP_ERR_INVALID, "position bias needs two buckets a side and a max_distance above half of a side's (got %zu, %zu)", b->buckets,
+                        b->max_distance);
+        if (b->buckets > ST_HIP_POSITION_BIAS_MOST_BUCKETS || b->max_distance > ST_HIP_POSITION_BIAS_MOST_DISTANCE)
+            return fail(ST_HIP_ERR_UNSUPPORTED, "position bias of %zu buckets to distance %zu exceeds the kernel's", b->buckets, b->max_distance);
+        if (contexts && !b->table) return fail(ST_HIP_ERR_INVALID, "position bias table is null");
+        if (a->heads > kMaxDim / ST_HIP_POSITION_BIAS_MOST_BUCKETS) return fail(ST_HIP_ERR_UNSUPPORTED, "position bias heads exceed the kernel's");
+    }
+    *work = rows != 0;
+    return ST_HIP_OK;
+}
+
+// One of the matrices of a trained attention, `width` bf16 columns.
+int check_training_rows(const st_hip_attention_training &a, const char *what, const void *at, size_t ld, size_t width)
+{
+    if (!at) return fail(ST_HIP_ERR_INVALID, "attention training: %s is null", what);
+    if (ld < width) return fail(ST_HIP_ERR_INVALID, "attention training: %s row stride %zu is smaller than its width %zu", what, ld, width);
+    if (ld > kMaxDim || ld % 8 != 0 || reinterpret_cast<uintptr_t>(at) % 16 != 0)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "attention training: %s needs a row stride that is a multiple of 8 and a 16-byte boundary", what);
+    if (!addressable(a.batch * a.sequence, ld, sizeof(uint16_t)) || ((a.sequence + 256) * ld + a.head_dim) * 2 >= 1ull << 31)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "attention training: a sequence of %s exceeds 2 GiB", what);
+    return ST_HIP_OK;
+}
+
 int check_kv_cache(const st_hip_kv_cache *c)
 {
     if (!c) return fail(ST_HIP_ERR_INVALID, "kv cache is null");
@@ -1411,6 +1487,75 @@ int st_hip_attention_kv_cache_bf16_dev(const st_hip_kv_cache *cache, size_t requ
     return launch_status(launch_attention_kv_cache_bf16(*cache, requests, rows, heads, scale, causal != 0, row_offsets, lengths, page_table, table_width,
                                                         q, ld_q, out, ld_out, as_stream(stream)),
                          "attention launch");
+}
+
+int st_hip_attention_training_bf16_dev(const st_hip_attention_training *shape, const uint16_t *q, size_t ld_q, const uint16_t *k, const uint16_t *v,
+                                       size_t ld_kv, uint16_t *out, size_t ld_out, float *lse, void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    bool work = false;
+    ST_HIP_CHECK(check_attention_training(shape, &work));
+    if (!work) return ST_HIP_OK;
+    const size_t width = shape->heads * shape->head_dim, kv_width = shape->kv_heads * shape->head_dim, rows = shape->batch * shape->sequence;
+    ST_HIP_CHECK(check_training_rows(*shape, "q", q, ld_q, width));
+    ST_HIP_CHECK(check_training_rows(*shape, "k", k, ld_kv, kv_width));
+    ST_HIP_CHECK(check_training_rows(*shape, "v", v, ld_kv, kv_width));
+    ST_HIP_CHECK(check_training_rows(*shape, "out", out, ld_out, width));
+    if (!lse) return fail(ST_HIP_ERR_INVALID, "attention training: lse is null");
+    const st_hip_position_bias *bias = shape->position_bias;
+    const Region read[] = {{q, rows, ld_q * 2, width * 2},
+                           {k, rows, ld_kv * 2, kv_width * 2},
+                           {v, rows, ld_kv * 2, kv_width * 2},
+                           flat(shape->lengths, shape->batch * sizeof(int32_t)),
+                           flat(bias ? bias->table : nullptr, bias ? bias->buckets * shape->heads * sizeof(float) : 0)};
+    const Region written[] = {{out, rows, ld_out * 2, width * 2}, flat(lse, rows * shape->heads * sizeof(float))};
+    ST_HIP_CHECK(check_regions("attention training", read, written));
+    return launch_status(launch_attention_training_bf16(*shape, q, ld_q, k, v, ld_kv, out, ld_out, lse, as_stream(stream)), "attention training launch");
+}
+
+int st_hip_attention_backward_bf16_dev(const st_hip_attention_training *shape, const uint16_t *q, size_t ld_q, const uint16_t *k, const uint16_t *v,
+                                       size_t ld_kv, const uint16_t *out, size_t ld_out, const float *lse, const uint16_t *grad_out, size_t ld_grad_out,
+                                       uint16_t *grad_q, size_t ld_grad_q, uint16_t *grad_k, uint16_t *grad_v, size_t ld_grad_kv, float *grad_table,
+                                       void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    bool work = false;
+    ST_HIP_CHECK(check_attention_training(shape, &work));
+    const st_hip_position_bias *bias = shape->position_bias;
+    if (grad_table && !bias) return fail(ST_HIP_ERR_INVALID, "attention training: a table's gradient without a position bias");
+    const size_t table_bytes = bias ? bias->buckets * shape->heads * sizeof(float) : 0;
+    if (!work) {  // no pair of a query and a key: the gradients of q, k and v are empty, the table's is 0
+        if (!grad_table || table_bytes == 0) return ST_HIP_OK;
+        return launch_status(launch_attention_backward_bf16(*shape, nullptr, 0, nullptr, nullptr, 0, nullptr, 0, nullptr, nullptr, 0, nullptr, 0, nullptr,
+                                                            nullptr, 0, grad_table, as_stream(stream)),
+                             "attention backward launch");
+    }
+    const size_t width = shape->heads * shape->head_dim, kv_width = shape->kv_heads * shape->head_dim, rows = shape->batch * shape->sequence;
+    ST_HIP_CHECK(check_training_rows(*shape, "q", q, ld_q, width));
+    ST_HIP_CHECK(check_training_rows(*shape, "k", k, ld_kv, kv_width));
+    ST_HIP_CHECK(check_training_rows(*shape, "v", v, ld_kv, kv_width));
+    ST_HIP_CHECK(check_training_rows(*shape, "out", out, ld_out, width));
+    ST_HIP_CHECK(check_training_rows(*shape, "grad_out", grad_out, ld_grad_out, width));
+    ST_HIP_CHECK(check_training_rows(*shape, "grad_q", grad_q, ld_grad_q, width));
+    ST_HIP_CHECK(check_training_rows(*shape, "grad_k", grad_k, ld_grad_kv, kv_width));
+    ST_HIP_CHECK(check_training_rows(*shape, "grad_v", grad_v, ld_grad_kv, kv_width));
+    if (!lse) return fail(ST_HIP_ERR_INVALID, "attention training: lse is null");
+    const Region read[] = {{q, rows, ld_q * 2, width * 2},
+                           {k, rows, ld_kv * 2, kv_width * 2},
+                           {v, rows, ld_kv * 2, kv_width * 2},
+                           {out, rows, ld_out * 2, width * 2},
+                           {grad_out, rows, ld_grad_out * 2, width * 2},
+                           flat(lse, rows * shape->heads * sizeof(float)),
+                           flat(shape->lengths, shape->batch * sizeof(int32_t)),
+                           flat(bias ? bias->table : nullptr, table_bytes)};
+    const Region written[] = {{grad_q, rows, ld_grad_q * 2, width * 2},
+                              {grad_k, rows, ld_grad_kv * 2, kv_width * 2},
+                              {grad_v, rows, ld_grad_kv * 2, kv_width * 2},
+                              flat(grad_table, table_bytes)};
+    ST_HIP_CHECK(check_regions("attention training", read, written));
+    return launch_status(launch_attention_backward_bf16(*shape, q, ld_q, k, v, ld_kv, out, ld_out, lse, grad_out, ld_grad_out, grad_q, ld_grad_q, grad_k,
+                                                        grad_v, ld_grad_kv, grad_table, as_stream(stream)),
+                         "attention backward launch");
 }
 
 int st_hip_row_softmax_f32_dev(size_t rows, size_t cols, const float *in, float *out, void *stream)

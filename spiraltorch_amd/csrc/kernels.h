@@ -216,6 +216,14 @@ hipError_t launch_rotary_f32(size_t rows, size_t sequence, size_t heads, size_t 
 hipError_t launch_rotary_bf16(size_t rows, size_t sequence, size_t heads, size_t head_dim, const st_hip_rotary &rotary, bool transposed,
                               const int32_t *positions, const uint16_t *in, size_t ld_in, uint16_t *out, size_t ld_out, hipStream_t stream);
 
+// Attention that is trained, in bf16 (see st_hip.h).  The backward pass uses the stream's scratch memory.
+hipError_t launch_attention_training_bf16(const st_hip_attention_training &shape, const uint16_t *q, size_t ld_q, const uint16_t *k, const uint16_t *v,
+                                          size_t ld_kv, uint16_t *out, size_t ld_out, float *lse, hipStream_t stream);
+hipError_t launch_attention_backward_bf16(const st_hip_attention_training &shape, const uint16_t *q, size_t ld_q, const uint16_t *k, const uint16_t *v,
+                                          size_t ld_kv, const uint16_t *out, size_t ld_out, const float *lse, const uint16_t *grad_out, size_t ld_grad_out,
+                                          uint16_t *grad_q, size_t ld_grad_q, uint16_t *grad_k, uint16_t *grad_v, size_t ld_grad_kv, float *grad_table,
+                                          hipStream_t stream);
+
 hipError_t launch_layer_norm_f32(size_t rows, size_t cols, const float *x, const float *residual,
                                  const float *gamma, const float *beta, float epsilon, float *out_f32,
                                  uint16_t *out_bf16, hipStream_t stream);

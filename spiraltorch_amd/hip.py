@@ -644,6 +644,40 @@ def attention_kv_cache_bf16_dev(cache: KvCache, requests, rows, heads, scale, ca
                                                           _stream_ptr(stream)))
 
 
+class PositionBias:
+    """A bias of attention scores learned by buckets of distance (st_hip_position_bias of include/st_hip.h): table (buckets, heads) f32 on the device."""
+
+    def __init__(self, buckets: int, max_distance: int, table, bidirectional: bool = False):
+        self.buckets, self.table = buckets, table
+        self._struct = _lib.PositionBiasStruct(buckets, max_distance, int(bool(bidirectional)), _address(table))
+
+
+class AttentionTraining:
+    """The shape of an attention that is trained (st_hip_attention_training of include/st_hip.h); lengths (batch) int32 on the device."""
+
+    def __init__(self, batch: int, heads: int, sequence: int, head_dim: int, scale: float, causal: bool = False, kv_heads: Optional[int] = None,
+                 lengths=None, position_bias: Optional[PositionBias] = None):
+        self._kept = (lengths, position_bias)
+        bias = None if position_bias is None else ctypes.pointer(position_bias._struct)
+        self._struct = _lib.AttentionTrainingStruct(batch, heads, heads if kv_heads is None else kv_heads, sequence, head_dim, scale,
+                                                    int(bool(causal)), _address(lengths), bias)
+        self._ref = ctypes.byref(self._struct)
+
+
+def attention_training_bf16_dev(shape: AttentionTraining, q, ld_q, k, v, ld_kv, out, ld_out, lse, stream=None) -> None:
+    """The forward pass of a trained attention: out (bf16) and lse (batch, heads, sequence) f32 (see st_hip_attention_training_bf16_dev)."""
+    _check(_lib.load().st_hip_attention_training_bf16_dev(shape._ref, _dev(q), ld_q, _dev(k), _dev(v), ld_kv, _dev(out), ld_out, _dev(lse),
+                                                          _stream_ptr(stream)))
+
+
+def attention_backward_bf16_dev(shape: AttentionTraining, q, ld_q, k, v, ld_kv, out, ld_out, lse, grad_out, ld_grad_out, grad_q, ld_grad_q, grad_k,
+                                grad_v, ld_grad_kv, grad_table=None, stream=None) -> None:
+    """Its backward pass: the gradients of q, k, v (bf16) and of the position bias's table (f32; see st_hip_attention_backward_bf16_dev)."""
+    _check(_lib.load().st_hip_attention_backward_bf16_dev(shape._ref, _dev(q), ld_q, _dev(k), _dev(v), ld_kv, _dev(out), ld_out, _dev(lse),
+                                                          _dev(grad_out), ld_grad_out, _dev(grad_q), ld_grad_q, _dev(grad_k), _dev(grad_v),
+                                                          ld_grad_kv, _dev(grad_table), _stream_ptr(stream)))
+
+
 def probe_mfma_bf16_dev(workgroups, iterations, operands, sink, stream=None) -> None:
     """A loop of bf16 matrix instructions on register operands (measurement aid; see st_hip_probe_mfma_bf16_dev)."""
     _check(_lib.load().st_hip_probe_mfma_bf16_dev(workgroups, iterations, _dev(operands), _dev(sink), _stream_ptr(stream)))

@@ -19,7 +19,8 @@ SCALARS = {"size_t": "usize", "int": "c_int", "float": "f32", "uint64_t": "u64",
            "st_hip_decoder_config": "StHipDecoderConfig", "st_hip_attention_plan": "StHipAttentionPlan",
            "st_hip_gemm_tile_plan": "StHipGemmTilePlan", "st_hip_gemm_split_plan": "StHipGemmSplitPlan",
            "st_hip_conv2d_split_plan": "StHipConv2dSplitPlan", "st_hip_conv2d_bf16_plan": "StHipConv2dBf16Plan",
-           "st_hip_kv_cache": "StHipKvCache", "st_hip_rotary": "StHipRotary"}
+           "st_hip_kv_cache": "StHipKvCache", "st_hip_rotary": "StHipRotary",
+           "st_hip_position_bias": "StHipPositionBias", "st_hip_attention_training": "StHipAttentionTraining"}
 RUST_KEYWORDS = {"in": "input", "type": "kind", "ref": "reference"}
 
 STRUCTS = '''/// `st_hip_device_props`.
@@ -165,6 +166,31 @@ pub struct StHipRotary {
     pub low_turns: f32,
     pub high_turns: f32,
     pub magnitude: f32,
+}
+
+/// `st_hip_position_bias`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct StHipPositionBias {
+    pub buckets: usize,
+    pub max_distance: usize,
+    pub bidirectional: c_int,
+    pub table: *const f32,
+}
+
+/// `st_hip_attention_training`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct StHipAttentionTraining {
+    pub batch: usize,
+    pub heads: usize,
+    pub kv_heads: usize,
+    pub sequence: usize,
+    pub head_dim: usize,
+    pub scale: f32,
+    pub causal: c_int,
+    pub lengths: *const i32,
+    pub position_bias: *const StHipPositionBias,
 }
 '''
 

@@ -150,6 +150,31 @@ pub struct StHipRotary {
     pub magnitude: f32,
 }
 
+/// `st_hip_position_bias`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct StHipPositionBias {
+    pub buckets: usize,
+    pub max_distance: usize,
+    pub bidirectional: c_int,
+    pub table: *const f32,
+}
+
+/// `st_hip_attention_training`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct StHipAttentionTraining {
+    pub batch: usize,
+    pub heads: usize,
+    pub kv_heads: usize,
+    pub sequence: usize,
+    pub head_dim: usize,
+    pub scale: f32,
+    pub causal: c_int,
+    pub lengths: *const i32,
+    pub position_bias: *const StHipPositionBias,
+}
+
 #[link(name = "sthip")]
 extern "C" {
     pub fn st_hip_init() -> c_int;
@@ -234,6 +259,8 @@ extern "C" {
     pub fn st_hip_kv_cache_append_f32_dev(cache: *const StHipKvCache, rows: usize, slots: *const i32, k: *const f32, v: *const f32, ld: usize, stream: *mut c_void) -> c_int;
     pub fn st_hip_kv_cache_append_bf16_dev(cache: *const StHipKvCache, rows: usize, slots: *const i32, k: *const u16, v: *const u16, ld: usize, stream: *mut c_void) -> c_int;
     pub fn st_hip_attention_kv_cache_bf16_dev(cache: *const StHipKvCache, requests: usize, rows: usize, heads: usize, scale: f32, causal: c_int, row_offsets: *const i32, lengths: *const i32, page_table: *const i32, table_width: usize, q: *const u16, ld_q: usize, out: *mut u16, ld_out: usize, stream: *mut c_void) -> c_int;
+    pub fn st_hip_attention_training_bf16_dev(shape: *const StHipAttentionTraining, q: *const u16, ld_q: usize, k: *const u16, v: *const u16, ld_kv: usize, out: *mut u16, ld_out: usize, lse: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn st_hip_attention_backward_bf16_dev(shape: *const StHipAttentionTraining, q: *const u16, ld_q: usize, k: *const u16, v: *const u16, ld_kv: usize, out: *const u16, ld_out: usize, lse: *const f32, grad_out: *const u16, ld_grad_out: usize, grad_q: *mut u16, ld_grad_q: usize, grad_k: *mut u16, grad_v: *mut u16, ld_grad_kv: usize, grad_table: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_probe_mfma_bf16_dev(workgroups: usize, iterations: usize, operands: *const u16, sink: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_probe_mfma_f32_dev(workgroups: usize, iterations: usize, operands: *const f32, sink: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_probe_stream_lds_dev(workgroups: usize, iterations: usize, region: *const c_void, region_bytes: usize, stream: *mut c_void) -> c_int;
