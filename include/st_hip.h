@@ -611,6 +611,28 @@ int st_hip_attention_backward_bf16_dev(const st_hip_attention_training *shape, c
                                        const uint16_t *grad_out, size_t ld_grad_out, uint16_t *grad_q, size_t ld_grad_q, uint16_t *grad_k,
                                        uint16_t *grad_v, size_t ld_grad_kv, float *grad_table, void *stream);
 
+/* What tokens are worth: for each of `rows` rows of `vocab` logits x (row stride ld), the log-probability of its token,
+ * x[token] - normalizer (0 for a token outside 0..vocab-1: a row that does not count); the entropy -sum p log p; the normalizer,
+ * log sum e^x; and the `top` likeliest alternatives, (rows, top), best first, equal ones in the order of their ids.  log_probs (with tokens),
+ * entropies and normalizers may each be NULL; top is at most vocab and 32.  Sums are f32.  Logits of -infinity have no probability; in a row of
+ * nothing else the normalizer and all log-probabilities are -infinity and the entropy is 0.  A row with NaN or +infinity gives NaN; NaN is
+ * no alternative (id -1 and NaN where there are too few).  Long rows of which there are few are cut over workgroups, whose parts go
+ * through the stream's scratch memory.  Results overlap neither what is read nor each other. */
+#define ST_HIP_LOG_PROBS_MOST_TOP 32
+int st_hip_token_log_probs_f32_dev(size_t rows, size_t vocab, const float *logits, size_t ld, const int32_t *tokens, float *log_probs,
+                                   float *entropies, float *normalizers, size_t top, int32_t *top_ids, float *top_log_probs, void *stream);
+int st_hip_token_log_probs_bf16_dev(size_t rows, size_t vocab, const uint16_t *logits, size_t ld, const int32_t *tokens, float *log_probs,
+                                    float *entropies, float *normalizers, size_t top, int32_t *top_ids, float *top_log_probs, void *stream);
+/* The logits' gradient, overwritten, of the log-probabilities' (NULL: 0; with tokens) and the entropies' (NULL: 0; with entropies, as the call
+ * above gave them), from its normalizers: g*([token] - p) - h*p*(log p + entropy), in f32 and rounded once.  A row that does not count
+ * has no g; a row of nothing but -infinity has the gradient 0.  grad_logits may be logits, with the same stride. */
+int st_hip_token_log_probs_backward_f32_dev(size_t rows, size_t vocab, const float *logits, size_t ld, const int32_t *tokens,
+                                            const float *normalizers, const float *entropies, const float *grad_log_probs,
+                                            const float *grad_entropies, float *grad_logits, size_t ld_grad, void *stream);
+int st_hip_token_log_probs_backward_bf16_dev(size_t rows, size_t vocab, const uint16_t *logits, size_t ld, const int32_t *tokens,
+                                             const float *normalizers, const float *entropies, const float *grad_log_probs,
+                                             const float *grad_entropies, uint16_t *grad_logits, size_t ld_grad, void *stream);
+
 /* ---- measurement aid ---------------------------------------------------------------------------- */
 /* A loop of nothing but bf16 matrix instructions (v_mfma_f32_32x32x16_bf16) on register operands: `workgroups` × 4
  * wavefronts each issue 32·iterations of them (2·32·32·16 flop each) on fragments read once from `operands` (device,

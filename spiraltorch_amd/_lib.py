@@ -214,6 +214,10 @@ SIGNATURES = {
     "st_hip_attention_backward_bf16_dev": (c_int, [POINTER(AttentionTrainingStruct), c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p,
                                                    c_size_t, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p, c_size_t,
                                                    c_void_p, c_void_p]),
+    "st_hip_token_log_probs_f32_dev": (c_int, [c_size_t, c_size_t, c_void_p, c_size_t] + [c_void_p] * 4 + [c_size_t] + [c_void_p] * 3),
+    "st_hip_token_log_probs_backward_f32_dev": (c_int, [c_size_t, c_size_t, c_void_p, c_size_t] + [c_void_p] * 6 + [c_size_t, c_void_p]),
+    "st_hip_token_log_probs_bf16_dev": (c_int, [c_size_t, c_size_t, c_void_p, c_size_t] + [c_void_p] * 4 + [c_size_t] + [c_void_p] * 3),
+    "st_hip_token_log_probs_backward_bf16_dev": (c_int, [c_size_t, c_size_t, c_void_p, c_size_t] + [c_void_p] * 6 + [c_size_t, c_void_p]),
     "st_hip_decoder_weight_count": (c_size_t, [POINTER(DecoderConfig)]),
     "st_hip_decoder_create": (c_int, [POINTER(DecoderConfig), c_void_p, c_size_t, POINTER(c_void_p)]),
     "st_hip_decoder_forward_dev": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),

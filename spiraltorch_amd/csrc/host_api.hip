@@ -403,6 +403,68 @@ int check_regions(const char *what, const Region (&read)[READ], const Region (&w
     return ST_HIP_OK;
 }
 
+// Rows of logits, or of their gradient.
+int check_logits(size_t rows, size_t vocab, const char *what, const void *at, size_t ld, size_t size)
+{
+    if (!at) return fail(ST_HIP_ERR_INVALID, "log-probabilities: %s are null", what);
+    if (ld < vocab) return fail(ST_HIP_ERR_INVALID, "log-probabilities: row stride %zu of the %s is smaller than the vocabulary's %zu", ld, what, vocab);
+    if (!addressable(rows, ld, size)) return fail(ST_HIP_ERR_INVALID, "log-probabilities: dimensions overflow");
+    if (reinterpret_cast<uintptr_t>(at) % size != 0) return fail(ST_HIP_ERR_INVALID, "log-probabilities: %s are not aligned to their type", what);
+    return ST_HIP_OK;
+}
+
+int check_vocabulary(size_t rows, size_t vocab)
+{
+    if (vocab == 0) return fail(ST_HIP_ERR_INVALID, "log-probabilities: the vocabulary is empty");
+    // (part sizes are rounded up, and a workgroup looks a round of 16-byte runs beyond the last)
+    if (rows > kMaxDim || vocab > kMaxDim - (1u << 17)) return fail(ST_HIP_ERR_UNSUPPORTED, "log-probabilities: dimension exceeds i32");
+    return ST_HIP_OK;
+}
+
+int token_log_probs(size_t rows, size_t vocab, const void *logits, size_t ld, size_t size, const int32_t *tokens, float *log_probs, float *entropies,
+                    float *normalizers, size_t top, int32_t *top_ids, float *top_log_probs, void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    ST_HIP_CHECK(check_vocabulary(rows, vocab));
+    if (top > vocab) return fail(ST_HIP_ERR_INVALID, "log-probabilities: %zu alternatives of a vocabulary of %zu", top, vocab);
+    if (top > ST_HIP_LOG_PROBS_MOST_TOP)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "log-probabilities: %zu alternatives are more than %d", top, ST_HIP_LOG_PROBS_MOST_TOP);
+    if (rows == 0) return ST_HIP_OK;
+    ST_HIP_CHECK(check_logits(rows, vocab, "logits", logits, ld, size));
+    if ((log_probs && !tokens) || (top && (!top_ids || !top_log_probs))) return fail(ST_HIP_ERR_INVALID, "log-probabilities received a null pointer");
+    if (!log_probs && !entropies && !normalizers && top == 0) return ST_HIP_OK;
+    const Region read[] = {{logits, rows, ld * size, vocab * size}, flat(log_probs ? tokens : nullptr, rows * sizeof(int32_t))};
+    const Region written[] = {flat(log_probs, rows * sizeof(float)), flat(entropies, rows * sizeof(float)), flat(normalizers, rows * sizeof(float)),
+                              flat(top_ids, rows * top * sizeof(int32_t)), flat(top_log_probs, rows * top * sizeof(float))};
+    ST_HIP_CHECK(check_regions("log-probabilities", read, written));
+    return launch_status(launch_token_log_probs(size == 2, rows, vocab, logits, ld, tokens, log_probs, entropies, normalizers, top, top_ids, top_log_probs,
+                                                as_stream(stream)),
+                         "log-probabilities launch");
+}
+
+int token_log_probs_backward(size_t rows, size_t vocab, const void *logits, size_t ld, size_t size, const int32_t *tokens, const float *normalizers,
+                             const float *entropies, const float *grad_log_probs, const float *grad_entropies, void *grad_logits, size_t ld_grad,
+                             void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    ST_HIP_CHECK(check_vocabulary(rows, vocab));
+    if (rows == 0) return ST_HIP_OK;
+    ST_HIP_CHECK(check_logits(rows, vocab, "logits", logits, ld, size));
+    ST_HIP_CHECK(check_logits(rows, vocab, "gradients", grad_logits, ld_grad, size));
+    if (!normalizers || (grad_log_probs && !tokens) || (grad_entropies && !entropies))
+        return fail(ST_HIP_ERR_INVALID, "log-probabilities received a null pointer");
+    const Region given{logits, rows, ld * size, vocab * size}, gradient{grad_logits, rows, ld_grad * size, vocab * size};
+    const bool in_place = logits == grad_logits && (ld == ld_grad || rows == 1);
+    const Region read[] = {flat(tokens, rows * sizeof(int32_t)), flat(normalizers, rows * sizeof(float)), flat(entropies, rows * sizeof(float)),
+                           flat(grad_log_probs, rows * sizeof(float)), flat(grad_entropies, rows * sizeof(float)),
+                           in_place ? Region{nullptr, 0, 0, 0} : given};
+    const Region written[] = {gradient};
+    ST_HIP_CHECK(check_regions("log-probabilities", read, written));
+    return launch_status(launch_token_log_probs_backward(size == 2, rows, vocab, logits, ld, tokens, normalizers, entropies, grad_log_probs, grad_entropies,
+                                                         grad_logits, ld_grad, as_stream(stream)),
+                         "log-probabilities backward launch");
+}
+
 int check_attention_training(const st_hip_attention_training *a, bool *work)
 {
     *work = false;
@@ -1556,6 +1618,34 @@ int st_hip_attention_backward_bf16_dev(const st_hip_attention_training *shape, c
     return launch_status(launch_attention_backward_bf16(*shape, q, ld_q, k, v, ld_kv, out, ld_out, lse, grad_out, ld_grad_out, grad_q, ld_grad_q, grad_k,
                                                         grad_v, ld_grad_kv, grad_table, as_stream(stream)),
                          "attention backward launch");
+}
+
+int st_hip_token_log_probs_f32_dev(size_t rows, size_t vocab, const float *logits, size_t ld, const int32_t *tokens, float *log_probs,
+                                   float *entropies, float *normalizers, size_t top, int32_t *top_ids, float *top_log_probs, void *stream)
+{
+    return token_log_probs(rows, vocab, logits, ld, sizeof(float), tokens, log_probs, entropies, normalizers, top, top_ids, top_log_probs, stream);
+}
+
+int st_hip_token_log_probs_backward_f32_dev(size_t rows, size_t vocab, const float *logits, size_t ld, const int32_t *tokens,
+                                            const float *normalizers, const float *entropies, const float *grad_log_probs,
+                                            const float *grad_entropies, float *grad_logits, size_t ld_grad, void *stream)
+{
+    return token_log_probs_backward(rows, vocab, logits, ld, sizeof(float), tokens, normalizers, entropies, grad_log_probs, grad_entropies, grad_logits, ld_grad,
+                                    stream);
+}
+
+int st_hip_token_log_probs_bf16_dev(size_t rows, size_t vocab, const uint16_t *logits, size_t ld, const int32_t *tokens, float *log_probs,
+                                   float *entropies, float *normalizers, size_t top, int32_t *top_ids, float *top_log_probs, void *stream)
+{
+    return token_log_probs(rows, vocab, logits, ld, sizeof(uint16_t), tokens, log_probs, entropies, normalizers, top, top_ids, top_log_probs, stream);
+}
+
+int st_hip_token_log_probs_backward_bf16_dev(size_t rows, size_t vocab, const uint16_t *logits, size_t ld, const int32_t *tokens,
+                                            const float *normalizers, const float *entropies, const float *grad_log_probs,
+                                            const float *grad_entropies, uint16_t *grad_logits, size_t ld_grad, void *stream)
+{
+    return token_log_probs_backward(rows, vocab, logits, ld, sizeof(uint16_t), tokens, normalizers, entropies, grad_log_probs, grad_entropies, grad_logits, ld_grad,
+                                    stream);
 }
 
 int st_hip_row_softmax_f32_dev(size_t rows, size_t cols, const float *in, float *out, void *stream)

@@ -224,6 +224,13 @@ hipError_t launch_attention_backward_bf16(const st_hip_attention_training &shape
                                           uint16_t *grad_q, size_t ld_grad_q, uint16_t *grad_k, uint16_t *grad_v, size_t ld_grad_kv, float *grad_table,
                                           hipStream_t stream);
 
+// Log-probabilities of given tokens and the logits' gradient, f32 or bf16 logits (see st_hip.h).
+hipError_t launch_token_log_probs(bool bf16, size_t rows, size_t vocab, const void *logits, size_t ld, const int32_t *tokens, float *log_probs,
+                                  float *entropies, float *normalizers, size_t top, int32_t *top_ids, float *top_log_probs, hipStream_t stream);
+hipError_t launch_token_log_probs_backward(bool bf16, size_t rows, size_t vocab, const void *logits, size_t ld, const int32_t *tokens,
+                                           const float *normalizers, const float *entropies, const float *grad_log_probs, const float *grad_entropies,
+                                           void *grad_logits, size_t ld_grad, hipStream_t stream);
+
 hipError_t launch_layer_norm_f32(size_t rows, size_t cols, const float *x, const float *residual,
                                  const float *gamma, const float *beta, float epsilon, float *out_f32,
                                  uint16_t *out_bf16, hipStream_t stream);

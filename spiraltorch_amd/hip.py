@@ -678,6 +678,37 @@ def attention_backward_bf16_dev(shape: AttentionTraining, q, ld_q, k, v, ld_kv, 
                                                           ld_grad_kv, _dev(grad_table), _stream_ptr(stream)))
 
 
+def token_log_probs_f32_dev(rows, vocab, logits, ld, tokens, log_probs, entropies, normalizers, top=0, top_ids=None, top_log_probs=None,
+                            stream=None) -> None:
+    """Log-probabilities of given tokens (int32), entropies, normalizers and the likeliest alternatives of rows of logits (see
+    st_hip_token_log_probs_f32_dev)."""
+    _check(_lib.load().st_hip_token_log_probs_f32_dev(rows, vocab, _dev(logits), ld, _dev(tokens), _dev(log_probs), _dev(entropies),
+                                                      _dev(normalizers), top, _dev(top_ids), _dev(top_log_probs), _stream_ptr(stream)))
+
+
+def token_log_probs_bf16_dev(rows, vocab, logits, ld, tokens, log_probs, entropies, normalizers, top=0, top_ids=None, top_log_probs=None,
+                             stream=None) -> None:
+    """token_log_probs_f32_dev on bf16 bit patterns."""
+    _check(_lib.load().st_hip_token_log_probs_bf16_dev(rows, vocab, _dev(logits), ld, _dev(tokens), _dev(log_probs), _dev(entropies),
+                                                       _dev(normalizers), top, _dev(top_ids), _dev(top_log_probs), _stream_ptr(stream)))
+
+
+def token_log_probs_backward_f32_dev(rows, vocab, logits, ld, tokens, normalizers, entropies, grad_log_probs, grad_entropies, grad_logits, ld_grad,
+                                     stream=None) -> None:
+    """The gradient of the logits from those of the log-probabilities and entropies, each of which may be None."""
+    _check(_lib.load().st_hip_token_log_probs_backward_f32_dev(rows, vocab, _dev(logits), ld, _dev(tokens), _dev(normalizers), _dev(entropies),
+                                                               _dev(grad_log_probs), _dev(grad_entropies), _dev(grad_logits), ld_grad,
+                                                               _stream_ptr(stream)))
+
+
+def token_log_probs_backward_bf16_dev(rows, vocab, logits, ld, tokens, normalizers, entropies, grad_log_probs, grad_entropies, grad_logits, ld_grad,
+                                      stream=None) -> None:
+    """token_log_probs_backward_f32_dev on bf16 bit patterns."""
+    _check(_lib.load().st_hip_token_log_probs_backward_bf16_dev(rows, vocab, _dev(logits), ld, _dev(tokens), _dev(normalizers), _dev(entropies),
+                                                                _dev(grad_log_probs), _dev(grad_entropies), _dev(grad_logits), ld_grad,
+                                                                _stream_ptr(stream)))
+
+
 def probe_mfma_bf16_dev(workgroups, iterations, operands, sink, stream=None) -> None:
     """A loop of bf16 matrix instructions on register operands (measurement aid; see st_hip_probe_mfma_bf16_dev)."""
     _check(_lib.load().st_hip_probe_mfma_bf16_dev(workgroups, iterations, _dev(operands), _dev(sink), _stream_ptr(stream)))
