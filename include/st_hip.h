@@ -611,6 +611,16 @@ int st_hip_attention_backward_bf16_dev(const st_hip_attention_training *shape, c
                                        const uint16_t *grad_out, size_t ld_grad_out, uint16_t *grad_q, size_t ld_grad_q, uint16_t *grad_k,
                                        uint16_t *grad_v, size_t ld_grad_kv, float *grad_table, void *stream);
 
+/* The backward pass of st_hip_attention_f32_dev: from its operands, its result and that result's gradient, the gradients of q, k, v and, where
+ * they are asked for (not NULL; with the bias), of z_bias (contexts, sequence) and attn_bias (contexts*sequence, sequence), all overwritten.
+ * A row whose every score is -infinity has the gradient 0.  f32 throughout; results do not depend on the order in which workgroups run,
+ * and what is written overlaps nothing else.  A context of q is within 2 GiB (ST_HIP_ERR_UNSUPPORTED).  Two numbers a row go through the
+ * stream's scratch memory. */
+int st_hip_attention_backward_f32_dev(size_t contexts, size_t sequence, size_t head_dim, float scale, int causal, const float *q,
+                                      const float *k, const float *v, const float *z_bias, const float *attn_bias, const float *out,
+                                      const float *grad_out, float *grad_q, float *grad_k, float *grad_v, float *grad_z_bias,
+                                      float *grad_attn_bias, void *stream);
+
 /* What tokens are worth: for each of `rows` rows of `vocab` logits x (row stride ld), the log-probability of its token,
  * x[token] - normalizer (0 for a token outside 0..vocab-1: a row that does not count); the entropy -sum p log p; the normalizer,
  * log sum e^x; and the `top` likeliest alternatives, (rows, top), best first, equal ones in the order of their ids.  log_probs (with tokens),

@@ -214,6 +214,7 @@ SIGNATURES = {
     "st_hip_attention_backward_bf16_dev": (c_int, [POINTER(AttentionTrainingStruct), c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p,
                                                    c_size_t, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p, c_void_p, c_size_t,
                                                    c_void_p, c_void_p]),
+    "st_hip_attention_backward_f32_dev": (c_int, [c_size_t, c_size_t, c_size_t, c_float, c_int] + [c_void_p] * 13),
     "st_hip_token_log_probs_f32_dev": (c_int, [c_size_t, c_size_t, c_void_p, c_size_t] + [c_void_p] * 4 + [c_size_t] + [c_void_p] * 3),
     "st_hip_token_log_probs_backward_f32_dev": (c_int, [c_size_t, c_size_t, c_void_p, c_size_t] + [c_void_p] * 6 + [c_size_t, c_void_p]),
     "st_hip_token_log_probs_bf16_dev": (c_int, [c_size_t, c_size_t, c_void_p, c_size_t] + [c_void_p] * 4 + [c_size_t] + [c_void_p] * 3),

@@ -1,0 +1,438 @@
+// The backward pass of f32 scaled-dot-product attention with its additive biases: the gradients of
+// softmax(scale·q·kᵀ + z_bias + attn_bias)·v with respect to all five, the probabilities worked out again.
+//
+//   p = exp(s − lse),  dv = pᵀ·g,  ds = p·(g·vᵀ − δ) with δ = Σ g·o,  dq = scale·ds·k,  dk = scale·dsᵀ·q,  dattn = ds,  dz = Σ_query ds
+//
+// Products run on v_mfma_f32_32x32x2_f32, whose 157 TFLOP/s bound the pass: eight products of 2·S²·D against the five that it cannot do
+// without (the scores once for lse, which the forward pass does not keep, and scores and g·vᵀ twice, for dq and for dk and dv).  That
+// instruction takes a value a lane from either operand, so that one copy of a tile in LDS serves rows and columns alike, and accumulators
+// go into the next product register by register.
+//
+// A workgroup owns 32 rows (queries for dq, keys for dk and dv), which its wavefronts all hold as B operands; they deal the tiles of 32
+// rows of the other two matrices out among themselves (wavefront w takes tiles w, w + WAVES, ...), each through LDS of its own, and add
+// up through LDS at the end, in the order of the wavefronts.  So 16 contexts of 1024 are 512 workgroups, and nothing waits for another
+// wavefront before the end.
+#include <algorithm>
+#include <cmath>
+
+#include "device_math.h"
+#include "kernels.h"
+
+namespace sthip {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRows = 32;
+
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+
+struct BackwardArgs {
+    const float *q, *k, *v, *z_bias, *attn_bias, *out, *grad_out;
+    float *grad_q, *grad_k, *grad_v, *grad_z_bias, *grad_attn_bias;
+    float *lse, *delta;  // (contexts, padded): lse·log2 e; rows behind the last +infinity and 0
+    int contexts, S, D, padded, tiles, swizzle;
+    float scale;
+    bool wide_bias;  // four neighbouring biases of a row are one aligned load
+};
+
+// Workgroup -> (context, tile), XCDs with whole contexts where they divide evenly; under a causal mask the longest tiles first.
+__host__ __device__ inline int2 decode(int contexts, int tiles, int swizzle, bool by_tile, bool last_first, unsigned block)
+{
+    const unsigned of_xcd = swizzle ? contexts >> 3 : contexts, first = swizzle ? (block & 7) * of_xcd : 0, i = swizzle ? block >> 3 : block;
+    const unsigned n = static_cast<unsigned>(tiles), tile = by_tile ? i / of_xcd : i % n;
+    return int2{static_cast<int>(first + (by_tile ? i % of_xcd : i / n)), static_cast<int>(last_first ? n - 1 - tile : tile)};
+}
+
+// A tile of 32 rows of DC values (a multiple of 32; zeros from D on) in LDS, its 16-byte chunks turned by the row: sixteen rows' same chunk lies
+// in sixteen places of the banks.
+template <int DC>
+struct Tile {
+    static constexpr int kWide = DC <= 32 ? 32 : DC <= 64 ? 64 : DC <= 128 ? 128 : 256;
+    static constexpr int kRow = kWide * 4, kBytes = kRows * kRow, kTurn = kWide / 4 < 16 ? kWide / 4 - 1 : 15;
+    static __device__ __forceinline__ unsigned place(unsigned row, unsigned chunk) { return row * kRow + (chunk ^ (row & kTurn)) * 16; }
+};
+
+// Rows of a context, zeros behind the last.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const float *first, int rows, int dim)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(first), 0, static_cast<int>(static_cast<unsigned>(rows) * dim * 4u), 0x00020000);
+}
+template <bool VEC>
+__device__ __forceinline__ f32x4 fetch4(const __amdgpu_buffer_rsrc_t &rows, int dim, int row, int column)
+{
+    const unsigned at = (static_cast<unsigned>(row) * dim + column) * 4u;
+    if (VEC) {
+        const u32x4_t raw = __builtin_amdgcn_raw_buffer_load_b128(rows, at, 0, 0);
+        return column < dim ? __builtin_bit_cast(f32x4, raw) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float raw = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, at + e * 4, 0, 0));
+        x[e] = column + e < dim ? raw : 0.0f;
+    }
+    return x;
+}
+
+template <int DC, bool VEC>
+__device__ __forceinline__ void load_tile(const __amdgpu_buffer_rsrc_t &rows, int dim, int first, unsigned char *to, int lane)
+{
+    constexpr int CHUNKS = DC / 4, STEPS = kRows * CHUNKS / 64, BATCH = STEPS % 8 == 0 ? 8 : 4;
+    static_assert(STEPS % BATCH == 0, "the last batch ends with the tile");
+#pragma unroll
+    for (int s = 0; s < STEPS; s += BATCH) {
+        f32x4 x[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int f = lane + 64 * (s + i);
+            x[i] = fetch4<VEC>(rows, dim, first + f / CHUNKS, f % CHUNKS * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int f = lane + 64 * (s + i);
+            *reinterpret_cast<f32x4 *>(to + Tile<DC>::place(f / CHUNKS, f % CHUNKS)) = x[i];
+        }
+    }
+}
+
+__device__ __forceinline__ f32x16 mfma(float a, float b, f32x16 sum) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, sum, 0, 0, 0); }
+__device__ constexpr int row_of(int r) { return (r >> 2) * 8 + (r & 3); }
+
+// tile · staysᵀ: accumulator registers are the tile's rows, lanes the rows that stay.
+template <int DC>
+__device__ __forceinline__ f32x16 product(const unsigned char *tile, const f32x4 (&stays)[DC / 8], int li, int lh)
+{
+    f32x16 sum = {};
+#pragma unroll
+    for (int g = 0; g < DC / 8; ++g) {
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(tile + Tile<DC>::place(li, 2 * g + lh));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = mfma(a[e], stays[g][e], sum);
+    }
+    return sum;
+}
+// sums += tileᵀ · weights: registers are the tile's columns, lanes the rows that stay.
+template <int DC>
+__device__ __forceinline__ void add_product(const unsigned char *tile, const f32x16 &weights, f32x16 (&sums)[DC / 32], int li, int lh)
+{
+    const unsigned base = ((li >> 2) ^ (4 * lh)) * 16 + (li & 3) * 4 + 4 * lh * Tile<DC>::kRow;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int dt = 0; dt < DC / 32; ++dt) {
+            const unsigned turn = ((dt * 8) ^ (row_of(r) & Tile<DC>::kTurn)) * 16;
+            sums[dt] = mfma(*reinterpret_cast<const float *>(tile + (base ^ turn) + row_of(r) * Tile<DC>::kRow), weights[r], sums[dt]);
+        }
+}
+
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The wavefronts' sums (a lane has its row, registers the columns), times `by`, into rows first .. first + 31 of a matrix.
+template <int DC, int WAVES>
+__device__ __forceinline__ void write_rows(const f32x16 (&sums)[DC / 32], float by, float *to, int first, int rows, int dim, unsigned char *lds)
+{
+    constexpr int STRIDE = DC + 4;
+    float *const parts = reinterpret_cast<float *>(lds);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, lh = lane >> 5;
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < DC / 32; ++dt)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+            *reinterpret_cast<f32x4 *>(parts + (wave * kRows + li) * STRIDE + dt * 32 + a * 8 + lh * 4) =
+                f32x4{sums[dt][a * 4], sums[dt][a * 4 + 1], sums[dt][a * 4 + 2], sums[dt][a * 4 + 3]};
+    __syncthreads();
+    for (int i = tid; i < kRows * dim; i += WAVES * 64) {
+        const int row = i / dim, column = i % dim;
+        if (first + row >= rows) break;
+        float sum = parts[row * STRIDE + column];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) sum += parts[(w * kRows + row) * STRIDE + column];
+        to[static_cast<size_t>(first + row) * dim + column] = sum * by;
+    }
+}
+
+// ---- lse, δ, dq: queries stay -----------------------------------------------------------------------------------------------------------
+template <int DC, int WAVES, bool VEC, bool CAUSAL>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <= 64 ? 2 : 1, 4))) void attention_f32_grad_q_kernel(BackwardArgs p)
+{
+    extern __shared__ __attribute__((aligned(16))) unsigned char backward_lds[];
+    __shared__ float maxima[WAVES][kRows], totals[WAVES][kRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
+    const int2 item = decode(p.contexts, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
+    const int context = item.x, q0 = item.y * kRows, my_q = q0 + li, S = p.S, D = p.D;
+    const size_t first = static_cast<size_t>(context) * S;
+    unsigned char *const k_tile = backward_lds + wave * 2 * Tile<DC>::kBytes, *const v_tile = k_tile + Tile<DC>::kBytes;
+    const __amdgpu_buffer_rsrc_t k_rows = rows_of(p.k + first * D, S, D), v_rows = rows_of(p.v + first * D, S, D);
+    f32x4 q[DC / 8], g[DC / 8];
+    float delta = 0.0f;
+    {
+        const __amdgpu_buffer_rsrc_t q_rows = rows_of(p.q + first * D, S, D), g_rows = rows_of(p.grad_out + first * D, S, D),
+                                     o_rows = rows_of(p.out + first * D, S, D);
+#pragma unroll
+        for (int c = 0; c < DC / 8; ++c) {
+            q[c] = fetch4<VEC>(q_rows, D, my_q, c * 8 + lh * 4);
+            g[c] = fetch4<VEC>(g_rows, D, my_q, c * 8 + lh * 4);
+            const f32x4 o = fetch4<VEC>(o_rows, D, my_q, c * 8 + lh * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) delta = fmaf(g[c][e], o[e], delta);
+        }
+    }
+    delta += __shfl_xor(delta, 32);
+    const float *const bias_row = p.attn_bias ? p.attn_bias + (first + my_q) * S : nullptr;
+    const int key_end = CAUSAL ? min(S, q0 + kRows) : S, last_key = CAUSAL ? min(my_q, S - 1) : S - 1;
+    // the scores of a tile, in units of log2 e
+    auto scores = [&](int key0) {
+        f32x16 s = product<DC>(k_tile, q, li, lh);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int key = key0 + a * 8 + lh * 4;
+            f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (bias_row && my_q < S) {
+                if (p.wide_bias) {
+                    if (key < S) bias = *reinterpret_cast<const f32x4 *>(bias_row + key);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (key + e < S) bias[e] = bias_row[key + e];
+                }
+            }
+            if (p.z_bias) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (key + e < S) bias[e] += p.z_bias[first + key + e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = fmaf(s[a * 4 + e], p.scale, bias[e]) * kLog2e;
+                s[a * 4 + e] = key + e > last_key ? -INFINITY : x;
+            }
+        }
+        return s;
+    };
+    float most = -INFINITY, total = 0.0f;
+    for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
+        load_tile<DC, VEC>(k_rows, D, key0, k_tile, lane);
+        wave_fence();
+        const f32x16 s = scores(key0);
+        float top = most;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+        const float safe = top == -INFINITY ? 0.0f : top;
+        total *= __builtin_amdgcn_exp2f(most - safe);
+        most = top;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) total += __builtin_amdgcn_exp2f(s[r] - safe);
+        wave_fence();
+    }
+    {
+        const float other = __shfl_xor(most, 32), other_total = __shfl_xor(total, 32), top = fmaxf(most, other), safe = top == -INFINITY ? 0.0f : top;
+        total = total * __builtin_amdgcn_exp2f(most - safe) + other_total * __builtin_amdgcn_exp2f(other - safe);
+        most = top;
+    }
+    if (lh == 0) {
+        maxima[wave][li] = most;
+        totals[wave][li] = total;
+    }
+    __syncthreads();
+    float top = maxima[0][li];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, maxima[w][li]);
+    const float safe = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum += totals[w][li] * __builtin_amdgcn_exp2f(maxima[w][li] - safe);
+    // (a row without keys: every p is 0)
+    const float lse = my_q < S && sum != 0.0f ? safe + __log2f(sum) : INFINITY;
+    if (wave == 0 && lh == 0) {
+        p.lse[static_cast<size_t>(context) * p.padded + my_q] = lse;
+        p.delta[static_cast<size_t>(context) * p.padded + my_q] = my_q < S ? delta : 0.0f;
+    }
+    f32x16 dq[DC / 32];
+#pragma unroll
+    for (int dt = 0; dt < DC / 32; ++dt) dq[dt] = f32x16{};
+    for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
+        load_tile<DC, VEC>(k_rows, D, key0, k_tile, lane);
+        load_tile<DC, VEC>(v_rows, D, key0, v_tile, lane);
+        wave_fence();
+        f32x16 s = scores(key0);
+        const f32x16 dp = product<DC>(v_tile, g, li, lh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - lse) * (dp[r] - delta);
+        add_product<DC>(k_tile, s, dq, li, lh);
+        wave_fence();
+    }
+    write_rows<DC, WAVES>(dq, p.scale, p.grad_q + first * D, q0, S, D, backward_lds);
+}
+
+// ---- dk, dv, the biases' gradients: keys stay -----------------------------------------------------------------------------------------------
+// Heads above 128 values have room for one of dk and dv in their registers, and take two launches.
+template <int DC, int WAVES, bool VEC, bool CAUSAL, bool DK, bool DV>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <= 64 ? 2 : 1, 4))) void attention_f32_grad_kv_kernel(BackwardArgs p)
+{
+    extern __shared__ __attribute__((aligned(16))) unsigned char backward_lds[];
+    __shared__ float totals[WAVES][kRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
+    const int2 item = decode(p.contexts, p.tiles, p.swizzle, CAUSAL, false, blockIdx.x);
+    const int context = item.x, k0 = item.y * kRows, my_key = k0 + li, S = p.S, D = p.D;
+    const size_t first = static_cast<size_t>(context) * S;
+    unsigned char *const q_tile = backward_lds + wave * 2 * Tile<DC>::kBytes, *const g_tile = q_tile + Tile<DC>::kBytes;
+    const __amdgpu_buffer_rsrc_t q_rows = rows_of(p.q + first * D, S, D), g_rows = rows_of(p.grad_out + first * D, S, D);
+    f32x4 k[DC / 8], v[DK ? DC / 8 : 1];
+    {
+        const __amdgpu_buffer_rsrc_t k_rows = rows_of(p.k + first * D, S, D), v_rows = rows_of(p.v + first * D, S, D);
+#pragma unroll
+        for (int c = 0; c < DC / 8; ++c) {
+            k[c] = fetch4<VEC>(k_rows, D, my_key, c * 8 + lh * 4);
+            if (DK) v[DK ? c : 0] = fetch4<VEC>(v_rows, D, my_key, c * 8 + lh * 4);
+        }
+    }
+    const float z = p.z_bias && my_key < S ? p.z_bias[first + my_key] : 0.0f;
+    f32x16 dk[DK ? DC / 32 : 1], dv[DV ? DC / 32 : 1];
+    if (DK)
+#pragma unroll
+        for (int dt = 0; dt < DC / 32; ++dt) dk[DK ? dt : 0] = f32x16{};
+    if (DV)
+#pragma unroll
+        for (int dt = 0; dt < DC / 32; ++dt) dv[DV ? dt : 0] = f32x16{};
+    float dz = 0.0f;
+    if (CAUSAL && DK && p.grad_attn_bias && my_key < S)  // queries before the tile do not see it
+        for (int q = wave * 2 + lh; q < k0; q += WAVES * 2) p.grad_attn_bias[(first + q) * S + my_key] = 0.0f;
+    for (int row0 = (CAUSAL ? k0 : 0) + wave * kRows; row0 < S; row0 += WAVES * kRows) {
+        load_tile<DC, VEC>(q_rows, D, row0, q_tile, lane);
+        load_tile<DC, VEC>(g_rows, D, row0, g_tile, lane);
+        wave_fence();
+        f32x16 s = product<DC>(q_tile, k, li, lh);
+        const float *const lse = p.lse + static_cast<size_t>(context) * p.padded + row0 + 4 * lh;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const f32x4 of = *reinterpret_cast<const f32x4 *>(lse + a * 8);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = a * 4 + e, row = row0 + row_of(r) + 4 * lh;
+                const float bias = p.attn_bias && row < S && my_key < S ? p.attn_bias[(first + row) * S + my_key] + z : z;
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale, bias) * kLog2e - of[e]);
+                s[r] = CAUSAL && my_key > row ? 0.0f : x;
+            }
+        }
+        if constexpr (DV) add_product<DC>(g_tile, s, dv, li, lh);
+        if constexpr (DK) {
+            f32x16 dp = product<DC>(g_tile, v, li, lh);
+            const float *const delta = p.delta + static_cast<size_t>(context) * p.padded + row0 + 4 * lh;
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const f32x4 of = *reinterpret_cast<const f32x4 *>(delta + a * 8);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = a * 4 + e, row = row0 + row_of(r) + 4 * lh;
+                    s[r] *= dp[r] - of[e];
+                    dz += s[r];
+                    if (p.grad_attn_bias && row < S && my_key < S) p.grad_attn_bias[(first + row) * S + my_key] = s[r];
+                }
+            }
+            add_product<DC>(q_tile, s, dk, li, lh);
+        }
+        wave_fence();
+    }
+    if constexpr (DK) {
+        if (p.grad_z_bias) {
+            dz += __shfl_xor(dz, 32);
+            if (lh == 0) totals[wave][li] = dz;
+            __syncthreads();
+            if (tid < kRows && my_key < S) {
+                float sum = totals[0][li];
+#pragma unroll
+                for (int w = 1; w < WAVES; ++w) sum += totals[w][li];
+                p.grad_z_bias[first + my_key] = sum;
+            }
+        }
+        write_rows<DC, WAVES>(dk, p.scale, p.grad_k + first * D, k0, S, D, backward_lds);
+    }
+    if constexpr (DV) write_rows<DC, WAVES>(dv, 1.0f, p.grad_v + first * D, k0, S, D, backward_lds);
+}
+
+template <class Kernel>
+hipError_t launch(Kernel kernel, const BackwardArgs &args, int waves, size_t lds, bool by_tile, bool last_first, hipStream_t stream)
+{
+    const size_t blocks = static_cast<size_t>(args.contexts) * args.tiles;
+    for (const size_t block : {static_cast<size_t>(0), blocks - 1}) {  // the grid is what the kernels' decode assumes
+        const int2 item = decode(args.contexts, args.tiles, args.swizzle, by_tile, last_first, static_cast<unsigned>(block));
+        if (blocks > kMaxDim || item.x < 0 || item.x >= args.contexts || item.y < 0 || item.y >= args.tiles) return hipErrorInvalidConfiguration;
+    }
+    const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+    if (rc != hipSuccess) return rc;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(waves * 64), lds, stream, args);
+    return hipGetLastError();
+}
+
+template <int DC, bool VEC, bool CAUSAL>
+hipError_t launch_variant(const BackwardArgs &args, hipStream_t stream)
+{
+    constexpr int WAVES = DC <= 128 ? 4 : 2;  // tiles of 256 values: 64 KiB a wavefront
+    constexpr size_t lds = std::max<size_t>(WAVES * 2 * Tile<DC>::kBytes, WAVES * kRows * (DC + 4) * sizeof(float));
+    hipError_t rc = launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
+    if (rc != hipSuccess) return rc;
+    if constexpr (DC <= 128) {
+        return launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, true, true>, args, WAVES, lds, CAUSAL, false, stream);
+    } else {
+        rc = launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, true, false>, args, WAVES, lds, CAUSAL, false, stream);
+        if (rc != hipSuccess) return rc;
+        return launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, false, true>, args, WAVES, lds, CAUSAL, false, stream);
+    }
+}
+
+template <int DC>
+hipError_t launch_width(const BackwardArgs &args, bool vec, bool causal, hipStream_t stream)
+{
+    if (vec) return causal ? launch_variant<DC, true, true>(args, stream) : launch_variant<DC, true, false>(args, stream);
+    return causal ? launch_variant<DC, false, true>(args, stream) : launch_variant<DC, false, false>(args, stream);
+}
+
+}  // namespace
+
+hipError_t launch_attention_backward_f32(size_t contexts, size_t sequence, size_t head_dim, float scale, bool causal, const float *q, const float *k,
+                                         const float *v, const float *z_bias, const float *attn_bias, const float *out, const float *grad_out,
+                                         float *grad_q, float *grad_k, float *grad_v, float *grad_z_bias, float *grad_attn_bias, hipStream_t stream)
+{
+    BackwardArgs args{};
+    args.q = q;
+    args.k = k;
+    args.v = v;
+    args.z_bias = z_bias;
+    args.attn_bias = attn_bias;
+    args.out = out;
+    args.grad_out = grad_out;
+    args.grad_q = grad_q;
+    args.grad_k = grad_k;
+    args.grad_v = grad_v;
+    args.grad_z_bias = grad_z_bias;
+    args.grad_attn_bias = grad_attn_bias;
+    args.contexts = static_cast<int>(contexts);
+    args.S = static_cast<int>(sequence);
+    args.D = static_cast<int>(head_dim);
+    args.tiles = static_cast<int>((sequence + kRows - 1) / kRows);
+    args.padded = args.tiles * kRows;
+    args.swizzle = contexts % 8 == 0;
+    args.scale = scale;
+    auto aligned = [](const void *at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; };
+    args.wide_bias = sequence % 4 == 0 && aligned(attn_bias);
+    const size_t rows = contexts * args.padded;
+    void *scratch = nullptr;
+    const hipError_t rc = stream_workspace(stream, 2 * rows * sizeof(float), &scratch);
+    if (rc != hipSuccess) return rc;
+    args.lse = static_cast<float *>(scratch);
+    args.delta = args.lse + rows;
+    const bool vec = head_dim % 4 == 0 && aligned(q) && aligned(k) && aligned(v) && aligned(out) && aligned(grad_out);
+    if (head_dim <= 32) return launch_width<32>(args, vec, causal, stream);
+    if (head_dim <= 64) return launch_width<64>(args, vec, causal, stream);
+    if (head_dim <= 96) return launch_width<96>(args, vec, causal, stream);
+    if (head_dim <= 128) return launch_width<128>(args, vec, causal, stream);
+    return launch_width<256>(args, vec, causal, stream);
+}
+
+}  // namespace sthip

@@ -1620,6 +1620,34 @@ int st_hip_attention_backward_bf16_dev(const st_hip_attention_training *shape, c
                          "attention backward launch");
 }
 
+int st_hip_attention_backward_f32_dev(size_t contexts, size_t sequence, size_t head_dim, float scale, int causal, const float *q, const float *k,
+                                      const float *v, const float *z_bias, const float *attn_bias, const float *out, const float *grad_out,
+                                      float *grad_q, float *grad_k, float *grad_v, float *grad_z_bias, float *grad_attn_bias, void *stream)
+{
+    ST_HIP_CHECK(ensure_init());
+    AttentionPlan plan;
+    ST_HIP_CHECK(plan_attention(contexts, sequence, head_dim, &plan));
+    if (!std::isfinite(scale))
+        return fail(ST_HIP_ERR_NONFINITE, "non-finite value encountered in scaled_dot_attention_scale: %g", static_cast<double>(scale));
+    if ((grad_z_bias && !z_bias) || (grad_attn_bias && !attn_bias))
+        return fail(ST_HIP_ERR_INVALID, "attention backward: a bias's gradient without the bias");
+    if (plan.rows == 0 || (head_dim == 0 && !grad_z_bias && !grad_attn_bias)) return ST_HIP_OK;
+    ST_HIP_CHECK(check_attention_kernel_limits(contexts, sequence, head_dim));
+    // (a tile's rows behind the last are looked up)
+    if (sequence > kMaxDim - 256 || (sequence + 256) * (head_dim + 8) * sizeof(float) >= 1ull << 31)
+        return fail(ST_HIP_ERR_UNSUPPORTED, "attention backward: a context of %zu x %zu exceeds 2 GiB", sequence, head_dim);
+    if (plan.bias_len > static_cast<size_t>(-1) / 8) return fail(ST_HIP_ERR_INVALID, "attention dimensions overflow");
+    if (head_dim && (!q || !k || !v || !out || !grad_out || !grad_q || !grad_k || !grad_v))
+        return fail(ST_HIP_ERR_INVALID, "attention received a null pointer; provide contiguous buffers");
+    const size_t matrix = plan.qkv_len * sizeof(float), row = plan.z_len * sizeof(float), square = plan.bias_len * sizeof(float);
+    const Region read[] = {flat(q, matrix), flat(k, matrix), flat(v, matrix), flat(z_bias, row), flat(attn_bias, square), flat(out, matrix), flat(grad_out, matrix)};
+    const Region written[] = {flat(grad_q, matrix), flat(grad_k, matrix), flat(grad_v, matrix), flat(grad_z_bias, row), flat(grad_attn_bias, square)};
+    ST_HIP_CHECK(check_regions("attention backward", read, written));
+    return launch_status(launch_attention_backward_f32(contexts, sequence, head_dim, scale, causal != 0, q, k, v, z_bias, attn_bias, out, grad_out, grad_q,
+                                                       grad_k, grad_v, grad_z_bias, grad_attn_bias, as_stream(stream)),
+                         "attention backward launch");
+}
+
 int st_hip_token_log_probs_f32_dev(size_t rows, size_t vocab, const float *logits, size_t ld, const int32_t *tokens, float *log_probs,
                                    float *entropies, float *normalizers, size_t top, int32_t *top_ids, float *top_log_probs, void *stream)
 {

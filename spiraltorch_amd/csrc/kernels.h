@@ -224,6 +224,10 @@ hipError_t launch_attention_backward_bf16(const st_hip_attention_training &shape
                                           uint16_t *grad_q, size_t ld_grad_q, uint16_t *grad_k, uint16_t *grad_v, size_t ld_grad_kv, float *grad_table,
                                           hipStream_t stream);
 
+// The backward pass of launch_attention_f32 (see st_hip.h).  Uses the stream's scratch memory.
+hipError_t launch_attention_backward_f32(size_t contexts, size_t sequence, size_t head_dim, float scale, bool causal, const float *q, const float *k,
+                                         const float *v, const float *z_bias, const float *attn_bias, const float *out, const float *grad_out,
+                                         float *grad_q, float *grad_k, float *grad_v, float *grad_z_bias, float *grad_attn_bias, hipStream_t stream);
 // Log-probabilities of given tokens and the logits' gradient, f32 or bf16 logits (see st_hip.h).
 hipError_t launch_token_log_probs(bool bf16, size_t rows, size_t vocab, const void *logits, size_t ld, const int32_t *tokens, float *log_probs,
                                   float *entropies, float *normalizers, size_t top, int32_t *top_ids, float *top_log_probs, hipStream_t stream);

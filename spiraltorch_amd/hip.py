@@ -678,6 +678,15 @@ def attention_backward_bf16_dev(shape: AttentionTraining, q, ld_q, k, v, ld_kv, 
                                                           ld_grad_kv, _dev(grad_table), _stream_ptr(stream)))
 
 
+def attention_backward_f32_dev(contexts, sequence, head_dim, scale, causal, q, k, v, z_bias, attn_bias, out, grad_out, grad_q, grad_k, grad_v,
+                               grad_z_bias=None, grad_attn_bias=None, stream=None) -> None:
+    """The backward pass of attention_f32_dev: the gradients of q, k, v and, where given, of the biases (see
+    st_hip_attention_backward_f32_dev)."""
+    _check(_lib.load().st_hip_attention_backward_f32_dev(contexts, sequence, head_dim, scale, int(bool(causal)), _dev(q), _dev(k), _dev(v),
+                                                         _dev(z_bias), _dev(attn_bias), _dev(out), _dev(grad_out), _dev(grad_q), _dev(grad_k),
+                                                         _dev(grad_v), _dev(grad_z_bias), _dev(grad_attn_bias), _stream_ptr(stream)))
+
+
 def token_log_probs_f32_dev(rows, vocab, logits, ld, tokens, log_probs, entropies, normalizers, top=0, top_ids=None, top_log_probs=None,
                             stream=None) -> None:
     """Log-probabilities of given tokens (int32), entropies, normalizers and the likeliest alternatives of rows of logits (see

@@ -261,6 +261,7 @@ extern "C" {
     pub fn st_hip_attention_kv_cache_bf16_dev(cache: *const StHipKvCache, requests: usize, rows: usize, heads: usize, scale: f32, causal: c_int, row_offsets: *const i32, lengths: *const i32, page_table: *const i32, table_width: usize, q: *const u16, ld_q: usize, out: *mut u16, ld_out: usize, stream: *mut c_void) -> c_int;
     pub fn st_hip_attention_training_bf16_dev(shape: *const StHipAttentionTraining, q: *const u16, ld_q: usize, k: *const u16, v: *const u16, ld_kv: usize, out: *mut u16, ld_out: usize, lse: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_attention_backward_bf16_dev(shape: *const StHipAttentionTraining, q: *const u16, ld_q: usize, k: *const u16, v: *const u16, ld_kv: usize, out: *const u16, ld_out: usize, lse: *const f32, grad_out: *const u16, ld_grad_out: usize, grad_q: *mut u16, ld_grad_q: usize, grad_k: *mut u16, grad_v: *mut u16, ld_grad_kv: usize, grad_table: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn st_hip_attention_backward_f32_dev(contexts: usize, sequence: usize, head_dim: usize, scale: f32, causal: c_int, q: *const f32, k: *const f32, v: *const f32, z_bias: *const f32, attn_bias: *const f32, out: *const f32, grad_out: *const f32, grad_q: *mut f32, grad_k: *mut f32, grad_v: *mut f32, grad_z_bias: *mut f32, grad_attn_bias: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_token_log_probs_f32_dev(rows: usize, vocab: usize, logits: *const f32, ld: usize, tokens: *const i32, log_probs: *mut f32, entropies: *mut f32, normalizers: *mut f32, top: usize, top_ids: *mut i32, top_log_probs: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_token_log_probs_bf16_dev(rows: usize, vocab: usize, logits: *const u16, ld: usize, tokens: *const i32, log_probs: *mut f32, entropies: *mut f32, normalizers: *mut f32, top: usize, top_ids: *mut i32, top_log_probs: *mut f32, stream: *mut c_void) -> c_int;
     pub fn st_hip_token_log_probs_backward_f32_dev(rows: usize, vocab: usize, logits: *const f32, ld: usize, tokens: *const i32, normalizers: *const f32, entropies: *const f32, grad_log_probs: *const f32, grad_entropies: *const f32, grad_logits: *mut f32, ld_grad: usize, stream: *mut c_void) -> c_int;

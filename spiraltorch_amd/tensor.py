@@ -491,6 +491,37 @@ class Tensor:
         return out._validate_result("scaled_dot_attention_output")  # pure.rs:4206-4210
 
 
+    def scaled_dot_attention_backward(self, keys: "Tensor", values: "Tensor", output: "Tensor", grad_output: "Tensor", *, contexts: int,
+                                      sequence: int, scale: float, z_bias: Optional["Tensor"] = None,
+                                      attn_bias: Optional["Tensor"] = None, causal: bool = False, backend: Optional[str] = None):
+        """The gradients of scaled_dot_attention from its operands, its output and that output's gradient: (queries, keys, values, z_bias or
+        None, attn_bias or None).  No reference counterpart."""
+        _resolve_backend(backend)
+        expected_rows = contexts * sequence
+        for t, shape in ((self, (expected_rows, self.cols)), (keys, (expected_rows, self.cols)), (values, (expected_rows, self.cols)),
+                         (output, (expected_rows, self.cols)), (grad_output, (expected_rows, self.cols)), (z_bias, (contexts, sequence)),
+                         (attn_bias, (expected_rows, sequence))):
+            if t is not None and t.shape() != shape:
+                raise TensorError("ShapeMismatch", f"left {t.shape()} right {shape}", left=t.shape(), right=shape)
+        if not np.isfinite(scale):
+            raise TensorError("NonFiniteValue", f"non-finite value encountered in scaled_dot_attention_scale: {scale}",
+                              label="scaled_dot_attention_scale")
+        for t, name in ((self, "query"), (keys, "key"), (values, "value"), (z_bias, "z_bias"), (attn_bias, "attn_bias"), (output, "output"),
+                        (grad_output, "grad_output")):
+            if t is not None:
+                t._require_finite(f"scaled_dot_attention_{name}")
+        if expected_rows == 0 or self.cols == 0:
+            return tuple(None if t is None else Tensor.zeros(*t.shape()) for t in (self, keys, values, z_bias, attn_bias))
+        gradients = [None if t is None else Tensor._on_device_result(*t.shape()) for t in (self, keys, values, z_bias, attn_bias)]
+        try:
+            hip.attention_backward_f32_dev(contexts, sequence, self.cols, scale, causal, self._device(), keys._device(), values._device(),
+                                           None if z_bias is None else z_bias._device(), None if attn_bias is None else attn_bias._device(),
+                                           output._device(), grad_output._device(), *(None if g is None else g._dev for g in gradients))
+        except hip.HipErr as err:
+            raise _backend_failure(err) from err
+        return tuple(None if g is None else g._validate_result("scaled_dot_attention_backward_output") for g in gradients)
+
+
 class Conv2d:
     """Conv2d layer of crates/st-nn/src/layers/conv.rs:607-1013 (forward and backward), with the optional fused
     activation the reference composes as a separate Relu layer.  `backward` accumulates into `weight_gradient` and
