@@ -17,8 +17,8 @@ namespace sthip {
 
 namespace {
 
-constexpr int kUnroll = 4;  // 16-byte loads that a thread has on their way
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kUnroll = 4;  // 16-byte loads that a thread of the backward pass has on their way
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1e30f;  // a difference beyond every exponential that is not 0, and whose products are finite
 
 typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
@@ -62,24 +62,26 @@ __device__ __forceinline__ float value_of_key(key_t key)
 }
 __device__ __forceinline__ int index_of_key(key_t key) { return static_cast<int>(~static_cast<unsigned>(key)); }
 
-// m, L and T of some values.  No value at all: L = 0.
+// m, L and T of some values; T in units of log2 e, as it is summed.  No value at all: L = 0.
 struct Sums {
     float m, l, t;
     static __device__ __forceinline__ Sums none() { return Sums{-FLT_MAX, 0.0f, 0.0f}; }
     __device__ __forceinline__ void raise(float to)
     {
         if (!(to > m)) return;
-        const float by = fmaxf(m - to, kFar), a = __builtin_amdgcn_exp2f(by * kLog2e);
+        const float by = fmaxf((m - to) * kLog2e, kFar), a = __builtin_amdgcn_exp2f(by);
         t = a * fmaf(by, l, t);
         l *= a;
         m = to;
     }
-    __device__ __forceinline__ void add(float x)  // m is not below x
+    // m is not below the value.  `ordinary`: m·log2 e is far from overflow, and the exponent is one multiply-add.
+    __device__ __forceinline__ void add(float x, bool ordinary)
     {
-        const float d = x - m, e = __builtin_amdgcn_exp2f(d * kLog2e);
+        const float d = ordinary ? fmaf(x, kLog2e, -m * kLog2e) : (x - m) * kLog2e, e = __builtin_amdgcn_exp2f(d);
         l += e;
         t = fmaf(e, fmaxf(d, kFar), t);  // (a value of -infinity adds nothing)
     }
+    __device__ __forceinline__ bool ordinary() const { return __all(fabsf(m) < 1e38f); }
     __device__ __forceinline__ void join(const Sums &other)
     {
         const float most = fmaxf(m, other.m);
@@ -91,24 +93,49 @@ struct Sums {
     }
     __device__ __forceinline__ void join_wave()
     {
-#pragma unroll
-        for (int by = 32; by > 0; by >>= 1) {
-            Sums other;
-            other.m = __shfl_xor(m, by);
-            other.l = __shfl_xor(l, by);
-            other.t = __shfl_xor(t, by);
-            join(other);
-        }
+        raise(wave_max(m));
+        l = wave_sum(l);
+        t = wave_sum(t);
     }
+    static __device__ __forceinline__ float wave_max(float v)
+    {
+        const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+        const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
+        auto rotated = [](float x, auto control) {
+            return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(control)::value, 0xf, 0xf, true));
+        };
+        v = fmaxf(v, rotated(v, std::integral_constant<int, 0x128>{}));  // row_ror:8, 4, 2, 1
+        v = fmaxf(v, rotated(v, std::integral_constant<int, 0x124>{}));
+        v = fmaxf(v, rotated(v, std::integral_constant<int, 0x122>{}));
+        return fmaxf(v, rotated(v, std::integral_constant<int, 0x121>{}));
+    }
+    __device__ __forceinline__ float log_l() const { return __log2f(l) * kLn2; }
+    __device__ __forceinline__ float lse() const { return l == 0.0f ? -INFINITY : m + log_l(); }
+    __device__ __forceinline__ float entropy() const { return l == 0.0f ? 0.0f : (__log2f(l) - t / l) * kLn2; }
 };
 
+// How many of the first `count` keys are larger.
+__device__ __forceinline__ int larger_keys(const key_t *keys, int count, key_t than)
+{
+    int larger = 0, j = 0;
+    for (; j + 8 <= count; j += 8) {  // eight reads on their way: one after the other would wait for each
+        key_t other[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) other[u] = keys[j + u];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) larger += other[u] > than;
+    }
+    for (; j < count; ++j) larger += keys[j] > than;
+    return larger;
+}
 // The best `top` of the first `count` keys, sorted, into `best`, by a group of threads: a key's place is the number of larger ones.
 __device__ __forceinline__ void rank_keys(const key_t *keys, int count, int top, key_t *best, int thread, int threads)
 {
     for (int i = thread; i < count; i += threads) {
         const key_t mine = keys[i];
-        int place = 0;
-        for (int j = 0; j < count; ++j) place += keys[j] > mine;
+        const int place = larger_keys(keys, count, mine);
         if (place < top) best[place] = mine;
     }
 }
@@ -116,9 +143,9 @@ __device__ __forceinline__ void rank_keys(const key_t *keys, int count, int top,
 template <typename T>
 __device__ __forceinline__ void write_row(const LogProbsArgs &p, int row, const Sums &s)
 {
-    const float lse = s.l == 0.0f ? -INFINITY : s.m + __log2f(s.l) * 0.6931471805599453f;
+    const float lse = s.lse();
     if (p.normalizers) p.normalizers[row] = lse;
-    if (p.entropies) p.entropies[row] = s.l == 0.0f ? 0.0f : __log2f(s.l) * 0.6931471805599453f - s.t / s.l;
+    if (p.entropies) p.entropies[row] = s.entropy();
     if (p.log_probs) {
         const int token = p.tokens[row];
         const bool counts = token >= 0 && token < p.vocab;
@@ -128,85 +155,114 @@ __device__ __forceinline__ void write_row(const LogProbsArgs &p, int row, const 
 }
 __device__ __forceinline__ void write_top(const LogProbsArgs &p, int row, int i, key_t key, const Sums &s)
 {
-    const float lse = s.l == 0.0f ? -INFINITY : s.m + __log2f(s.l) * 0.6931471805599453f;
+    const float lse = s.lse();
     const size_t at = static_cast<size_t>(row) * p.top + i;
     p.top_ids[at] = key ? index_of_key(key) : -1;
     p.top_log_probs[at] = !key ? NAN : lse == -INFINITY ? -INFINITY : value_of_key(key) - lse;
 }
 
-// How many keys a group of `waves` wavefronts may find in a round, `top` lanes of each with all their values at the most.
-constexpr int kLaneValues(int size) { return kUnroll * 16 / size + 1; }
-__host__ __device__ constexpr int keys_of_round(int waves, int size, int top) { return waves * top * kLaneValues(size); }
+// What a wavefront's list has room for: the best so far and a round of `runs` 16-byte runs a lane, in which no more than `top` lanes with all their
+// values (one of them from the part's edges) have anything to add.
+__host__ __device__ constexpr int room_of(int runs, int size, int top) { return top + top * (runs * 16 / size + 1); }
 
-// WAVES wavefronts to a part of a row: all four of a workgroup, or one.
-template <typename T, int WAVES, bool TOP>
+// A number that at least `top` of the lanes' values reach, and few more: the top-th largest of them but for its last six bits, which tell equal
+// ones apart here.
+__device__ __forceinline__ unsigned wave_bound(unsigned ordered, int top)
+{
+    const unsigned mine = (ordered & ~63u) | (63u - (threadIdx.x & 63));
+    int place = 0;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) place += static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) > mine;
+    const int which = __ffsll(__ballot(place == top - 1)) - 1;
+    return static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(mine), which)) & ~63u;
+}
+
+// The next number below a finite one; -infinity for that and, as it comes from a bound without its last bits, for NaN.
+__device__ __forceinline__ float below(float x)
+{
+    if (!(x > -INFINITY)) return -INFINITY;
+    const float y = x + 0.0f;  // -0 is 0
+    return y == 0.0f ? -1e-45f : __uint_as_float(__float_as_uint(y) + (y > 0.0f ? ~0u : 1u));
+}
+
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// WAVES wavefronts to a part of a row: all four of a workgroup, or one.  A round: RUNS 16-byte runs a lane, those of the next one on their way
+// meanwhile.  Every wavefront keeps a list of its own of what may be among the best, and they are put together at the end.
+template <typename T, int WAVES, int RUNS, bool TOP>
 __global__ __launch_bounds__(256) void token_log_probs_kernel(LogProbsArgs p)
 {
     constexpr int N = 16 / sizeof(T), THREADS = WAVES * 64, GROUPS = 4 / WAVES;
-    extern __shared__ __attribute__((aligned(16))) key_t log_probs_lds[];  // of every group: best [top], then keys [top + two rounds]
+    extern __shared__ __attribute__((aligned(16))) key_t log_probs_lds[];  // of every wavefront: best [top], then keys
     __shared__ Sums wave_sums[4];
     __shared__ int counts[4];
-    __shared__ key_t bounds[4];
-    const int tid = threadIdx.x % THREADS, group = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS), lane = tid & 63;
-    const long long item = static_cast<long long>(blockIdx.x) * GROUPS + group;
-    const bool works = item < static_cast<long long>(p.rows) * p.parts;  // (all of a group, and of a workgroup of one)
-    auto sync = [] {
-        if (WAVES > 1) {
-            __syncthreads();
-        } else {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
-    };
-    if (!works) return;
+    __shared__ float reached[4];  // by `top` values of a wavefront's list
+    const int tid = threadIdx.x % THREADS, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = tid & 63;
+    const long long item = static_cast<long long>(blockIdx.x) * GROUPS + wave / WAVES;
+    if (item >= static_cast<long long>(p.rows) * p.parts) return;  // (all of a workgroup of one part)
     const int row = static_cast<int>(item / p.parts), part = static_cast<int>(item % p.parts);
     const int from = part * p.part_size, to = min(p.vocab, from + p.part_size);
     const T *const x = static_cast<const T *>(p.logits) + row * p.ld;
-    const int round = keys_of_round(WAVES, sizeof(T), p.top), held = 2 * p.top + 2 * round;
-    key_t *const best = log_probs_lds + group * held, *const keys = best + p.top;
-    int *const count = counts + group;
-    key_t *const bound = bounds + group;
-    if (TOP) {
-        if (tid == 0) {
-            *count = 0;
-            *bound = 0;
-        }
-        sync();
-    }
-    // 16-byte runs from the first boundary within the part; what stands before and behind them is one value a thread
+    const int top = p.top, room = TOP ? room_of(RUNS, sizeof(T), top) : 0;
+    key_t *const best = log_probs_lds + wave * (top + room), *const keys = best + top;
+    // 16-byte runs from the first boundary within the part; what stands before and behind them is one value a thread, in the first and in the
+    // last round: of equal values, those of later rounds have the higher index
     const int ahead = min(to - from, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x + from) % 16) % 16 / sizeof(T)));
-    const int runs = (to - from - ahead) / N, first = from + ahead, edges = to - from - runs * N;
+    const int runs = (to - from - ahead) / N, first = from + ahead, behind = first + runs * N;
     const u32x4_t *const run_at = reinterpret_cast<const u32x4_t *>(x + first);
-    Sums sums = Sums::none();
-    for (int at = 0; at == 0 || at < runs; at += THREADS * kUnroll) {
-        u32x4_t loaded[kUnroll];
+    constexpr unsigned nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;  // -infinity
+    u32x4_t next[RUNS];
+    auto load = [&](int at) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < RUNS; ++u) {
             const int i = at + u * THREADS + tid;
-            constexpr unsigned nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;  // -infinity
-            loaded[u] = i < runs ? run_at[i] : u32x4_t{nothing, nothing, nothing, nothing};
+            next[u] = u32x4_t{nothing, nothing, nothing, nothing};
+            if (i < runs) next[u] = run_at[i];
         }
-        float edge = -INFINITY;
-        const int edge_at = tid < ahead ? from + tid : first + runs * N + tid - ahead;
-        if (at == 0 && tid < edges) edge = value_of(x[edge_at]);
-        float most = edge;
+    };
+    load(0);
+    if (TOP && WAVES > 1) {
+        if (lane == 0) reached[wave] = -INFINITY;
+        __syncthreads();
+    }
+    const bool has_head = tid < ahead, has_tail = tid >= 8 && behind + tid - 8 < to;  // (fewer than eight of each, a lane for each)
+    const float edge = has_head ? value_of(x[from + tid]) : has_tail ? value_of(x[behind + tid - 8]) : -INFINITY;
+    const int edge_at = has_head ? from + tid : behind + tid - 8;
+    Sums sums = Sums::none();
+    int count = 0;             // of the wavefront's list
+    float above = -INFINITY;   // what is not above it is not among the best
+    for (int at = 0; at == 0 || at < runs; at += THREADS * RUNS) {
+        u32x4_t loaded[RUNS];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
+        for (int u = 0; u < RUNS; ++u) loaded[u] = next[u];
+        const bool begins = at == 0, ends = at + THREADS * RUNS >= runs;
+        if (!ends) load(at + THREADS * RUNS);
+        const bool has_edge = (begins && has_head) || (ends && has_tail);
+        float most = has_edge ? fmaxf(edge, -INFINITY) : -INFINITY;  // (never NaN)
+#pragma unroll
+        for (int u = 0; u < RUNS; ++u)
 #pragma unroll
             for (int i = 0; i < N; ++i) most = fmaxf(most, value_at<T>(loaded[u], i));
         sums.raise(most);
+        auto add_all = [&](bool ordinary) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
+            for (int u = 0; u < RUNS; ++u)
 #pragma unroll
-            for (int i = 0; i < N; ++i) sums.add(value_at<T>(loaded[u], i));
-        if (at == 0 && tid < edges) sums.add(edge);
+                for (int i = 0; i < N; ++i) sums.add(value_at<T>(loaded[u], i), ordinary);
+        };
+        if (sums.ordinary()) add_all(true);
+        else add_all(false);
+        if (has_edge) sums.add(edge, false);
         if (TOP) {
-            const key_t least = *bound;
             // every value this lane has in the round, with its index
             auto each = [&](auto &&of) {
-                if (at == 0 && tid < edges) of(edge, edge_at);
+                if (has_edge) of(edge, edge_at);
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
+                for (int u = 0; u < RUNS; ++u) {
                     const int run = at + u * THREADS + tid;
                     if (run < runs) {
 #pragma unroll
@@ -214,61 +270,123 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(LogProbsArgs p)
                     }
                 }
             };
-            bool may = least == 0 || most >= value_of_key(least);
-            key_t mine = 0;
-            if (__any(may)) {
-                if (may) each([&](float v, int index) {
-                    if (v == v) mine = max(mine, key_of(v, index));  // (NaN is no alternative)
-                });
-                may = mine > least;
-                key_t lower = least + 1;
-                if (__popcll(__ballot(may)) > p.top) {  // the best of more than `top` lanes: what is below the top-th of them is not among the best
+            auto compact = [&] {
+                rank_keys(keys, count, top, best, lane, 64);
+                wave_fence();
+                count = min(count, top);
+                if (lane < count) keys[lane] = best[lane];
+                if (count == top) {
+                    above = value_of_key(best[top - 1]);  // equal ones to come have a higher index
+                    if (WAVES > 1 && lane == 0) __hip_atomic_store(&reached[wave], above, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                }
+                wave_fence();
+            };
+            if (begins) {
+                above = below(value_of_key(static_cast<key_t>(wave_bound(static_cast<unsigned>(key_of(most, 0) >> 32), top)) << 32));
+            } else if (WAVES > 1) {  // what `top` values of another wavefront reach; equal ones here may have a lower index than those
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w)
+                    above = fmaxf(above, below(__hip_atomic_load(&reached[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)));
+            }
+            // (-infinity: everything but NaN may be among the best, -infinity too)
+            if (__any(most > above) || above == -INFINITY) {
+                // How many values the lane adds, as many as there is room for; where many reach the bound and are equal, below the top-th of
+                // the lanes' best keys is nothing to add.
+                key_t lower = 0;
+                bool by_key = above == -INFINITY;
+                auto found = [&] {
+                    unsigned n = 0;
+                    if (by_key) {
+                        each([&](float v, int index) { n += v >= above && key_of(v, index) >= lower; });
+                    } else {  // (lanes without a run have -infinity in its place)
+                        n += has_edge && edge > above;
+#pragma unroll
+                        for (int u = 0; u < RUNS; ++u)
+#pragma unroll
+                            for (int i = 0; i < N; ++i) n += value_at<T>(loaded[u], i) > above;
+                    }
+                    return n;
+                };
+                unsigned mine = 0, up_to = 0;
+                int all = 0;
+                auto rank = [&] {
+                    mine = found();
+                    up_to = wave_scan(mine, [](unsigned a, unsigned b) { return a + b; });
+                    all = __builtin_amdgcn_readlane(static_cast<int>(up_to), 63);
+                };
+                rank();
+                if (count + all > room && count > top) {
+                    compact();
+                    by_key = above == -INFINITY;
+                    rank();
+                }
+                if (count + all > room) {
+                    key_t highest = 0;
+                    each([&](float v, int index) {
+                        if (by_key ? v >= above : v > above) highest = max(highest, key_of(v, index));
+                    });
                     int place = 0;
                     for (int j = 0; j < 64; ++j) {
-                        const key_t other = static_cast<key_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), j)) << 32 |
-                                            static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(mine), j));
-                        place += other > mine;
+                        const key_t other =
+                            static_cast<key_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(highest >> 32), j))) << 32 |
+                            static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(highest), j));
+                        place += other > highest;
                     }
-                    const int which = __ffsll(__ballot(place == p.top - 1 && mine != 0)) - 1;
-                    lower = static_cast<key_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), which)) << 32 |
-                            static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(mine), which));
-                    may = mine >= lower;
+                    // (more than `top` lanes have some, or they would have room)
+                    const int which = __ffsll(__ballot(place == top - 1)) - 1;
+                    lower = static_cast<key_t>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(highest >> 32), which))) << 32 |
+                            static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(highest), which));
+                    by_key = true;
+                    rank();
                 }
-                if (may) each([&](float v, int index) {
-                    if (v != v) return;
-                    const key_t key = key_of(v, index);
-                    if (key >= lower) keys[atomicAdd(count, 1)] = key;
-                });
-            }
-            sync();
-            const int found = *count;
-            const bool last = at + THREADS * kUnroll >= runs;
-            // the first round gives a bound to begin with; later ones only where another might not fit
-            if (last || at == 0 || found > p.top + round) {
-                rank_keys(keys, found, p.top, best, tid, THREADS);
-                sync();
-                const int kept = min(found, p.top);
-                for (int i = tid; i < kept; i += THREADS) keys[i] = best[i];
-                if (tid == 0) {
-                    *count = kept;
-                    if (found >= p.top) *bound = best[p.top - 1];
+                int place = count + static_cast<int>(up_to - mine);
+                if (mine) {
+                    if (by_key) each([&](float v, int index) {
+                        if (v >= above && key_of(v, index) >= lower) keys[place++] = key_of(v, index);
+                    });
+                    else each([&](float v, int index) {
+                        if (v > above) keys[place++] = key_of(v, index);
+                    });
                 }
+                count += all;
+                wave_fence();
+                // a first bound of its own, and a better one when the list has grown
+                if (count > 2 * top + 32 || (begins && !ends)) compact();
             }
-            sync();
         }
     }
     sums.join_wave();
-    if (WAVES > 1) {
-        if (lane == 0) wave_sums[threadIdx.x >> 6] = sums;
+    if (WAVES == 1) {
+        if (TOP) {
+            rank_keys(keys, count, top, best, lane, 64);
+            wave_fence();
+        }
+    } else {
+        if (lane == 0) {
+            wave_sums[wave] = sums;
+            counts[wave] = count;
+        }
         __syncthreads();
         sums = wave_sums[0];
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) sums.join(wave_sums[w]);
+        if (TOP) {
+            key_t *const list = log_probs_lds + top;
+            for (int i = lane; i < counts[wave]; i += 64) {  // a wavefront's keys among everyone's
+                const key_t mine = keys[i];
+                int place = 0;
+                for (int w = 0; w < WAVES; ++w) place += larger_keys(list + w * (top + room), counts[w], mine);
+                if (place < top) log_probs_lds[place] = mine;  // the first wavefront's `best`
+            }
+            count = 0;
+            for (int w = 0; w < WAVES; ++w) count += counts[w];
+            __syncthreads();
+        }
     }
-    const int kept = TOP ? *count : 0;
+    const key_t *const sorted = WAVES == 1 ? best : log_probs_lds;
     if (p.parts == 1) {
         if (tid == 0) write_row<T>(p, row, sums);
-        if (TOP && tid < p.top) write_top(p, row, tid, tid < kept ? best[tid] : 0, sums);
+        if (TOP && tid < top) write_top(p, row, tid, tid < count ? sorted[tid] : 0, sums);
     } else {
         float *const to_sums = p.part_sums + item * 3;
         if (tid == 0) {
@@ -276,7 +394,7 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(LogProbsArgs p)
             to_sums[1] = sums.l;
             to_sums[2] = sums.t;
         }
-        if (TOP && tid < p.top) p.part_keys[item * p.top + tid] = tid < kept ? best[tid] : 0;
+        if (TOP && tid < top) p.part_keys[item * top + tid] = tid < count ? sorted[tid] : 0;
     }
 }
 
@@ -285,31 +403,49 @@ constexpr int kMostParts = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void token_log_probs_join_kernel(LogProbsArgs p)
 {
-    __shared__ key_t keys[kMostParts * ST_HIP_LOG_PROBS_MOST_TOP], best[ST_HIP_LOG_PROBS_MOST_TOP];
+    constexpr int KEYS = kMostParts * ST_HIP_LOG_PROBS_MOST_TOP / 256;  // of a thread
+    __shared__ key_t keys[KEYS * 256], best[ST_HIP_LOG_PROBS_MOST_TOP];
     __shared__ Sums all;
     __shared__ int count;
-    const int row = blockIdx.x, tid = threadIdx.x;
-    if (tid == 0) count = 0;
-    if (tid < p.top) best[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < p.parts * p.top; i += 256) {
-        const key_t key = p.part_keys[static_cast<long long>(row) * p.parts * p.top + i];
-        if (key) keys[atomicAdd(&count, 1)] = key;
+    __shared__ unsigned least;
+    const int row = blockIdx.x, tid = threadIdx.x, found = p.parts * p.top;
+    const key_t *const part_keys = p.part_keys + static_cast<long long>(row) * found;
+    // everything that is read, on its way at once
+    key_t mine[KEYS];
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) mine[i] = i * 256 + tid < found ? part_keys[i * 256 + tid] : 0;
+    // A number that at least `top` keys reach: the top-th largest of the parts' first ones, or, of few parts, the least of their r-th ones with
+    // parts * r not below top.
+    const int rank = p.parts >= p.top ? 0 : (p.top + p.parts - 1) / p.parts - 1;
+    const unsigned of_part = tid < p.parts && p.top ? static_cast<unsigned>(part_keys[tid * p.top + rank] >> 32) : 0;
+    Sums sums = Sums::none();
+    if (tid < p.parts) {
+        const float *const from = p.part_sums + (static_cast<long long>(row) * p.parts + tid) * 3;
+        sums = Sums{from[0], from[1], from[2]};
     }
+    if (tid < p.top) best[tid] = 0;
     if (tid < 64) {
-        Sums sums = Sums::none();
-        if (tid < p.parts) {
-            const float *const from = p.part_sums + (static_cast<long long>(row) * p.parts + tid) * 3;
-            sums.m = from[0];
-            sums.l = from[1];
-            sums.t = from[2];
-        }
         sums.join_wave();
+        unsigned bound = 0;
+        if (p.top && rank == 0) {
+            bound = wave_bound(of_part, p.top);
+        } else if (p.top) {
+            bound = tid < p.parts ? of_part : ~0u;
+#pragma unroll
+            for (int by = 32; by > 0; by >>= 1) bound = min(bound, static_cast<unsigned>(__shfl_xor(static_cast<int>(bound), by)));
+        }
         if (tid == 0) {
             all = sums;
-            write_row<T>(p, row, sums);
+            least = bound;
+            count = 0;
         }
     }
+    __syncthreads();
+    const unsigned from = least;
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i)
+        if (mine[i] && static_cast<unsigned>(mine[i] >> 32) >= from) keys[atomicAdd(&count, 1)] = mine[i];
+    if (tid == 0) write_row<T>(p, row, sums);
     __syncthreads();
     rank_keys(keys, count, p.top, best, tid, 256);
     __syncthreads();
@@ -393,10 +529,10 @@ __global__ __launch_bounds__(256) void token_log_probs_grad_kernel(LogProbsGradA
 
 // A wavefront takes a row of up to so many bytes, a workgroup longer ones.
 constexpr size_t kWaveRow = 4096;
-// Rows are cut into parts where there are fewer than workgroups to fill the chip with, of 16 KiB or more.
+// Rows are cut into parts where there are fewer than workgroups to fill the chip with, of 8 KiB (two runs a thread) or more.
 int parts_of(size_t rows, size_t vocab, size_t size, size_t most)
 {
-    const size_t wanted = (512 + rows - 1) / rows, possible = vocab * size / (16u << 10);
+    const size_t wanted = (512 + rows - 1) / rows, possible = vocab * size / (8u << 10);
     return static_cast<int>(std::max<size_t>(1, std::min({wanted, possible, most})));
 }
 
@@ -420,16 +556,24 @@ hipError_t launch_forward(LogProbsArgs args, hipStream_t stream)
         args.part_keys = static_cast<key_t *>(scratch);
         args.part_sums = reinterpret_cast<float *>(static_cast<unsigned char *>(scratch) + keys);
     }
-    const size_t lds = args.top ? groups * (2 * args.top + 2 * keys_of_round(wave ? 1 : 4, sizeof(T), args.top)) * sizeof(key_t) : 0;
-    auto run = [&](auto kernel) {
+    auto run = [&](auto waves, auto runs, auto top) {
+        auto kernel = token_log_probs_kernel<T, decltype(waves)::value, decltype(runs)::value, decltype(top)::value>;
+        const size_t keys = args.top ? args.top + room_of(decltype(runs)::value, sizeof(T), args.top) : 0;
+        const size_t lds = 4 * keys * sizeof(key_t);
         const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
         if (rc != hipSuccess) return rc;
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), lds, stream, args);
         return hipGetLastError();
     };
-    hipError_t rc;
-    if (wave) rc = args.top ? run(token_log_probs_kernel<T, 1, true>) : run(token_log_probs_kernel<T, 1, false>);
-    else rc = args.top ? run(token_log_probs_kernel<T, 4, true>) : run(token_log_probs_kernel<T, 4, false>);
+    // no more runs to a round than a lane has
+    auto with_runs = [&](auto waves, auto top) {
+        const size_t of_lane = args.part_size * sizeof(T) / (16 * 64 * decltype(waves)::value);
+        if (of_lane <= 1) return run(waves, std::integral_constant<int, 1>{}, top);
+        if (of_lane <= 2) return run(waves, std::integral_constant<int, 2>{}, top);
+        return run(waves, std::integral_constant<int, 4>{}, top);
+    };
+    auto with_top = [&](auto waves) { return args.top ? with_runs(waves, std::true_type{}) : with_runs(waves, std::false_type{}); };
+    const hipError_t rc = wave ? with_top(std::integral_constant<int, 1>{}) : with_top(std::integral_constant<int, 4>{});
     if (rc != hipSuccess || args.parts == 1) return rc;
     hipLaunchKernelGGL(token_log_probs_join_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, args);
     return hipGetLastError();
