@@ -50,6 +50,8 @@ struct TrainingArgs {
     int batch, heads, kv_heads, group, S;
     unsigned ld_q, ld_kv, ld_out, ld_grad_out, ld_grad_q, ld_grad_kv;
     int tiles, swizzle;
+    int parts;          // workgroups to a tile of keys
+    float *part_sums;   // of dk and dv, f32: (parts, 2, rows, kv_heads * head_dim)
     float scale;
     Buckets buckets;
 };
@@ -57,13 +59,15 @@ struct TrainingArgs {
 struct Item {
     int context, tile;
 };
-// Workgroup -> (context, tile): each XCD (workgroup id mod 8) keeps whole contexts where they divide evenly, so that what comes by stays
-// in its L2; under a causal mask the longest tiles of all its contexts run first.
-__host__ __device__ inline Item decode(int contexts, int tiles, int swizzle, bool by_tile, bool last_first, unsigned block)
+// Workgroup -> (context, tile), `group` neighbouring contexts sharing keys: each XCD (workgroup id mod 8) keeps whole groups where they divide
+// evenly, so that what comes by stays in its L2, every eighth one, so that a batch's long sequences are spread over them; under a causal
+// mask the longest tiles of all its contexts run first.
+__host__ __device__ inline Item decode(int groups, int group, int tiles, int swizzle, bool by_tile, bool last_first, unsigned block)
 {
-    const unsigned of_xcd = swizzle ? contexts >> 3 : contexts, first = swizzle ? (block & 7) * of_xcd : 0, i = swizzle ? block >> 3 : block;
-    const unsigned n = static_cast<unsigned>(tiles), tile = by_tile ? i / of_xcd : i % n;
-    return Item{static_cast<int>(first + (by_tile ? i % of_xcd : i / n)), static_cast<int>(last_first ? n - 1 - tile : tile)};
+    const unsigned contexts = static_cast<unsigned>(groups) * group, of_xcd = swizzle ? contexts >> 3 : contexts, i = swizzle ? block >> 3 : block;
+    const unsigned n = static_cast<unsigned>(tiles), tile = by_tile ? i / of_xcd : i % n, j = by_tile ? i % of_xcd : i / n;
+    const unsigned context = swizzle ? (j / group * 8 + (block & 7)) * group + j % group : j;
+    return Item{static_cast<int>(context), static_cast<int>(last_first ? n - 1 - tile : tile)};
 }
 
 // A 64-row stage in LDS: rows of D values as they are in memory, their 16-byte chunks swapped about so that neither kind of read meets
@@ -162,13 +166,19 @@ __device__ __forceinline__ bf16x8 packed(const f32x16 &x, int j)
 // The accumulator register's row within its 32, for lanes 0 to 31; lanes 32 to 63 hold the fourth row behind it.
 __device__ constexpr int row_of(int r) { return (r >> 2) * 8 + (r & 3); }
 
-// What a key `distance` behind its query (negative: before it) is given, for distances of −far .. far: bias[distance + far], in units of
-// log2 e.  Beyond them it is that of the ends.
+// Biases and sums by distance hold those of -far - 64 .. far + 64: a 32x32 block whose distances are not all beyond `far` on one side lies within.
+constexpr int kMargin = 64;
+__host__ __device__ inline int distances_of(int far) { return 2 * far + 2 * kMargin + 1; }
+
+// Where distances lie among those that a block's registers are given: bias[from + row_of(r)], or the one bias of a block beyond `far`.
+__device__ __forceinline__ bool near(int d0, int far) { return d0 - 31 < far && d0 + 31 > -far; }
+
+// What a key `distance` behind its query (negative: before it) is given: bias[distance + far + 64], in units of log2 e.
 __device__ __forceinline__ void fill_bias(const TrainingArgs &p, int head, float *bias, int tid)
 {
     const Buckets &b = p.buckets;
-    for (int i = tid; i <= 2 * b.far; i += 256) {
-        const int distance = i - b.far, m = b.bidirectional ? abs(distance) : max(-distance, 0);
+    for (int i = tid; i < distances_of(b.far); i += 256) {
+        const int distance = min(max(i - b.far - kMargin, -b.far), b.far), m = b.bidirectional ? abs(distance) : max(-distance, 0);
         int bucket = b.bidirectional && distance > 0 ? b.side : 0;
         for (int j = 1; j < b.side; ++j) bucket += m >= b.first[j];
         bias[i] = p.table[static_cast<size_t>(bucket) * p.heads + head] * kLog2e;
@@ -206,7 +216,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
     float *const bias = reinterpret_cast<float *>(training_lds + 4 * BYTES);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
 
-    const Item item = decode(p.batch * p.heads, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
+    const Item item = decode(p.batch * p.kv_heads, p.group, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
     const int b = item.context / p.heads, h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
     const int length = length_of(p, b);
     uint16_t *const out_row = p.out + (static_cast<size_t>(b) * p.S + my_q) * p.ld_out + static_cast<size_t>(h) * D;
@@ -242,22 +252,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
     for (int t = 0; t < DT; ++t) oacc[t] = f32x16{};
     float run_max = -INFINITY, run_sum = 0.0f;
 
-    auto compute = [&](auto may_mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
-        constexpr bool MAY_MASK = decltype(may_mask_tag)::value;
+    // (One body for stages with masked keys and without: with two, the accumulators are copied where the two meet, behind their last product.)
+    auto compute = [&](const unsigned char *ks, const unsigned char *vs, int key0) {
         f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
             for (int t = 0; t < 2; ++t) s[t] = mfma(reader.row_fragment(ks, t, c), qf[c], s[t]);
         if (BIAS) {
-            const int at = key0 - my_q + 4 * lh, far = p.buckets.far;
+            const int far = p.buckets.far;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t) {
+                const int d0 = key0 + t * 32 - wq0;
+                if (near(d0, far)) {
+                    const float *const of = bias + d0 - li + 4 * lh + far + kMargin;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], by, bias[min(max(at + t * 32 + row_of(r), -far), far) + far]);
+                    for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], by, of[row_of(r)]);
+                } else {
+                    const float of = bias[d0 > 0 ? distances_of(far) - 1 : 0];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], by, of);
+                }
+            }
         }
         float most = -INFINITY;
-        if (MAY_MASK) {
+        if (key0 + kStage > (CAUSAL ? min(length, wq0 + 1) : length)) {
             const int last = (CAUSAL ? min(my_q, length - 1) : length - 1) - key0 - 4 * lh;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -299,16 +318,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
     };
 
     const int key_end = CAUSAL ? min(length, q0 + kStay) : length, stages = (key_end + kStage - 1) / kStage;
-    const int seen = CAUSAL ? min(length, wq0 + 32) : length, plain = (CAUSAL ? min(length, wq0 + 1) : length) / kStage;
+    const int seen = CAUSAL ? min(length, wq0 + 32) : length;
     moving.store(training_lds, training_lds + BYTES, tid);
     __syncthreads();
-    int t = 0;
-    for (; t < stages; ++t) {
+    for (int t = 0; t < stages; ++t) {
         const bool more = t + 1 < stages;
         if (more) moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, (t + 1) * kStage, tid);
         const unsigned char *const ks = training_lds + (t & 1) * 2 * BYTES;
-        if (t < plain) compute(std::false_type{}, ks, ks + BYTES, t * kStage);
-        else if (t * kStage < seen) compute(std::true_type{}, ks, ks + BYTES, t * kStage);
+        if (t * kStage < seen) compute(ks, ks + BYTES, t * kStage);
         if (more) moving.store(training_lds + ((t + 1) & 1) * 2 * BYTES, training_lds + ((t + 1) & 1) * 2 * BYTES + BYTES, tid);
         __syncthreads();
     }
@@ -321,12 +338,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
 }
 
 // ---- backward: dq, δ, the bias's gradient -------------------------------------------------------------------------------------------
-// By distance: `bins` (of a wavefront) holds sums of ds for distances of −far − 64 .. far + 64.
-constexpr int kBinsMargin = 64;
-__host__ __device__ inline int bins_width(int far) { return 2 * far + 2 * kBinsMargin + 1; }
-
 // Adds a 32×32 block's ds (a lane has query q0 + li, its registers keys key0 + row_of(r) + 4·lh), whose distances lie around d0 = key0 − q0, to
-// the bins: every register's values go to the lanes that stand for their distances modulo 32, by a permutation of the lanes, the
+// the bins (of a wavefront, sums of ds by distance): every register's values go to the lanes that stand for their distances modulo 32, by a permutation of the lanes, the
 // non-negative and the negative ones apart; then 64 distances are added at once, each by one lane.
 __device__ __forceinline__ void add_by_distance(const f32x16 &ds, int d0, int far, float *bins, int lane)
 {
@@ -342,7 +355,7 @@ __device__ __forceinline__ void add_by_distance(const f32x16 &ds, int d0, int fa
     }
     upper += __shfl_xor(upper, 32);
     lower += __shfl_xor(lower, 32);
-    float *const at = bins + d0 + (lh ? li - 32 : li) + far + kBinsMargin;
+    float *const at = bins + d0 + (lh ? li - 32 : li) + far + kMargin;
     *at += lh ? lower : upper;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the next block's lanes stand for other distances
     __builtin_amdgcn_wave_barrier();
@@ -354,12 +367,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     constexpr int KC = D / 16, DT = D / 32, BYTES = Stage<D>::kBytes;
     extern __shared__ __attribute__((aligned(16))) unsigned char training_lds[];  // [K, V][2]; bias; bins of four wavefronts
     float *const bias = reinterpret_cast<float *>(training_lds + 4 * BYTES);
-    const int far = p.buckets.far, width = bins_width(far);
-    float *const all_bins = bias + 2 * far + 1;
+    const int far = p.buckets.far, width = distances_of(far);
+    float *const all_bins = bias + width;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
     float *const bins = all_bins + wave * width;
 
-    const Item item = decode(p.batch * p.heads, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
+    const Item item = decode(p.batch * p.kv_heads, p.group, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
     const int b = item.context / p.heads, h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
     const int length = length_of(p, b);
     const bool to_table = BIAS && p.partial != nullptr;
@@ -403,16 +416,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     const float by = p.scale * kLog2e, shift = -lse * kLog2e;
 
     // p of a 32-key block from its products
-    auto weights = [&](auto may_mask_tag, f32x16 &s, int key0) {
-        constexpr bool MAY_MASK = decltype(may_mask_tag)::value;
-        const int at = key0 - my_q + 4 * lh, last = (CAUSAL ? min(my_q, length - 1) : length - 1) - key0 - 4 * lh;
+    auto weights = [&](f32x16 &s, int key0) {
+        if (BIAS) {
+            const int d0 = key0 - wq0;
+            if (near(d0, far)) {
+                const float *const of = bias + d0 - li + 4 * lh + far + kMargin;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float x = fmaf(s[r], by, shift);
-            if (BIAS) x += bias[min(max(at + row_of(r), -far), far) + far];
-            x = __builtin_amdgcn_exp2f(x);
-            if (MAY_MASK && row_of(r) > last) x = 0.0f;
-            s[r] = x;
+                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of[row_of(r)]);
+            } else {
+                const float of = bias[d0 > 0 ? width - 1 : 0];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(BIAS ? s[r] + shift : fmaf(s[r], by, shift));
+        if (key0 + 32 > (CAUSAL ? min(length, wq0 + 1) : length)) {
+            const int last = (CAUSAL ? min(my_q, length - 1) : length - 1) - key0 - 4 * lh;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (row_of(r) > last) s[r] = 0.0f;
         }
     };
     auto products = [&](const unsigned char *ks, const unsigned char *vs, int t, f32x16 &s, f32x16 &dp) {
@@ -425,7 +448,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         }
     };
     const int key_end = CAUSAL ? min(length, q0 + kStay) : length, stages = (key_end + kStage - 1) / kStage;
-    const int seen = CAUSAL ? min(length, wq0 + 32) : length, plain = (CAUSAL ? min(length, wq0 + 1) : length) / kStage;
+    const int seen = CAUSAL ? min(length, wq0 + 32) : length;
     auto walk = [&](auto &&body) {
         moving.store(training_lds, training_lds + BYTES, tid);
         __syncthreads();
@@ -433,28 +456,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
             const bool more = t + 1 < stages;
             if (more) moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, (t + 1) * kStage, tid);
             const unsigned char *const ks = training_lds + (t & 1) * 2 * BYTES;
-            if (t < plain) body(std::false_type{}, ks, ks + BYTES, t * kStage);
-            else if (t * kStage < seen) body(std::true_type{}, ks, ks + BYTES, t * kStage);
+            if (t * kStage < seen) body(ks, ks + BYTES, t * kStage);
             if (more) moving.store(training_lds + ((t + 1) & 1) * 2 * BYTES, training_lds + ((t + 1) & 1) * 2 * BYTES + BYTES, tid);
             __syncthreads();
         }
     };
-    // do·o carries the roundings of o, a step of bf16 in all: little where ds is rounded to bf16 anyway, but the table's gradient is f32 and
-    // adds ds over whole diagonals.  There δ is Σ p·dp, at the price of both products again.
-    if (to_table) {
+    // do·o carries the roundings of o, which are to those of ds (rounded to bf16 as well) as one to the root of the keys.  The table's gradient
+    // though is f32 and adds ds over whole diagonals, and a sequence may have few keys: there δ is Σ p·dp, at the price of both products again
+    // (of one stage, where the sequence is short).
+    if (to_table || length <= kStage) {
         delta = 0.0f;
-        walk([&](auto may_mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
+        walk([&](const unsigned char *ks, const unsigned char *vs, int key0) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 f32x16 s, dp;
                 products(ks, vs, t, s, dp);
-                weights(may_mask_tag, s, key0 + t * 32);
+                weights(s, key0 + t * 32);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) delta = fmaf(s[r], dp[r], delta);
             }
         });
         delta += __shfl_xor(delta, 32);
-        moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, 0, tid);
+        if (stages > 1) moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, 0, tid);
     }
     if (lh == 0 && my_q < length) *delta_row = delta;
 
@@ -462,17 +485,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 #pragma unroll
     for (int t = 0; t < DT; ++t) dq[t] = f32x16{};
     float before = 0.0f, behind = 0.0f;  // ds of blocks beyond `far`
-    walk([&](auto may_mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
+    walk([&](const unsigned char *ks, const unsigned char *vs, int key0) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x16 s, dp;
             products(ks, vs, t, s, dp);
-            weights(may_mask_tag, s, key0 + t * 32);
+            weights(s, key0 + t * 32);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
             if (to_table) {
                 const int d0 = key0 + t * 32 - wq0;
-                if (d0 - 31 < far && d0 + 31 > -far) {
+                if (near(d0, far)) {
                     add_by_distance(s, d0, far, bins, lane);
                 } else {
                     float sum = 0.0f;
@@ -508,19 +531,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 __global__ __launch_bounds__(256) void position_bias_grad_kernel(const float *partial, float *grad_table, int batch, int heads, int tiles, Buckets buckets)
 {
     __shared__ float sums[4];
-    const int bucket = blockIdx.x / heads, h = blockIdx.x % heads, far = buckets.far, width = bins_width(far);
+    const int bucket = blockIdx.x / heads, h = blockIdx.x % heads, far = buckets.far, width = distances_of(far);
     const bool behind = buckets.bidirectional && bucket >= buckets.side;
     const int j = behind ? bucket - buckets.side : bucket;
     // the distances' sizes: from `low` to below `high`
-    int low = buckets.first[j], high = j + 1 < buckets.side ? buckets.first[j + 1] : far + kBinsMargin + 1;
+    int low = buckets.first[j], high = j + 1 < buckets.side ? buckets.first[j + 1] : far + kMargin + 1;
     if (behind) low = max(low, 1);  // 0 is on the other side
     int first = behind ? low : -(high - 1), last = behind ? high - 1 : -low;  // distances
-    if (!buckets.bidirectional && j == 0) last = far + kBinsMargin;  // all keys ahead
-    const long long run = max(last - first + 1, 0), all = run * batch * tiles;
+    if (!buckets.bidirectional && j == 0) last = far + kMargin;  // all keys ahead
+    // Threads side by side take neighbouring distances, as many as the bucket has (up to a wavefront), and the others further workgroups' sums.
+    const int run = max(last - first + 1, 0), parts = batch * tiles;
+    int wide = 1;
+    while (wide < 64 && wide < run) wide *= 2;
     float sum = 0.0f;
-    for (long long i = threadIdx.x; i < all; i += 256) {
-        const long long part = i / run, context = part / tiles * heads + h;
-        sum += partial[(context * tiles + part % tiles) * width + first + i % run + far + kBinsMargin];
+    const int distance = threadIdx.x % wide;
+#pragma unroll 4
+    for (int part = threadIdx.x / wide; part < parts; part += 256 / wide) {
+        const size_t context = static_cast<size_t>(part / tiles) * heads + h;
+        const float *const from = partial + (context * tiles + part % tiles) * width + first + far + kMargin;
+        for (int d = distance; d < run; d += wide) sum += from[d];
     }
     sum = wave_sum(sum);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
@@ -538,12 +567,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     const int far = p.buckets.far;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
 
-    const Item item = decode(p.batch * p.kv_heads, p.tiles, p.swizzle, CAUSAL, false, blockIdx.x);
-    const int b = item.context / p.kv_heads, kv_head = item.context % p.kv_heads, k0 = item.tile * kStay, wk0 = k0 + wave * 32, my_key = wk0 + li;
+    const Item item = decode(p.batch * p.kv_heads, 1, p.tiles * p.parts, p.swizzle, CAUSAL, false, blockIdx.x);
+    const int tile = item.tile / p.parts, part = item.tile % p.parts;
+    const int b = item.context / p.kv_heads, kv_head = item.context % p.kv_heads, k0 = tile * kStay, wk0 = k0 + wave * 32, my_key = wk0 + li;
     const int length = length_of(p, b);
     const size_t grad_at = (static_cast<size_t>(b) * p.S + my_key) * p.ld_grad_kv + static_cast<size_t>(kv_head) * D;
     if (k0 >= length) {
-        if (my_key < p.S) {
+        if (p.parts == 1 && my_key < p.S) {
             store_zeros<D>(p.grad_k + grad_at, lh);
             store_zeros<D>(p.grad_v + grad_at, lh);
         }
@@ -565,81 +595,118 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         dk[t] = f32x16{};
         dv[t] = f32x16{};
     }
-    const int first_stage = CAUSAL ? k0 / kStage : 0, stages = (length + kStage - 1) / kStage;
+    // The stages of all heads that share the keys, one after the other; a part takes its share of them.
+    const int first_stage = CAUSAL ? k0 / kStage : 0, of_head = (length + kStage - 1) / kStage - first_stage;
+    const long long all = static_cast<long long>(of_head) * p.group;
+    const int begin = static_cast<int>(all * part / p.parts), end = static_cast<int>(all * (part + 1) / p.parts);
     Moving<D> moving;
     float statistic = 0.0f;
-    for (int head = kv_head * p.group; head < (kv_head + 1) * p.group; ++head) {
+    auto load = [&](int i) {
+        const int head = kv_head * p.group + i / of_head, first = (first_stage + i % of_head) * kStage;
         const __amdgpu_buffer_rsrc_t q_rows =
             rows_of(p.q + static_cast<size_t>(b) * p.S * p.ld_q + static_cast<size_t>(head) * D, p.ld_q, length, D);
         const __amdgpu_buffer_rsrc_t g_rows =
             rows_of(p.grad_out + static_cast<size_t>(b) * p.S * p.ld_grad_out + static_cast<size_t>(head) * D, p.ld_grad_out, length, D);
         const size_t of_context = (static_cast<size_t>(b) * p.heads + head) * p.S;
-        auto load = [&](int stage) {
-            moving.load(q_rows, p.ld_q, g_rows, p.ld_grad_out, stage * kStage, tid);
-            const int row = stage * kStage + (tid & 63);
-            if (tid < 64) {
-                const float lse = row < length ? p.lse[of_context + row] : INFINITY;
-                statistic = lse == -INFINITY ? -INFINITY : -lse * kLog2e;  // rows without keys: every p is 0
-            } else if (tid < 128) {
-                statistic = row < length ? p.delta[of_context + row] : 0.0f;
+        moving.load(q_rows, p.ld_q, g_rows, p.ld_grad_out, first, tid);
+        const int row = first + (tid & 63);
+        if (tid < 64) {
+            const float lse = row < length ? p.lse[of_context + row] : INFINITY;
+            statistic = lse == -INFINITY ? -INFINITY : -lse * kLog2e;  // rows without keys: every p is 0
+        } else if (tid < 128) {
+            statistic = row < length ? p.delta[of_context + row] : 0.0f;
+        }
+    };
+    auto store = [&](int buffer) {
+        moving.store(training_lds + buffer * 2 * BYTES, training_lds + buffer * 2 * BYTES + BYTES, tid);
+        if (tid < 128) statistics[buffer * 2 * kStage + tid] = statistic;
+    };
+    auto compute = [&](int buffer, int row0) {
+        const unsigned char *const qs = training_lds + buffer * 2 * BYTES, *const gs = qs + BYTES;
+        const float *const of_rows = statistics + buffer * 2 * kStage + 4 * lh;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                s = mfma(reader.row_fragment(qs, t, c), kf[c], s);
+                dp = mfma(reader.row_fragment(gs, t, c), vf[c], dp);
             }
-        };
-        auto store = [&](int buffer) {
-            moving.store(training_lds + buffer * 2 * BYTES, training_lds + buffer * 2 * BYTES + BYTES, tid);
-            if (tid < 128) statistics[buffer * 2 * kStage + tid] = statistic;
-        };
-        auto compute = [&](auto may_mask_tag, int buffer, int row0) {
-            constexpr bool MAY_MASK = decltype(may_mask_tag)::value;
-            const unsigned char *const qs = training_lds + buffer * 2 * BYTES, *const gs = qs + BYTES;
-            const float *const of_rows = statistics + buffer * 2 * kStage + 4 * lh;
+            if (BIAS) {
+                const int d0 = wk0 - row0 - t * 32;
+                if (near(d0, far)) {
+                    const float *const of = bias + d0 + li - 4 * lh + far + kMargin - row_of(15);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x16 s = f32x16{}, dp = f32x16{};
+                    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of[row_of(15) - row_of(r)]);
+                } else {
+                    const float of = bias[d0 > 0 ? distances_of(far) - 1 : 0];
 #pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    s = mfma(reader.row_fragment(qs, t, c), kf[c], s);
-                    dp = mfma(reader.row_fragment(gs, t, c), vf[c], dp);
+                    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of);
                 }
+            }
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const f32x4 shift = *reinterpret_cast<const f32x4 *>(of_rows + t * 32 + a * 8);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = a * 4 + e;
+                    s[r] = __builtin_amdgcn_exp2f(BIAS ? s[r] + shift[e] : fmaf(s[r], by, shift[e]));
+                }
+            }
+            if (CAUSAL && row0 + t * 32 < wk0 + 31) {
                 const int at = my_key - row0 - t * 32 - 4 * lh;  // the key's distance from row 0
 #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const f32x4 shift = *reinterpret_cast<const f32x4 *>(of_rows + t * 32 + a * 8);
-                    const f32x4 delta = *reinterpret_cast<const f32x4 *>(of_rows + kStage + t * 32 + a * 8);
+                for (int r = 0; r < 16; ++r)
+                    if (at > row_of(r)) s[r] = 0.0f;
+            }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = a * 4 + e;
-                        float x = fmaf(s[r], by, shift[e]);
-                        if (BIAS) x += bias[min(max(at - row_of(r), -far), far) + far];
-                        x = __builtin_amdgcn_exp2f(x);
-                        if (MAY_MASK && CAUSAL && at > row_of(r)) x = 0.0f;
-                        s[r] = x;
-                        dp[r] = x * (dp[r] - delta[e]);
-                    }
-                }
+            for (int a = 0; a < 4; ++a) {
+                const f32x4 delta = *reinterpret_cast<const f32x4 *>(of_rows + kStage + t * 32 + a * 8);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const bf16x8 pf = packed(s, j), df = packed(dp, j);
+                for (int e = 0; e < 4; ++e) dp[a * 4 + e] = s[a * 4 + e] * (dp[a * 4 + e] - delta[e]);
+            }
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        dv[dt] = mfma(reader.column_fragment(gs, 2 * t + j, dt), pf, dv[dt]);
-                        dk[dt] = mfma(reader.column_fragment(qs, 2 * t + j, dt), df, dk[dt]);
-                    }
+            for (int j = 0; j < 2; ++j) {
+                const bf16x8 pf = packed(s, j), df = packed(dp, j);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    dv[dt] = mfma(reader.column_fragment(gs, 2 * t + j, dt), pf, dv[dt]);
+                    dk[dt] = mfma(reader.column_fragment(qs, 2 * t + j, dt), df, dk[dt]);
                 }
             }
-        };
-        load(first_stage);
-        if (BIAS) fill_bias(p, head, bias, tid);
-        store(first_stage & 1);
-        __syncthreads();
-        for (int t = first_stage; t < stages; ++t) {
-            const bool more = t + 1 < stages;
-            if (more) load(t + 1);
-            const int row0 = t * kStage;
-            if (!CAUSAL || row0 >= wk0 + 31) compute(std::false_type{}, t & 1, row0);
-            else if (row0 + kStage > wk0) compute(std::true_type{}, t & 1, row0);
-            if (more) store((t + 1) & 1);
-            __syncthreads();
         }
+    };
+    if (begin < end) {
+        load(begin);
+        if (BIAS) fill_bias(p, kv_head * p.group + begin / of_head, bias, tid);
+        store(begin & 1);
+    }
+    __syncthreads();
+    for (int i = begin; i < end; ++i) {
+        const bool more = i + 1 < end;
+        if (more) load(i + 1);
+        const int row0 = (first_stage + i % of_head) * kStage;
+        if (!CAUSAL || row0 + kStage > wk0) compute(i & 1, row0);
+        if (BIAS && more && (i + 1) % of_head == 0) {  // another head: its biases, when this one's have been read
+            __syncthreads();
+            fill_bias(p, kv_head * p.group + (i + 1) / of_head, bias, tid);
+        }
+        if (more) store((i + 1) & 1);
+        __syncthreads();
+    }
+    if (p.parts > 1) {
+        if (my_key >= length) return;
+        const size_t rows = static_cast<size_t>(p.batch) * p.S, width = static_cast<size_t>(p.kv_heads) * D;
+        float *const to = p.part_sums + ((static_cast<size_t>(part) * 2 * rows + static_cast<size_t>(b) * p.S + my_key) * width + static_cast<size_t>(kv_head) * D);
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = t * 32 + g * 8 + lh * 4;
+                *reinterpret_cast<f32x4 *>(to + d) = f32x4{dk[t][g * 4], dk[t][g * 4 + 1], dk[t][g * 4 + 2], dk[t][g * 4 + 3]};
+                *reinterpret_cast<f32x4 *>(to + rows * width + d) = f32x4{dv[t][g * 4], dv[t][g * 4 + 1], dv[t][g * 4 + 2], dv[t][g * 4 + 3]};
+            }
+        return;
     }
     if (my_key < length) {
         store_row<D>(p.grad_k + grad_at, dk, p.scale, lh);
@@ -650,30 +717,61 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     }
 }
 
+// The parts of dk and dv together, four values a thread.
+__global__ __launch_bounds__(256) void attention_grad_kv_parts_kernel(TrainingArgs p, int width)
+{
+    const size_t rows = static_cast<size_t>(p.batch) * p.S, units = rows * (width / 4);
+    const bool of_v = blockIdx.y == 1;
+    uint16_t *const to = of_v ? p.grad_v : p.grad_k;
+    const float by = of_v ? 1.0f : p.scale;
+    for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < units; i += static_cast<size_t>(gridDim.x) * 256) {
+        const size_t row = i / (width / 4), column = i % (width / 4) * 4;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (static_cast<int>(row % p.S) < length_of(p, static_cast<int>(row / p.S))) {
+            const float *from = p.part_sums + (of_v ? rows * width : 0) + row * width + column;
+            for (int part = 0; part < p.parts; ++part, from += 2 * rows * width) sum += *reinterpret_cast<const f32x4 *>(from);
+        }
+        const u32x2_t words = {pack_bf16x2_rne(sum[0] * by, sum[1] * by), pack_bf16x2_rne(sum[2] * by, sum[3] * by)};
+        *reinterpret_cast<u32x2_t *>(to + row * p.ld_grad_kv + column) = words;
+    }
+}
+
 // ---- launches -----------------------------------------------------------------------------------------------------------------------
 // The check before a launch: the grid is what the decode assumes, and its first and last workgroups lie inside.
-bool grid_consistent(int contexts, int tiles, int swizzle, bool by_tile, bool last_first, size_t blocks, int S)
+bool grid_consistent(int groups, int group, int tiles, int parts, int swizzle, bool by_tile, bool last_first, size_t blocks, int S)
 {
-    if (contexts <= 0 || tiles <= 0 || blocks > kMaxDim || blocks != static_cast<size_t>(contexts) * tiles) return false;
-    if (static_cast<long long>(tiles) * kStay < S || static_cast<long long>(tiles - 1) * kStay >= S || (swizzle && contexts % 8 != 0)) return false;
+    const size_t contexts = static_cast<size_t>(groups) * group, of_context = static_cast<size_t>(tiles) * parts;
+    if (contexts == 0 || tiles <= 0 || blocks > kMaxDim || blocks != contexts * of_context) return false;
+    if (static_cast<long long>(tiles) * kStay < S || static_cast<long long>(tiles - 1) * kStay >= S || (swizzle && groups % 8 != 0)) return false;
     for (const size_t block : {static_cast<size_t>(0), blocks - 1}) {
-        const Item item = decode(contexts, tiles, swizzle, by_tile, last_first, static_cast<unsigned>(block));
-        if (item.context < 0 || item.context >= contexts || item.tile < 0 || item.tile >= tiles) return false;
+        const Item item = decode(groups, group, tiles * parts, swizzle, by_tile, last_first, static_cast<unsigned>(block));
+        if (item.context < 0 || static_cast<size_t>(item.context) >= contexts || item.tile < 0 || item.tile >= tiles * parts) return false;
     }
     return true;
 }
 
+// `group`: of the contexts that share keys, 1 where they are one.
 template <class Kernel>
-hipError_t launch(Kernel kernel, TrainingArgs &args, int contexts, bool by_tile, bool last_first, size_t lds_bytes, hipStream_t stream)
+hipError_t launch(Kernel kernel, TrainingArgs &args, int group, int parts, bool by_tile, bool last_first, size_t lds_bytes, hipStream_t stream)
 {
+    const int groups = args.batch * args.kv_heads;
     args.tiles = (args.S + kStay - 1) / kStay;
-    args.swizzle = contexts % 8 == 0;
-    const size_t blocks = static_cast<size_t>(contexts) * args.tiles;
-    if (!grid_consistent(contexts, args.tiles, args.swizzle, by_tile, last_first, blocks, args.S)) return hipErrorInvalidConfiguration;
+    args.swizzle = groups % 8 == 0;
+    const size_t blocks = static_cast<size_t>(groups) * group * args.tiles * parts;
+    if (!grid_consistent(groups, group, args.tiles, parts, args.swizzle, by_tile, last_first, blocks, args.S)) return hipErrorInvalidConfiguration;
     const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds_bytes));
     if (rc != hipSuccess) return rc;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), lds_bytes, stream, args);
     return hipGetLastError();
+}
+
+// Workgroups to a tile of keys: two rounds of the chip where one workgroup a tile would not be one, none with less than eight stages.
+int parts_of_keys(size_t groups, size_t group, size_t sequence, size_t head_dim)
+{
+    const size_t tiles = groups * ((sequence + kStay - 1) / kStay), round = head_dim == 64 ? 512 : 256;
+    if (tiles >= round) return 1;
+    const size_t stages = (sequence + kStage - 1) / kStage * group;
+    return static_cast<int>(std::max<size_t>(1, std::min({2 * round / tiles, stages / 8, static_cast<size_t>(16)})));
 }
 
 // Runs `body(d, causal, biased)` with the three as compile-time constants.
@@ -737,8 +835,8 @@ hipError_t launch_attention_training_bf16(const st_hip_attention_training &shape
     return with_variant(shape.head_dim, shape.causal != 0, biased, [&](auto d, auto causal, auto bias) {
         constexpr int D = decltype(d)::value;
         constexpr bool CAUSAL = decltype(causal)::value, BIAS = decltype(bias)::value;
-        const size_t lds = 4 * Stage<D>::kBytes + (BIAS ? (2 * args.buckets.far + 1) * sizeof(float) : 0);
-        return launch(attention_training_kernel<D, CAUSAL, BIAS>, args, args.batch * args.heads, CAUSAL, CAUSAL, lds, stream);
+        const size_t lds = 4 * Stage<D>::kBytes + (BIAS ? distances_of(args.buckets.far) * sizeof(float) : 0);
+        return launch(attention_training_kernel<D, CAUSAL, BIAS>, args, args.group, 1, CAUSAL, CAUSAL, lds, stream);
     });
 }
 
@@ -765,22 +863,32 @@ hipError_t launch_attention_backward_bf16(const st_hip_attention_training &shape
     const size_t contexts = shape.batch * shape.heads, tiles = (shape.sequence + kStay - 1) / kStay;
     if (contexts * tiles == 0) return add_up(nullptr, 0);
     const size_t deltas = (contexts * shape.sequence + 63) / 64 * 64;
-    const size_t sums = grad_table ? contexts * tiles * bins_width(args.buckets.far) : 0;
+    const size_t sums = grad_table ? contexts * tiles * distances_of(args.buckets.far) : 0;
+    const size_t kv_width = shape.kv_heads * shape.head_dim, sums_padded = (sums + 63) / 64 * 64;
+    args.parts = parts_of_keys(shape.batch * shape.kv_heads, args.group, shape.sequence, shape.head_dim);
+    const size_t part_sums = args.parts > 1 ? args.parts * 2 * shape.batch * shape.sequence * kv_width : 0;
     void *scratch = nullptr;
-    hipError_t rc = stream_workspace(stream, (deltas + sums) * sizeof(float), &scratch);
+    hipError_t rc = stream_workspace(stream, (deltas + sums_padded + part_sums) * sizeof(float), &scratch);
     if (rc != hipSuccess) return rc;
     args.delta = static_cast<float *>(scratch);
     args.partial = grad_table ? args.delta + deltas : nullptr;
+    args.part_sums = args.delta + deltas + sums_padded;
     rc = with_variant(shape.head_dim, shape.causal != 0, biased, [&](auto d, auto causal, auto bias) {
         constexpr int D = decltype(d)::value;
         constexpr bool CAUSAL = decltype(causal)::value, BIAS = decltype(bias)::value;
-        const size_t distances = BIAS ? 2 * args.buckets.far + 1 : 0;
-        const size_t lds_q = 4 * Stage<D>::kBytes + (distances + (grad_table ? 4 * bins_width(args.buckets.far) : 0)) * sizeof(float);
-        const hipError_t first = launch(attention_grad_q_kernel<D, CAUSAL, BIAS>, args, args.batch * args.heads, CAUSAL, CAUSAL, lds_q, stream);
+        const size_t distances = BIAS ? distances_of(args.buckets.far) : 0;
+        const size_t lds_q = 4 * Stage<D>::kBytes + (grad_table ? 5 : 1) * distances * sizeof(float);
+        const hipError_t first = launch(attention_grad_q_kernel<D, CAUSAL, BIAS>, args, args.group, 1, CAUSAL, CAUSAL, lds_q, stream);
         if (first != hipSuccess) return first;
         const size_t lds_kv = 4 * Stage<D>::kBytes + (4 * kStage + distances) * sizeof(float);
-        return launch(attention_grad_kv_kernel<D, CAUSAL, BIAS>, args, args.batch * args.kv_heads, CAUSAL, false, lds_kv, stream);
+        return launch(attention_grad_kv_kernel<D, CAUSAL, BIAS>, args, 1, args.parts, CAUSAL, false, lds_kv, stream);
     });
+    if (rc == hipSuccess && args.parts > 1) {
+        const size_t units = shape.batch * shape.sequence * kv_width / 4;
+        hipLaunchKernelGGL(attention_grad_kv_parts_kernel, dim3(static_cast<unsigned>(std::min<size_t>((units + 255) / 256, 4096)), 2), dim3(256), 0, stream, args,
+                           static_cast<int>(kv_width));
+        rc = hipGetLastError();
+    }
     if (rc != hipSuccess || !grad_table) return rc;
     return add_up(args.partial, tiles);
 }
