@@ -170,8 +170,10 @@ __device__ constexpr int row_of(int r) { return (r >> 2) * 8 + (r & 3); }
 constexpr int kMargin = 64;
 __host__ __device__ inline int distances_of(int far) { return 2 * far + 2 * kMargin + 1; }
 
-// Where distances lie among those that a block's registers are given: bias[from + row_of(r)], or the one bias of a block beyond `far`.
+// Whether some distance of a 32x32 block, d0 - 31 .. d0 + 31, is not beyond `far`.
 __device__ __forceinline__ bool near(int d0, int far) { return d0 - 31 < far && d0 + 31 > -far; }
+// Where a block's distances begin among those held: those of a block beyond `far` are all the same, as they are 32 behind it.
+__device__ __forceinline__ int window(int d0, int far) { return min(max(d0, -far - 32), far + 32) + far + kMargin; }
 
 // What a key `distance` behind its query (negative: before it) is given: bias[distance + far + 64], in units of log2 e.
 __device__ __forceinline__ void fill_bias(const TrainingArgs &p, int head, float *bias, int tid)
@@ -252,31 +254,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
     for (int t = 0; t < DT; ++t) oacc[t] = f32x16{};
     float run_max = -INFINITY, run_sum = 0.0f;
 
-    // (One body for stages with masked keys and without: with two, the accumulators are copied where the two meet, behind their last product.)
-    auto compute = [&](const unsigned char *ks, const unsigned char *vs, int key0) {
+    auto compute = [&](auto mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
         f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
             for (int t = 0; t < 2; ++t) s[t] = mfma(reader.row_fragment(ks, t, c), qf[c], s[t]);
         if (BIAS) {
-            const int far = p.buckets.far;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int d0 = key0 + t * 32 - wq0;
-                if (near(d0, far)) {
-                    const float *const of = bias + d0 - li + 4 * lh + far + kMargin;
+                const float *const of = bias + window(key0 + t * 32 - wq0, p.buckets.far) - li + 4 * lh;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], by, of[row_of(r)]);
-                } else {
-                    const float of = bias[d0 > 0 ? distances_of(far) - 1 : 0];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], by, of);
-                }
+                for (int r = 0; r < 16; ++r) s[t][r] = fmaf(s[t][r], by, of[row_of(r)]);
             }
         }
         float most = -INFINITY;
-        if (key0 + kStage > (CAUSAL ? min(length, wq0 + 1) : length)) {
+        if (decltype(mask_tag)::value) {
             const int last = (CAUSAL ? min(my_q, length - 1) : length - 1) - key0 - 4 * lh;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -318,17 +311,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
     };
 
     const int key_end = CAUSAL ? min(length, q0 + kStay) : length, stages = (key_end + kStage - 1) / kStage;
-    const int seen = CAUSAL ? min(length, wq0 + 32) : length;
+    const int seen = CAUSAL ? min(length, wq0 + 32) : length, plain = (CAUSAL ? min(length, q0) : length) / kStage;
     moving.store(training_lds, training_lds + BYTES, tid);
     __syncthreads();
-    for (int t = 0; t < stages; ++t) {
+    auto step = [&](auto mask_tag, int t) {
         const bool more = t + 1 < stages;
         if (more) moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, (t + 1) * kStage, tid);
         const unsigned char *const ks = training_lds + (t & 1) * 2 * BYTES;
-        if (t * kStage < seen) compute(ks, ks + BYTES, t * kStage);
+        if (!decltype(mask_tag)::value || t * kStage < seen) compute(mask_tag, ks, ks + BYTES, t * kStage);
         if (more) moving.store(training_lds + ((t + 1) & 1) * 2 * BYTES, training_lds + ((t + 1) & 1) * 2 * BYTES + BYTES, tid);
         __syncthreads();
-    }
+    };
+    // Stages without masked keys in a loop of their own: where a body branches, the accumulators are copied behind its last product, and the
+    // compiler makes masks of all scores in either case.
+    int t = 0;
+    for (; t < plain; ++t) step(std::false_type{}, t);
+    for (; t < stages; ++t) step(std::true_type{}, t);
     const float total = run_sum + __shfl_xor(run_sum, 32);
     if (my_q >= p.S) return;
     const bool live = my_q < length && total > 0.0f;
@@ -416,22 +414,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     const float by = p.scale * kLog2e, shift = -lse * kLog2e;
 
     // p of a 32-key block from its products
-    auto weights = [&](f32x16 &s, int key0) {
+    auto weights = [&](auto mask_tag, f32x16 &s, int key0) {
         if (BIAS) {
-            const int d0 = key0 - wq0;
-            if (near(d0, far)) {
-                const float *const of = bias + d0 - li + 4 * lh + far + kMargin;
+            const float *const of = bias + window(key0 - wq0, far) - li + 4 * lh;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of[row_of(r)]);
-            } else {
-                const float of = bias[d0 > 0 ? width - 1 : 0];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of);
-            }
+            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of[row_of(r)]);
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(BIAS ? s[r] + shift : fmaf(s[r], by, shift));
-        if (key0 + 32 > (CAUSAL ? min(length, wq0 + 1) : length)) {
+        if (decltype(mask_tag)::value) {
             const int last = (CAUSAL ? min(my_q, length - 1) : length - 1) - key0 - 4 * lh;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -448,30 +439,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         }
     };
     const int key_end = CAUSAL ? min(length, q0 + kStay) : length, stages = (key_end + kStage - 1) / kStage;
-    const int seen = CAUSAL ? min(length, wq0 + 32) : length;
+    const int seen = CAUSAL ? min(length, wq0 + 32) : length, plain = (CAUSAL ? min(length, q0) : length) / kStage;
     auto walk = [&](auto &&body) {
         moving.store(training_lds, training_lds + BYTES, tid);
         __syncthreads();
-        for (int t = 0; t < stages; ++t) {
+        auto step = [&](auto mask_tag, int t) {
             const bool more = t + 1 < stages;
             if (more) moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, (t + 1) * kStage, tid);
             const unsigned char *const ks = training_lds + (t & 1) * 2 * BYTES;
-            if (t * kStage < seen) body(ks, ks + BYTES, t * kStage);
+            if (!decltype(mask_tag)::value || t * kStage < seen) body(mask_tag, ks, ks + BYTES, t * kStage);
             if (more) moving.store(training_lds + ((t + 1) & 1) * 2 * BYTES, training_lds + ((t + 1) & 1) * 2 * BYTES + BYTES, tid);
             __syncthreads();
-        }
+        };
+        int t = 0;  // (as in the forward pass)
+        for (; t < plain; ++t) step(std::false_type{}, t);
+        for (; t < stages; ++t) step(std::true_type{}, t);
     };
     // do·o carries the roundings of o, which are to those of ds (rounded to bf16 as well) as one to the root of the keys.  The table's gradient
     // though is f32 and adds ds over whole diagonals, and a sequence may have few keys: there δ is Σ p·dp, at the price of both products again
     // (of one stage, where the sequence is short).
     if (to_table || length <= kStage) {
         delta = 0.0f;
-        walk([&](const unsigned char *ks, const unsigned char *vs, int key0) {
+        walk([&](auto mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 f32x16 s, dp;
                 products(ks, vs, t, s, dp);
-                weights(s, key0 + t * 32);
+                weights(mask_tag, s, key0 + t * 32);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) delta = fmaf(s[r], dp[r], delta);
             }
@@ -485,12 +479,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 #pragma unroll
     for (int t = 0; t < DT; ++t) dq[t] = f32x16{};
     float before = 0.0f, behind = 0.0f;  // ds of blocks beyond `far`
-    walk([&](const unsigned char *ks, const unsigned char *vs, int key0) {
+    walk([&](auto mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x16 s, dp;
             products(ks, vs, t, s, dp);
-            weights(s, key0 + t * 32);
+            weights(mask_tag, s, key0 + t * 32);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
             if (to_table) {
@@ -539,16 +533,16 @@ __global__ __launch_bounds__(256) void position_bias_grad_kernel(const float *pa
     if (behind) low = max(low, 1);  // 0 is on the other side
     int first = behind ? low : -(high - 1), last = behind ? high - 1 : -low;  // distances
     if (!buckets.bidirectional && j == 0) last = far + kMargin;  // all keys ahead
-    // Threads side by side take neighbouring distances, as many as the bucket has (up to a wavefront), and the others further workgroups' sums.
+    // Threads side by side take neighbouring distances, up to sixteen, and the others further workgroups' sums.
     const int run = max(last - first + 1, 0), parts = batch * tiles;
     int wide = 1;
-    while (wide < 64 && wide < run) wide *= 2;
+    while (wide < 16 && wide < run) wide *= 2;
     float sum = 0.0f;
     const int distance = threadIdx.x % wide;
-#pragma unroll 4
     for (int part = threadIdx.x / wide; part < parts; part += 256 / wide) {
         const size_t context = static_cast<size_t>(part / tiles) * heads + h;
         const float *const from = partial + (context * tiles + part % tiles) * width + first + far + kMargin;
+#pragma unroll 8
         for (int d = distance; d < run; d += wide) sum += from[d];
     }
     sum = wave_sum(sum);
@@ -601,8 +595,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     const int begin = static_cast<int>(all * part / p.parts), end = static_cast<int>(all * (part + 1) / p.parts);
     Moving<D> moving;
     float statistic = 0.0f;
-    auto load = [&](int i) {
-        const int head = kv_head * p.group + i / of_head, first = (first_stage + i % of_head) * kStage;
+    auto load = [&](int head, int stage) {
+        const int first = stage * kStage;
         const __amdgpu_buffer_rsrc_t q_rows =
             rows_of(p.q + static_cast<size_t>(b) * p.S * p.ld_q + static_cast<size_t>(head) * D, p.ld_q, length, D);
         const __amdgpu_buffer_rsrc_t g_rows =
@@ -621,7 +615,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         moving.store(training_lds + buffer * 2 * BYTES, training_lds + buffer * 2 * BYTES + BYTES, tid);
         if (tid < 128) statistics[buffer * 2 * kStage + tid] = statistic;
     };
-    auto compute = [&](int buffer, int row0) {
+    auto compute = [&](auto mask_tag, int buffer, int row0) {
         const unsigned char *const qs = training_lds + buffer * 2 * BYTES, *const gs = qs + BYTES;
         const float *const of_rows = statistics + buffer * 2 * kStage + 4 * lh;
 #pragma unroll
@@ -633,16 +627,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
                 dp = mfma(reader.row_fragment(gs, t, c), vf[c], dp);
             }
             if (BIAS) {
-                const int d0 = wk0 - row0 - t * 32;
-                if (near(d0, far)) {
-                    const float *const of = bias + d0 + li - 4 * lh + far + kMargin - row_of(15);
+                const float *const of = bias + window(wk0 - row0 - t * 32, far) + li - 4 * lh - row_of(15);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of[row_of(15) - row_of(r)]);
-                } else {
-                    const float of = bias[d0 > 0 ? distances_of(far) - 1 : 0];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of);
-                }
+                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of[row_of(15) - row_of(r)]);
             }
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
@@ -653,7 +640,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
                     s[r] = __builtin_amdgcn_exp2f(BIAS ? s[r] + shift[e] : fmaf(s[r], by, shift[e]));
                 }
             }
-            if (CAUSAL && row0 + t * 32 < wk0 + 31) {
+            if (decltype(mask_tag)::value) {
                 const int at = my_key - row0 - t * 32 - 4 * lh;  // the key's distance from row 0
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -676,23 +663,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
             }
         }
     };
+    const int last_stage = first_stage + of_head;
+    int head = 0, stage = first_stage;
     if (begin < end) {
-        load(begin);
-        if (BIAS) fill_bias(p, kv_head * p.group + begin / of_head, bias, tid);
-        store(begin & 1);
+        head = begin / of_head;
+        stage = first_stage + begin % of_head;
+        head += kv_head * p.group;
+        load(head, stage);
+        if (BIAS) fill_bias(p, head, bias, tid);
+        store(stage & 1);
     }
     __syncthreads();
-    for (int i = begin; i < end; ++i) {
-        const bool more = i + 1 < end;
-        if (more) load(i + 1);
-        const int row0 = (first_stage + i % of_head) * kStage;
-        if (!CAUSAL || row0 + kStage > wk0) compute(i & 1, row0);
-        if (BIAS && more && (i + 1) % of_head == 0) {  // another head: its biases, when this one's have been read
+    int buffer = stage & 1;
+    for (int left = end - begin; left > 0;) {
+        auto step = [&](auto mask_tag) {
+            const int row0 = stage * kStage;
+            const bool more = --left > 0, next_head = ++stage == last_stage;
+            if (next_head) {
+                ++head;
+                stage = first_stage;
+            }
+            if (more) load(head, stage);
+            if (!decltype(mask_tag)::value || row0 + kStage > wk0) compute(mask_tag, buffer, row0);
+            if (BIAS && more && next_head) {  // another head's biases, when this one's have been read
+                __syncthreads();
+                fill_bias(p, head, bias, tid);
+            }
+            buffer ^= 1;
+            if (more) store(buffer);
             __syncthreads();
-            fill_bias(p, kv_head * p.group + (i + 1) / of_head, bias, tid);
-        }
-        if (more) store((i + 1) & 1);
-        __syncthreads();
+            return more && !next_head;
+        };
+        // the stages that hold a key's own place or queries before it, then the others of the head, as in the forward pass
+        bool same = true;
+        while (CAUSAL && same && stage * kStage < k0 + kStay) same = step(std::true_type{});
+        while (same) same = step(std::false_type{});
     }
     if (p.parts > 1) {
         if (my_key >= length) return;
