@@ -413,29 +413,53 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     if (lse == -INFINITY) lse = INFINITY;  // a row without keys: every p is 0
     const float by = p.scale * kLog2e, shift = -lse * kLog2e;
 
-    // p of a 32-key block from its products
-    auto weights = [&](auto mask_tag, f32x16 &s, int key0) {
-        if (BIAS) {
-            const float *const of = bias + window(key0 - wq0, far) - li + 4 * lh;
+    // A stage is two blocks of 32 keys.  Its products are dealt out in steps of one chunk, with what is read from LDS `AHEAD` steps early and
+    // the other block's softmax spread over the steps: there are one or two wavefronts to a SIMD, and nothing else hides the reads' way
+    // or the exponentials.
+    constexpr int AHEAD = D == 64 ? 2 : 4, STEPS = D / 16, EACH = 16 / STEPS;
+    struct Block {
+        f32x16 s, dp;
+        float bias[BIAS ? 16 : 1];
+    };
+    // scores and dp of both blocks; `behind(t, step)` goes on with the first block while the second one's products run
+    auto products = [&](const unsigned char *ks, const unsigned char *vs, int key0, Block (&blocks)[2], auto &&ahead, auto &&behind) {
+        bf16x8 ring_k[AHEAD], ring_v[AHEAD];
+        auto load = [&](int i) {
+            ring_k[i % AHEAD] = reader.row_fragment(ks, i / KC, i % KC);
+            ring_v[i % AHEAD] = reader.row_fragment(vs, i / KC, i % KC);
+        };
+        auto load_bias = [&](int t) {
+            if (!BIAS) return;
+            const float *const of = bias + window(key0 + t * 32 - wq0, far) - li + 4 * lh;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of[row_of(r)]);
-        }
+            for (int r = 0; r < 16; ++r) blocks[t].bias[BIAS ? r : 0] = of[row_of(r)];
+        };
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(BIAS ? s[r] + shift : fmaf(s[r], by, shift));
-        if (decltype(mask_tag)::value) {
-            const int last = (CAUSAL ? min(my_q, length - 1) : length - 1) - key0 - 4 * lh;
+        for (int i = 0; i < AHEAD; ++i) load(i);
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (row_of(r) > last) s[r] = 0.0f;
+        for (int i = 0; i < 2 * KC; ++i) {
+            Block &x = blocks[i / KC];
+            if (i % KC == 0) {
+                x.s = f32x16{};
+                x.dp = f32x16{};
+                load_bias(i / KC);
+            }
+            x.s = mfma(ring_k[i % AHEAD], qf[i % KC], x.s);
+            x.dp = mfma(ring_v[i % AHEAD], gf[i % KC], x.dp);
+            if (i + AHEAD < 2 * KC) load(i + AHEAD);
+            else ahead(i + AHEAD - 2 * KC);
+            if (i >= KC) behind(0, i - KC);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto products = [&](const unsigned char *ks, const unsigned char *vs, int t, f32x16 &s, f32x16 &dp) {
-        s = f32x16{};
-        dp = f32x16{};
+    // p of EACH registers of a block
+    auto weights = [&](auto mask_tag, Block &x, int key0, int step) {
+        const int last = (CAUSAL ? min(my_q, length - 1) : length - 1) - key0 - 4 * lh;
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            s = mfma(reader.row_fragment(ks, t, c), qf[c], s);
-            dp = mfma(reader.row_fragment(vs, t, c), gf[c], dp);
+        for (int r = step * EACH; r < (step + 1) * EACH; ++r) {
+            const float score = BIAS ? fmaf(x.s[r], by, x.bias[BIAS ? r : 0]) + shift : fmaf(x.s[r], by, shift);
+            const float weight = __builtin_amdgcn_exp2f(score);
+            x.s[r] = decltype(mask_tag)::value && row_of(r) > last ? 0.0f : weight;
         }
     };
     const int key_end = CAUSAL ? min(length, q0 + kStay) : length, stages = (key_end + kStage - 1) / kStage;
@@ -461,14 +485,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     if (to_table || length <= kStage) {
         delta = 0.0f;
         walk([&](auto mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
+            Block blocks[2];
+            auto add = [&](int t, int step) {
+                weights(mask_tag, blocks[t], key0 + t * 32, step);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x16 s, dp;
-                products(ks, vs, t, s, dp);
-                weights(mask_tag, s, key0 + t * 32);
+                for (int r = step * EACH; r < (step + 1) * EACH; ++r) delta = fmaf(blocks[t].s[r], blocks[t].dp[r], delta);
+            };
+            products(ks, vs, key0, blocks, [](int) {}, add);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) delta = fmaf(s[r], dp[r], delta);
-            }
+            for (int step = 0; step < STEPS; ++step) add(1, step);
         });
         delta += __shfl_xor(delta, 32);
         if (stages > 1) moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, 0, tid);
@@ -480,30 +505,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     for (int t = 0; t < DT; ++t) dq[t] = f32x16{};
     float before = 0.0f, behind = 0.0f;  // ds of blocks beyond `far`
     walk([&](auto mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
+        Block blocks[2];
+        bf16x8 ring[AHEAD], df[2][2];
+        auto load = [&](int m) { ring[m % AHEAD] = reader.column_fragment(ks, m / DT, m % DT); };
+        auto grads = [&](int t, int step) {
+            Block &x = blocks[t];
+            weights(mask_tag, x, key0 + t * 32, step);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x16 s, dp;
-            products(ks, vs, t, s, dp);
-            weights(mask_tag, s, key0 + t * 32);
+            for (int r = step * EACH; r < (step + 1) * EACH; ++r) x.s[r] *= x.dp[r] - delta;
+            if ((step + 1) * EACH % 8 == 0) df[t][(step + 1) * EACH / 8 - 1] = packed(x.s, (step + 1) * EACH / 8 - 1);
+        };
+        products(ks, vs, key0, blocks, load, grads);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
-            if (to_table) {
+        for (int m = 0; m < 4 * DT; ++m) {
+            dq[m % DT] = mfma(ring[m % AHEAD], df[m / (2 * DT)][m / DT % 2], dq[m % DT]);
+            if (m + AHEAD < 4 * DT) load(m + AHEAD);
+            if (m < 2 * DT) grads(1, m);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (to_table) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
                 const int d0 = key0 + t * 32 - wq0;
                 if (near(d0, far)) {
-                    add_by_distance(s, d0, far, bins, lane);
+                    add_by_distance(blocks[t].s, d0, far, bins, lane);
                 } else {
                     float sum = 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) sum += s[r];
+                    for (int r = 0; r < 16; ++r) sum += blocks[t].s[r];
                     if (d0 > 0) behind += sum;
                     else before += sum;
                 }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const bf16x8 df = packed(s, j);
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) dq[dt] = mfma(reader.column_fragment(ks, 2 * t + j, dt), df, dq[dt]);
             }
         }
     });
@@ -615,52 +647,76 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         moving.store(training_lds + buffer * 2 * BYTES, training_lds + buffer * 2 * BYTES + BYTES, tid);
         if (tid < 128) statistics[buffer * 2 * kStage + tid] = statistic;
     };
+    // (In steps, as in the dq kernel.)
+    constexpr int AHEAD = D == 64 ? 2 : 4, STEPS = D / 16, EACH = 16 / STEPS;
     auto compute = [&](auto mask_tag, int buffer, int row0) {
         const unsigned char *const qs = training_lds + buffer * 2 * BYTES, *const gs = qs + BYTES;
         const float *const of_rows = statistics + buffer * 2 * kStage + 4 * lh;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x16 s = f32x16{}, dp = f32x16{};
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                s = mfma(reader.row_fragment(qs, t, c), kf[c], s);
-                dp = mfma(reader.row_fragment(gs, t, c), vf[c], dp);
-            }
-            if (BIAS) {
-                const float *const of = bias + window(wk0 - row0 - t * 32, far) + li - 4 * lh - row_of(15);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], by, of[row_of(15) - row_of(r)]);
-            }
-#pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                const f32x4 shift = *reinterpret_cast<const f32x4 *>(of_rows + t * 32 + a * 8);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = a * 4 + e;
-                    s[r] = __builtin_amdgcn_exp2f(BIAS ? s[r] + shift[e] : fmaf(s[r], by, shift[e]));
-                }
-            }
-            if (decltype(mask_tag)::value) {
-                const int at = my_key - row0 - t * 32 - 4 * lh;  // the key's distance from row 0
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (at > row_of(r)) s[r] = 0.0f;
-            }
+        f32x16 s[2], dp[2];
+        f32x4 shift[4], delta[4];  // of the rows of the block whose softmax is next
+        float of_bias[BIAS ? 16 : 1];
+        bf16x8 ring_q[AHEAD], ring_g[AHEAD], pf[2][2], df[2][2];
+        auto load_rows = [&](int i) {
+            ring_q[i % AHEAD] = reader.row_fragment(qs, i / KC, i % KC);
+            ring_g[i % AHEAD] = reader.row_fragment(gs, i / KC, i % KC);
+        };
+        auto load_columns = [&](int m) {
+            ring_q[m % AHEAD] = reader.column_fragment(qs, m / DT, m % DT);
+            ring_g[m % AHEAD] = reader.column_fragment(gs, m / DT, m % DT);
+        };
+        auto load_statistics = [&](int t) {
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
-                const f32x4 delta = *reinterpret_cast<const f32x4 *>(of_rows + kStage + t * 32 + a * 8);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) dp[a * 4 + e] = s[a * 4 + e] * (dp[a * 4 + e] - delta[e]);
+                shift[a] = *reinterpret_cast<const f32x4 *>(of_rows + t * 32 + a * 8);
+                delta[a] = *reinterpret_cast<const f32x4 *>(of_rows + kStage + t * 32 + a * 8);
             }
+            if (!BIAS) return;
+            const float *const of = bias + window(wk0 - row0 - t * 32, far) + li - 4 * lh - row_of(15);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const bf16x8 pf = packed(s, j), df = packed(dp, j);
+            for (int r = 0; r < 16; ++r) of_bias[BIAS ? r : 0] = of[row_of(15) - row_of(r)];
+        };
+        auto grads = [&](int t, int step) {
+            const int at = my_key - row0 - t * 32 - 4 * lh;  // the key's distance from the block's first row
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    dv[dt] = mfma(reader.column_fragment(gs, 2 * t + j, dt), pf, dv[dt]);
-                    dk[dt] = mfma(reader.column_fragment(qs, 2 * t + j, dt), df, dk[dt]);
-                }
+            for (int r = step * EACH; r < (step + 1) * EACH; ++r) {
+                const float of_row = shift[r >> 2][r & 3];
+                float x = __builtin_amdgcn_exp2f(BIAS ? fmaf(s[t][r], by, of_bias[BIAS ? r : 0]) + of_row : fmaf(s[t][r], by, of_row));
+                if (decltype(mask_tag)::value && at > row_of(r)) x = 0.0f;
+                s[t][r] = x;
+                dp[t][r] = x * (dp[t][r] - delta[r >> 2][r & 3]);
             }
+            if ((step + 1) * EACH % 8 == 0) {
+                const int j = (step + 1) * EACH / 8 - 1;
+                pf[t][j] = packed(s[t], j);
+                df[t][j] = packed(dp[t], j);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) load_rows(i);
+#pragma unroll
+        for (int i = 0; i < 2 * KC; ++i) {
+            const int t = i / KC, c = i % KC;
+            if (c == 0) {
+                s[t] = f32x16{};
+                dp[t] = f32x16{};
+            }
+            if (i == KC - AHEAD) load_statistics(0);
+            s[t] = mfma(ring_q[i % AHEAD], kf[c], s[t]);
+            dp[t] = mfma(ring_g[i % AHEAD], vf[c], dp[t]);
+            if (i + AHEAD < 2 * KC) load_rows(i + AHEAD);
+            else load_columns(i + AHEAD - 2 * KC);
+            if (i >= KC) grads(0, i - KC);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        load_statistics(1);
+#pragma unroll
+        for (int m = 0; m < 4 * DT; ++m) {
+            const int t = m / (2 * DT), j = m / DT % 2, dt = m % DT;
+            dv[dt] = mfma(ring_g[m % AHEAD], pf[t][j], dv[dt]);
+            dk[dt] = mfma(ring_q[m % AHEAD], df[t][j], dk[dt]);
+            if (m + AHEAD < 4 * DT) load_columns(m + AHEAD);
+            if (m < 2 * DT) grads(1, m);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     const int last_stage = first_stage + of_head;
