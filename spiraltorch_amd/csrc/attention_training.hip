@@ -152,6 +152,10 @@ struct Moving {
     }
 };
 
+// Every load has arrived.  Before a loop that works on what was loaded ahead of it: where the compiler sees such a load pending at the loop's head,
+// it waits within the loop, and there for the next stage's loads as well.
+__device__ __forceinline__ void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 sum) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, sum, 0, 0, 0); }
 
 // Accumulator registers 8j .. 8j + 7 as a B operand.
@@ -312,6 +316,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
 
     const int key_end = CAUSAL ? min(length, q0 + kStay) : length, stages = (key_end + kStage - 1) / kStage;
     const int seen = CAUSAL ? min(length, wq0 + 32) : length, plain = (CAUSAL ? min(length, q0) : length) / kStage;
+    wait_for_loads();
     moving.store(training_lds, training_lds + BYTES, tid);
     __syncthreads();
     auto step = [&](auto mask_tag, int t) {
@@ -465,6 +470,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     const int key_end = CAUSAL ? min(length, q0 + kStay) : length, stages = (key_end + kStage - 1) / kStage;
     const int seen = CAUSAL ? min(length, wq0 + 32) : length, plain = (CAUSAL ? min(length, q0) : length) / kStage;
     auto walk = [&](auto &&body) {
+        wait_for_loads();
         moving.store(training_lds, training_lds + BYTES, tid);
         __syncthreads();
         auto step = [&](auto mask_tag, int t) {
@@ -729,6 +735,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         if (BIAS) fill_bias(p, head, bias, tid);
         store(stage & 1);
     }
+    wait_for_loads();
     __syncthreads();
     int buffer = stage & 1;
     for (int left = end - begin; left > 0;) {
