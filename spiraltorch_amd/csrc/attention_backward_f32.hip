@@ -75,40 +75,58 @@ __device__ __forceinline__ f32x4 fetch4(const __amdgpu_buffer_rsrc_t &rows, int 
     return x;
 }
 
+typedef __attribute__((address_space(3))) void *lds_void_ptr;
+// A tile on its way straight into LDS, 16 bytes (VEC) or 4 a lane: what lies at a place is fetched by the lane that stands for it.  Rows behind the
+// last and columns from `dim` on are beyond the descriptor, and zeros.
 template <int DC, bool VEC>
 __device__ __forceinline__ void load_tile(const __amdgpu_buffer_rsrc_t &rows, int dim, int first, unsigned char *to, int lane)
 {
-    constexpr int CHUNKS = DC / 4, STEPS = kRows * CHUNKS / 64, BATCH = STEPS % 8 == 0 ? 8 : 4;
-    static_assert(STEPS % BATCH == 0, "the last batch ends with the tile");
+    constexpr int SIZE = VEC ? 16 : 4, STEPS = Tile<DC>::kBytes / (64 * SIZE);
+    asm volatile("" : "+v"(lane));  // (the places are worked out every time: kept for all steps, they would be registers the products need)
 #pragma unroll
-    for (int s = 0; s < STEPS; s += BATCH) {
-        f32x4 x[BATCH];
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int f = lane + 64 * (s + i);
-            x[i] = fetch4<VEC>(rows, dim, first + f / CHUNKS, f % CHUNKS * 4);
-        }
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int f = lane + 64 * (s + i);
-            *reinterpret_cast<f32x4 *>(to + Tile<DC>::place(f / CHUNKS, f % CHUNKS)) = x[i];
-        }
+    for (int s = 0; s < STEPS; ++s) {
+        const unsigned at = (s * 64 + lane) * SIZE, row = at / Tile<DC>::kRow, chunk = (at % Tile<DC>::kRow / 16) ^ (row & Tile<DC>::kTurn);
+        const unsigned column = chunk * 4 + at % 16 / 4;
+        const unsigned from = column < static_cast<unsigned>(dim) ? ((first + row) * static_cast<unsigned>(dim) + column) * 4u : 0x80000000u;
+        if (VEC) __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (lds_void_ptr)(to + s * 64 * SIZE), 16, from, 0, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (lds_void_ptr)(to + s * 64 * SIZE), 4, from, 0, 0, 0);
     }
+}
+__device__ __forceinline__ void wait_for_loads()
+{
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Up to 32 rows of S biases, zeros behind the last: loads beyond them give 0, and stores are dropped.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bias_rows(const float *first, int rows, int S)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(first), 0, static_cast<int>(static_cast<unsigned>(min(rows, kRows)) * S * 4u), 0x00020000);
 }
 
 __device__ __forceinline__ f32x16 mfma(float a, float b, f32x16 sum) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, sum, 0, 0, 0); }
 __device__ constexpr int row_of(int r) { return (r >> 2) * 8 + (r & 3); }
 
+// What a product reads from LDS is on its way some instructions early: a read takes longer than the matrix instruction that it feeds, and there
+// are one or two wavefronts to a SIMD.
 // tile · staysᵀ: accumulator registers are the tile's rows, lanes the rows that stay.
 template <int DC>
 __device__ __forceinline__ f32x16 product(const unsigned char *tile, const f32x4 (&stays)[DC / 8], int li, int lh)
 {
+    constexpr int AHEAD = 2;
     f32x16 sum = {};
+    f32x4 ring[AHEAD];
+    auto load = [&](int g) { ring[g % AHEAD] = *reinterpret_cast<const f32x4 *>(tile + Tile<DC>::place(li, 2 * g + lh)); };
+#pragma unroll
+    for (int g = 0; g < AHEAD; ++g) load(g);
 #pragma unroll
     for (int g = 0; g < DC / 8; ++g) {
-        const f32x4 a = *reinterpret_cast<const f32x4 *>(tile + Tile<DC>::place(li, 2 * g + lh));
+        const f32x4 a = ring[g % AHEAD];
+        if (g + AHEAD < DC / 8) load(g + AHEAD);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum = mfma(a[e], stays[g][e], sum);
+        __builtin_amdgcn_sched_barrier(0);
     }
     return sum;
 }
@@ -116,19 +134,30 @@ __device__ __forceinline__ f32x16 product(const unsigned char *tile, const f32x4
 template <int DC>
 __device__ __forceinline__ void add_product(const unsigned char *tile, const f32x16 &weights, f32x16 (&sums)[DC / 32], int li, int lh)
 {
+    constexpr int AHEAD = 8, DT = DC / 32, STEPS = 16 * DT;
     const unsigned base = ((li >> 2) ^ (4 * lh)) * 16 + (li & 3) * 4 + 4 * lh * Tile<DC>::kRow;
+    float ring[AHEAD];
+    auto load = [&](int n) {
+        const int row = row_of(n / DT);
+        const unsigned turn = ((n % DT * 8) ^ (row & Tile<DC>::kTurn)) * 16;
+        ring[n % AHEAD] = *reinterpret_cast<const float *>(tile + (base ^ turn) + row * Tile<DC>::kRow);
+    };
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int n = 0; n < AHEAD; ++n) load(n);
 #pragma unroll
-        for (int dt = 0; dt < DC / 32; ++dt) {
-            const unsigned turn = ((dt * 8) ^ (row_of(r) & Tile<DC>::kTurn)) * 16;
-            sums[dt] = mfma(*reinterpret_cast<const float *>(tile + (base ^ turn) + row_of(r) * Tile<DC>::kRow), weights[r], sums[dt]);
-        }
+    for (int n = 0; n < STEPS; ++n) {
+        sums[n % DT] = mfma(ring[n % AHEAD], weights[n / DT], sums[n % DT]);
+        if (n + AHEAD < STEPS) load(n + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
-__device__ __forceinline__ void wave_fence()
+// What the wavefront reads from LDS has been read, before loads into the same place.
+__device__ __forceinline__ void wait_for_reads()
 {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_s_waitcnt(0xc07f);
     __builtin_amdgcn_wave_barrier();
 }
 
@@ -184,29 +213,36 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         }
     }
     delta += __shfl_xor(delta, 32);
-    const float *const bias_row = p.attn_bias ? p.attn_bias + (first + my_q) * S : nullptr;
     const int key_end = CAUSAL ? min(S, q0 + kRows) : S, last_key = CAUSAL ? min(my_q, S - 1) : S - 1;
+    const __amdgpu_buffer_rsrc_t biases = bias_rows(p.attn_bias + (first + q0) * S, S - q0, S), z_biases = bias_rows(p.z_bias + first, 1, S);
+    // A tile's biases, four keys at a time; what is behind a row's last key is masked with it.
+    struct Biases {
+        f32x4 of_pair[4], of_key[4];
+    };
+    auto load_biases = [&](int key0, Biases &to) {
+        auto load = [&](const __amdgpu_buffer_rsrc_t &from, unsigned at) {
+            if (p.wide_bias) return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at * 4u, 0, 0));
+            f32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, (at + e) * 4u, 0, 0));
+            return x;
+        };
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const unsigned key = key0 + a * 8 + lh * 4;
+            if (p.attn_bias) to.of_pair[a] = load(biases, static_cast<unsigned>(li) * S + key);
+            if (p.z_bias) to.of_key[a] = load(z_biases, key);
+        }
+    };
     // the scores of a tile, in units of log2 e
-    auto scores = [&](int key0) {
-        f32x16 s = product<DC>(k_tile, q, li, lh);
+    auto scores = [&](const unsigned char *tile, const Biases &with, int key0) {
+        f32x16 s = product<DC>(tile, q, li, lh);
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
             const int key = key0 + a * 8 + lh * 4;
             f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (bias_row && my_q < S) {
-                if (p.wide_bias) {
-                    if (key < S) bias = *reinterpret_cast<const f32x4 *>(bias_row + key);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (key + e < S) bias[e] = bias_row[key + e];
-                }
-            }
-            if (p.z_bias) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (key + e < S) bias[e] += p.z_bias[first + key + e];
-            }
+            if (p.attn_bias) bias += with.of_pair[a];
+            if (p.z_bias) bias += with.of_key[a];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float x = fmaf(s[a * 4 + e], p.scale, bias[e]) * kLog2e;
@@ -216,10 +252,15 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         return s;
     };
     float most = -INFINITY, total = 0.0f;
-    for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
-        load_tile<DC, VEC>(k_rows, D, key0, k_tile, lane);
-        wave_fence();
-        const f32x16 s = scores(key0);
+    // (the wavefront's two tiles take turns)
+    if (wave * kRows < key_end) load_tile<DC, VEC>(k_rows, D, wave * kRows, k_tile, lane);
+    for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
+        Biases with;
+        wait_for_loads();
+        wait_for_reads();
+        load_biases(key0, with);
+        if (key0 + WAVES * kRows < key_end) load_tile<DC, VEC>(k_rows, D, key0 + WAVES * kRows, turn ? k_tile : v_tile, lane);
+        const f32x16 s = scores(turn ? v_tile : k_tile, with, key0);
         float top = most;
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
@@ -228,7 +269,6 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         most = top;
 #pragma unroll
         for (int r = 0; r < 16; ++r) total += __builtin_amdgcn_exp2f(s[r] - safe);
-        wave_fence();
     }
     {
         const float other = __shfl_xor(most, 32), other_total = __shfl_xor(total, 32), top = fmaxf(most, other), safe = top == -INFINITY ? 0.0f : top;
@@ -256,16 +296,28 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     f32x16 dq[DC / 32];
 #pragma unroll
     for (int dt = 0; dt < DC / 32; ++dt) dq[dt] = f32x16{};
+    auto load_keys = [&](int key0) {
+        if (key0 < key_end) load_tile<DC, VEC>(k_rows, D, key0, k_tile, lane);
+    };
+    auto load_values = [&](int key0) {
+        if (key0 < key_end) load_tile<DC, VEC>(v_rows, D, key0, v_tile, lane);
+    };
+    wait_for_reads();
+    load_keys(wave * kRows);
+    load_values(wave * kRows);
     for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
-        load_tile<DC, VEC>(k_rows, D, key0, k_tile, lane);
-        load_tile<DC, VEC>(v_rows, D, key0, v_tile, lane);
-        wave_fence();
-        f32x16 s = scores(key0);
+        Biases with;
+        wait_for_loads();
+        load_biases(key0, with);
         const f32x16 dp = product<DC>(v_tile, g, li, lh);
+        wait_for_reads();
+        load_values(key0 + WAVES * kRows);  // each tile's successor as soon as it has been read
+        f32x16 s = scores(k_tile, with, key0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - lse) * (dp[r] - delta);
         add_product<DC>(k_tile, s, dq, li, lh);
-        wave_fence();
+        wait_for_reads();
+        load_keys(key0 + WAVES * kRows);
     }
     write_rows<DC, WAVES>(dq, p.scale, p.grad_q + first * D, q0, S, D, backward_lds);
 }
@@ -303,41 +355,59 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     float dz = 0.0f;
     if (CAUSAL && DK && p.grad_attn_bias && my_key < S)  // queries before the tile do not see it
         for (int q = wave * 2 + lh; q < k0; q += WAVES * 2) p.grad_attn_bias[(first + q) * S + my_key] = 0.0f;
-    for (int row0 = (CAUSAL ? k0 : 0) + wave * kRows; row0 < S; row0 += WAVES * kRows) {
-        load_tile<DC, VEC>(q_rows, D, row0, q_tile, lane);
-        load_tile<DC, VEC>(g_rows, D, row0, g_tile, lane);
-        wave_fence();
-        f32x16 s = product<DC>(q_tile, k, li, lh);
-        const float *const lse = p.lse + static_cast<size_t>(context) * p.padded + row0 + 4 * lh;
+    auto load_queries = [&](int row0) {
+        if (row0 < S) load_tile<DC, VEC>(q_rows, D, row0, q_tile, lane);
+    };
+    auto load_grads = [&](int row0) {
+        if (row0 < S) load_tile<DC, VEC>(g_rows, D, row0, g_tile, lane);
+    };
+    const int start = (CAUSAL ? k0 : 0) + wave * kRows;
+    load_queries(start);
+    load_grads(start);
+    for (int row0 = start; row0 < S; row0 += WAVES * kRows) {
+        // the biases of the lane's key; beyond the descriptor for a key behind the last
+        const unsigned at = my_key < S ? (4u * lh * S + my_key) * 4u : 0x80000000u;
+        float bias[16];
+        f32x4 lse[4], delta[4];
+        const size_t of_rows = static_cast<size_t>(context) * p.padded + row0 + 4 * lh;
+        wait_for_loads();
+        if (p.attn_bias) {
+            const __amdgpu_buffer_rsrc_t biases = bias_rows(p.attn_bias + (first + row0) * S, S - row0, S);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) bias[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(biases, at + row_of(r) * S * 4u, 0, 0));
+        }
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-            const f32x4 of = *reinterpret_cast<const f32x4 *>(lse + a * 8);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = a * 4 + e, row = row0 + row_of(r) + 4 * lh;
-                const float bias = p.attn_bias && row < S && my_key < S ? p.attn_bias[(first + row) * S + my_key] + z : z;
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale, bias) * kLog2e - of[e]);
-                s[r] = CAUSAL && my_key > row ? 0.0f : x;
-            }
+            lse[a] = *reinterpret_cast<const f32x4 *>(p.lse + of_rows + a * 8);
+            if (DK) delta[a] = *reinterpret_cast<const f32x4 *>(p.delta + of_rows + a * 8);
         }
+        f32x16 s = product<DC>(q_tile, k, li, lh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float with = p.attn_bias ? bias[r] + z : z;
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale, with) * kLog2e - lse[r >> 2][r & 3]);
+            s[r] = CAUSAL && my_key > row0 + row_of(r) + 4 * lh ? 0.0f : x;
+        }
+        f32x16 dp;
+        if constexpr (DK) dp = product<DC>(g_tile, v, li, lh);
         if constexpr (DV) add_product<DC>(g_tile, s, dv, li, lh);
+        wait_for_reads();
+        load_grads(row0 + WAVES * kRows);  // each tile's successor as soon as it has been read
         if constexpr (DK) {
-            f32x16 dp = product<DC>(g_tile, v, li, lh);
-            const float *const delta = p.delta + static_cast<size_t>(context) * p.padded + row0 + 4 * lh;
 #pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                const f32x4 of = *reinterpret_cast<const f32x4 *>(delta + a * 8);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = a * 4 + e, row = row0 + row_of(r) + 4 * lh;
-                    s[r] *= dp[r] - of[e];
-                    dz += s[r];
-                    if (p.grad_attn_bias && row < S && my_key < S) p.grad_attn_bias[(first + row) * S + my_key] = s[r];
-                }
+            for (int r = 0; r < 16; ++r) {
+                s[r] *= dp[r] - delta[r >> 2][r & 3];
+                dz += s[r];
             }
             add_product<DC>(q_tile, s, dk, li, lh);
+            if (p.grad_attn_bias) {
+                const __amdgpu_buffer_rsrc_t grads = bias_rows(p.grad_attn_bias + (first + row0) * S, S - row0, S);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[r]), grads, at + row_of(r) * S * 4u, 0, 0);
+            }
         }
-        wave_fence();
+        wait_for_reads();
+        load_queries(row0 + WAVES * kRows);
     }
     if constexpr (DK) {
         if (p.grad_z_bias) {
@@ -420,7 +490,7 @@ hipError_t launch_attention_backward_f32(size_t contexts, size_t sequence, size_
     args.swizzle = contexts % 8 == 0;
     args.scale = scale;
     auto aligned = [](const void *at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; };
-    args.wide_bias = sequence % 4 == 0 && aligned(attn_bias);
+    args.wide_bias = sequence % 4 == 0 && aligned(attn_bias) && aligned(z_bias);
     const size_t rows = contexts * args.padded;
     void *scratch = nullptr;
     const hipError_t rc = stream_workspace(stream, 2 * rows * sizeof(float), &scratch);
