@@ -191,6 +191,20 @@ __device__ __forceinline__ void fill_bias(const TrainingArgs &p, int head, float
     }
 }
 
+// The sequence that is taken as the `place`-th: of a padded batch of up to 64, in the order of their lengths, the longest first, as those that begin
+// last are what the launch waits for.
+__device__ __forceinline__ int sequence_at(const TrainingArgs &p, int place, int lane)
+{
+    if (!p.lengths || p.batch > 64) return place;
+    const int mine = lane < p.batch ? min(max(p.lengths[lane], 0), p.S) : -1;
+    int before = 0;
+    for (int j = 0; j < p.batch; ++j) {
+        const int other = __builtin_amdgcn_readlane(mine, j);
+        before += other > mine || (other == mine && j < lane);
+    }
+    return __ffsll(__ballot(before == place)) - 1;
+}
+
 __device__ __forceinline__ int length_of(const TrainingArgs &p, int batch) { return p.lengths ? min(max(p.lengths[batch], 0), p.S) : p.S; }
 
 // One head's 32 rows as they left the matrix cores: a lane has its row's values 4 at a time.
@@ -223,10 +237,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
 
     const Item item = decode(p.batch * p.kv_heads, p.group, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
-    const int b = item.context / p.heads, h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
+    const int b = sequence_at(p, item.context / p.heads, lane), h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
+    const size_t context = static_cast<size_t>(b) * p.heads + h;
     const int length = length_of(p, b);
     uint16_t *const out_row = p.out + (static_cast<size_t>(b) * p.S + my_q) * p.ld_out + static_cast<size_t>(h) * D;
-    float *const lse = p.lse + static_cast<size_t>(item.context) * p.S;
+    float *const lse = p.lse + context * p.S;
     if (q0 >= length) {
         if (my_q < p.S) {
             store_zeros<D>(out_row, lh);
@@ -376,12 +391,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     float *const bins = all_bins + wave * width;
 
     const Item item = decode(p.batch * p.kv_heads, p.group, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
-    const int b = item.context / p.heads, h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
+    const int b = sequence_at(p, item.context / p.heads, lane), h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
+    const size_t context = static_cast<size_t>(b) * p.heads + h;
     const int length = length_of(p, b);
     const bool to_table = BIAS && p.partial != nullptr;
-    float *const partial = to_table ? p.partial + (static_cast<size_t>(item.context) * p.tiles + item.tile) * width : nullptr;
+    float *const partial = to_table ? p.partial + (context * p.tiles + item.tile) * width : nullptr;
     uint16_t *const grad_row = p.grad_q + (static_cast<size_t>(b) * p.S + my_q) * p.ld_grad_q + static_cast<size_t>(h) * D;
-    float *const delta_row = p.delta + static_cast<size_t>(item.context) * p.S + my_q;
+    float *const delta_row = p.delta + context * p.S + my_q;
     if (q0 >= length) {
         if (my_q < p.S) store_zeros<D>(grad_row, lh);
         if (to_table)
@@ -414,7 +430,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         for (int e = 0; e < 8; ++e) delta = fmaf(static_cast<float>(gf[c][e]), static_cast<float>(of[e]), delta);
     }
     delta += __shfl_xor(delta, 32);
-    float lse = my_q < length ? p.lse[static_cast<size_t>(item.context) * p.S + my_q] : INFINITY;
+    float lse = my_q < length ? p.lse[context * p.S + my_q] : INFINITY;
     if (lse == -INFINITY) lse = INFINITY;  // a row without keys: every p is 0
     const float by = p.scale * kLog2e, shift = -lse * kLog2e;
 
@@ -601,7 +617,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 
     const Item item = decode(p.batch * p.kv_heads, 1, p.tiles * p.parts, p.swizzle, CAUSAL, false, blockIdx.x);
     const int tile = item.tile / p.parts, part = item.tile % p.parts;
-    const int b = item.context / p.kv_heads, kv_head = item.context % p.kv_heads, k0 = tile * kStay, wk0 = k0 + wave * 32, my_key = wk0 + li;
+    const int b = sequence_at(p, item.context / p.kv_heads, lane), kv_head = item.context % p.kv_heads, k0 = tile * kStay, wk0 = k0 + wave * 32, my_key = wk0 + li;
     const int length = length_of(p, b);
     const size_t grad_at = (static_cast<size_t>(b) * p.S + my_key) * p.ld_grad_kv + static_cast<size_t>(kv_head) * D;
     if (k0 >= length) {
