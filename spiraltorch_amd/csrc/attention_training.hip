@@ -126,29 +126,25 @@ __device__ __forceinline__ u32x4_t fetch8(const __amdgpu_buffer_rsrc_t &rows, un
     return __builtin_amdgcn_raw_buffer_load_b128(rows, (static_cast<unsigned>(row) * ld + column) * 2u, 0, 0);
 }
 
-// Two matrices' stages on their way: from memory into registers, and into LDS when the stage before has been read.
+// A matrix's stages on their way from memory straight into LDS, 16 bytes a lane: no registers, and no instructions to store them.  A wavefront's
+// instruction fills 1 KiB; what lies at a place is fetched by the lane that stands for it.
+typedef __attribute__((address_space(3))) void *lds_void_ptr;
 template <int D>
-struct Moving {
-    u32x4_t a[Stage<D>::kLoads], b[Stage<D>::kLoads];
-    __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t &rows_a, unsigned ld_a, const __amdgpu_buffer_rsrc_t &rows_b, unsigned ld_b, int first,
-                                         int tid)
+struct Mover {
+    static constexpr int kRows = 1024 / Stage<D>::kRow;  // of an instruction; those of the four wavefronts together hold every turn once or twice
+    unsigned from, ld;                                   // of this lane in the first instruction, bytes; row stride, bytes
+    int wave;
+    __device__ __forceinline__ Mover(unsigned ld_values, int lane, int wave) : ld(ld_values * 2u), wave(wave)
     {
-#pragma unroll
-        for (int r = 0; r < Stage<D>::kLoads; ++r) {
-            const int f = tid + 256 * r, row = f / (D / 8), column = f % (D / 8) * 8;
-            a[r] = fetch8(rows_a, ld_a, first + row, column);
-            b[r] = fetch8(rows_b, ld_b, first + row, column);
-        }
+        constexpr int LANES = Stage<D>::kRow / 16;
+        const unsigned row = wave * kRows + lane / LANES, held = Stage<D>::place(row, lane % LANES) - row * Stage<D>::kRow;  // (a turn undoes itself)
+        from = row * ld + held;
     }
-    __device__ __forceinline__ void store(unsigned char *to_a, unsigned char *to_b, int tid) const
+    __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t &rows, int first, unsigned char *to) const
     {
 #pragma unroll
-        for (int r = 0; r < Stage<D>::kLoads; ++r) {
-            const int f = tid + 256 * r;
-            const unsigned at = Stage<D>::place(f / (D / 8), f % (D / 8));
-            *reinterpret_cast<u32x4_t *>(to_a + at) = a[r];
-            *reinterpret_cast<u32x4_t *>(to_b + at) = b[r];
-        }
+        for (int i = 0; i < Stage<D>::kLoads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (lds_void_ptr)(to + (i * 4 + wave) * 1024), 16, from + (first + i * 4 * kRows) * ld, 0, 0, 0);
     }
 };
 
@@ -254,8 +250,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
     const __amdgpu_buffer_rsrc_t q_rows = rows_of(p.q + first_q, p.ld_q, length, D), k_rows = rows_of(p.k + first_k, p.ld_kv, length, D),
                                  v_rows = rows_of(p.v + first_k, p.ld_kv, length, D);
     const Reader<D> reader(lane);
-    Moving<D> moving;
-    moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, 0, tid);
+    const Mover<D> mover(p.ld_kv, lane, wave);
+    auto load = [&](int t) {
+        unsigned char *const to = training_lds + (t & 1) * 2 * BYTES;
+        mover.load(k_rows, t * kStage, to);
+        mover.load(v_rows, t * kStage, to + BYTES);
+    };
+    load(0);
     if (BIAS) fill_bias(p, h, bias, tid);
     // Without biases the running maximum is kept in units of the product q·k; a negative scale goes into q's signs for that.
     bf16x8 qf[KC];
@@ -332,14 +333,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
     const int key_end = CAUSAL ? min(length, q0 + kStay) : length, stages = (key_end + kStage - 1) / kStage;
     const int seen = CAUSAL ? min(length, wq0 + 32) : length, plain = (CAUSAL ? min(length, q0) : length) / kStage;
     wait_for_loads();
-    moving.store(training_lds, training_lds + BYTES, tid);
     __syncthreads();
     auto step = [&](auto mask_tag, int t) {
-        const bool more = t + 1 < stages;
-        if (more) moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, (t + 1) * kStage, tid);
+        if (t + 1 < stages) load(t + 1);
         const unsigned char *const ks = training_lds + (t & 1) * 2 * BYTES;
         if (!decltype(mask_tag)::value || t * kStage < seen) compute(mask_tag, ks, ks + BYTES, t * kStage);
-        if (more) moving.store(training_lds + ((t + 1) & 1) * 2 * BYTES, training_lds + ((t + 1) & 1) * 2 * BYTES + BYTES, tid);
+        wait_for_loads();
         __syncthreads();
     };
     // Stages without masked keys in a loop of their own: where a body branches, the accumulators are copied behind its last product, and the
@@ -380,7 +379,7 @@ __device__ __forceinline__ void add_by_distance(const f32x16 &ds, int d0, int fa
 }
 
 template <int D, bool CAUSAL, bool BIAS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, 4))) void attention_grad_q_kernel(TrainingArgs p)
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BIAS && D == 128 ? 1 : 2, 4))) void attention_grad_q_kernel(TrainingArgs p)
 {
     constexpr int KC = D / 16, DT = D / 32, BYTES = Stage<D>::kBytes;
     extern __shared__ __attribute__((aligned(16))) unsigned char training_lds[];  // [K, V][2]; bias; bins of four wavefronts
@@ -412,8 +411,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         rows_of(p.grad_out + static_cast<size_t>(b) * p.S * p.ld_grad_out + static_cast<size_t>(h) * D, p.ld_grad_out, length, D);
     const __amdgpu_buffer_rsrc_t o_rows = rows_of(p.out_read + static_cast<size_t>(b) * p.S * p.ld_out + static_cast<size_t>(h) * D, p.ld_out, length, D);
     const Reader<D> reader(lane);
-    Moving<D> moving;
-    moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, 0, tid);
+    const Mover<D> mover(p.ld_kv, lane, wave);
+    auto load_stage = [&](int t) {
+        unsigned char *const to = training_lds + (t & 1) * 2 * BYTES;
+        mover.load(k_rows, t * kStage, to);
+        mover.load(v_rows, t * kStage, to + BYTES);
+    };
+    load_stage(0);
     if (BIAS) {
         fill_bias(p, h, bias, tid);
         if (to_table)
@@ -437,7 +441,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     // A stage is two blocks of 32 keys.  Its products are dealt out in steps of one chunk, with what is read from LDS `AHEAD` steps early and
     // the other block's softmax spread over the steps: there are one or two wavefronts to a SIMD, and nothing else hides the reads' way
     // or the exponentials.
-    constexpr int AHEAD = D == 64 ? 2 : 4, STEPS = D / 16, EACH = 16 / STEPS;
+    constexpr int AHEAD = BIAS && D == 128 ? 4 : D == 64 ? 2 : 1, STEPS = D / 16, EACH = 16 / STEPS;
     struct Block {
         f32x16 s, dp;
         float bias[BIAS ? 16 : 1];
@@ -487,14 +491,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     const int seen = CAUSAL ? min(length, wq0 + 32) : length, plain = (CAUSAL ? min(length, q0) : length) / kStage;
     auto walk = [&](auto &&body) {
         wait_for_loads();
-        moving.store(training_lds, training_lds + BYTES, tid);
         __syncthreads();
         auto step = [&](auto mask_tag, int t) {
-            const bool more = t + 1 < stages;
-            if (more) moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, (t + 1) * kStage, tid);
+            if (t + 1 < stages) load_stage(t + 1);
             const unsigned char *const ks = training_lds + (t & 1) * 2 * BYTES;
             if (!decltype(mask_tag)::value || t * kStage < seen) body(mask_tag, ks, ks + BYTES, t * kStage);
-            if (more) moving.store(training_lds + ((t + 1) & 1) * 2 * BYTES, training_lds + ((t + 1) & 1) * 2 * BYTES + BYTES, tid);
+            wait_for_loads();
             __syncthreads();
         };
         int t = 0;  // (as in the forward pass)
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
             for (int step = 0; step < STEPS; ++step) add(1, step);
         });
         delta += __shfl_xor(delta, 32);
-        if (stages > 1) moving.load(k_rows, p.ld_kv, v_rows, p.ld_kv, 0, tid);
+        if (stages > 1) load_stage(0);
     }
     if (lh == 0 && my_q < length) *delta_row = delta;
 
@@ -647,16 +649,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     const int first_stage = CAUSAL ? k0 / kStage : 0, of_head = (length + kStage - 1) / kStage - first_stage;
     const long long all = static_cast<long long>(of_head) * p.group;
     const int begin = static_cast<int>(all * part / p.parts), end = static_cast<int>(all * (part + 1) / p.parts);
-    Moving<D> moving;
+    const Mover<D> mover_q(p.ld_q, lane, wave), mover_g(p.ld_grad_out, lane, wave);
     float statistic = 0.0f;
-    auto load = [&](int head, int stage) {
+    auto load = [&](int head, int stage, int buffer) {
         const int first = stage * kStage;
         const __amdgpu_buffer_rsrc_t q_rows =
             rows_of(p.q + static_cast<size_t>(b) * p.S * p.ld_q + static_cast<size_t>(head) * D, p.ld_q, length, D);
         const __amdgpu_buffer_rsrc_t g_rows =
             rows_of(p.grad_out + static_cast<size_t>(b) * p.S * p.ld_grad_out + static_cast<size_t>(head) * D, p.ld_grad_out, length, D);
         const size_t of_context = (static_cast<size_t>(b) * p.heads + head) * p.S;
-        moving.load(q_rows, p.ld_q, g_rows, p.ld_grad_out, first, tid);
+        unsigned char *const to = training_lds + buffer * 2 * BYTES;
+        mover_q.load(q_rows, first, to);
+        mover_g.load(g_rows, first, to + BYTES);
         const int row = first + (tid & 63);
         if (tid < 64) {
             const float lse = row < length ? p.lse[of_context + row] : INFINITY;
@@ -666,7 +670,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         }
     };
     auto store = [&](int buffer) {
-        moving.store(training_lds + buffer * 2 * BYTES, training_lds + buffer * 2 * BYTES + BYTES, tid);
         if (tid < 128) statistics[buffer * 2 * kStage + tid] = statistic;
     };
     // (In steps, as in the dq kernel.)
@@ -747,13 +750,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         head = begin / of_head;
         stage = first_stage + begin % of_head;
         head += kv_head * p.group;
-        load(head, stage);
+        load(head, stage, 0);
         if (BIAS) fill_bias(p, head, bias, tid);
-        store(stage & 1);
+        store(0);
     }
     wait_for_loads();
     __syncthreads();
-    int buffer = stage & 1;
+    int buffer = 0;
     for (int left = end - begin; left > 0;) {
         auto step = [&](auto mask_tag) {
             const int row0 = stage * kStage;
@@ -762,7 +765,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
                 ++head;
                 stage = first_stage;
             }
-            if (more) load(head, stage);
+            if (more) load(head, stage, buffer ^ 1);
             if (!decltype(mask_tag)::value || row0 + kStage > wk0) compute(mask_tag, buffer, row0);
             if (BIAS && more && next_head) {  // another head's biases, when this one's have been read
                 __syncthreads();
@@ -770,6 +773,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
             }
             buffer ^= 1;
             if (more) store(buffer);
+            wait_for_loads();
             __syncthreads();
             return more && !next_head;
         };
