@@ -441,7 +441,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BIAS && D =
     // A stage is two blocks of 32 keys.  Its products are dealt out in steps of one chunk, with what is read from LDS `AHEAD` steps early and
     // the other block's softmax spread over the steps: there are one or two wavefronts to a SIMD, and nothing else hides the reads' way
     // or the exponentials.
-    constexpr int AHEAD = BIAS && D == 128 ? 4 : D == 64 ? 2 : 1, STEPS = D / 16, EACH = 16 / STEPS;
+    constexpr int AHEAD = BIAS && D == 128 ? 4 : 1, STEPS = D / 16, EACH = 16 / STEPS;
     struct Block {
         f32x16 s, dp;
         float bias[BIAS ? 16 : 1];
