@@ -1,6 +1,7 @@
 """Log-probabilities of given tokens, entropies, the likeliest alternatives and the logits' gradient against 64 bits."""
 import numpy as np
 import pytest
+import torch
 
 from spiraltorch_amd import inputs
 
@@ -236,3 +237,86 @@ def test_gradient_of_nothing(hip):
     hip.token_log_probs_backward_f32_dev(2, 100, call.d_x, 100, None, call.d["lse"], None, None, None, d_y, 100)
     hip.device_synchronize()
     assert (d_y.to_array(np.float32, (2, 100)) == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_rows_far_into_the_memory(hip, kind):
+    """Logits of 9 GB: the last rows' results, and gradients, are those that they have alone."""
+    rng = np.random.default_rng(4)
+    size = 4 if kind == "f32" else 2
+    vocab, rows = 60001, 9 * 10**9 // size // 60001
+    x = make(rng, 3, vocab, kind)
+    tokens, g = rng.integers(0, vocab, 3).astype(np.int32), rng.normal(size=3).astype(np.float32)
+    alone = Call(hip, x, vocab, tokens, kind, 4)
+    alone.forward()
+    want = alone.results()
+    backward = hip.token_log_probs_backward_f32_dev if kind == "f32" else hip.token_log_probs_backward_bf16_dev
+    d_g, d_y = hip.DeviceBuffer.from_array(g), hip.DeviceBuffer(3 * vocab * size)
+    backward(3, vocab, alone.d_x, vocab, alone.d_tokens, alone.d["lse"], alone.d["entropies"], d_g, d_g, d_y, vocab)
+    hip.device_synchronize()
+    want_y = d_y.to_array(x.dtype, x.shape)
+    d_x = hip.DeviceBuffer(rows * vocab * size)
+    d_x.zero()
+    d_x.upload(x, (rows - 3) * vocab * size)
+    d_tokens = hip.DeviceBuffer.from_array(np.concatenate([np.zeros(rows - 3, np.int32), tokens]))
+    d_all = hip.DeviceBuffer.from_array(np.concatenate([np.zeros(rows - 3, np.float32), g]))
+    out = [hip.DeviceBuffer(rows * 4) for _ in range(3)]
+    d_ids, d_top = hip.DeviceBuffer(rows * 16), hip.DeviceBuffer(rows * 16)
+    forward = hip.token_log_probs_f32_dev if kind == "f32" else hip.token_log_probs_bf16_dev
+    forward(rows, vocab, d_x, vocab, d_tokens, *out, 4, d_ids, d_top)
+    hip.device_synchronize()
+    got = {name: buf.to_array(np.float32, rows)[-3:] for name, buf in zip(("log_probs", "entropies", "lse"), out)}
+    for name, value in got.items():
+        # (few rows are cut into parts, whose sums are put together in another order)
+        assert np.abs(value - want[name]).max() < 1e-4, name
+    assert (d_ids.to_array(np.int32, (rows, 4))[-3:] == want["ids"]).all()
+    backward(rows, vocab, d_x, vocab, d_tokens, out[2], out[1], d_all, d_all, d_x, vocab)
+    hip.device_synchronize()
+    y = np.empty((3, vocab), x.dtype)
+    hip._check(hip._lib.load().st_hip_memcpy_d2h(y.ctypes.data, d_x.at((rows - 3) * vocab * size), y.nbytes, None))
+    off = np.abs(floats(y) - floats(want_y))
+    assert (off <= 2e-4 * np.abs(floats(want_y)) + (U * np.abs(floats(want_y)) * 2 if kind == "bf16" else 0) + 1e-9).all()
+
+
+def test_the_same_bits_again(hip):
+    rng = np.random.default_rng(8)
+    for rows, vocab in ((1, 100000), (70, 30000), (500, 700)):
+        call = Call(hip, make(rng, rows, vocab, "bf16"), vocab, rng.integers(0, vocab, rows), "bf16", 16)
+        call.forward()
+        first = call.results()
+        for _ in range(3):
+            call.forward()
+            for name, value in call.results().items():
+                assert (value == first[name]).all(), name
+
+
+def test_parts_captured_and_replayed(hip):
+    """A row that is cut into parts, recorded on a stream without scratch memory."""
+    x = torch.randn(2, 90000, device="cuda")
+    tokens = torch.tensor([5, 89999], dtype=torch.int32, device="cuda")
+    out = [torch.empty(2, device="cuda") for _ in range(3)]
+    ids, top = torch.empty(2, 9, dtype=torch.int32, device="cuda"), torch.empty(2, 9, device="cuda")
+    call = lambda stream: hip.token_log_probs_f32_dev(2, 90000, x.data_ptr(), 90000, tokens.data_ptr(), *(o.data_ptr() for o in out), 9, ids.data_ptr(),
+                                                      top.data_ptr(), stream=stream)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        call(torch.cuda.current_stream().cuda_stream)
+    try:
+        for replay in range(4):
+            x.mul_(-0.9)
+            call(None)
+            torch.cuda.synchronize()
+            want = [o.clone() for o in (*out, ids, top)]
+            for o in (*out, ids, top):
+                o.fill_(7)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            torch.cuda.synchronize()
+            for got, first in zip((*out, ids, top), want):
+                assert torch.equal(got, first), replay
+    finally:
+        del graph
+        hip.release_scratch(stream.cuda_stream)
+        hip.release_scratch(None)
