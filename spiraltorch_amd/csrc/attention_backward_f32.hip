@@ -162,7 +162,7 @@ __device__ __forceinline__ void wait_for_reads()
 }
 
 // The wavefronts' sums (a lane has its row, registers the columns), times `by`, into rows first .. first + 31 of a matrix.
-template <int DC, int WAVES>
+template <int DC, int WAVES, bool VEC>
 __device__ __forceinline__ void write_rows(const f32x16 (&sums)[DC / 32], float by, float *to, int first, int rows, int dim, unsigned char *lds)
 {
     constexpr int STRIDE = DC + 4;
@@ -176,13 +176,24 @@ __device__ __forceinline__ void write_rows(const f32x16 (&sums)[DC / 32], float 
             *reinterpret_cast<f32x4 *>(parts + (wave * kRows + li) * STRIDE + dt * 32 + a * 8 + lh * 4) =
                 f32x4{sums[dt][a * 4], sums[dt][a * 4 + 1], sums[dt][a * 4 + 2], sums[dt][a * 4 + 3]};
     __syncthreads();
-    for (int i = tid; i < kRows * dim; i += WAVES * 64) {
-        const int row = i / dim, column = i % dim;
-        if (first + row >= rows) break;
-        float sum = parts[row * STRIDE + column];
+    constexpr int UNIT = VEC ? 4 : 1, OF_ROW = DC / UNIT;
+#pragma unroll 4
+    for (int i = tid; i < kRows * OF_ROW; i += WAVES * 64) {
+        const int row = i / OF_ROW, column = i % OF_ROW * UNIT;
+        if (first + row >= rows || column >= dim) continue;
+        const float *const from = parts + row * STRIDE + column;
+        float *const at = to + static_cast<size_t>(first + row) * dim + column;
+        if constexpr (VEC) {
+            f32x4 sum = *reinterpret_cast<const f32x4 *>(from);
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) sum += parts[(w * kRows + row) * STRIDE + column];
-        to[static_cast<size_t>(first + row) * dim + column] = sum * by;
+            for (int w = 1; w < WAVES; ++w) sum += *reinterpret_cast<const f32x4 *>(from + w * kRows * STRIDE);
+            *reinterpret_cast<f32x4 *>(at) = sum * by;
+        } else {
+            float sum = *from;
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) sum += from[w * kRows * STRIDE];
+            *at = sum * by;
+        }
     }
 }
 
@@ -198,6 +209,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     const size_t first = static_cast<size_t>(context) * S;
     unsigned char *const k_tile = backward_lds + wave * 2 * Tile<DC>::kBytes, *const v_tile = k_tile + Tile<DC>::kBytes;
     const __amdgpu_buffer_rsrc_t k_rows = rows_of(p.k + first * D, S, D), v_rows = rows_of(p.v + first * D, S, D);
+    const int key_end = CAUSAL ? min(S, q0 + kRows) : S, last_key = CAUSAL ? min(my_q, S - 1) : S - 1;
+    if (wave * kRows < key_end) load_tile<DC, VEC>(k_rows, D, wave * kRows, k_tile, lane);
     f32x4 q[DC / 8], g[DC / 8];
     float delta = 0.0f;
     {
@@ -213,7 +226,6 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         }
     }
     delta += __shfl_xor(delta, 32);
-    const int key_end = CAUSAL ? min(S, q0 + kRows) : S, last_key = CAUSAL ? min(my_q, S - 1) : S - 1;
     const __amdgpu_buffer_rsrc_t biases = bias_rows(p.attn_bias + (first + q0) * S, S - q0, S), z_biases = bias_rows(p.z_bias + first, 1, S);
     // A tile's biases, four keys at a time; what is behind a row's last key is masked with it.
     struct Biases {
@@ -253,7 +265,6 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     };
     float most = -INFINITY, total = 0.0f;
     // (the wavefront's two tiles take turns)
-    if (wave * kRows < key_end) load_tile<DC, VEC>(k_rows, D, wave * kRows, k_tile, lane);
     for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
         Biases with;
         wait_for_loads();
@@ -270,6 +281,15 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
 #pragma unroll
         for (int r = 0; r < 16; ++r) total += __builtin_amdgcn_exp2f(s[r] - safe);
     }
+    auto load_keys = [&](int key0) {
+        if (key0 < key_end) load_tile<DC, VEC>(k_rows, D, key0, k_tile, lane);
+    };
+    auto load_values = [&](int key0) {
+        if (key0 < key_end) load_tile<DC, VEC>(v_rows, D, key0, v_tile, lane);
+    };
+    wait_for_reads();
+    load_values(wave * kRows);
+    load_keys(wave * kRows);
     {
         const float other = __shfl_xor(most, 32), other_total = __shfl_xor(total, 32), top = fmaxf(most, other), safe = top == -INFINITY ? 0.0f : top;
         total = total * __builtin_amdgcn_exp2f(most - safe) + other_total * __builtin_amdgcn_exp2f(other - safe);
@@ -296,15 +316,6 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     f32x16 dq[DC / 32];
 #pragma unroll
     for (int dt = 0; dt < DC / 32; ++dt) dq[dt] = f32x16{};
-    auto load_keys = [&](int key0) {
-        if (key0 < key_end) load_tile<DC, VEC>(k_rows, D, key0, k_tile, lane);
-    };
-    auto load_values = [&](int key0) {
-        if (key0 < key_end) load_tile<DC, VEC>(v_rows, D, key0, v_tile, lane);
-    };
-    wait_for_reads();
-    load_keys(wave * kRows);
-    load_values(wave * kRows);
     for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
         Biases with;
         wait_for_loads();
@@ -319,7 +330,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         wait_for_reads();
         load_keys(key0 + WAVES * kRows);
     }
-    write_rows<DC, WAVES>(dq, p.scale, p.grad_q + first * D, q0, S, D, backward_lds);
+    write_rows<DC, WAVES, VEC>(dq, p.scale, p.grad_q + first * D, q0, S, D, backward_lds);
 }
 
 // ---- dk, dv, the biases' gradients: keys stay -----------------------------------------------------------------------------------------------
@@ -335,6 +346,15 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     const size_t first = static_cast<size_t>(context) * S;
     unsigned char *const q_tile = backward_lds + wave * 2 * Tile<DC>::kBytes, *const g_tile = q_tile + Tile<DC>::kBytes;
     const __amdgpu_buffer_rsrc_t q_rows = rows_of(p.q + first * D, S, D), g_rows = rows_of(p.grad_out + first * D, S, D);
+    auto load_queries = [&](int row0) {
+        if (row0 < S) load_tile<DC, VEC>(q_rows, D, row0, q_tile, lane);
+    };
+    auto load_grads = [&](int row0) {
+        if (row0 < S) load_tile<DC, VEC>(g_rows, D, row0, g_tile, lane);
+    };
+    const int start = (CAUSAL ? k0 : 0) + wave * kRows;
+    load_queries(start);
+    load_grads(start);
     f32x4 k[DC / 8], v[DK ? DC / 8 : 1];
     {
         const __amdgpu_buffer_rsrc_t k_rows = rows_of(p.k + first * D, S, D), v_rows = rows_of(p.v + first * D, S, D);
@@ -355,15 +375,6 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     float dz = 0.0f;
     if (CAUSAL && DK && p.grad_attn_bias && my_key < S)  // queries before the tile do not see it
         for (int q = wave * 2 + lh; q < k0; q += WAVES * 2) p.grad_attn_bias[(first + q) * S + my_key] = 0.0f;
-    auto load_queries = [&](int row0) {
-        if (row0 < S) load_tile<DC, VEC>(q_rows, D, row0, q_tile, lane);
-    };
-    auto load_grads = [&](int row0) {
-        if (row0 < S) load_tile<DC, VEC>(g_rows, D, row0, g_tile, lane);
-    };
-    const int start = (CAUSAL ? k0 : 0) + wave * kRows;
-    load_queries(start);
-    load_grads(start);
     for (int row0 = start; row0 < S; row0 += WAVES * kRows) {
         // the biases of the lane's key; beyond the descriptor for a key behind the last
         const unsigned at = my_key < S ? (4u * lh * S + my_key) * 4u : 0x80000000u;
@@ -421,9 +432,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
                 p.grad_z_bias[first + my_key] = sum;
             }
         }
-        write_rows<DC, WAVES>(dk, p.scale, p.grad_k + first * D, k0, S, D, backward_lds);
+        write_rows<DC, WAVES, VEC>(dk, p.scale, p.grad_k + first * D, k0, S, D, backward_lds);
     }
-    if constexpr (DV) write_rows<DC, WAVES>(dv, 1.0f, p.grad_v + first * D, k0, S, D, backward_lds);
+    if constexpr (DV) write_rows<DC, WAVES, VEC>(dv, 1.0f, p.grad_v + first * D, k0, S, D, backward_lds);
 }
 
 template <class Kernel>
@@ -497,7 +508,8 @@ hipError_t launch_attention_backward_f32(size_t contexts, size_t sequence, size_
     if (rc != hipSuccess) return rc;
     args.lse = static_cast<float *>(scratch);
     args.delta = args.lse + rows;
-    const bool vec = head_dim % 4 == 0 && aligned(q) && aligned(k) && aligned(v) && aligned(out) && aligned(grad_out);
+    const bool vec = head_dim % 4 == 0 && aligned(q) && aligned(k) && aligned(v) && aligned(out) && aligned(grad_out) &&
+                     aligned(grad_q) && aligned(grad_k) && aligned(grad_v);
     if (head_dim <= 32) return launch_width<32>(args, vec, causal, stream);
     if (head_dim <= 64) return launch_width<64>(args, vec, causal, stream);
     if (head_dim <= 96) return launch_width<96>(args, vec, causal, stream);
