@@ -451,10 +451,9 @@ hipError_t launch(Kernel kernel, const BackwardArgs &args, int waves, size_t lds
     return hipGetLastError();
 }
 
-template <int DC, bool VEC, bool CAUSAL>
-hipError_t launch_variant(const BackwardArgs &args, hipStream_t stream)
+template <int DC, int WAVES, bool VEC, bool CAUSAL>
+hipError_t launch_waves(const BackwardArgs &args, hipStream_t stream)
 {
-    constexpr int WAVES = DC <= 128 ? 4 : 2;  // tiles of 256 values: 64 KiB a wavefront
     constexpr size_t lds = std::max<size_t>(WAVES * 2 * Tile<DC>::kBytes, WAVES * kRows * (DC + 4) * sizeof(float));
     hipError_t rc = launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
     if (rc != hipSuccess) return rc;
@@ -464,6 +463,18 @@ hipError_t launch_variant(const BackwardArgs &args, hipStream_t stream)
         rc = launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, true, false>, args, WAVES, lds, CAUSAL, false, stream);
         if (rc != hipSuccess) return rc;
         return launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, false, true>, args, WAVES, lds, CAUSAL, false, stream);
+    }
+}
+
+template <int DC, bool VEC, bool CAUSAL>
+hipError_t launch_variant(const BackwardArgs &args, hipStream_t stream)
+{
+    if constexpr (DC > 128) {
+        return launch_waves<DC, 2, VEC, CAUSAL>(args, stream);  // 64 KiB of tiles a wavefront
+    } else if constexpr (DC > 64) {
+        return static_cast<size_t>(args.contexts) * args.tiles >= 512 ? launch_waves<DC, 2, VEC, CAUSAL>(args, stream) : launch_waves<DC, 4, VEC, CAUSAL>(args, stream);
+    } else {
+        return launch_waves<DC, 4, VEC, CAUSAL>(args, stream);
     }
 }
 
