@@ -31,9 +31,10 @@ struct BackwardArgs {
     const float *q, *k, *v, *z_bias, *attn_bias, *out, *grad_out;
     float *grad_q, *grad_k, *grad_v, *grad_z_bias, *grad_attn_bias;
     float *lse, *delta;  // (contexts, padded): lse·log2 e; rows behind the last +infinity and 0
-    int contexts, S, D, padded, tiles, swizzle;
+    float *pairs;        // ds, (contexts, S, pair_row): grad_attn_bias, or scratch, or null where dq works it out again
+    int contexts, S, D, padded, tiles, swizzle, pair_row;
     float scale;
-    bool wide_bias;  // four neighbouring biases of a row are one aligned load
+    bool wide_bias, wide_pairs;  // four neighbouring values of a row are one aligned load
 };
 
 // Workgroup -> (context, tile), XCDs with whole contexts where they divide evenly; under a causal mask the longest tiles first.
@@ -99,10 +100,18 @@ __device__ __forceinline__ void wait_for_loads()
     __builtin_amdgcn_wave_barrier();
 }
 
-// Up to 32 rows of S biases, zeros behind the last: loads beyond them give 0, and stores are dropped.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t bias_rows(const float *first, int rows, int S)
+// Up to 32 rows of biases, or of ds, zeros behind the last: loads beyond them give 0, and stores are dropped.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bias_rows(const float *first, int rows, int row)
 {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(first), 0, static_cast<int>(static_cast<unsigned>(min(rows, kRows)) * S * 4u), 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(first), 0, static_cast<int>(static_cast<unsigned>(min(rows, kRows)) * row * 4u), 0x00020000);
+}
+__device__ __forceinline__ f32x4 bias4(const __amdgpu_buffer_rsrc_t &from, unsigned at, bool wide)
+{
+    if (wide) return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at * 4u, 0, 0));
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, (at + e) * 4u, 0, 0));
+    return x;
 }
 
 __device__ __forceinline__ f32x16 mfma(float a, float b, f32x16 sum) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, sum, 0, 0, 0); }
@@ -198,7 +207,7 @@ __device__ __forceinline__ void write_rows(const f32x16 (&sums)[DC / 32], float 
 }
 
 // ---- lse, δ, dq: queries stay -----------------------------------------------------------------------------------------------------------
-template <int DC, int WAVES, bool VEC, bool CAUSAL>
+template <int DC, int WAVES, bool VEC, bool CAUSAL, bool DQ>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <= 64 ? 2 : 1, 4))) void attention_f32_grad_q_kernel(BackwardArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char backward_lds[];
@@ -232,18 +241,11 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         f32x4 of_pair[4], of_key[4];
     };
     auto load_biases = [&](int key0, Biases &to) {
-        auto load = [&](const __amdgpu_buffer_rsrc_t &from, unsigned at) {
-            if (p.wide_bias) return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at * 4u, 0, 0));
-            f32x4 x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, (at + e) * 4u, 0, 0));
-            return x;
-        };
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
             const unsigned key = key0 + a * 8 + lh * 4;
-            if (p.attn_bias) to.of_pair[a] = load(biases, static_cast<unsigned>(li) * S + key);
-            if (p.z_bias) to.of_key[a] = load(z_biases, key);
+            if (p.attn_bias) to.of_pair[a] = bias4(biases, static_cast<unsigned>(li) * S + key, p.wide_bias);
+            if (p.z_bias) to.of_key[a] = bias4(z_biases, key, p.wide_bias);
         }
     };
     // the scores of a tile, in units of log2 e
@@ -287,9 +289,11 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     auto load_values = [&](int key0) {
         if (key0 < key_end) load_tile<DC, VEC>(v_rows, D, key0, v_tile, lane);
     };
-    wait_for_reads();
-    load_values(wave * kRows);
-    load_keys(wave * kRows);
+    if constexpr (DQ) {
+        wait_for_reads();
+        load_values(wave * kRows);
+        load_keys(wave * kRows);
+    }
     {
         const float other = __shfl_xor(most, 32), other_total = __shfl_xor(total, 32), top = fmaxf(most, other), safe = top == -INFINITY ? 0.0f : top;
         total = total * __builtin_amdgcn_exp2f(most - safe) + other_total * __builtin_amdgcn_exp2f(other - safe);
@@ -313,22 +317,59 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         p.lse[static_cast<size_t>(context) * p.padded + my_q] = lse;
         p.delta[static_cast<size_t>(context) * p.padded + my_q] = my_q < S ? delta : 0.0f;
     }
+    if constexpr (DQ) {
+        f32x16 dq[DC / 32];
+#pragma unroll
+        for (int dt = 0; dt < DC / 32; ++dt) dq[dt] = f32x16{};
+        for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
+            Biases with;
+            wait_for_loads();
+            load_biases(key0, with);
+            const f32x16 dp = product<DC>(v_tile, g, li, lh);
+            wait_for_reads();
+            load_values(key0 + WAVES * kRows);  // each tile's successor as soon as it has been read
+            f32x16 s = scores(k_tile, with, key0);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - lse) * (dp[r] - delta);
+            add_product<DC>(k_tile, s, dq, li, lh);
+            wait_for_reads();
+            load_keys(key0 + WAVES * kRows);
+        }
+        write_rows<DC, WAVES, VEC>(dq, p.scale, p.grad_q + first * D, q0, S, D, backward_lds);
+    }
+}
+
+// dq = scale·ds·k where the pass for dk and dv has left ds.
+template <int DC, int WAVES, bool VEC, bool CAUSAL>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <= 128 ? 2 : 1, 4))) void attention_f32_grad_q_of_pairs_kernel(BackwardArgs p)
+{
+    extern __shared__ __attribute__((aligned(16))) unsigned char backward_lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
+    const int2 item = decode(p.contexts, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
+    const int context = item.x, q0 = item.y * kRows, my_q = q0 + li, S = p.S, D = p.D;
+    const size_t first = static_cast<size_t>(context) * S;
+    const int key_end = CAUSAL ? min(S, q0 + kRows) : S, last_key = CAUSAL ? min(my_q, S - 1) : S - 1;
+    unsigned char *const tiles = backward_lds + wave * 2 * Tile<DC>::kBytes;  // they take turns
+    const __amdgpu_buffer_rsrc_t k_rows = rows_of(p.k + first * D, S, D), pairs = bias_rows(p.pairs + (first + q0) * p.pair_row, S - q0, p.pair_row);
+    f32x4 ds[4];
+    auto load = [&](int key0, int turn) {
+        if (key0 >= key_end) return;
+        load_tile<DC, VEC>(k_rows, D, key0, tiles + turn * Tile<DC>::kBytes, lane);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) ds[a] = bias4(pairs, static_cast<unsigned>(li) * p.pair_row + key0 + a * 8 + lh * 4, p.wide_pairs);
+    };
     f32x16 dq[DC / 32];
 #pragma unroll
     for (int dt = 0; dt < DC / 32; ++dt) dq[dt] = f32x16{};
-    for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
-        Biases with;
+    load(wave * kRows, 0);
+    for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
+        f32x16 weights;
         wait_for_loads();
-        load_biases(key0, with);
-        const f32x16 dp = product<DC>(v_tile, g, li, lh);
         wait_for_reads();
-        load_values(key0 + WAVES * kRows);  // each tile's successor as soon as it has been read
-        f32x16 s = scores(k_tile, with, key0);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - lse) * (dp[r] - delta);
-        add_product<DC>(k_tile, s, dq, li, lh);
-        wait_for_reads();
-        load_keys(key0 + WAVES * kRows);
+        for (int r = 0; r < 16; ++r) weights[r] = key0 + row_of(r) + 4 * lh > last_key ? 0.0f : ds[r >> 2][r & 3];
+        load(key0 + WAVES * kRows, turn ^ 1);
+        add_product<DC>(tiles + turn * Tile<DC>::kBytes, weights, dq, li, lh);
     }
     write_rows<DC, WAVES, VEC>(dq, p.scale, p.grad_q + first * D, q0, S, D, backward_lds);
 }
@@ -411,10 +452,11 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
                 dz += s[r];
             }
             add_product<DC>(q_tile, s, dk, li, lh);
-            if (p.grad_attn_bias) {
-                const __amdgpu_buffer_rsrc_t grads = bias_rows(p.grad_attn_bias + (first + row0) * S, S - row0, S);
+            if (p.pairs) {
+                const __amdgpu_buffer_rsrc_t pairs = bias_rows(p.pairs + (first + row0) * p.pair_row, S - row0, p.pair_row);
+                const unsigned to = my_key < S ? (4u * lh * p.pair_row + my_key) * 4u : 0x80000000u;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[r]), grads, at + row_of(r) * S * 4u, 0, 0);
+                for (int r = 0; r < 16; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[r]), pairs, to + row_of(r) * p.pair_row * 4u, 0, 0);
             }
         }
         wait_for_reads();
@@ -437,6 +479,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     if constexpr (DV) write_rows<DC, WAVES, VEC>(dv, 1.0f, p.grad_v + first * D, k0, S, D, backward_lds);
 }
 
+// Values of ds that are kept from dk's pass for dq's where nobody asked for them: 128 MiB.
+constexpr size_t kPairsKept = 32u << 20;
+
 template <class Kernel>
 hipError_t launch(Kernel kernel, const BackwardArgs &args, int waves, size_t lds, bool by_tile, bool last_first, hipStream_t stream)
 {
@@ -455,15 +500,18 @@ template <int DC, int WAVES, bool VEC, bool CAUSAL>
 hipError_t launch_waves(const BackwardArgs &args, hipStream_t stream)
 {
     constexpr size_t lds = std::max<size_t>(WAVES * 2 * Tile<DC>::kBytes, WAVES * kRows * (DC + 4) * sizeof(float));
-    hipError_t rc = launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
+    hipError_t rc = args.pairs ? launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL, false>, args, WAVES, lds, CAUSAL, CAUSAL, stream)
+                               : launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL, true>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
     if (rc != hipSuccess) return rc;
     if constexpr (DC <= 128) {
-        return launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, true, true>, args, WAVES, lds, CAUSAL, false, stream);
+        rc = launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, true, true>, args, WAVES, lds, CAUSAL, false, stream);
     } else {
         rc = launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, true, false>, args, WAVES, lds, CAUSAL, false, stream);
         if (rc != hipSuccess) return rc;
-        return launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, false, true>, args, WAVES, lds, CAUSAL, false, stream);
+        rc = launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, false, true>, args, WAVES, lds, CAUSAL, false, stream);
     }
+    if (rc != hipSuccess || !args.pairs) return rc;
+    return launch(attention_f32_grad_q_of_pairs_kernel<DC, WAVES, VEC, CAUSAL>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
 }
 
 template <int DC, bool VEC, bool CAUSAL>
@@ -513,11 +561,15 @@ hipError_t launch_attention_backward_f32(size_t contexts, size_t sequence, size_
     args.scale = scale;
     auto aligned = [](const void *at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; };
     args.wide_bias = sequence % 4 == 0 && aligned(attn_bias) && aligned(z_bias);
-    const size_t rows = contexts * args.padded;
+    const size_t rows = contexts * args.padded, pair_row = grad_attn_bias ? sequence : (sequence + 3) / 4 * 4;
+    const size_t kept = !grad_attn_bias && contexts * sequence * pair_row <= kPairsKept ? contexts * sequence * pair_row : 0;
     void *scratch = nullptr;
-    const hipError_t rc = stream_workspace(stream, 2 * rows * sizeof(float), &scratch);
+    const hipError_t rc = stream_workspace(stream, (kept + 2 * rows) * sizeof(float), &scratch);
     if (rc != hipSuccess) return rc;
-    args.lse = static_cast<float *>(scratch);
+    args.pairs = grad_attn_bias ? grad_attn_bias : kept ? static_cast<float *>(scratch) : nullptr;
+    args.pair_row = static_cast<int>(pair_row);
+    args.wide_pairs = pair_row % 4 == 0 && aligned(args.pairs);
+    args.lse = static_cast<float *>(scratch) + kept;
     args.delta = args.lse + rows;
     const bool vec = head_dim % 4 == 0 && aligned(q) && aligned(k) && aligned(v) && aligned(out) && aligned(grad_out) &&
                      aligned(grad_q) && aligned(grad_k) && aligned(grad_v);
