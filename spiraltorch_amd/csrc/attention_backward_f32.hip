@@ -45,13 +45,11 @@ __host__ __device__ inline int2 decode(int contexts, int tiles, int swizzle, boo
     return int2{static_cast<int>(first + (by_tile ? i % of_xcd : i / n)), static_cast<int>(last_first ? n - 1 - tile : tile)};
 }
 
-// A tile of 32 rows of DC values (a multiple of 32; zeros from D on) in LDS, its 16-byte chunks turned by the row: sixteen rows' same chunk lies
-// in sixteen places of the banks.
+// A tile of 32 rows of DC values (a multiple of 16; zeros from D on) in LDS.  A row is an odd number of 16-byte chunks, the last of them empty: sixteen
+// rows' same chunk lies in sixteen places of the banks, and where a value lies is a lane's place and a constant.
 template <int DC>
 struct Tile {
-    static constexpr int kWide = DC <= 32 ? 32 : DC <= 64 ? 64 : DC <= 128 ? 128 : 256;
-    static constexpr int kRow = kWide * 4, kBytes = kRows * kRow, kTurn = kWide / 4 < 16 ? kWide / 4 - 1 : 15;
-    static __device__ __forceinline__ unsigned place(unsigned row, unsigned chunk) { return row * kRow + (chunk ^ (row & kTurn)) * 16; }
+    static constexpr int kChunks = DC / 4 + 1, kRow = kChunks * 16, kBytes = (kRows * kChunks + 63) / 64 * 1024, kAcross = (DC + 31) / 32;
 };
 
 // Rows of a context, zeros behind the last.
@@ -86,9 +84,8 @@ __device__ __forceinline__ void load_tile(const __amdgpu_buffer_rsrc_t &rows, in
     asm volatile("" : "+v"(lane));  // (the places are worked out every time: kept for all steps, they would be registers the products need)
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        const unsigned at = (s * 64 + lane) * SIZE, row = at / Tile<DC>::kRow, chunk = (at % Tile<DC>::kRow / 16) ^ (row & Tile<DC>::kTurn);
-        const unsigned column = chunk * 4 + at % 16 / 4;
-        const unsigned from = column < static_cast<unsigned>(dim) ? ((first + row) * static_cast<unsigned>(dim) + column) * 4u : 0x80000000u;
+        const unsigned at = (s * 64 + lane) * SIZE, row = at / Tile<DC>::kRow, column = at % Tile<DC>::kRow / 4;
+        const unsigned from = column < static_cast<unsigned>(dim) && row < kRows ? ((first + row) * static_cast<unsigned>(dim) + column) * 4u : 0x80000000u;
         if (VEC) __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (lds_void_ptr)(to + s * 64 * SIZE), 16, from, 0, 0, 0);
         else __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (lds_void_ptr)(to + s * 64 * SIZE), 4, from, 0, 0, 0);
     }
@@ -126,7 +123,8 @@ __device__ __forceinline__ f32x16 product(const unsigned char *tile, const f32x4
     constexpr int AHEAD = 2;
     f32x16 sum = {};
     f32x4 ring[AHEAD];
-    auto load = [&](int g) { ring[g % AHEAD] = *reinterpret_cast<const f32x4 *>(tile + Tile<DC>::place(li, 2 * g + lh)); };
+    const unsigned char *const mine = tile + li * Tile<DC>::kRow + lh * 16;
+    auto load = [&](int g) { ring[g % AHEAD] = *reinterpret_cast<const f32x4 *>(mine + g * 32); };
 #pragma unroll
     for (int g = 0; g < AHEAD; ++g) load(g);
 #pragma unroll
@@ -141,16 +139,12 @@ __device__ __forceinline__ f32x16 product(const unsigned char *tile, const f32x4
 }
 // sums += tileᵀ · weights: registers are the tile's columns, lanes the rows that stay.
 template <int DC>
-__device__ __forceinline__ void add_product(const unsigned char *tile, const f32x16 &weights, f32x16 (&sums)[DC / 32], int li, int lh)
+__device__ __forceinline__ void add_product(const unsigned char *tile, const f32x16 &weights, f32x16 (&sums)[Tile<DC>::kAcross], int li, int lh)
 {
-    constexpr int AHEAD = 8, DT = DC / 32, STEPS = 16 * DT;
-    const unsigned base = ((li >> 2) ^ (4 * lh)) * 16 + (li & 3) * 4 + 4 * lh * Tile<DC>::kRow;
+    constexpr int AHEAD = 8, DT = Tile<DC>::kAcross, STEPS = 16 * DT;
+    const unsigned char *const mine = tile + 4 * lh * Tile<DC>::kRow + li * 4;
     float ring[AHEAD];
-    auto load = [&](int n) {
-        const int row = row_of(n / DT);
-        const unsigned turn = ((n % DT * 8) ^ (row & Tile<DC>::kTurn)) * 16;
-        ring[n % AHEAD] = *reinterpret_cast<const float *>(tile + (base ^ turn) + row * Tile<DC>::kRow);
-    };
+    auto load = [&](int n) { ring[n % AHEAD] = *reinterpret_cast<const float *>(mine + row_of(n / DT) * Tile<DC>::kRow + n % DT * 128); };
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) load(n);
 #pragma unroll
@@ -172,14 +166,14 @@ __device__ __forceinline__ void wait_for_reads()
 
 // The wavefronts' sums (a lane has its row, registers the columns), times `by`, into rows first .. first + 31 of a matrix.
 template <int DC, int WAVES, bool VEC>
-__device__ __forceinline__ void write_rows(const f32x16 (&sums)[DC / 32], float by, float *to, int first, int rows, int dim, unsigned char *lds)
+__device__ __forceinline__ void write_rows(const f32x16 (&sums)[Tile<DC>::kAcross], float by, float *to, int first, int rows, int dim, unsigned char *lds)
 {
-    constexpr int STRIDE = DC + 4;
+    constexpr int STRIDE = Tile<DC>::kAcross * 32 + 4;
     float *const parts = reinterpret_cast<float *>(lds);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, lh = lane >> 5;
     __syncthreads();
 #pragma unroll
-    for (int dt = 0; dt < DC / 32; ++dt)
+    for (int dt = 0; dt < Tile<DC>::kAcross; ++dt)
 #pragma unroll
         for (int a = 0; a < 4; ++a)
             *reinterpret_cast<f32x4 *>(parts + (wave * kRows + li) * STRIDE + dt * 32 + a * 8 + lh * 4) =
@@ -318,9 +312,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         p.delta[static_cast<size_t>(context) * p.padded + my_q] = my_q < S ? delta : 0.0f;
     }
     if constexpr (DQ) {
-        f32x16 dq[DC / 32];
+        f32x16 dq[Tile<DC>::kAcross];
 #pragma unroll
-        for (int dt = 0; dt < DC / 32; ++dt) dq[dt] = f32x16{};
+        for (int dt = 0; dt < Tile<DC>::kAcross; ++dt) dq[dt] = f32x16{};
         for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
             Biases with;
             wait_for_loads();
@@ -358,9 +352,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
 #pragma unroll
         for (int a = 0; a < 4; ++a) ds[a] = bias4(pairs, static_cast<unsigned>(li) * p.pair_row + key0 + a * 8 + lh * 4, p.wide_pairs);
     };
-    f32x16 dq[DC / 32];
+    f32x16 dq[Tile<DC>::kAcross];
 #pragma unroll
-    for (int dt = 0; dt < DC / 32; ++dt) dq[dt] = f32x16{};
+    for (int dt = 0; dt < Tile<DC>::kAcross; ++dt) dq[dt] = f32x16{};
     load(wave * kRows, 0);
     for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
         f32x16 weights;
@@ -406,13 +400,13 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         }
     }
     const float z = p.z_bias && my_key < S ? p.z_bias[first + my_key] : 0.0f;
-    f32x16 dk[DK ? DC / 32 : 1], dv[DV ? DC / 32 : 1];
+    f32x16 dk[DK ? Tile<DC>::kAcross : 1], dv[DV ? Tile<DC>::kAcross : 1];
     if (DK)
 #pragma unroll
-        for (int dt = 0; dt < DC / 32; ++dt) dk[DK ? dt : 0] = f32x16{};
+        for (int dt = 0; dt < Tile<DC>::kAcross; ++dt) dk[DK ? dt : 0] = f32x16{};
     if (DV)
 #pragma unroll
-        for (int dt = 0; dt < DC / 32; ++dt) dv[DV ? dt : 0] = f32x16{};
+        for (int dt = 0; dt < Tile<DC>::kAcross; ++dt) dv[DV ? dt : 0] = f32x16{};
     float dz = 0.0f;
     if (CAUSAL && DK && p.grad_attn_bias && my_key < S)  // queries before the tile do not see it
         for (int q = wave * 2 + lh; q < k0; q += WAVES * 2) p.grad_attn_bias[(first + q) * S + my_key] = 0.0f;
@@ -479,8 +473,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     if constexpr (DV) write_rows<DC, WAVES, VEC>(dv, 1.0f, p.grad_v + first * D, k0, S, D, backward_lds);
 }
 
-// Values of ds that are kept from dk's pass for dq's where nobody asked for them: 128 MiB.
-constexpr size_t kPairsKept = 32u << 20;
+// Values of ds that are kept from dk's pass for dq's where nobody asked for them: 256 MiB.
+constexpr size_t kPairsKept = 64u << 20;
 
 template <class Kernel>
 hipError_t launch(Kernel kernel, const BackwardArgs &args, int waves, size_t lds, bool by_tile, bool last_first, hipStream_t stream)
@@ -499,7 +493,7 @@ hipError_t launch(Kernel kernel, const BackwardArgs &args, int waves, size_t lds
 template <int DC, int WAVES, bool VEC, bool CAUSAL>
 hipError_t launch_waves(const BackwardArgs &args, hipStream_t stream)
 {
-    constexpr size_t lds = std::max<size_t>(WAVES * 2 * Tile<DC>::kBytes, WAVES * kRows * (DC + 4) * sizeof(float));
+    constexpr size_t lds = std::max<size_t>(WAVES * 2 * Tile<DC>::kBytes, WAVES * kRows * (Tile<DC>::kAcross * 32 + 4) * sizeof(float));
     hipError_t rc = args.pairs ? launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL, false>, args, WAVES, lds, CAUSAL, CAUSAL, stream)
                                : launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL, true>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
     if (rc != hipSuccess) return rc;
@@ -520,7 +514,7 @@ hipError_t launch_variant(const BackwardArgs &args, hipStream_t stream)
     if constexpr (DC > 128) {
         return launch_waves<DC, 2, VEC, CAUSAL>(args, stream);  // 64 KiB of tiles a wavefront
     } else if constexpr (DC > 64) {
-        return static_cast<size_t>(args.contexts) * args.tiles >= 512 ? launch_waves<DC, 2, VEC, CAUSAL>(args, stream) : launch_waves<DC, 4, VEC, CAUSAL>(args, stream);
+        return static_cast<size_t>(args.contexts) * args.tiles >= (CAUSAL ? 768 : 2048) ? launch_waves<DC, 2, VEC, CAUSAL>(args, stream) : launch_waves<DC, 4, VEC, CAUSAL>(args, stream);
     } else {
         return launch_waves<DC, 4, VEC, CAUSAL>(args, stream);
     }
@@ -575,6 +569,7 @@ hipError_t launch_attention_backward_f32(size_t contexts, size_t sequence, size_
                      aligned(grad_q) && aligned(grad_k) && aligned(grad_v);
     if (head_dim <= 32) return launch_width<32>(args, vec, causal, stream);
     if (head_dim <= 64) return launch_width<64>(args, vec, causal, stream);
+    if (head_dim <= 80) return launch_width<80>(args, vec, causal, stream);
     if (head_dim <= 96) return launch_width<96>(args, vec, causal, stream);
     if (head_dim <= 128) return launch_width<128>(args, vec, causal, stream);
     return launch_width<256>(args, vec, causal, stream);
