@@ -14,6 +14,7 @@
 // wavefront before the end.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "device_math.h"
 #include "kernels.h"
@@ -75,21 +76,46 @@ __device__ __forceinline__ f32x4 fetch4(const __amdgpu_buffer_rsrc_t &rows, int 
 }
 
 typedef __attribute__((address_space(3))) void *lds_void_ptr;
-// A tile on its way straight into LDS, 16 bytes (VEC) or 4 a lane: what lies at a place is fetched by the lane that stands for it.  Rows behind the
-// last and columns from `dim` on are beyond the descriptor, and zeros.
-template <int DC, bool VEC>
-__device__ __forceinline__ void load_tile(const __amdgpu_buffer_rsrc_t &rows, int dim, int first, unsigned char *to, int lane)
+typedef __attribute__((address_space(3))) void *lds_void_ptr;
+// Rows first .. first + 31 of a context's `rows` on their way straight into LDS, 16 bytes (VEC) or 4 a lane and step: what lies at a place is fetched by
+// the lane that stands for it, from beyond the descriptor (zeros) where it stands for no value.  The matrix instructions wait for what a wavefront
+// computes between them, so that wide loads find where a step's values come from in a table in LDS, which a wavefront writes with its FIRST tile (every
+// one writes the same, so that none waits for another).
+template <int DC, bool VEC, bool FIRST>
+__device__ __forceinline__ void load_tile(const float *matrix, int rows, int dim, int first, unsigned char *to, unsigned char *places, int lane)
 {
     constexpr int SIZE = VEC ? 16 : 4, STEPS = Tile<DC>::kBytes / (64 * SIZE);
-    asm volatile("" : "+v"(lane));  // (the places are worked out every time: kept for all steps, they would be registers the products need)
+    constexpr unsigned OF_ROW = Tile<DC>::kRow / SIZE, DOWN = 64 / OF_ROW, ACROSS = 64 % OF_ROW * (SIZE / 4);
+    const __amdgpu_buffer_rsrc_t from = rows_of(matrix + static_cast<size_t>(first) * dim, min(rows - first, kRows), dim);
+    asm volatile("" : "+v"(lane));  // (kept for all steps, the places would be registers the products need)
+    unsigned row = lane / OF_ROW, column = lane % OF_ROW * (SIZE / 4);
+    unsigned *const table = reinterpret_cast<unsigned *>(places) + lane;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        const unsigned at = (s * 64 + lane) * SIZE, row = at / Tile<DC>::kRow, column = at % Tile<DC>::kRow / 4;
-        const unsigned from = column < static_cast<unsigned>(dim) && row < kRows ? ((first + row) * static_cast<unsigned>(dim) + column) * 4u : 0x80000000u;
-        if (VEC) __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (lds_void_ptr)(to + s * 64 * SIZE), 16, from, 0, 0, 0);
-        else __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, (lds_void_ptr)(to + s * 64 * SIZE), 4, from, 0, 0, 0);
+        unsigned at;
+        if (VEC && !FIRST) {
+            at = table[s * 64];
+        } else {
+            at = column < static_cast<unsigned>(dim) && row < kRows ? (row * static_cast<unsigned>(dim) + column) * 4u : 0x80000000u;
+            if (VEC) table[s * 64] = at;
+            row += DOWN;
+            column += ACROSS;
+            if (column >= OF_ROW * (SIZE / 4)) {
+                row += 1;
+                column -= OF_ROW * (SIZE / 4);
+            }
+        }
+        if (VEC) __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void_ptr)(to + s * 64 * SIZE), 16, at, 0, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void_ptr)(to + s * 64 * SIZE), 4, at, 0, 0, 0);
+    }
+    if (VEC && FIRST) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
+template <int DC, bool VEC>
+constexpr size_t kPlaces = VEC ? Tile<DC>::kBytes / 4 : 0;  // bytes of the table
+
 __device__ __forceinline__ void wait_for_loads()
 {
     __builtin_amdgcn_s_waitcnt(0x0f70);
@@ -211,9 +237,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     const int context = item.x, q0 = item.y * kRows, my_q = q0 + li, S = p.S, D = p.D;
     const size_t first = static_cast<size_t>(context) * S;
     unsigned char *const k_tile = backward_lds + wave * 2 * Tile<DC>::kBytes, *const v_tile = k_tile + Tile<DC>::kBytes;
-    const __amdgpu_buffer_rsrc_t k_rows = rows_of(p.k + first * D, S, D), v_rows = rows_of(p.v + first * D, S, D);
+    unsigned char *const places = backward_lds + WAVES * 2 * Tile<DC>::kBytes;
     const int key_end = CAUSAL ? min(S, q0 + kRows) : S, last_key = CAUSAL ? min(my_q, S - 1) : S - 1;
-    if (wave * kRows < key_end) load_tile<DC, VEC>(k_rows, D, wave * kRows, k_tile, lane);
+    if (wave * kRows < key_end) load_tile<DC, VEC, true>(p.k + first * D, S, D, wave * kRows, k_tile, places, lane);
     f32x4 q[DC / 8], g[DC / 8];
     float delta = 0.0f;
     {
@@ -266,7 +292,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         wait_for_loads();
         wait_for_reads();
         load_biases(key0, with);
-        if (key0 + WAVES * kRows < key_end) load_tile<DC, VEC>(k_rows, D, key0 + WAVES * kRows, turn ? k_tile : v_tile, lane);
+        if (key0 + WAVES * kRows < key_end) load_tile<DC, VEC, false>(p.k + first * D, S, D, key0 + WAVES * kRows, turn ? k_tile : v_tile, places, lane);
         const f32x16 s = scores(turn ? v_tile : k_tile, with, key0);
         float top = most;
 #pragma unroll
@@ -278,10 +304,10 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         for (int r = 0; r < 16; ++r) total += __builtin_amdgcn_exp2f(s[r] - safe);
     }
     auto load_keys = [&](int key0) {
-        if (key0 < key_end) load_tile<DC, VEC>(k_rows, D, key0, k_tile, lane);
+        if (key0 < key_end) load_tile<DC, VEC, false>(p.k + first * D, S, D, key0, k_tile, places, lane);
     };
     auto load_values = [&](int key0) {
-        if (key0 < key_end) load_tile<DC, VEC>(v_rows, D, key0, v_tile, lane);
+        if (key0 < key_end) load_tile<DC, VEC, false>(p.v + first * D, S, D, key0, v_tile, places, lane);
     };
     if constexpr (DQ) {
         wait_for_reads();
@@ -344,25 +370,26 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     const size_t first = static_cast<size_t>(context) * S;
     const int key_end = CAUSAL ? min(S, q0 + kRows) : S, last_key = CAUSAL ? min(my_q, S - 1) : S - 1;
     unsigned char *const tiles = backward_lds + wave * 2 * Tile<DC>::kBytes;  // they take turns
-    const __amdgpu_buffer_rsrc_t k_rows = rows_of(p.k + first * D, S, D), pairs = bias_rows(p.pairs + (first + q0) * p.pair_row, S - q0, p.pair_row);
+    unsigned char *const places = backward_lds + WAVES * 2 * Tile<DC>::kBytes;
+    const __amdgpu_buffer_rsrc_t pairs = bias_rows(p.pairs + (first + q0) * p.pair_row, S - q0, p.pair_row);
     f32x4 ds[4];
-    auto load = [&](int key0, int turn) {
+    auto load = [&](auto starts, int key0, int turn) {
         if (key0 >= key_end) return;
-        load_tile<DC, VEC>(k_rows, D, key0, tiles + turn * Tile<DC>::kBytes, lane);
+        load_tile<DC, VEC, decltype(starts)::value>(p.k + first * D, S, D, key0, tiles + turn * Tile<DC>::kBytes, places, lane);
 #pragma unroll
         for (int a = 0; a < 4; ++a) ds[a] = bias4(pairs, static_cast<unsigned>(li) * p.pair_row + key0 + a * 8 + lh * 4, p.wide_pairs);
     };
     f32x16 dq[Tile<DC>::kAcross];
 #pragma unroll
     for (int dt = 0; dt < Tile<DC>::kAcross; ++dt) dq[dt] = f32x16{};
-    load(wave * kRows, 0);
+    load(std::true_type{}, wave * kRows, 0);
     for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
         f32x16 weights;
         wait_for_loads();
         wait_for_reads();
 #pragma unroll
         for (int r = 0; r < 16; ++r) weights[r] = key0 + row_of(r) + 4 * lh > last_key ? 0.0f : ds[r >> 2][r & 3];
-        load(key0 + WAVES * kRows, turn ^ 1);
+        load(std::false_type{}, key0 + WAVES * kRows, turn ^ 1);
         add_product<DC>(tiles + turn * Tile<DC>::kBytes, weights, dq, li, lh);
     }
     write_rows<DC, WAVES, VEC>(dq, p.scale, p.grad_q + first * D, q0, S, D, backward_lds);
@@ -380,15 +407,15 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     const int context = item.x, k0 = item.y * kRows, my_key = k0 + li, S = p.S, D = p.D;
     const size_t first = static_cast<size_t>(context) * S;
     unsigned char *const q_tile = backward_lds + wave * 2 * Tile<DC>::kBytes, *const g_tile = q_tile + Tile<DC>::kBytes;
-    const __amdgpu_buffer_rsrc_t q_rows = rows_of(p.q + first * D, S, D), g_rows = rows_of(p.grad_out + first * D, S, D);
-    auto load_queries = [&](int row0) {
-        if (row0 < S) load_tile<DC, VEC>(q_rows, D, row0, q_tile, lane);
+    unsigned char *const places = backward_lds + WAVES * 2 * Tile<DC>::kBytes;
+    auto load_queries = [&](auto starts, int row0) {
+        if (row0 < S) load_tile<DC, VEC, decltype(starts)::value>(p.q + first * D, S, D, row0, q_tile, places, lane);
     };
     auto load_grads = [&](int row0) {
-        if (row0 < S) load_tile<DC, VEC>(g_rows, D, row0, g_tile, lane);
+        if (row0 < S) load_tile<DC, VEC, false>(p.grad_out + first * D, S, D, row0, g_tile, places, lane);
     };
     const int start = (CAUSAL ? k0 : 0) + wave * kRows;
-    load_queries(start);
+    load_queries(std::true_type{}, start);
     load_grads(start);
     f32x4 k[DC / 8], v[DK ? DC / 8 : 1];
     {
@@ -454,7 +481,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
             }
         }
         wait_for_reads();
-        load_queries(row0 + WAVES * kRows);
+        load_queries(std::false_type{}, row0 + WAVES * kRows);
     }
     if constexpr (DK) {
         if (p.grad_z_bias) {
@@ -493,7 +520,7 @@ hipError_t launch(Kernel kernel, const BackwardArgs &args, int waves, size_t lds
 template <int DC, int WAVES, bool VEC, bool CAUSAL>
 hipError_t launch_waves(const BackwardArgs &args, hipStream_t stream)
 {
-    constexpr size_t lds = std::max<size_t>(WAVES * 2 * Tile<DC>::kBytes, WAVES * kRows * (Tile<DC>::kAcross * 32 + 4) * sizeof(float));
+    constexpr size_t lds = std::max<size_t>(WAVES * 2 * Tile<DC>::kBytes + kPlaces<DC, VEC>, WAVES * kRows * (Tile<DC>::kAcross * 32 + 4) * sizeof(float));
     hipError_t rc = args.pairs ? launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL, false>, args, WAVES, lds, CAUSAL, CAUSAL, stream)
                                : launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL, true>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
     if (rc != hipSuccess) return rc;
