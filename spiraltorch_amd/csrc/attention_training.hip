@@ -584,9 +584,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BIAS && D =
 }
 
 // The table's gradient: a workgroup adds the workgroups' sums for the distances of one bucket and head, in an order of its own.
-__global__ __launch_bounds__(256) void position_bias_grad_kernel(const float *partial, float *grad_table, int batch, int heads, int tiles, Buckets buckets)
+constexpr int kTableThreads = 1024;
+__global__ __launch_bounds__(kTableThreads) void position_bias_grad_kernel(const float *partial, float *grad_table, int batch, int heads, int tiles, Buckets buckets)
 {
-    __shared__ float sums[4];
+    __shared__ float sums[kTableThreads / 64];
     const int bucket = blockIdx.x / heads, h = blockIdx.x % heads, far = buckets.far, width = distances_of(far);
     const bool behind = buckets.bidirectional && bucket >= buckets.side;
     const int j = behind ? bucket - buckets.side : bucket;
@@ -601,7 +602,7 @@ __global__ __launch_bounds__(256) void position_bias_grad_kernel(const float *pa
     while (wide < 16 && wide < run) wide *= 2;
     float sum = 0.0f;
     const int distance = threadIdx.x % wide;
-    for (int part = threadIdx.x / wide; part < parts; part += 256 / wide) {
+    for (int part = threadIdx.x / wide; part < parts; part += kTableThreads / wide) {
         const size_t context = static_cast<size_t>(part / tiles) * heads + h;
         const float *const from = partial + (context * tiles + part % tiles) * width + first + far + kMargin;
 #pragma unroll 8
@@ -610,7 +611,12 @@ __global__ __launch_bounds__(256) void position_bias_grad_kernel(const float *pa
     sum = wave_sum(sum);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) grad_table[static_cast<size_t>(bucket) * heads + h] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    if (threadIdx.x == 0) {
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kTableThreads / 64; ++w) sum += sums[w];
+        grad_table[static_cast<size_t>(bucket) * heads + h] = sum;
+    }
 }
 
 // ---- backward: dk, dv ---------------------------------------------------------------------------------------------------------------
@@ -968,7 +974,7 @@ hipError_t launch_attention_backward_bf16(const st_hip_attention_training &shape
     args.ld_grad_kv = static_cast<unsigned>(ld_grad_kv);
     const bool biased = shape.position_bias != nullptr;
     auto add_up = [&](const float *partial, size_t tiles) {
-        hipLaunchKernelGGL(position_bias_grad_kernel, dim3(static_cast<unsigned>(args.buckets.count * args.heads)), dim3(256), 0, stream, partial, grad_table,
+        hipLaunchKernelGGL(position_bias_grad_kernel, dim3(static_cast<unsigned>(args.buckets.count * args.heads)), dim3(kTableThreads), 0, stream, partial, grad_table,
                            args.batch, args.heads, static_cast<int>(tiles), args.buckets);
         return hipGetLastError();
     };
