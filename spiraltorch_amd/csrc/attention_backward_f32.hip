@@ -3,15 +3,22 @@
 //
 //   p = exp(s − lse),  dv = pᵀ·g,  ds = p·(g·vᵀ − δ) with δ = Σ g·o,  dq = scale·ds·k,  dk = scale·dsᵀ·q,  dattn = ds,  dz = Σ_query ds
 //
-// Products run on v_mfma_f32_32x32x2_f32, whose 157 TFLOP/s bound the pass: eight products of 2·S²·D against the five that it cannot do
-// without (the scores once for lse, which the forward pass does not keep, and scores and g·vᵀ twice, for dq and for dk and dv).  That
-// instruction takes a value a lane from either operand, so that one copy of a tile in LDS serves rows and columns alike, and accumulators
+// Products run on v_mfma_f32_32x32x2_f32, whose 157 TFLOP/s bound the pass, and on nothing narrower: the operands are f32, and gradients of bf16
+// products would not be this function's.  Six products of 2·S²·D against the five that it cannot do without: the scores twice, once for lse,
+// which the forward pass does not keep.  One launch works out lse and δ; one dk, dv and the biases' gradients, and leaves ds; one takes dq from
+// ds.  Where nobody asks for ds (attn_bias's gradient) and it is above kPairsKept, the first launch works out dq as well, with eight products.
+// That instruction takes a value a lane from either operand, so that one copy of a tile in LDS serves rows and columns alike, and accumulators
 // go into the next product register by register.
 //
 // A workgroup owns 32 rows (queries for dq, keys for dk and dv), which its wavefronts all hold as B operands; they deal the tiles of 32
 // rows of the other two matrices out among themselves (wavefront w takes tiles w, w + WAVES, ...), each through LDS of its own, and add
 // up through LDS at the end, in the order of the wavefronts.  So 16 contexts of 1024 are 512 workgroups, and nothing waits for another
-// wavefront before the end.
+// wavefront before the end.  No atomics: the same call gives the same bits.
+//
+// 16 contexts of 1024 x 64 with both biases and all five gradients take 143 µs in three launches (44, 91, 29 µs by themselves), 75 TFLOP/s of
+// needed products where a large library product reaches 154; 96 causal ones of 333 x 80 take 109 µs.  What is left: with the rows that stay, the
+// sums and a tile's scores in registers there are two wavefronts a SIMD (one above 64 values a head), and the softmax's instructions and a
+// tile's wait stand beside the products only where the other wavefront has some.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -500,7 +507,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     if constexpr (DV) write_rows<DC, WAVES, VEC>(dv, 1.0f, p.grad_v + first * D, k0, S, D, backward_lds);
 }
 
-// Values of ds that are kept from dk's pass for dq's where nobody asked for them: 256 MiB.
+// Values of ds that are kept from dk's pass for dq's where nobody asked for them: 256 MiB, as much as the last-level cache holds.  Kept and worked out
+// again: 16 contexts of 1024 x 64 145 and 170 µs, 4 of 2048 x 80 217 and 270, 96 causal ones of 333 x 80 134 and 139.
 constexpr size_t kPairsKept = 64u << 20;
 
 template <class Kernel>
@@ -541,7 +549,11 @@ hipError_t launch_variant(const BackwardArgs &args, hipStream_t stream)
     if constexpr (DC > 128) {
         return launch_waves<DC, 2, VEC, CAUSAL>(args, stream);  // 64 KiB of tiles a wavefront
     } else if constexpr (DC > 64) {
-        return static_cast<size_t>(args.contexts) * args.tiles >= (CAUSAL ? 768 : 2048) ? launch_waves<DC, 2, VEC, CAUSAL>(args, stream) : launch_waves<DC, 4, VEC, CAUSAL>(args, stream);
+        // One wavefront a SIMD: two workgroups of two a compute unit cover each other's waits where there are enough of them, and a causal mask's
+        // uneven ones even out (longest first).  Two and four wavefronts: 96 causal contexts of 333 x 80 (1056 workgroups) 134 and 151 µs, 48
+        // (528) 93 and 92; 64 of 1024 x 128 without a mask (2048) 1375 and 1432, 96 of 333 x 96 (1056) 269 and 246.
+        const bool many = static_cast<size_t>(args.contexts) * args.tiles >= (CAUSAL ? 768 : 2048);
+        return many ? launch_waves<DC, 2, VEC, CAUSAL>(args, stream) : launch_waves<DC, 4, VEC, CAUSAL>(args, stream);
     } else {
         return launch_waves<DC, 4, VEC, CAUSAL>(args, stream);
     }

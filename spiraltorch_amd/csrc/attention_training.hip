@@ -187,11 +187,14 @@ __device__ __forceinline__ void fill_bias(const TrainingArgs &p, int head, float
     }
 }
 
-// The sequence that is taken as the `place`-th: of a padded batch of up to 64, in the order of their lengths, the longest first, as those that begin
-// last are what the launch waits for.
+// The sequence that is taken as the `place`-th: of a padded batch of up to 64 without a causal mask, in the order of their lengths, the longest
+// first, as those that begin last are what the launch waits for: a pass over 8 sequences of 90 to 1500 tokens on 12 heads of 64 takes 152 µs so
+// against 178 in the order given, 16 of 200 to 512 120 against 127.  Under a causal mask the longest tiles run first anyhow (32 of 64 to 1024 on
+// 8 heads: 135 sorted, 131 not).
+template <bool CAUSAL>
 __device__ __forceinline__ int sequence_at(const TrainingArgs &p, int place, int lane)
 {
-    if (!p.lengths || p.batch > 64) return place;
+    if (CAUSAL || !p.lengths || p.batch > 64) return place;
     const int mine = lane < p.batch ? min(max(p.lengths[lane], 0), p.S) : -1;
     int before = 0;
     for (int j = 0; j < p.batch; ++j) {
@@ -233,7 +236,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4))) voi
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
 
     const Item item = decode(p.batch * p.kv_heads, p.group, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
-    const int b = sequence_at(p, item.context / p.heads, lane), h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
+    const int b = sequence_at<CAUSAL>(p, item.context / p.heads, lane), h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
     const size_t context = static_cast<size_t>(b) * p.heads + h;
     const int length = length_of(p, b);
     uint16_t *const out_row = p.out + (static_cast<size_t>(b) * p.S + my_q) * p.ld_out + static_cast<size_t>(h) * D;
@@ -389,7 +392,7 @@ __device__ __forceinline__ void grad_q(const TrainingArgs &p, unsigned char *tra
     float *const bins = all_bins + wave * width;
 
     const Item item = decode(p.batch * p.kv_heads, p.group, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
-    const int b = sequence_at(p, item.context / p.heads, lane), h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
+    const int b = sequence_at<CAUSAL>(p, item.context / p.heads, lane), h = item.context % p.heads, q0 = item.tile * kStay, wq0 = q0 + wave * 32, my_q = wq0 + li;
     const size_t context = static_cast<size_t>(b) * p.heads + h;
     const int length = length_of(p, b);
     const bool to_table = BIAS && p.partial != nullptr;
@@ -630,7 +633,7 @@ __device__ __forceinline__ void grad_kv(const TrainingArgs &p, unsigned char *tr
 
     const Item item = decode(p.batch * p.kv_heads, 1, p.tiles * p.parts, p.swizzle, CAUSAL, false, blockIdx.x);
     const int tile = item.tile / p.parts, part = item.tile % p.parts;
-    const int b = sequence_at(p, item.context / p.kv_heads, lane), kv_head = item.context % p.kv_heads, k0 = tile * kStay, wk0 = k0 + wave * 32, my_key = wk0 + li;
+    const int b = sequence_at<CAUSAL>(p, item.context / p.kv_heads, lane), kv_head = item.context % p.kv_heads, k0 = tile * kStay, wk0 = k0 + wave * 32, my_key = wk0 + li;
     const int length = length_of(p, b);
     const size_t grad_at = (static_cast<size_t>(b) * p.S + my_key) * p.ld_grad_kv + static_cast<size_t>(kv_head) * D;
     if (k0 >= length) {

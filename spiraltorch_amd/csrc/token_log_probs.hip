@@ -3,7 +3,10 @@
 //   lse = log Σ e^x,  log p = x − lse,  H = −Σ p log p = log L − T / L  with  L = Σ e^(x−m),  T = Σ e^(x−m)·(x − m),  m = max x
 //   dx = g·([x is the token's] − p) − h·p·(log p + H)   for gradients g of the token's log p and h of H
 //
-// Memory bounds both: the forward pass reads the logits once, with the running maximum, L and T in every thread (f32), and collects the
+// Memory bounds both where there are many rows (8192 of 50001 in bf16: forward 819 MB in 199 µs, 4.1 TB/s, backward 1.64 GB in 325 µs, 5.0 TB/s;
+// a copy reaches 4.9), latency where there are few (one row of 131072 with the first 20: 11.7 µs, of which 8.7 the parts and 3 putting them
+// together; a workgroup that finds itself the last of its row and does that at once takes longer, 44 µs, for the fences between the
+// chip's caches).  The forward pass reads the logits once, with the running maximum, L and T in every thread (f32), and collects the
 // likeliest alternatives on the way; the backward pass reads them once and writes once.  A value stands for itself in an integer key
 // (order of the value, then the lower index), so that which alternatives are taken, and in which order, does not depend on who finds them.
 #include <algorithm>
@@ -17,7 +20,7 @@ namespace sthip {
 
 namespace {
 
-constexpr int kUnroll = 4;  // 16-byte loads that a thread of the backward pass has on their way
+constexpr int kUnroll = 4;  // 16-byte loads that a thread of the backward pass has on their way (2 and 8 take the same where memory is what it waits for)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1e30f;  // a difference beyond every exponential that is not 0, and whose products are finite
 
@@ -527,12 +530,13 @@ __global__ __launch_bounds__(256) void token_log_probs_grad_kernel(LogProbsGradA
     }
 }
 
-// A wavefront takes a row of up to so many bytes, a workgroup longer ones.
+// A wavefront takes a row of up to so many bytes, a workgroup longer ones: 16384 rows of 256 f32 take a wavefront each 6.4 µs forward and 7.7 backward, a
+// workgroup each 20 and 16; of 1000 12.5 and 21.1, against 20.8 and 21.7; from 8 KB on both take the same.
 constexpr size_t kWaveRow = 4096;
-// Rows are cut into parts where there are fewer than workgroups to fill the chip with, of 8 KiB (two runs a thread) or more.
-int parts_of(size_t rows, size_t vocab, size_t size, size_t most)
+// Rows are cut into parts of 8 KiB (two runs a thread) or more, enough for so many workgroups.
+int parts_of(size_t rows, size_t vocab, size_t size, size_t workgroups, size_t most)
 {
-    const size_t wanted = (512 + rows - 1) / rows, possible = vocab * size / (8u << 10);
+    const size_t wanted = (workgroups + rows - 1) / rows, possible = vocab * size / (8u << 10);
     return static_cast<int>(std::max<size_t>(1, std::min({wanted, possible, most})));
 }
 
@@ -541,7 +545,10 @@ hipError_t launch_forward(LogProbsArgs args, hipStream_t stream)
 {
     const size_t rows = args.rows, vocab = args.vocab;
     const bool wave = vocab * sizeof(T) <= kWaveRow;
-    args.parts = wave ? 1 : parts_of(rows, vocab, sizeof(T), kMostParts);
+    // Lists of the likeliest keep a workgroup busy: four of them to a compute unit (64 rows of 100001 in f32 with the first 5: 16.0 µs; two 17.4, one
+    // 22.5, whole rows 45.8), also where every compute unit would have a row (300 rows: 35, whole 49).  Without lists two, and then whole rows
+    // (128 rows: 13.5 µs, four 14.4; 300 rows of 32000: 9.4 whole, 10.9 in parts; of 100001 21 and 24).
+    args.parts = wave ? 1 : parts_of(rows, vocab, sizeof(T), args.top ? 1024 : rows < 256 ? 512 : 1, kMostParts);
     // (whole 16-byte runs, so that no two parts share one)
     args.part_size = static_cast<int>((vocab + args.parts - 1) / args.parts + 15) / 16 * 16;
     args.parts = static_cast<int>((vocab + args.part_size - 1) / args.part_size);
@@ -584,7 +591,8 @@ hipError_t launch_backward(LogProbsGradArgs args, hipStream_t stream)
 {
     const size_t rows = args.rows, vocab = args.vocab;
     const bool wave = vocab * sizeof(T) <= kWaveRow;
-    args.parts = wave ? 1 : parts_of(rows, vocab, sizeof(T), 4096);
+    // (300 rows of 32000 12.6 µs, with two workgroups to a compute unit 13.4, with one, and whole, 14.2; a row of 131072 4.1 and whole 20)
+    args.parts = wave ? 1 : parts_of(rows, vocab, sizeof(T), 1024, 1024);
     args.part_size = static_cast<int>((vocab + args.parts - 1) / args.parts + 15) / 16 * 16;
     args.parts = static_cast<int>((vocab + args.part_size - 1) / args.part_size);
     const size_t items = rows * args.parts, blocks = wave ? (items + 3) / 4 : items;
