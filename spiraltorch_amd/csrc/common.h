@@ -29,6 +29,7 @@ inline bool checked_mul(size_t a, size_t b, size_t *out)
 }
 
 constexpr size_t kMaxDim = 0x7fffffffu;  // dims must fit i32 (crates/st-tensor/src/backend/hip_dense.rs:55-73)
+constexpr size_t kMostWorkgroups = (1u << 24) - 1;  // of 256 threads to a launch, whose threads are counted in 32 bits
 
 inline hipStream_t as_stream(void *stream) { return static_cast<hipStream_t>(stream); }
 

@@ -410,6 +410,7 @@ int check_logits(size_t rows, size_t vocab, const char *what, const void *at, si
     if (ld < vocab) return fail(ST_HIP_ERR_INVALID, "log-probabilities: row stride %zu of the %s is smaller than the vocabulary's %zu", ld, what, vocab);
     if (!addressable(rows, ld, size)) return fail(ST_HIP_ERR_INVALID, "log-probabilities: dimensions overflow");
     if (reinterpret_cast<uintptr_t>(at) % size != 0) return fail(ST_HIP_ERR_INVALID, "log-probabilities: %s are not aligned to their type", what);
+    if (rows > kMostWorkgroups) return fail(ST_HIP_ERR_UNSUPPORTED, "log-probabilities: %zu rows are more than %zu", rows, kMostWorkgroups);
     return ST_HIP_OK;
 }
 
@@ -484,6 +485,8 @@ int check_attention_training(const st_hip_attention_training *a, bool *work)
     // (the kernels look up to a tile of 128 rows behind the last)
     if (a->batch > kMaxDim || width > kMaxDim || a->sequence > kMaxDim - 256 || rows > kMaxDim)
         return fail(ST_HIP_ERR_UNSUPPORTED, "attention dimension exceeds i32");
+    const size_t tiles = contexts * ((a->sequence + 127) / 128);
+    if (tiles > kMostWorkgroups) return fail(ST_HIP_ERR_UNSUPPORTED, "attention training: %zu tiles of 128 rows are more than %zu", tiles, kMostWorkgroups);
     if (const st_hip_position_bias *b = a->position_bias) {
         if (b->bidirectional && b->buckets % 2 != 0) return fail(ST_HIP_ERR_INVALID, "position bias buckets %zu are odd on two sides", b->buckets);
         const size_t side = b->bidirectional ? b->buckets / 2 : b->buckets;
@@ -493,7 +496,7 @@ int check_attention_training(const st_hip_attention_training *a, bool *work)
         if (b->buckets > ST_HIP_POSITION_BIAS_MOST_BUCKETS || b->max_distance > ST_HIP_POSITION_BIAS_MOST_DISTANCE)
             return fail(ST_HIP_ERR_UNSUPPORTED, "position bias of %zu buckets to distance %zu exceeds the kernel's", b->buckets, b->max_distance);
         if (contexts && !b->table) return fail(ST_HIP_ERR_INVALID, "position bias table is null");
-        if (a->heads > kMaxDim / ST_HIP_POSITION_BIAS_MOST_BUCKETS) return fail(ST_HIP_ERR_UNSUPPORTED, "position bias heads exceed the kernel's");
+        if (a->heads > kMostWorkgroups / 4 / ST_HIP_POSITION_BIAS_MOST_BUCKETS) return fail(ST_HIP_ERR_UNSUPPORTED, "position bias heads exceed the kernel's");
     }
     *work = rows != 0;
     return ST_HIP_OK;
@@ -1636,6 +1639,8 @@ int st_hip_attention_backward_f32_dev(size_t contexts, size_t sequence, size_t h
     // (a tile's rows behind the last are looked up)
     if (sequence > kMaxDim - 256 || (sequence + 256) * (head_dim + 8) * sizeof(float) >= 1ull << 31)
         return fail(ST_HIP_ERR_UNSUPPORTED, "attention backward: a context of %zu x %zu exceeds 2 GiB", sequence, head_dim);
+    const size_t tiles = contexts * ((sequence + 31) / 32);
+    if (tiles > kMostWorkgroups) return fail(ST_HIP_ERR_UNSUPPORTED, "attention backward: %zu tiles of 32 rows are more than %zu", tiles, kMostWorkgroups);
     if (plan.bias_len > static_cast<size_t>(-1) / 8) return fail(ST_HIP_ERR_INVALID, "attention dimensions overflow");
     if (head_dim && (!q || !k || !v || !out || !grad_out || !grad_q || !grad_k || !grad_v))
         return fail(ST_HIP_ERR_INVALID, "attention received a null pointer; provide contiguous buffers");

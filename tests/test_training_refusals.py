@@ -129,3 +129,21 @@ def test_log_probs(stub, kind, size):  # noqa: F811
                 f"ld=208, ld_grad=208, grad_logits=1*M + {100 * size}": "taken", f"ld=208, ld_grad=208, grad_logits=1*M + {99 * size}": "invalid",
                 "rows=2**31": "unsupported", "grad_logits=7*M + 1": "invalid"}
     assert answers(stub, f"hip.token_log_probs_backward_{kind}_dev", base, expected) == list(expected.values())
+
+
+def test_more_workgroups_than_a_launch_has(stub):  # noqa: F811
+    """A launch counts its threads in 32 bits: 2^24 workgroups of 256 are one too many."""
+    far = "logits=M, ld=1, tokens=2**40, log_probs=2**41, entropies=None, normalizers=None, top=0, top_ids=None, top_log_probs=None"
+    assert answers(stub, "hip.token_log_probs_f32_dev", f"rows=2**24 - 1, vocab=1, {far}", {"": "taken", "rows=2**24": "unsupported"}) == ["taken", "unsupported"]
+    back = "logits=M, ld=1, tokens=None, normalizers=2**40, entropies=None, grad_log_probs=None, grad_entropies=None, grad_logits=2**41, ld_grad=1"
+    expected = {"": "taken", "rows=2**24": "unsupported"}
+    assert answers(stub, "hip.token_log_probs_backward_bf16_dev", f"rows=2**24 - 1, vocab=1, {back}", expected) == list(expected.values())
+    wide = "q=M, ld_q=64, k=2**41, v=2**42, ld_kv=64, out=2**43, ld_out=64, lse=2**44"
+    expected = {"": "taken", shape("2**24, 1, 1, 64, 0.125"): "unsupported", shape("2**23, 1, 129, 64, 0.125"): "unsupported",
+                shape("2**23 - 1, 2, 1, 64, 0.125, kv_heads=1") + ", ld_q=128, ld_out=128": "taken",
+                shape("1, 2**14, 1, 64, 0.125, position_bias=hip.PositionBias(8, 100, 2**45)") + ", ld_q=2**20, ld_kv=2**20, ld_out=2**20": "unsupported"}
+    assert answers(stub, "hip.attention_training_bf16_dev", f"{shape('2**24 - 1, 1, 1, 64, 0.125')}, {wide}", expected) == list(expected.values())
+    base = ("contexts=2**24 - 1, sequence=1, head_dim=1, scale=1.0, causal=False, q=M, k=2**41, v=2**42, z_bias=None, attn_bias=None, out=2**43, grad_out=2**44, "
+            "grad_q=2**45, grad_k=2**46, grad_v=2**47")
+    expected = {"": "taken", "contexts=2**24": "unsupported", "contexts=2**23, sequence=33": "unsupported"}
+    assert answers(stub, "hip.attention_backward_f32_dev", base, expected) == list(expected.values())
