@@ -598,8 +598,8 @@ typedef struct {
  * sees no key.  q, out: heads*head_dim columns; k, v: kv_heads*head_dim columns, row stride ld_kv.  Rows behind a sequence's length are
  * not read, and their results are 0 (lse: -infinity), as are those of rows whose every key has a bias of -infinity.
  * The products take bf16 and accumulate in f32, the softmax is f32; its weights are rounded to bf16 for the second product, and so is out.
- * Row strides (values) multiples of 8, buffers 16-byte aligned, and a sequence of a head within 2 GiB of its first row, else
- * ST_HIP_ERR_UNSUPPORTED.  What is written overlaps nothing else; columns of one matrix that do not meet may be given. */
+ * Row strides (values) multiples of 8, buffers 16-byte aligned, a sequence of a head within 2 GiB of its first row and fewer than 2^24 tiles
+ * of 128 rows of a head, else ST_HIP_ERR_UNSUPPORTED.  What is written overlaps nothing else; columns of one matrix that do not meet may be given. */
 int st_hip_attention_training_bf16_dev(const st_hip_attention_training *shape, const uint16_t *q, size_t ld_q, const uint16_t *k,
                                        const uint16_t *v, size_t ld_kv, uint16_t *out, size_t ld_out, float *lse, void *stream);
 /* The backward pass, from what the forward pass was given and gave, and out's gradient: grad_q, grad_k, grad_v (bf16; those of shared
@@ -615,7 +615,7 @@ int st_hip_attention_backward_bf16_dev(const st_hip_attention_training *shape, c
  * they are asked for (not NULL; with the bias), of z_bias (contexts, sequence) and attn_bias (contexts*sequence, sequence), all overwritten.
  * A row whose every score is -infinity has the gradient 0.  f32 throughout; results do not depend on the order in which workgroups run,
  * and what is written overlaps nothing else.  A context of q is within 2 GiB (ST_HIP_ERR_UNSUPPORTED).  Two numbers a row go through the
- * stream's scratch memory. */
+ * stream's scratch memory and, unless attn_bias's gradient is asked for, the scores' gradients where these are no more than 256 MiB. */
 int st_hip_attention_backward_f32_dev(size_t contexts, size_t sequence, size_t head_dim, float scale, int causal, const float *q,
                                       const float *k, const float *v, const float *z_bias, const float *attn_bias, const float *out,
                                       const float *grad_out, float *grad_q, float *grad_k, float *grad_v, float *grad_z_bias,
@@ -627,7 +627,7 @@ int st_hip_attention_backward_f32_dev(size_t contexts, size_t sequence, size_t h
  * entropies and normalizers may each be NULL; top is at most vocab and 32.  Sums are f32.  Logits of -infinity have no probability; in a row of
  * nothing else the normalizer and all log-probabilities are -infinity and the entropy is 0.  A row with NaN or +infinity gives NaN; NaN is
  * no alternative (id -1 and NaN where there are too few).  Long rows of which there are few are cut over workgroups, whose parts go
- * through the stream's scratch memory.  Results overlap neither what is read nor each other. */
+ * through the stream's scratch memory.  Results overlap neither what is read nor each other.  Fewer than 2^24 rows. */
 #define ST_HIP_LOG_PROBS_MOST_TOP 32
 int st_hip_token_log_probs_f32_dev(size_t rows, size_t vocab, const float *logits, size_t ld, const int32_t *tokens, float *log_probs,
                                    float *entropies, float *normalizers, size_t top, int32_t *top_ids, float *top_log_probs, void *stream);
