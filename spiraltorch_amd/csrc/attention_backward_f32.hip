@@ -41,7 +41,7 @@ struct BackwardArgs {
     float *lse, *delta;  // (contexts, padded): lse·log2 e; rows behind the last +infinity and 0
     float *pairs;        // ds, (contexts, S, pair_row): grad_attn_bias, or scratch, or null where dq works it out again
     int contexts, S, D, padded, tiles, swizzle, pair_row;
-    float scale;
+    float scale, keep;  // ds counts `keep` times: once, or, where there is one key, not at all (the roundings of p and dp would leave something of it)
     bool wide_bias, wide_pairs;  // four neighbouring values of a row are one aligned load
 };
 
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
             wait_for_reads();
             load_keys(key0 + WAVES * kRows);
         }
-        write_rows<DC, WAVES, VEC>(dq, p.scale, p.grad_q + first * D, q0, S, D, backward_lds);
+        write_rows<DC, WAVES, VEC>(dq, p.scale * p.keep, p.grad_q + first * D, q0, S, D, backward_lds);
     }
 }
 
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         load(std::false_type{}, key0 + WAVES * kRows, turn ^ 1);
         add_product<DC>(tiles + turn * Tile<DC>::kBytes, weights, dq, li, lh);
     }
-    write_rows<DC, WAVES, VEC>(dq, p.scale, p.grad_q + first * D, q0, S, D, backward_lds);
+    write_rows<DC, WAVES, VEC>(dq, p.scale * p.keep, p.grad_q + first * D, q0, S, D, backward_lds);
 }
 
 // ---- dk, dv, the biases' gradients: keys stay -----------------------------------------------------------------------------------------------
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
                 const __amdgpu_buffer_rsrc_t pairs = bias_rows(p.pairs + (first + row0) * p.pair_row, S - row0, p.pair_row);
                 const unsigned to = my_key < S ? (4u * lh * p.pair_row + my_key) * 4u : 0x80000000u;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[r]), pairs, to + row_of(r) * p.pair_row * 4u, 0, 0);
+                for (int r = 0; r < 16; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[r] * p.keep), pairs, to + row_of(r) * p.pair_row * 4u, 0, 0);
             }
         }
         wait_for_reads();
@@ -499,10 +499,10 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
                 float sum = totals[0][li];
 #pragma unroll
                 for (int w = 1; w < WAVES; ++w) sum += totals[w][li];
-                p.grad_z_bias[first + my_key] = sum;
+                p.grad_z_bias[first + my_key] = sum * p.keep;
             }
         }
-        write_rows<DC, WAVES, VEC>(dk, p.scale, p.grad_k + first * D, k0, S, D, backward_lds);
+        write_rows<DC, WAVES, VEC>(dk, p.scale * p.keep, p.grad_k + first * D, k0, S, D, backward_lds);
     }
     if constexpr (DV) write_rows<DC, WAVES, VEC>(dv, 1.0f, p.grad_v + first * D, k0, S, D, backward_lds);
 }
@@ -592,6 +592,7 @@ hipError_t launch_attention_backward_f32(size_t contexts, size_t sequence, size_
     args.padded = args.tiles * kRows;
     args.swizzle = contexts % 8 == 0;
     args.scale = scale;
+    args.keep = sequence == 1 ? 0.0f : 1.0f;
     auto aligned = [](const void *at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; };
     args.wide_bias = sequence % 4 == 0 && aligned(attn_bias) && aligned(z_bias);
     const size_t rows = contexts * args.padded, pair_row = grad_attn_bias ? sequence : (sequence + 3) / 4 * 4;

@@ -447,7 +447,8 @@ __device__ __forceinline__ void grad_q(const TrainingArgs &p, unsigned char *tra
     }
     delta += __shfl_xor(delta, 32);
     float lse = my_q < length ? p.lse[context * p.S + my_q] : INFINITY;
-    if (lse == -INFINITY) lse = INFINITY;  // a row without keys: every p is 0
+    // A row without keys: every p is 0.  So is ds where there is one key, exactly: the roundings of p and dp would leave something.
+    if (lse == -INFINITY || length == 1) lse = INFINITY;
     const float by = p.scale * kLog2e, shift = -lse * kLog2e;
 
     // A stage is two blocks of 32 keys.  Its products are dealt out in steps of one chunk, with what is read from LDS `AHEAD` steps early and
@@ -809,6 +810,10 @@ __device__ __forceinline__ void grad_kv(const TrainingArgs &p, unsigned char *tr
         bool same = true;
         while (CAUSAL && same && stage * kStage < k0 + kStay) same = step(std::true_type{});
         while (same) same = step(std::false_type{});
+    }
+    if (length == 1) {  // (ds, as in the dq kernel)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) dk[t] *= 0.0f;
     }
     if (p.parts > 1) {
         if (my_key >= length) return;

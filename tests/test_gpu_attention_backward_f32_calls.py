@@ -151,3 +151,20 @@ def test_two_threads_on_streams_of_their_own(hip):
     for case, first in zip(cases, want):
         for name, a in case.results().items():
             assert torch.equal(a, first[name]), name
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("d", [1, 64, 80, 200])
+def test_a_single_key_has_all_of_every_row(hip, d, biased, causal):
+    """Its weight is 1 whatever the scores, and everything but dv exactly 0."""
+    case = Buffers(d, 37, 1, d, causal, biased)
+    case.x["out"].copy_(case.x["v"])
+    case.run(hip)
+    got = case.results()
+    for name in got.keys() - {"dv"}:
+        assert (got[name] == 0).all(), name
+    # p = 2^(s - lse) with lse = s + log2(1), s below 16 rounded twice (to 2^-21 each at the most) in units of log2 e: off by less than 2^-20, and rounded
+    s = (case.x["q"] * case.x["k"]).sum((1, 2)) * case.scale + (case.x["z"][:, 0] + case.x["bias"][:, 0, 0] if biased else 0)
+    assert s.abs().max() * 1.4427 < 15.9
+    assert ((got["dv"] - case.x["g"]).abs() <= 2.0**-20 * case.x["g"].abs()).all()

@@ -314,3 +314,15 @@ def test_two_threads_on_streams_of_their_own(hip):
     for case, first in zip(cases, want):
         for name, value in case.results().items():
             assert (value == first[name]).all(), name
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,n,lengths,buckets", [(3, 3, 1, None, 0), (4, 2, 1, None, 8), (2, 1, 1500, [1, 1, 0], 0), (2, 2, 40, [1, 0, 1], 8)])
+def test_a_single_key_has_all_of_its_row(hip, heads, kv_heads, n, lengths, buckets, causal, dim):
+    """Its weight is 1 whatever the score, and the gradients of queries, keys and biases exactly 0."""
+    case = Case(hip, 31, 3, heads, kv_heads, n, dim, causal, lengths, buckets=buckets, far=20 if buckets else 0)
+    case.check()
+    got = case.results()
+    for name in got.keys() - {"out", "lse", "dv"}:
+        assert (got[name] == 0).all(), name
