@@ -320,3 +320,27 @@ def test_parts_captured_and_replayed(hip):
         del graph
         hip.release_scratch(stream.cuda_stream)
         hip.release_scratch(None)
+
+
+@pytest.mark.parametrize("vocab", [2, 4, 40, 5001])
+def test_the_entropy_goes_with_the_normalizer(hip, vocab):
+    """The gradient of the entropy sums to 0 over a row to its own terms' rounding, also where one token has nearly all: there log p + H is small beside
+    what the normalizer's rounding moves log p by (half a step of 8 to 16: 8 f), which the entropy moves with."""
+    rng = np.random.default_rng(vocab)
+    rows = 64
+    x = rng.normal(size=(rows, vocab)).astype(np.float32)
+    tokens = rng.integers(0, vocab, rows)
+    x[np.arange(rows), tokens] += 10.0 + np.log(vocab)
+    x = np.minimum(x, 15.0).astype(np.float32) if vocab < 100 else x
+    call = Call(hip, x, vocab, tokens, "f32")
+    call.check()
+    ones, d_y = hip.DeviceBuffer.from_array(np.ones(rows, np.float32)), hip.DeviceBuffer.from_array(np.zeros((rows, vocab), np.float32))
+    hip.token_log_probs_backward_f32_dev(rows, vocab, call.at(), call.ld, call.d_tokens, call.d["lse"], call.d["entropies"], None, ones, d_y, vocab)
+    hip.device_synchronize()
+    y = d_y.to_array(np.float32, (rows, vocab)).astype(np.float64)
+    lse, p, log_p, entropies, _, _ = oracle(call.values(), call.tokens)
+    assert (np.abs(lse) < 32).all()
+    # a term: p's exponent rounded twice (2 f |log p| each) and its result, log p and H and their sum rounded, the product twice; and H, the sum of
+    # what up to vocab / 64 + 80 additions leave of T / L
+    size = (p * (np.abs(log_p) + entropies[:, None]) * (8 + 4 * np.abs(log_p))).sum(1) + (vocab / 64 + 80 + 4 * 40) * entropies
+    assert (np.abs(y.sum(1)) <= F * size).all(), np.max(np.abs(y.sum(1)) / (F * size))
