@@ -20,6 +20,7 @@
 // of which 16 each are the bytes).
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "device_math.h"
@@ -37,7 +38,7 @@ typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 typedef s16x4 __attribute__((address_space(3))) *lds_s16x4_ptr;
 
-// The buckets of one side: bucket j begins at distance first[j].
+// The buckets of one side: bucket j begins at distance first[j]; what is behind the last one's begins nowhere.
 struct Buckets {
     int count, side, far;  // of both sides; of one; from `far` on the last one
     int bidirectional;
@@ -186,8 +187,10 @@ __device__ __forceinline__ void fill_bias(const TrainingArgs &p, int head, float
     const Buckets &b = p.buckets;
     for (int i = tid; i < distances_of(b.far); i += 256) {
         const int distance = min(max(i - b.far - kMargin, -b.far), b.far), m = b.bidirectional ? abs(distance) : max(-distance, 0);
-        int bucket = b.bidirectional && distance > 0 ? b.side : 0;
-        for (int j = 1; j < b.side; ++j) bucket += m >= b.first[j];
+        int bucket = b.bidirectional && distance > 0 ? b.side - 1 : -1;
+        for (int j = 0; j < b.side; j += 16)  // sixteen at a load (a pass over a single token 39 µs; one after the other 48)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) bucket += m >= b.first[j + e];
         bias[i] = p.table[static_cast<size_t>(bucket) * p.heads + head] * kLog2e;
     }
 }
@@ -962,6 +965,7 @@ TrainingArgs arguments(const st_hip_attention_training &shape, const uint16_t *q
             while (m < to.far && !reached(m)) ++m;
             to.first[j] = m;
         }
+        std::fill(to.first + to.side, to.first + ST_HIP_POSITION_BIAS_MOST_BUCKETS, std::numeric_limits<int>::max());
     }
     return args;
 }
