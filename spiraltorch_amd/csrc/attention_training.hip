@@ -682,7 +682,9 @@ __device__ __forceinline__ void grad_kv(const TrainingArgs &p, unsigned char *tr
     const long long all = static_cast<long long>(of_head) * p.group;
     const int begin = static_cast<int>(all * part / p.parts), end = static_cast<int>(all * (part + 1) / p.parts);
     const Mover<D> mover_q(p.ld_q, lane, wave), mover_g(p.ld_grad_out, lane, wave);
+    // A stage's lse and δ, a row a thread: what is made of them waits for the store, as it would wait here for the whole stage's loads.
     float statistic = 0.0f;
+    int statistic_row = 0;
     auto load = [&](int head, int stage, int buffer) {
         const int first = stage * kStage;
         const __amdgpu_buffer_rsrc_t q_rows =
@@ -691,18 +693,15 @@ __device__ __forceinline__ void grad_kv(const TrainingArgs &p, unsigned char *tr
             rows_of(p.grad_out + static_cast<size_t>(b) * p.S * p.ld_grad_out + static_cast<size_t>(head) * D, p.ld_grad_out, length, D);
         const size_t of_context = (static_cast<size_t>(b) * p.heads + head) * p.S;
         unsigned char *const to = training_lds + buffer * 2 * BYTES;
+        statistic_row = first + (tid & 63);
+        statistic = (tid < 64 ? p.lse : p.delta)[of_context + min(statistic_row, length - 1)];
         mover_q.load(q_rows, first, to);
         mover_g.load(g_rows, first, to + BYTES);
-        const int row = first + (tid & 63);
-        if (tid < 64) {
-            const float lse = row < length ? p.lse[of_context + row] : INFINITY;
-            statistic = lse == -INFINITY ? -INFINITY : -lse * kLog2e;  // rows without keys: every p is 0
-        } else if (tid < 128) {
-            statistic = row < length ? p.delta[of_context + row] : 0.0f;
-        }
     };
     auto store = [&](int buffer) {
-        if (tid < 128) statistics[buffer * 2 * kStage + tid] = statistic;
+        const bool within = statistic_row < length;
+        const float shift = within && statistic != -INFINITY ? -statistic * kLog2e : -INFINITY;  // rows without keys: every p is 0
+        if (tid < 128) statistics[buffer * 2 * kStage + tid] = tid < 64 ? shift : within ? statistic : 0.0f;
     };
     // (In steps, as in the dq kernel.)
     constexpr int AHEAD = D == 64 ? 2 : 4, STEPS = D / 16, EACH = 16 / STEPS;
