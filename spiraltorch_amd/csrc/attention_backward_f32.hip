@@ -135,9 +135,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t bias_rows(const float *first, 
 {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(first), 0, static_cast<int>(static_cast<unsigned>(min(rows, kRows)) * row * 4u), 0x00020000);
 }
-__device__ __forceinline__ f32x4 bias4(const __amdgpu_buffer_rsrc_t &from, unsigned at, bool wide)
+// (Which of both is known where it is compiled: loads on two sides of a branch are waited for where the sides meet.)
+template <bool WIDE>
+__device__ __forceinline__ f32x4 bias4(const __amdgpu_buffer_rsrc_t &from, unsigned at)
 {
-    if (wide) return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at * 4u, 0, 0));
+    if (WIDE) return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at * 4u, 0, 0));
     f32x4 x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, (at + e) * 4u, 0, 0));
@@ -267,49 +269,63 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     struct Biases {
         f32x4 of_pair[4], of_key[4];
     };
-    auto load_biases = [&](int key0, Biases &to) {
+    auto load_biases = [&](auto wide, int key0, Biases &to) {
+        constexpr bool WIDE = decltype(wide)::value;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
             const unsigned key = key0 + a * 8 + lh * 4;
-            if (p.attn_bias) to.of_pair[a] = bias4(biases, static_cast<unsigned>(li) * S + key, p.wide_bias);
-            if (p.z_bias) to.of_key[a] = bias4(z_biases, key, p.wide_bias);
+            if (p.attn_bias) to.of_pair[a] = bias4<WIDE>(biases, static_cast<unsigned>(li) * S + key);
+            if (p.z_bias) to.of_key[a] = bias4<WIDE>(z_biases, key);
+        }
+    };
+    auto sum_of = [&](const Biases &from, f32x4 (&to)[4]) {
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            to[a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.attn_bias) to[a] += from.of_pair[a];
+            if (p.z_bias) to[a] += from.of_key[a];
+            asm volatile("" : "+v"(to[a]));
         }
     };
     // the scores of a tile, in units of log2 e
-    auto scores = [&](const unsigned char *tile, const Biases &with, int key0) {
+    auto scores = [&](const unsigned char *tile, const f32x4 (&with)[4], int key0) {
         f32x16 s = product<DC>(tile, q, li, lh);
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
             const int key = key0 + a * 8 + lh * 4;
-            f32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (p.attn_bias) bias += with.of_pair[a];
-            if (p.z_bias) bias += with.of_key[a];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = fmaf(s[a * 4 + e], p.scale, bias[e]) * kLog2e;
+                const float x = fmaf(s[a * 4 + e], p.scale, with[a][e]) * kLog2e;
                 s[a * 4 + e] = key + e > last_key ? -INFINITY : x;
             }
         }
         return s;
     };
     float most = -INFINITY, total = 0.0f;
-    // (the wavefront's two tiles take turns)
-    for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
-        Biases with;
-        wait_for_loads();
-        wait_for_reads();
-        load_biases(key0, with);
-        if (key0 + WAVES * kRows < key_end) load_tile<DC, VEC, false>(p.k + first * D, S, D, key0 + WAVES * kRows, turn ? k_tile : v_tile, places, lane);
-        const f32x16 s = scores(turn ? v_tile : k_tile, with, key0);
-        float top = most;
+    // (the wavefront's two tiles take turns; biases come with their tile, as what is waited for behind the next tile's loads is waited for with them)
+    auto sweep = [&](auto wide) {
+        Biases next;
+        load_biases(wide, wave * kRows, next);
+        for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
+            f32x4 with[4];
+            wait_for_loads();
+            wait_for_reads();
+            sum_of(next, with);
+            load_biases(wide, key0 + WAVES * kRows, next);
+            if (key0 + WAVES * kRows < key_end) load_tile<DC, VEC, false>(p.k + first * D, S, D, key0 + WAVES * kRows, turn ? k_tile : v_tile, places, lane);
+            const f32x16 s = scores(turn ? v_tile : k_tile, with, key0);
+            float top = most;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
-        const float safe = top == -INFINITY ? 0.0f : top;
-        total *= __builtin_amdgcn_exp2f(most - safe);
-        most = top;
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+            const float safe = top == -INFINITY ? 0.0f : top;
+            total *= __builtin_amdgcn_exp2f(most - safe);
+            most = top;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) total += __builtin_amdgcn_exp2f(s[r] - safe);
-    }
+            for (int r = 0; r < 16; ++r) total += __builtin_amdgcn_exp2f(s[r] - safe);
+        }
+    };
+    if (p.wide_bias) sweep(std::true_type{});
+    else sweep(std::false_type{});
     auto load_keys = [&](int key0) {
         if (key0 < key_end) load_tile<DC, VEC, false>(p.k + first * D, S, D, key0, k_tile, places, lane);
     };
@@ -348,20 +364,26 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         f32x16 dq[Tile<DC>::kAcross];
 #pragma unroll
         for (int dt = 0; dt < Tile<DC>::kAcross; ++dt) dq[dt] = f32x16{};
-        for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
-            Biases with;
-            wait_for_loads();
-            load_biases(key0, with);
-            const f32x16 dp = product<DC>(v_tile, g, li, lh);
-            wait_for_reads();
-            load_values(key0 + WAVES * kRows);  // each tile's successor as soon as it has been read
-            f32x16 s = scores(k_tile, with, key0);
+        auto second = [&](auto wide) {
+            for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
+                Biases biases_of;
+                f32x4 with[4];
+                wait_for_loads();
+                load_biases(wide, key0, biases_of);
+                const f32x16 dp = product<DC>(v_tile, g, li, lh);
+                sum_of(biases_of, with);
+                wait_for_reads();
+                load_values(key0 + WAVES * kRows);  // each tile's successor as soon as it has been read
+                f32x16 s = scores(k_tile, with, key0);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - lse) * (dp[r] - delta);
-            add_product<DC>(k_tile, s, dq, li, lh);
-            wait_for_reads();
-            load_keys(key0 + WAVES * kRows);
-        }
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - lse) * (dp[r] - delta);
+                add_product<DC>(k_tile, s, dq, li, lh);
+                wait_for_reads();
+                load_keys(key0 + WAVES * kRows);
+            }
+        };
+        if (p.wide_bias) second(std::true_type{});
+        else second(std::false_type{});
         write_rows<DC, WAVES, VEC>(dq, p.scale * p.keep, p.grad_q + first * D, q0, S, D, backward_lds);
     }
 }
@@ -380,25 +402,29 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     unsigned char *const places = backward_lds + WAVES * 2 * Tile<DC>::kBytes;
     const __amdgpu_buffer_rsrc_t pairs = bias_rows(p.pairs + (first + q0) * p.pair_row, S - q0, p.pair_row);
     f32x4 ds[4];
-    auto load = [&](auto starts, int key0, int turn) {
-        if (key0 >= key_end) return;
-        load_tile<DC, VEC, decltype(starts)::value>(p.k + first * D, S, D, key0, tiles + turn * Tile<DC>::kBytes, places, lane);
-#pragma unroll
-        for (int a = 0; a < 4; ++a) ds[a] = bias4(pairs, static_cast<unsigned>(li) * p.pair_row + key0 + a * 8 + lh * 4, p.wide_pairs);
-    };
     f32x16 dq[Tile<DC>::kAcross];
 #pragma unroll
     for (int dt = 0; dt < Tile<DC>::kAcross; ++dt) dq[dt] = f32x16{};
-    load(std::true_type{}, wave * kRows, 0);
-    for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
-        f32x16 weights;
-        wait_for_loads();
-        wait_for_reads();
+    auto sweep = [&](auto wide) {
+        auto load = [&](auto starts, int key0, int turn) {
+            if (key0 >= key_end) return;
+            load_tile<DC, VEC, decltype(starts)::value>(p.k + first * D, S, D, key0, tiles + turn * Tile<DC>::kBytes, places, lane);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) weights[r] = key0 + row_of(r) + 4 * lh > last_key ? 0.0f : ds[r >> 2][r & 3];
-        load(std::false_type{}, key0 + WAVES * kRows, turn ^ 1);
-        add_product<DC>(tiles + turn * Tile<DC>::kBytes, weights, dq, li, lh);
-    }
+            for (int a = 0; a < 4; ++a) ds[a] = bias4<decltype(wide)::value>(pairs, static_cast<unsigned>(li) * p.pair_row + key0 + a * 8 + lh * 4);
+        };
+        load(std::true_type{}, wave * kRows, 0);
+        for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
+            f32x16 weights;
+            wait_for_loads();
+            wait_for_reads();
+#pragma unroll
+            for (int r = 0; r < 16; ++r) weights[r] = key0 + row_of(r) + 4 * lh > last_key ? 0.0f : ds[r >> 2][r & 3];
+            load(std::false_type{}, key0 + WAVES * kRows, turn ^ 1);
+            add_product<DC>(tiles + turn * Tile<DC>::kBytes, weights, dq, li, lh);
+        }
+    };
+    if (p.wide_pairs) sweep(std::true_type{});
+    else sweep(std::false_type{});
     write_rows<DC, WAVES, VEC>(dq, p.scale * p.keep, p.grad_q + first * D, q0, S, D, backward_lds);
 }
 
@@ -471,6 +497,11 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         f32x16 dp;
         if constexpr (DK) dp = product<DC>(g_tile, v, li, lh);
         if constexpr (DV) add_product<DC>(g_tile, s, dv, li, lh);
+        // (what was loaded into registers is used before the next loads: these stand behind a branch, where waiting for others is waiting for them)
+        if constexpr (DK) {
+#pragma unroll
+            for (int a = 0; a < 4; ++a) asm volatile("" : "+v"(delta[a]));
+        }
         wait_for_reads();
         load_grads(row0 + WAVES * kRows);  // each tile's successor as soon as it has been read
         if constexpr (DK) {
