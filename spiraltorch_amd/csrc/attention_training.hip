@@ -394,6 +394,18 @@ __device__ __forceinline__ void add_by_distance(const f32x16 &ds, int d0, int fa
     __builtin_amdgcn_wave_barrier();
 }
 
+// A sum over a whole row, with what each addition lost: the sums of ds by distance cancel to a small part of what is added, of a long sequence's last
+// bucket above all.
+struct LongSum {
+    float sum = 0.0f, lost = 0.0f;
+    __device__ __forceinline__ void add(float x)
+    {
+        const float y = x - lost, to = sum + y;
+        lost = (to - sum) - y;
+        sum = to;
+    }
+};
+
 template <int D, bool CAUSAL, bool BIAS>
 __device__ __forceinline__ void grad_q(const TrainingArgs &p, unsigned char *training_lds)  // [K, V][2]; bias; bins of four wavefronts
 {
@@ -521,21 +533,30 @@ __device__ __forceinline__ void grad_q(const TrainingArgs &p, unsigned char *tra
     };
     // do·o carries the roundings of o, which are to those of ds (rounded to bf16 as well) as one to the root of the keys.  The table's gradient
     // though is f32 and adds ds over whole diagonals, and a sequence may have few keys: there δ is Σ p·dp, at the price of both products again
-    // (of one stage, where the sequence is short).
+    // (of one stage, where the sequence is short), and over Σ p, which lse's rounding makes a little less or more than 1: so a row's ds add up to 0, and
+    // nothing of that is summed over whole columns.
     if (to_table || length <= kStage) {
-        delta = 0.0f;
+        LongSum delta_sum, total_sum;
         walk([&](auto mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
             Block blocks[2];
+            float of_delta = 0.0f, of_total = 0.0f;
             auto add = [&](int t, int step) {
                 weights(mask_tag, blocks[t], key0 + t * 32, step);
 #pragma unroll
-                for (int r = step * EACH; r < (step + 1) * EACH; ++r) delta = fmaf(blocks[t].s[r], blocks[t].dp[r], delta);
+                for (int r = step * EACH; r < (step + 1) * EACH; ++r) {
+                    of_delta = fmaf(blocks[t].s[r], blocks[t].dp[r], of_delta);
+                    of_total += blocks[t].s[r];
+                }
             };
             products(ks, vs, key0, blocks, [](int) {}, add);
 #pragma unroll
             for (int step = 0; step < STEPS; ++step) add(1, step);
+            delta_sum.add(of_delta);
+            total_sum.add(of_total);
         });
-        delta += __shfl_xor(delta, 32);
+        delta = delta_sum.sum + __shfl_xor(delta_sum.sum, 32);
+        const float total = total_sum.sum + __shfl_xor(total_sum.sum, 32);
+        if (total > 0.0f) delta /= total;
         if (stages > 1) load_stage(0);
     }
     if (lh == 0 && my_q < length) *delta_row = delta;
@@ -543,7 +564,7 @@ __device__ __forceinline__ void grad_q(const TrainingArgs &p, unsigned char *tra
     f32x16 dq[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) dq[t] = f32x16{};
-    float before = 0.0f, behind = 0.0f;  // ds of blocks beyond `far`
+    LongSum before, behind;  // ds of blocks beyond `far`
     walk([&](auto mask_tag, const unsigned char *ks, const unsigned char *vs, int key0) {
         Block blocks[2];
         bf16x8 ring[AHEAD], df[2][2];
@@ -573,8 +594,8 @@ __device__ __forceinline__ void grad_q(const TrainingArgs &p, unsigned char *tra
                     float sum = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sum += blocks[t].s[r];
-                    if (d0 > 0) behind += sum;
-                    else before += sum;
+                    if (d0 > 0) behind.add(sum);
+                    else before.add(sum);
                 }
             }
         }
@@ -582,11 +603,10 @@ __device__ __forceinline__ void grad_q(const TrainingArgs &p, unsigned char *tra
     if (my_q < length) store_row<D>(grad_row, dq, p.scale, lh);
     else if (my_q < p.S) store_zeros<D>(grad_row, lh);
     if (to_table) {
-        before = wave_sum(before);
-        behind = wave_sum(behind);
+        const float all_before = wave_sum(before.sum), all_behind = wave_sum(behind.sum);
         if (lane == 0) {
-            bins[0] += before;
-            bins[width - 1] += behind;
+            bins[0] += all_before;
+            bins[width - 1] += all_behind;
         }
         __syncthreads();
         for (int i = tid; i < width; i += 256) partial[i] = (all_bins[i] + all_bins[width + i]) + (all_bins[2 * width + i] + all_bins[3 * width + i]);
