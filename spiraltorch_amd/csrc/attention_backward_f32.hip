@@ -15,7 +15,7 @@
 // up through LDS at the end, in the order of the wavefronts.  So 16 contexts of 1024 are 512 workgroups, and nothing waits for another
 // wavefront before the end.  No atomics: the same call gives the same bits.
 //
-// 16 contexts of 1024 x 64 with both biases and all five gradients take 143 µs in three launches (44, 91, 29 µs by themselves), 75 TFLOP/s of
+// 16 contexts of 1024 x 64 with both biases and all five gradients take 136 µs in three launches (38, 90, 26 µs by themselves), 79 TFLOP/s of
 // needed products where a large library product reaches 154; 96 causal ones of 333 x 80 take 109 µs.  What is left: with the rows that stay, the
 // sums and a tile's scores in registers there are two wavefronts a SIMD (one above 64 values a head), and the softmax's instructions and a
 // tile's wait stand beside the products only where the other wavefront has some.

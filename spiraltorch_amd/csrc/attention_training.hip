@@ -15,8 +15,8 @@
 // where δ is worked out exactly), for results that do not depend on the order of workgroups, and no f32 copy of dq in memory.
 //
 // What bounds it: on a long sequence the matrix cores and what is issued between their instructions (8192 causal tokens, 32 heads on 8 of 128:
-// forward 540 µs, 1.02 PFLOP/s of unmasked products, dq 715, 1.15, dk and dv 1355, 0.81; a large library product reaches 1.31), on shorter ones
-// how full the chip is and how long a tile's loads, first products and results take (16 sequences of 1024 on 8 heads of 64: 32, 41 and 55 µs,
+// forward 515 µs, 1.07 PFLOP/s of unmasked products, dq 690, 1.2, dk and dv 1075, 1.02; a large library product reaches 1.31), on shorter ones
+// how full the chip is and how long a tile's loads, first products and results take (16 sequences of 1024 on 8 heads of 64: 32, 40 and 52 µs,
 // of which 16 each are the bytes).
 #include <algorithm>
 #include <cmath>
@@ -659,8 +659,8 @@ __global__ __launch_bounds__(kTableThreads) void position_bias_grad_kernel(const
 
 // ---- backward: dk, dv ---------------------------------------------------------------------------------------------------------------
 // Keys and values stay, q and do come by: four products, and 4·D/32 accumulators, which at heads of 128 leave one wavefront a SIMD: a stage's reads
-// from LDS run four steps ahead of their products then, but what neither covers shows (of 1355 µs at 8192 tokens the matrix instructions
-// alone are 645).
+// from LDS run four steps ahead of their products then, but what neither covers shows (of 1075 µs at 8192 tokens the matrix instructions
+// alone are 645, and the reads from LDS, 64 KB of a wavefront's for 64 of them, take as long).
 template <int D, bool CAUSAL, bool BIAS>
 __device__ __forceinline__ void grad_kv(const TrainingArgs &p, unsigned char *training_lds)  // [Q, dO][2]; [lse, δ][2]; bias
 {
