@@ -615,7 +615,8 @@ int st_hip_attention_backward_bf16_dev(const st_hip_attention_training *shape, c
  * they are asked for (not NULL; with the bias), of z_bias (contexts, sequence) and attn_bias (contexts*sequence, sequence), all overwritten.
  * A row whose every score is -infinity has the gradient 0.  f32 throughout; results do not depend on the order in which workgroups run,
  * and what is written overlaps nothing else.  A context of q is within 2 GiB (ST_HIP_ERR_UNSUPPORTED).  Two numbers a row go through the
- * stream's scratch memory and, unless attn_bias's gradient is asked for, the scores' gradients where these are no more than 256 MiB. */
+ * stream's scratch memory and, unless attn_bias's gradient is asked for, the scores' gradients where these are no more than 256 MiB; of few
+ * contexts also workgroups' sums (up to 50 MB). */
 int st_hip_attention_backward_f32_dev(size_t contexts, size_t sequence, size_t head_dim, float scale, int causal, const float *q,
                                       const float *k, const float *v, const float *z_bias, const float *attn_bias, const float *out,
                                       const float *grad_out, float *grad_q, float *grad_k, float *grad_v, float *grad_z_bias,

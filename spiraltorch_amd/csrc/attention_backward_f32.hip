@@ -13,7 +13,8 @@
 // A workgroup owns 32 rows (queries for dq, keys for dk and dv), which its wavefronts all hold as B operands; they deal the tiles of 32
 // rows of the other two matrices out among themselves (wavefront w takes tiles w, w + WAVES, ...), each through LDS of its own, and add
 // up through LDS at the end, in the order of the wavefronts.  So 16 contexts of 1024 are 512 workgroups, and nothing waits for another
-// wavefront before the end.  No atomics: the same call gives the same bits.
+// wavefront before the end.  Few contexts of many tiles have several workgroups a tile, whose sums a further launch adds.  No atomics: the same call
+// gives the same bits.
 //
 // 16 contexts of 1024 x 64 with both biases and all five gradients take 136 µs in three launches (38, 90, 26 µs by themselves), 79 TFLOP/s of
 // needed products where a large library product reaches 154; 96 causal ones of 333 x 80 take 109 µs.  What is left: with the rows that stay, the
@@ -41,6 +42,10 @@ struct BackwardArgs {
     float *lse, *delta;  // (contexts, padded): lse·log2 e; rows behind the last +infinity and 0
     float *pairs;        // ds, (contexts, S, pair_row): grad_attn_bias, or scratch, or null where dq works it out again
     int contexts, S, D, padded, tiles, swizzle, pair_row;
+    // Workgroups to a tile, each of which takes every parts-th of the others' rounds; then sums of theirs, (parts, ...), not scaled yet: of rows, of keys,
+    // and the rows' maxima and totals.
+    int parts;
+    float *part_q, *part_k, *part_v, *part_z, *part_max, *part_total;
     float scale, keep;  // ds counts `keep` times: once, or, where there is one key, not at all (the roundings of p and dp would leave something of it)
     bool wide_bias, wide_pairs;  // four neighbouring values of a row are one aligned load
 };
@@ -242,13 +247,14 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     extern __shared__ __attribute__((aligned(16))) unsigned char backward_lds[];
     __shared__ float maxima[WAVES][kRows], totals[WAVES][kRows];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
-    const int2 item = decode(p.contexts, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
-    const int context = item.x, q0 = item.y * kRows, my_q = q0 + li, S = p.S, D = p.D;
+    const int2 item = decode(p.contexts, p.tiles * p.parts, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
+    const int context = item.x, part = item.y % p.parts, q0 = item.y / p.parts * kRows, my_q = q0 + li, S = p.S, D = p.D;
+    const int begin = (part * WAVES + wave) * kRows, step = p.parts * WAVES * kRows;  // the wavefront's first tile, and to its next one
     const size_t first = static_cast<size_t>(context) * S;
     unsigned char *const k_tile = backward_lds + wave * 2 * Tile<DC>::kBytes, *const v_tile = k_tile + Tile<DC>::kBytes;
     unsigned char *const places = backward_lds + WAVES * 2 * Tile<DC>::kBytes;
     const int key_end = CAUSAL ? min(S, q0 + kRows) : S, last_key = CAUSAL ? min(my_q, S - 1) : S - 1;
-    if (wave * kRows < key_end) load_tile<DC, VEC, true>(p.k + first * D, S, D, wave * kRows, k_tile, places, lane);
+    if (begin < key_end) load_tile<DC, VEC, true>(p.k + first * D, S, D, begin, k_tile, places, lane);
     f32x4 q[DC / 8], g[DC / 8];
     float delta = 0.0f;
     {
@@ -305,14 +311,14 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     // (the wavefront's two tiles take turns; biases come with their tile, as what is waited for behind the next tile's loads is waited for with them)
     auto sweep = [&](auto wide) {
         Biases next;
-        load_biases(wide, wave * kRows, next);
-        for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
+        load_biases(wide, begin, next);
+        for (int key0 = begin, turn = 0; key0 < key_end; key0 += step, turn ^= 1) {
             f32x4 with[4];
             wait_for_loads();
             wait_for_reads();
             sum_of(next, with);
-            load_biases(wide, key0 + WAVES * kRows, next);
-            if (key0 + WAVES * kRows < key_end) load_tile<DC, VEC, false>(p.k + first * D, S, D, key0 + WAVES * kRows, turn ? k_tile : v_tile, places, lane);
+            load_biases(wide, key0 + step, next);
+            if (key0 + step < key_end) load_tile<DC, VEC, false>(p.k + first * D, S, D, key0 + step, turn ? k_tile : v_tile, places, lane);
             const f32x16 s = scores(turn ? v_tile : k_tile, with, key0);
             float top = most;
 #pragma unroll
@@ -334,8 +340,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     };
     if constexpr (DQ) {
         wait_for_reads();
-        load_values(wave * kRows);
-        load_keys(wave * kRows);
+        load_values(begin);
+        load_keys(begin);
     }
     {
         const float other = __shfl_xor(most, 32), other_total = __shfl_xor(total, 32), top = fmaxf(most, other), safe = top == -INFINITY ? 0.0f : top;
@@ -357,15 +363,21 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     // (a row without keys: every p is 0)
     const float lse = my_q < S && sum != 0.0f ? safe + __log2f(sum) : INFINITY;
     if (wave == 0 && lh == 0) {
-        p.lse[static_cast<size_t>(context) * p.padded + my_q] = lse;
-        p.delta[static_cast<size_t>(context) * p.padded + my_q] = my_q < S ? delta : 0.0f;
+        const size_t at = static_cast<size_t>(context) * p.padded + my_q, of_part = static_cast<size_t>(part) * p.contexts * p.padded;
+        if (p.parts > 1) {
+            p.part_max[of_part + at] = top;
+            p.part_total[of_part + at] = sum;
+        } else {
+            p.lse[at] = lse;
+        }
+        if (part == 0) p.delta[at] = my_q < S ? delta : 0.0f;
     }
     if constexpr (DQ) {
         f32x16 dq[Tile<DC>::kAcross];
 #pragma unroll
         for (int dt = 0; dt < Tile<DC>::kAcross; ++dt) dq[dt] = f32x16{};
         auto second = [&](auto wide) {
-            for (int key0 = wave * kRows; key0 < key_end; key0 += WAVES * kRows) {
+            for (int key0 = begin; key0 < key_end; key0 += step) {
                 Biases biases_of;
                 f32x4 with[4];
                 wait_for_loads();
@@ -373,13 +385,13 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
                 const f32x16 dp = product<DC>(v_tile, g, li, lh);
                 sum_of(biases_of, with);
                 wait_for_reads();
-                load_values(key0 + WAVES * kRows);  // each tile's successor as soon as it has been read
+                load_values(key0 + step);  // each tile's successor as soon as it has been read
                 f32x16 s = scores(k_tile, with, key0);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - lse) * (dp[r] - delta);
                 add_product<DC>(k_tile, s, dq, li, lh);
                 wait_for_reads();
-                load_keys(key0 + WAVES * kRows);
+                load_keys(key0 + step);
             }
         };
         if (p.wide_bias) second(std::true_type{});
@@ -394,8 +406,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char backward_lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
-    const int2 item = decode(p.contexts, p.tiles, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
-    const int context = item.x, q0 = item.y * kRows, my_q = q0 + li, S = p.S, D = p.D;
+    const int2 item = decode(p.contexts, p.tiles * p.parts, p.swizzle, CAUSAL, CAUSAL, blockIdx.x);
+    const int context = item.x, part = item.y % p.parts, q0 = item.y / p.parts * kRows, my_q = q0 + li, S = p.S, D = p.D;
+    const int begin = (part * WAVES + wave) * kRows, step = p.parts * WAVES * kRows;  // the wavefront's first tile, and to its next one
     const size_t first = static_cast<size_t>(context) * S;
     const int key_end = CAUSAL ? min(S, q0 + kRows) : S, last_key = CAUSAL ? min(my_q, S - 1) : S - 1;
     unsigned char *const tiles = backward_lds + wave * 2 * Tile<DC>::kBytes;  // they take turns
@@ -412,20 +425,21 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
 #pragma unroll
             for (int a = 0; a < 4; ++a) ds[a] = bias4<decltype(wide)::value>(pairs, static_cast<unsigned>(li) * p.pair_row + key0 + a * 8 + lh * 4);
         };
-        load(std::true_type{}, wave * kRows, 0);
-        for (int key0 = wave * kRows, turn = 0; key0 < key_end; key0 += WAVES * kRows, turn ^= 1) {
+        load(std::true_type{}, begin, 0);
+        for (int key0 = begin, turn = 0; key0 < key_end; key0 += step, turn ^= 1) {
             f32x16 weights;
             wait_for_loads();
             wait_for_reads();
 #pragma unroll
             for (int r = 0; r < 16; ++r) weights[r] = key0 + row_of(r) + 4 * lh > last_key ? 0.0f : ds[r >> 2][r & 3];
-            load(std::false_type{}, key0 + WAVES * kRows, turn ^ 1);
+            load(std::false_type{}, key0 + step, turn ^ 1);
             add_product<DC>(tiles + turn * Tile<DC>::kBytes, weights, dq, li, lh);
         }
     };
     if (p.wide_pairs) sweep(std::true_type{});
     else sweep(std::false_type{});
-    write_rows<DC, WAVES, VEC>(dq, p.scale * p.keep, p.grad_q + first * D, q0, S, D, backward_lds);
+    if (p.parts > 1) write_rows<DC, WAVES, VEC>(dq, 1.0f, p.part_q + (static_cast<size_t>(part) * p.contexts * S + first) * D, q0, S, D, backward_lds);
+    else write_rows<DC, WAVES, VEC>(dq, p.scale * p.keep, p.grad_q + first * D, q0, S, D, backward_lds);
 }
 
 // ---- dk, dv, the biases' gradients: keys stay -----------------------------------------------------------------------------------------------
@@ -436,8 +450,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     extern __shared__ __attribute__((aligned(16))) unsigned char backward_lds[];
     __shared__ float totals[WAVES][kRows];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, lh = lane >> 5;
-    const int2 item = decode(p.contexts, p.tiles, p.swizzle, CAUSAL, false, blockIdx.x);
-    const int context = item.x, k0 = item.y * kRows, my_key = k0 + li, S = p.S, D = p.D;
+    const int2 item = decode(p.contexts, p.tiles * p.parts, p.swizzle, CAUSAL, false, blockIdx.x);
+    const int context = item.x, part = item.y % p.parts, k0 = item.y / p.parts * kRows, my_key = k0 + li, S = p.S, D = p.D;
+    const int step = p.parts * WAVES * kRows;
     const size_t first = static_cast<size_t>(context) * S;
     unsigned char *const q_tile = backward_lds + wave * 2 * Tile<DC>::kBytes, *const g_tile = q_tile + Tile<DC>::kBytes;
     unsigned char *const places = backward_lds + WAVES * 2 * Tile<DC>::kBytes;
@@ -447,7 +462,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
     auto load_grads = [&](int row0) {
         if (row0 < S) load_tile<DC, VEC, false>(p.grad_out + first * D, S, D, row0, g_tile, places, lane);
     };
-    const int start = (CAUSAL ? k0 : 0) + wave * kRows;
+    const int start = (CAUSAL ? k0 : 0) + (part * WAVES + wave) * kRows;
     load_queries(std::true_type{}, start);
     load_grads(start);
     f32x4 k[DC / 8], v[DK ? DC / 8 : 1];
@@ -469,8 +484,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
         for (int dt = 0; dt < Tile<DC>::kAcross; ++dt) dv[DV ? dt : 0] = f32x16{};
     float dz = 0.0f;
     if (CAUSAL && DK && p.grad_attn_bias && my_key < S)  // queries before the tile do not see it
-        for (int q = wave * 2 + lh; q < k0; q += WAVES * 2) p.grad_attn_bias[(first + q) * S + my_key] = 0.0f;
-    for (int row0 = start; row0 < S; row0 += WAVES * kRows) {
+        for (int q = (part * WAVES + wave) * 2 + lh; q < k0; q += p.parts * WAVES * 2) p.grad_attn_bias[(first + q) * S + my_key] = 0.0f;
+    for (int row0 = start; row0 < S; row0 += step) {
         // the biases of the lane's key; beyond the descriptor for a key behind the last
         const unsigned at = my_key < S ? (4u * lh * S + my_key) * 4u : 0x80000000u;
         float bias[16];
@@ -503,7 +518,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
             for (int a = 0; a < 4; ++a) asm volatile("" : "+v"(delta[a]));
         }
         wait_for_reads();
-        load_grads(row0 + WAVES * kRows);  // each tile's successor as soon as it has been read
+        load_grads(row0 + step);  // each tile's successor as soon as it has been read
         if constexpr (DK) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -519,7 +534,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
             }
         }
         wait_for_reads();
-        load_queries(std::false_type{}, row0 + WAVES * kRows);
+        load_queries(std::false_type{}, row0 + step);
     }
     if constexpr (DK) {
         if (p.grad_z_bias) {
@@ -530,25 +545,65 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DC <
                 float sum = totals[0][li];
 #pragma unroll
                 for (int w = 1; w < WAVES; ++w) sum += totals[w][li];
-                p.grad_z_bias[first + my_key] = sum * p.keep;
+                if (p.parts > 1) p.part_z[static_cast<size_t>(part) * p.contexts * S + first + my_key] = sum;
+                else p.grad_z_bias[first + my_key] = sum * p.keep;
             }
         }
-        write_rows<DC, WAVES, VEC>(dk, p.scale * p.keep, p.grad_k + first * D, k0, S, D, backward_lds);
+        if (p.parts > 1) write_rows<DC, WAVES, VEC>(dk, 1.0f, p.part_k + (static_cast<size_t>(part) * p.contexts * S + first) * D, k0, S, D, backward_lds);
+        else write_rows<DC, WAVES, VEC>(dk, p.scale * p.keep, p.grad_k + first * D, k0, S, D, backward_lds);
     }
-    if constexpr (DV) write_rows<DC, WAVES, VEC>(dv, 1.0f, p.grad_v + first * D, k0, S, D, backward_lds);
+    if constexpr (DV) {
+        float *const to = p.parts > 1 ? p.part_v + static_cast<size_t>(part) * p.contexts * S * D : p.grad_v;
+        write_rows<DC, WAVES, VEC>(dv, 1.0f, to + first * D, k0, S, D, backward_lds);
+    }
+}
+
+// The parts of rows' log-sum-exps together.
+__global__ __launch_bounds__(256) void attention_f32_join_lse_kernel(BackwardArgs p)
+{
+    const size_t rows = static_cast<size_t>(p.contexts) * p.padded, at = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= rows) return;
+    float top = p.part_max[at];
+    for (int part = 1; part < p.parts; ++part) top = fmaxf(top, p.part_max[part * rows + at]);
+    const float safe = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    for (int part = 0; part < p.parts; ++part) sum += p.part_total[part * rows + at] * __builtin_amdgcn_exp2f(p.part_max[part * rows + at] - safe);
+    p.lse[at] = static_cast<int>(at % p.padded) < p.S && sum != 0.0f ? safe + __log2f(sum) : INFINITY;
+}
+// The parts of the gradients together, in their order.
+__global__ __launch_bounds__(256) void attention_f32_join_kernel(BackwardArgs p)
+{
+    const size_t rows = static_cast<size_t>(p.contexts) * p.S, values = blockIdx.y == 3 ? rows : rows * p.D;
+    const float *const from = blockIdx.y == 0 ? p.part_q : blockIdx.y == 1 ? p.part_k : blockIdx.y == 2 ? p.part_v : p.part_z;
+    float *const to = blockIdx.y == 0 ? p.grad_q : blockIdx.y == 1 ? p.grad_k : blockIdx.y == 2 ? p.grad_v : p.grad_z_bias;
+    const float by = blockIdx.y < 2 ? p.scale : 1.0f;  // (more than one part has more than one key)
+    if (!to) return;
+    for (size_t at = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; at < values; at += static_cast<size_t>(gridDim.x) * 256) {
+        float sum = from[at];
+        for (int part = 1; part < p.parts; ++part) sum += from[part * values + at];
+        to[at] = sum * by;
+    }
 }
 
 // Values of ds that are kept from dk's pass for dq's where nobody asked for them: 256 MiB, as much as the last-level cache holds.  Kept and worked out
 // again: 16 contexts of 1024 x 64 145 and 170 µs, 4 of 2048 x 80 217 and 270, 96 causal ones of 333 x 80 134 and 139.
 constexpr size_t kPairsKept = 64u << 20;
 
+// Workgroups to a tile: as many as the chip has room for at once where one a tile would be half of that or less, of two rounds or more each.  3 causal
+// contexts of 659 x 256 with biases take 195 µs so and 490 with one a tile, 8 of 512 x 128 64 and 78; 16 of 512 x 128, one a tile, 82.
+int parts_of(size_t workgroups, size_t tiles, size_t head_dim)
+{
+    const size_t room = head_dim <= 64 ? 512 : 256, rounds = tiles / (head_dim <= 128 ? 4 : 2);
+    return static_cast<int>(std::max<size_t>(1, std::min({room / workgroups, rounds / 2, static_cast<size_t>(16)})));
+}
+
 template <class Kernel>
 hipError_t launch(Kernel kernel, const BackwardArgs &args, int waves, size_t lds, bool by_tile, bool last_first, hipStream_t stream)
 {
-    const size_t blocks = static_cast<size_t>(args.contexts) * args.tiles;
+    const size_t blocks = static_cast<size_t>(args.contexts) * args.tiles * args.parts;
     for (const size_t block : {static_cast<size_t>(0), blocks - 1}) {  // the grid is what the kernels' decode assumes
-        const int2 item = decode(args.contexts, args.tiles, args.swizzle, by_tile, last_first, static_cast<unsigned>(block));
-        if (blocks > kMaxDim || item.x < 0 || item.x >= args.contexts || item.y < 0 || item.y >= args.tiles) return hipErrorInvalidConfiguration;
+        const int2 item = decode(args.contexts, args.tiles * args.parts, args.swizzle, by_tile, last_first, static_cast<unsigned>(block));
+        if (blocks > kMaxDim || item.x < 0 || item.x >= args.contexts || item.y < 0 || item.y >= args.tiles * args.parts) return hipErrorInvalidConfiguration;
     }
     const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
     if (rc != hipSuccess) return rc;
@@ -563,6 +618,12 @@ hipError_t launch_waves(const BackwardArgs &args, hipStream_t stream)
     hipError_t rc = args.pairs ? launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL, false>, args, WAVES, lds, CAUSAL, CAUSAL, stream)
                                : launch(attention_f32_grad_q_kernel<DC, WAVES, VEC, CAUSAL, true>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
     if (rc != hipSuccess) return rc;
+    if (args.parts > 1) {
+        hipLaunchKernelGGL(attention_f32_join_lse_kernel, dim3(static_cast<unsigned>((static_cast<size_t>(args.contexts) * args.padded + 255) / 256)), dim3(256), 0,
+                           stream, args);
+        rc = hipGetLastError();
+        if (rc != hipSuccess) return rc;
+    }
     if constexpr (DC <= 128) {
         rc = launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, true, true>, args, WAVES, lds, CAUSAL, false, stream);
     } else {
@@ -571,7 +632,11 @@ hipError_t launch_waves(const BackwardArgs &args, hipStream_t stream)
         rc = launch(attention_f32_grad_kv_kernel<DC, WAVES, VEC, CAUSAL, false, true>, args, WAVES, lds, CAUSAL, false, stream);
     }
     if (rc != hipSuccess || !args.pairs) return rc;
-    return launch(attention_f32_grad_q_of_pairs_kernel<DC, WAVES, VEC, CAUSAL>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
+    rc = launch(attention_f32_grad_q_of_pairs_kernel<DC, WAVES, VEC, CAUSAL>, args, WAVES, lds, CAUSAL, CAUSAL, stream);
+    if (rc != hipSuccess || args.parts == 1) return rc;
+    const size_t values = static_cast<size_t>(args.contexts) * args.S * std::max(args.D, 1);
+    hipLaunchKernelGGL(attention_f32_join_kernel, dim3(static_cast<unsigned>(std::min<size_t>((values + 255) / 256, 2048)), 4), dim3(256), 0, stream, args);
+    return hipGetLastError();
 }
 
 template <int DC, bool VEC, bool CAUSAL>
@@ -628,14 +693,23 @@ hipError_t launch_attention_backward_f32(size_t contexts, size_t sequence, size_
     args.wide_bias = sequence % 4 == 0 && aligned(attn_bias) && aligned(z_bias);
     const size_t rows = contexts * args.padded, pair_row = grad_attn_bias ? sequence : (sequence + 3) / 4 * 4;
     const size_t kept = !grad_attn_bias && contexts * sequence * pair_row <= kPairsKept ? contexts * sequence * pair_row : 0;
+    const size_t values = (contexts * sequence * head_dim + 63) / 64 * 64, keys = (contexts * sequence + 63) / 64 * 64;
+    args.parts = grad_attn_bias || kept ? parts_of(contexts * args.tiles, args.tiles, head_dim) : 1;
+    const size_t of_parts = args.parts > 1 ? args.parts * (3 * values + keys + 2 * rows) : 0;
     void *scratch = nullptr;
-    const hipError_t rc = stream_workspace(stream, (kept + 2 * rows) * sizeof(float), &scratch);
+    const hipError_t rc = stream_workspace(stream, (kept + 2 * rows + of_parts) * sizeof(float), &scratch);
     if (rc != hipSuccess) return rc;
     args.pairs = grad_attn_bias ? grad_attn_bias : kept ? static_cast<float *>(scratch) : nullptr;
     args.pair_row = static_cast<int>(pair_row);
     args.wide_pairs = pair_row % 4 == 0 && aligned(args.pairs);
     args.lse = static_cast<float *>(scratch) + kept;
     args.delta = args.lse + rows;
+    args.part_q = args.delta + rows;
+    args.part_k = args.part_q + args.parts * values;
+    args.part_v = args.part_k + args.parts * values;
+    args.part_z = args.part_v + args.parts * values;
+    args.part_max = args.part_z + args.parts * keys;
+    args.part_total = args.part_max + args.parts * rows;
     const bool vec = head_dim % 4 == 0 && aligned(q) && aligned(k) && aligned(v) && aligned(out) && aligned(grad_out) &&
                      aligned(grad_q) && aligned(grad_k) && aligned(grad_v);
     if (head_dim <= 32) return launch_width<32>(args, vec, causal, stream);

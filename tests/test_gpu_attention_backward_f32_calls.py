@@ -168,3 +168,57 @@ def test_a_single_key_has_all_of_every_row(hip, d, biased, causal):
     s = (case.x["q"] * case.x["k"]).sum((1, 2)) * case.scale + (case.x["z"][:, 0] + case.x["bias"][:, 0, 0] if biased else 0)
     assert s.abs().max() * 1.4427 < 15.9
     assert ((got["dv"] - case.x["g"]).abs() <= 2.0**-20 * case.x["g"].abs()).all()
+
+
+PARTS = [(1, 1000, 64), (2, 700, 80), (1, 1024, 128), (1, 530, 256), (3, 401, 200), (1, 1500, 8), (2, 999, 31), (1, 2048, 96)]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("contexts,n,d", PARTS)
+def test_few_long_contexts(hip, contexts, n, d, biased, causal):
+    """Several workgroups to a tile, whose sums are added up behind them; keys that biases bar, and a row that sees nothing."""
+    case = Buffers(n + d, contexts, n, d, causal, biased)
+    if biased:
+        case.x["z"][0, n // 3:n // 2] = -torch.inf
+        case.x["bias"][0, n - 5] = -torch.inf
+        case.x["bias"][contexts - 1, 40, ::2] = -torch.inf
+    want = case.want(list(range(contexts)))
+    case.x["out"].copy_(torch.from_numpy(want["out"][0].astype(np.float32)))
+    torch.cuda.synchronize()
+    case.run(hip)
+    first = case.results()
+    for name, a in first.items():
+        plain.check(a.cpu().numpy(), want[name], name)
+    for a in case.y.values():
+        a.fill_(7)
+    torch.cuda.synchronize()
+    case.run(hip)
+    for name, a in case.results().items():
+        assert torch.equal(a, first[name]), name
+
+
+def test_few_long_contexts_captured_and_replayed(hip):
+    case, larger = Buffers(21, 1, 1100, 64, True, True), Buffers(22, 1, 2000, 96, False, False)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        case.run(hip, torch.cuda.current_stream().cuda_stream)
+    try:
+        for replay in range(3):
+            case.x["q"].mul_(-0.5)
+            torch.cuda.synchronize()
+            case.run(hip)
+            want = case.results()
+            for a in case.y.values():
+                a.fill_(7)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            for name, a in case.results().items():
+                assert torch.equal(a, want[name]), (replay, name)
+            larger.run(hip, stream.cuda_stream)  # grows the stream's scratch
+            torch.cuda.synchronize()
+    finally:
+        del graph
+        hip.release_scratch(stream.cuda_stream)
+        hip.release_scratch(None)
